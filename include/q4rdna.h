@@ -326,6 +326,154 @@ int q4rdna_pack(const float *w, uint32_t rows, uint32_t columns, int algorithm, 
  * product (source/q4rdna_cpu_experiment.cpp:270-271). */
 int q4rdna_dequantize(const q4rdna_weight *w, float *out, void *stream);
 
+/* ---- the rest of a decoder layer -------------------------------------------
+ * What a program runs between the GEMVs above: cache append, attention and
+ * norm.  No reference counterpart (its llama.cpp host runs these).  The
+ * launches are asynchronous on `stream`; activations are fp32, fp16 or bf16
+ * and every sum, softmax statistic and norm is kept in fp32. */
+#define Q4RDNA_F32 0
+#define Q4RDNA_F16 1
+#define Q4RDNA_BF16 2
+
+/* A paged key/value cache of one layer, in caller-owned device buffers.
+ * Pages are blocks of Q4RDNA_KV_BLOCK tokens.  A full block holds int8 codes
+ * with one fp32 scale per head for K and one for V (x = code * scale).  The
+ * last, partly filled block of a sequence is held in the sequence's slot with
+ * 16-bit codes, as two int8 planes (256 * high + low, |code| <= 32512), and an
+ * fp32 scale per token and head (absmax / 32512).  When a block fills, its
+ * scale becomes 256 * the largest of its tokens' scales and each code
+ * rint(code16 * (token scale / scale)): every number is rounded to 16 bits
+ * once and to 8 bits once, so the cache's bytes do not depend on the chunks in
+ * which the tokens arrive, and a full page never changes again (sequences may
+ * share it).  A slot holds two blocks, used in turn: a sequence may be cut
+ * back to any length >= 64 * (length / 64 - 1), its last full block included,
+ * and be appended to from there, as long as no other sequence reads that page.
+ *
+ * The order of codes within a block of one head, 16 bytes per lane of a
+ * 64-lane int8 matrix instruction:
+ *   K  token 16 n + c, number 64 s + 16 g + j at (((n * D/64 + s) * 4 + g) * 16 + c) * 16 + j
+ *   V  token 16 a + 4 g + b, number 16 n + c  at ((n * 4 + g) * 16 + c) * 16 + 4 a + b
+ * A token with a number that is not finite has the scale NaN and reads as NaN,
+ * and so does its block once full; one whose largest number is under 1e-30
+ * reads as zero. */
+#define Q4RDNA_KV_BLOCK 64
+typedef struct q4rdna_kv_cache {
+    int8_t *pages;        /* [page_count][kv_heads][2 (K, V)][64 * head_dim], 16-byte aligned */
+    float *scales;        /* [page_count][kv_heads][2], 8-byte aligned */
+    int8_t *open;         /* [slot_count][2][kv_heads][4 (K high, K low, V high, V low)][64 * head_dim], 16-byte aligned */
+    float *open_scales;   /* [slot_count][2][kv_heads][2 (K, V)][64], 16-byte aligned */
+    uint32_t *faults;     /* counts what the kernels refused (see q4rdna_kv_batch), or NULL */
+    uint32_t page_count;
+    uint32_t slot_count;
+    uint32_t kv_heads;
+    uint32_t head_dim;    /* 64 or 128 */
+    int32_t device;
+    uint32_t reserved;
+} q4rdna_kv_cache;
+
+/* The sequences of one step, shared by the calls of all layers.  The arrays
+ * are device memory and are read when the kernels run, so a captured graph
+ * may be replayed with other lengths, tables and slots in them.  Sequence i
+ * has `past[i]` tokens in the cache before the step and the step's tokens
+ * cu_tokens[i] .. cu_tokens[i + 1] - 1 (cu_tokens NULL: one token each,
+ * tokens == sequences) at the positions past[i], past[i] + 1, ...  Its token t
+ * lies in page table[i * table_width + t / 64].  slots[i] is its slot (NULL:
+ * slot i).  max_tokens bounds every sequence's tokens in the step.
+ * The kernels check what they read: a sequence whose entries are out of range
+ * (tokens outside the step's or more than max_tokens, past < 0, past + tokens
+ * > 64 * table_width, a bad slot) is skipped, its results not written; a page
+ * outside the cache is not written, and rows that need to read it come out as
+ * NaN.  Each adds to *faults. */
+typedef struct q4rdna_kv_batch {
+    const int32_t *past;      /* [sequences] */
+    const int32_t *cu_tokens; /* [sequences + 1], ascending, or NULL */
+    const int32_t *table;     /* [sequences][table_width] */
+    const int32_t *slots;     /* [sequences] or NULL */
+    uint32_t sequences;       /* at most 65535 */
+    uint32_t tokens;          /* of all sequences in this step */
+    uint32_t max_tokens;
+    uint32_t table_width;     /* at most 2^24 */
+} q4rdna_kv_batch;
+
+/* Rows of activations [tokens][heads][head_dim]: the numbers of a head are
+ * contiguous, the strides are in elements. */
+typedef struct q4rdna_kv_rows {
+    void *data;
+    int64_t token_stride;
+    int64_t head_stride;
+} q4rdna_kv_rows;
+
+/* Append the step's keys and values.  Each head's row of q and k is first
+ * normalised (x * rsqrt(mean x^2 + eps) * weight) where q_norm / k_norm is
+ * given, then its first `rotary` numbers are rotated by the token's position
+ * p: pairs (x_i, x_{i + rotary/2}), or (x_{2i}, x_{2i+1}) with `interleaved`,
+ * become (a cos - b sin, b cos + a sin) with cos[p][i], sin[p][i].  Rotated q
+ * goes to q_out (which may be q); rotated k and v go into the cache.
+ * rotary is a multiple of 8 up to head_dim, 0 for no rotation; a sequence that
+ * reaches past the `positions` rows of cos and sin is skipped as above. */
+typedef struct q4rdna_kv_append_desc {
+    uint32_t dtype;           /* of k, v, q and q_out */
+    uint32_t q_heads;         /* a multiple of kv_heads; 0: no q */
+    q4rdna_kv_rows k, v, q, q_out;
+    const float *cos, *sin;   /* [positions][rotary / 2], 16-byte aligned */
+    uint32_t positions;
+    uint32_t rotary;
+    uint32_t interleaved;
+    float eps;
+    const float *q_norm, *k_norm; /* [head_dim], 16-byte aligned, or NULL */
+} q4rdna_kv_append_desc;
+int q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
+                     const q4rdna_kv_append_desc *desc, void *stream);
+
+/* Attention of the step's query tokens, after q4rdna_kv_append of the same
+ * batch: out = sum_t softmax_t(scale * q . k_t) v_t over the tokens t <= p of
+ * the query's sequence (t > p - window where window > 0), p its position.
+ * Query head h reads kv head h / (q_heads / kv_heads).  lse (may be NULL)
+ * receives log sum_t exp(scale * q . k_t), [tokens][q_heads].  Calls that
+ * split a sequence use scratch per (device, stream), under the rules of the
+ * GEMVs' scratch above: make one call of a shape on the stream before
+ * capturing it. */
+typedef struct q4rdna_kv_attend_desc {
+    uint32_t dtype;           /* of q and out */
+    uint32_t q_heads;
+    q4rdna_kv_rows q, out;
+    float *lse;
+    float scale;
+    uint32_t window;
+} q4rdna_kv_attend_desc;
+int q4rdna_kv_attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
+                     const q4rdna_kv_attend_desc *desc, void *stream);
+
+/* The cache's tokens past[i] .. past[i] + count - 1 as numbers, in the order of
+ * the batch's tokens: k and v [tokens][kv_heads][head_dim] of `dtype`.  The
+ * sequence's length must be past[i] + count (its last, open block is found by
+ * it); past 0 reads it whole. */
+int q4rdna_kv_read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dtype,
+                   const q4rdna_kv_rows *k, const q4rdna_kv_rows *v, void *stream);
+
+/* Residual add with the norms before and after it, per row:
+ *   h = residual + scale * gate * post(y)    post(y) = y * rsqrt(mean y^2 + eps) * post_weight, or y
+ *   n = h * rsqrt(mean h^2 + eps) * weight
+ * y NULL: h = residual.  gate NULL: 1; gate_stride 0: one gate for all rows.
+ * post_weight, h and n may be NULL (no norm of y, output not wanted).  n uses
+ * h before its rounding to dtype.  h may be residual or y and n may be y or
+ * residual, with the same strides; other overlaps are not allowed.  Strides
+ * are in elements; width is at most Q4RDNA_NORM_MAX_WIDTH. */
+#define Q4RDNA_NORM_MAX_WIDTH 16384
+typedef struct q4rdna_add_norm_desc {
+    uint32_t dtype;           /* of residual, y, gate, h and n */
+    uint32_t rows;
+    uint32_t width;
+    float scale;
+    float eps;
+    uint32_t reserved;
+    const void *residual, *y, *gate;
+    void *h, *n;
+    int64_t residual_stride, y_stride, gate_stride, h_stride, n_stride;
+    const float *post_weight, *weight; /* [width]; weight may be NULL only where n is */
+} q4rdna_add_norm_desc;
+int q4rdna_add_norm(const q4rdna_add_norm_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,330 @@
+// Entry points of the decoder-layer operators (include/q4rdna.h): argument
+// checks, attention's scratch and the launches.  All compute runs in the
+// kernels of q4rdna_cache.hip, q4rdna_attend.hip and q4rdna_norm.hip.
+#include "q4rdna_layer.h"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <exception>
+#include <map>
+#include <mutex>
+#include <utility>
+#include <vector>
+
+#include "q4rdna_runtime.h"
+
+namespace {
+
+using q4rdna::set_error;
+
+bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+uint32_t size_of(uint32_t dtype) { return dtype == Q4RDNA_F32 ? 4 : 2; }
+
+// No exception leaves a C entry point.
+template <typename F>
+int guarded(F body) {
+    try {
+        return body();
+    } catch (const std::exception &e) {
+        return set_error(Q4RDNA_ERR_MEMORY, "%s", e.what());
+    }
+}
+
+int launched(hipError_t e, const char *what) {
+    return e == hipSuccess ? Q4RDNA_OK : set_error(Q4RDNA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+int check_device(int device) {
+    int current = -1;
+    if (hipGetDevice(&current) != hipSuccess || current != device)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "the cache lives on device %d, the current device is %d", device, current);
+    return Q4RDNA_OK;
+}
+
+// Compute units per device, looked up once.
+std::atomic<uint32_t> g_cus[64];
+
+uint32_t cu_count(int device) {
+    if (device < 0 || device >= 64) return 256;
+    uint32_t n = g_cus[device].load(std::memory_order_relaxed);
+    if (n != 0) return n;
+    int v = 0;
+    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || v <= 0) v = 256;
+    g_cus[device].store(static_cast<uint32_t>(v), std::memory_order_relaxed);
+    return static_cast<uint32_t>(v);
+}
+
+// Checks that need no device come first, so a malformed call is refused the
+// same way with and without one.
+int check_cache(const q4rdna_kv_cache *c) {
+    if (c == nullptr || c->pages == nullptr || c->scales == nullptr || c->open == nullptr || c->open_scales == nullptr)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "null cache or cache buffer");
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "head_dim is %u: 64 and 128 are supported", c->head_dim);
+    if (c->kv_heads == 0 || c->kv_heads > 1024 || c->page_count == 0 || c->page_count > 0x7fffffffu || c->slot_count == 0 ||
+        c->slot_count > 0x7fffffffu)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "cache of %u pages, %u slots, %u kv heads", c->page_count, c->slot_count,
+                         c->kv_heads);
+    if (!aligned(c->pages, 16) || !aligned(c->scales, 8) || !aligned(c->open, 16) || !aligned(c->open_scales, 16) ||
+        !aligned(c->faults, 4))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned cache buffer");
+    return Q4RDNA_OK;
+}
+
+int check_batch(const q4rdna_kv_batch *b) {
+    if (b == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null batch");
+    if (b->sequences == 0 || b->tokens == 0) return Q4RDNA_OK;  // nothing to do
+    if (b->past == nullptr || b->table == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null past or table");
+    if (!aligned(b->past, 4) || !aligned(b->cu_tokens, 4) || !aligned(b->table, 4) || !aligned(b->slots, 4))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned batch array");
+    if (b->sequences > 65535 || b->tokens > 0x3fffffffu || b->table_width == 0 || b->table_width > (1u << 24))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "step of %u sequences, %u tokens, %u table columns", b->sequences, b->tokens,
+                         b->table_width);
+    if (b->max_tokens == 0 || (b->cu_tokens == nullptr && (b->tokens != b->sequences || b->max_tokens != 1)))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of %u sequences, at most %u each: without cu_tokens each has one",
+                         b->tokens, b->sequences, b->max_tokens);
+    return Q4RDNA_OK;
+}
+
+int check_rows(const q4rdna_kv_rows &r, uint32_t dtype, const char *name) {
+    if (r.data == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null %s", name);
+    if (!aligned(r.data, size_of(dtype))) return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned %s", name);
+    return Q4RDNA_OK;
+}
+
+int check_dtype(uint32_t dtype) {
+    return dtype > Q4RDNA_BF16 ? set_error(Q4RDNA_ERR_ARGUMENT, "unknown dtype %u", dtype) : Q4RDNA_OK;
+}
+
+int check_heads(uint32_t q_heads, uint32_t kv_heads) {
+    if (q_heads == 0 || q_heads % kv_heads != 0 || q_heads > 65536)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "%u query heads over %u kv heads", q_heads, kv_heads);
+    return Q4RDNA_OK;
+}
+
+// Whether every row starts at a multiple of `elements`.
+bool wide_rows(const q4rdna_kv_rows &r, uint32_t dtype, int64_t elements) {
+    return aligned(r.data, elements * size_of(dtype)) && r.token_stride % elements == 0 && r.head_stride % elements == 0;
+}
+
+// Attention's partial results and arrival counters per (device, stream), under
+// the same rules as the GEMVs' exchange slots (q4rdna_runtime.cpp): outgrown
+// buffers are kept, since launches still queued and captured graphs use them,
+// and nothing is allocated while the stream is being captured.
+struct Scratch {
+    float *partials = nullptr;
+    size_t floats = 0;
+    uint32_t *arrived = nullptr;
+    size_t jobs = 0;
+};
+std::mutex g_scratch_mu;
+std::map<std::pair<int, hipStream_t>, Scratch> g_scratch;
+std::vector<void *> g_retired;
+
+bool stream_captured(hipStream_t stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return status == hipStreamCaptureStatusActive;
+}
+
+// Device memory while other streams may be under capture: relaxed mode, and
+// zeros (where asked for) in the order of the stream.
+hipError_t relaxed_malloc(void **p, size_t bytes, bool zero, hipStream_t stream) {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    hipError_t e = hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) return e;
+    e = hipMalloc(p, bytes);
+    if (e == hipSuccess && zero && (e = hipMemsetAsync(*p, 0, bytes, stream)) != hipSuccess) (void)hipFree(*p);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    return e;
+}
+
+int get_scratch(int device, hipStream_t stream, size_t floats, size_t jobs, Scratch *out) {
+    std::lock_guard<std::mutex> lock(g_scratch_mu);
+    Scratch &s = g_scratch[{device, stream}];
+    if (s.floats < floats || s.jobs < jobs) {
+        if (stream_captured(stream))
+            return set_error(Q4RDNA_ERR_MEMORY, "attention scratch: it cannot grow while its stream is being captured");
+        g_retired.reserve(g_retired.size() + 2);
+        if (s.floats < floats) {
+            const size_t count = std::max(floats, 2 * s.floats);
+            void *p = nullptr;
+            const hipError_t e = relaxed_malloc(&p, count * sizeof(float), false, stream);
+            if (e != hipSuccess) return set_error(Q4RDNA_ERR_MEMORY, "attention scratch: %s", hipGetErrorString(e));
+            if (s.partials != nullptr) g_retired.push_back(s.partials);
+            s.partials = static_cast<float *>(p);
+            s.floats = count;
+        }
+        if (s.jobs < jobs) {
+            const size_t count = std::max(jobs, 2 * s.jobs);
+            void *p = nullptr;
+            const hipError_t e = relaxed_malloc(&p, count * sizeof(uint32_t), true, stream);
+            if (e != hipSuccess) return set_error(Q4RDNA_ERR_MEMORY, "attention scratch: %s", hipGetErrorString(e));
+            if (s.arrived != nullptr) g_retired.push_back(s.arrived);
+            s.arrived = static_cast<uint32_t *>(p);
+            s.jobs = count;
+        }
+    }
+    *out = s;
+    return Q4RDNA_OK;
+}
+
+int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4rdna_kv_append_desc *desc, void *stream) {
+    int rc;
+    if ((rc = check_cache(cache)) != Q4RDNA_OK || (rc = check_batch(batch)) != Q4RDNA_OK) return rc;
+    if (desc == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null descriptor");
+    if (batch->sequences == 0 || batch->tokens == 0) return Q4RDNA_OK;
+    if ((rc = check_dtype(desc->dtype)) != Q4RDNA_OK || (rc = check_rows(desc->k, desc->dtype, "k")) != Q4RDNA_OK ||
+        (rc = check_rows(desc->v, desc->dtype, "v")) != Q4RDNA_OK)
+        return rc;
+    if (desc->q_heads != 0 && ((rc = check_heads(desc->q_heads, cache->kv_heads)) != Q4RDNA_OK ||
+                               (rc = check_rows(desc->q, desc->dtype, "q")) != Q4RDNA_OK ||
+                               (rc = check_rows(desc->q_out, desc->dtype, "q_out")) != Q4RDNA_OK))
+        return rc;
+    if (desc->rotary % 8 != 0 || desc->rotary > cache->head_dim)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "rotary is %u: a multiple of 8 up to head_dim is needed", desc->rotary);
+    if (desc->rotary != 0 && (desc->cos == nullptr || desc->sin == nullptr || !aligned(desc->cos, 16) || !aligned(desc->sin, 16)))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "cos and sin have to be 16-byte aligned tables");
+    if (!aligned(desc->q_norm, 16) || !aligned(desc->k_norm, 16))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned norm weight");
+    const uint64_t kv_units = q4rdna::kv_places(*batch) * cache->kv_heads;
+    const uint64_t q_units = (static_cast<uint64_t>(batch->tokens) * desc->q_heads + q4rdna::kAppendQRows - 1) / q4rdna::kAppendQRows;
+    if (kv_units + q_units > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
+    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    q4rdna::AppendArgs a{};
+    a.cache = *cache;
+    a.batch = *batch;
+    a.d = *desc;
+    a.kv_units = static_cast<uint32_t>(kv_units);
+    a.q_units = static_cast<uint32_t>(q_units);
+    a.wide = wide_rows(desc->k, desc->dtype, 4) && wide_rows(desc->v, desc->dtype, 4) &&
+             (desc->q_heads == 0 || (wide_rows(desc->q, desc->dtype, 4) && wide_rows(desc->q_out, desc->dtype, 4)));
+    return launched(q4rdna::launch_append(a, static_cast<hipStream_t>(stream)), "kv_append");
+}
+
+int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4rdna_kv_attend_desc *desc, void *stream) {
+    int rc;
+    if ((rc = check_cache(cache)) != Q4RDNA_OK || (rc = check_batch(batch)) != Q4RDNA_OK) return rc;
+    if (desc == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null descriptor");
+    if (batch->sequences == 0 || batch->tokens == 0) return Q4RDNA_OK;
+    if ((rc = check_dtype(desc->dtype)) != Q4RDNA_OK || (rc = check_heads(desc->q_heads, cache->kv_heads)) != Q4RDNA_OK ||
+        (rc = check_rows(desc->q, desc->dtype, "q")) != Q4RDNA_OK || (rc = check_rows(desc->out, desc->dtype, "out")) != Q4RDNA_OK)
+        return rc;
+    if (!std::isfinite(desc->scale) || desc->scale < 0.0f)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "scale is %g: a finite number >= 0 is needed", static_cast<double>(desc->scale));
+    if (!aligned(desc->lse, 4)) return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned lse");
+    q4rdna::AttendArgs a{};
+    a.cache = *cache;
+    a.batch = *batch;
+    a.d = *desc;
+    a.group = desc->q_heads / cache->kv_heads;
+    const uint64_t most_rows = static_cast<uint64_t>(std::min(batch->max_tokens, batch->tokens)) * a.group;
+    const uint32_t rows = q4rdna::attend_few_rows(static_cast<uint32_t>(std::min<uint64_t>(most_rows, 1u << 30)));
+    const uint64_t row_groups = (most_rows + rows - 1) / rows;
+    if (row_groups * cache->kv_heads > 65535)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of a sequence are too many for one call", batch->max_tokens);
+    a.row_groups = static_cast<uint32_t>(row_groups);
+    a.wide = wide_rows(desc->q, desc->dtype, 16 / size_of(desc->dtype));
+    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    // Enough workgroups for four per CU, no more than a block for each wave.
+    const uint64_t jobs = row_groups * cache->kv_heads * batch->sequences;
+    const uint64_t most_blocks = desc->window == 0 ? batch->table_width
+                                                   : std::min<uint64_t>(batch->table_width, (static_cast<uint64_t>(desc->window) + batch->max_tokens) / q4rdna::kKvBlock + 2);
+    uint64_t splits = 4ull * cu_count(cache->device) / jobs;
+    splits = std::min(splits, (most_blocks + 3) / 4);
+    a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 256)));
+    if (a.splits > 1) {
+        Scratch s;
+        const size_t slots = jobs * a.splits * rows;
+        if ((rc = get_scratch(cache->device, static_cast<hipStream_t>(stream), slots * (cache->head_dim + 2), jobs, &s)) != Q4RDNA_OK)
+            return rc;
+        a.partials = s.partials;
+        a.arrived = s.arrived;
+    }
+    return launched(q4rdna::launch_attend_few(a, rows, static_cast<hipStream_t>(stream)), "kv_attend");
+}
+
+int read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dtype, const q4rdna_kv_rows *k,
+         const q4rdna_kv_rows *v, void *stream) {
+    int rc;
+    if ((rc = check_cache(cache)) != Q4RDNA_OK || (rc = check_batch(batch)) != Q4RDNA_OK) return rc;
+    if (k == nullptr || v == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null rows");
+    if (batch->sequences == 0 || batch->tokens == 0) return Q4RDNA_OK;
+    if ((rc = check_dtype(dtype)) != Q4RDNA_OK || (rc = check_rows(*k, dtype, "k")) != Q4RDNA_OK ||
+        (rc = check_rows(*v, dtype, "v")) != Q4RDNA_OK)
+        return rc;
+    const uint64_t units = q4rdna::kv_places(*batch) * cache->kv_heads;
+    if (units > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
+    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    q4rdna::ReadArgs a{};
+    a.cache = *cache;
+    a.batch = *batch;
+    a.k = *k;
+    a.v = *v;
+    a.dtype = dtype;
+    a.units = static_cast<uint32_t>(units);
+    return launched(q4rdna::launch_read(a, static_cast<hipStream_t>(stream)), "kv_read");
+}
+
+int add_norm(const q4rdna_add_norm_desc *desc, void *stream) {
+    if (desc == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null descriptor");
+    const q4rdna_add_norm_desc &d = *desc;
+    int rc;
+    if ((rc = check_dtype(d.dtype)) != Q4RDNA_OK) return rc;
+    if (d.width == 0 || d.width > Q4RDNA_NORM_MAX_WIDTH || d.rows > 0x7fffffffu)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "%u rows of %u: 1 to %d numbers a row are supported", d.rows, d.width,
+                         Q4RDNA_NORM_MAX_WIDTH);
+    if (d.rows == 0 || (d.h == nullptr && d.n == nullptr)) return Q4RDNA_OK;
+    if (d.residual == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "null residual");
+    if (d.n != nullptr && d.weight == nullptr) return set_error(Q4RDNA_ERR_ARGUMENT, "n needs a weight");
+    if (d.y == nullptr && (d.gate != nullptr || d.post_weight != nullptr))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "a gate or a norm of y without y");
+    if (d.reserved != 0) return set_error(Q4RDNA_ERR_ARGUMENT, "reserved is not zero");
+    const uint32_t size = size_of(d.dtype);
+    const void *const buffers[] = {d.residual, d.y, d.gate, d.h, d.n};
+    const int64_t strides[] = {d.residual_stride, d.y_stride, d.gate_stride, d.h_stride, d.n_stride};
+    bool wide = d.width % (16 / size) == 0 && aligned(d.weight, 16) && aligned(d.post_weight, 16);
+    for (int i = 0; i < 5; ++i) {
+        if (!aligned(buffers[i], size)) return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned buffer");
+        if (buffers[i] != nullptr) wide = wide && aligned(buffers[i], 16) && strides[i] % (16 / size) == 0;
+    }
+    if (!aligned(d.weight, 4) || !aligned(d.post_weight, 4)) return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned weight");
+    if (d.h == d.n) return set_error(Q4RDNA_ERR_ARGUMENT, "h and n are one buffer");
+    for (int o = 3; o < 5; ++o)
+        for (int i = 0; i < 3; ++i)
+            if (buffers[o] != nullptr && buffers[o] == buffers[i] && (strides[o] != strides[i] || (i == 2 && d.rows > 1)))
+                return set_error(Q4RDNA_ERR_ARGUMENT, "an output over an input with another stride, or over the gate");
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess) return set_error(Q4RDNA_ERR_HIP, "no current device");
+    return launched(q4rdna::launch_add_norm(d, wide, cu_count(device), static_cast<hipStream_t>(stream)), "add_norm");
+}
+
+}  // namespace
+
+extern "C" {
+
+int q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4rdna_kv_append_desc *desc,
+                     void *stream) {
+    return guarded([&] { return append(cache, batch, desc, stream); });
+}
+
+int q4rdna_kv_attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4rdna_kv_attend_desc *desc,
+                     void *stream) {
+    return guarded([&] { return attend(cache, batch, desc, stream); });
+}
+
+int q4rdna_kv_read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dtype, const q4rdna_kv_rows *k,
+                   const q4rdna_kv_rows *v, void *stream) {
+    return guarded([&] { return read(cache, batch, dtype, k, v, stream); });
+}
+
+int q4rdna_add_norm(const q4rdna_add_norm_desc *desc, void *stream) {
+    return guarded([&] { return add_norm(desc, stream); });
+}
+
+}  // extern "C"

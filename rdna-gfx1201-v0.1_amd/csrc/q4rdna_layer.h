@@ -1,0 +1,67 @@
+// Internal interface of the decoder-layer operators: the kernels of
+// q4rdna_cache.hip (append, read), q4rdna_attend.hip and q4rdna_norm.hip, and
+// their entry points in q4rdna_layer.cpp.  Not part of the C ABI.
+#pragma once
+
+#include <hip/hip_runtime_api.h>
+#include <stdint.h>
+
+#include "q4rdna.h"
+
+namespace q4rdna {
+
+constexpr uint32_t kKvBlock = Q4RDNA_KV_BLOCK;
+
+// The 16-bit codes' largest magnitude, 127 * 256: code = 256 * high + low with
+// low in [-128, 127] keeps high in [-127, 127].
+constexpr int kKvCode16 = 32512;
+// Below this largest magnitude a token counts as zero: its 16-bit scale and
+// the reciprocal of it stay far from the subnormal numbers.
+constexpr float kKvZero = 1e-30f;
+
+struct AppendArgs {
+    q4rdna_kv_cache cache;
+    q4rdna_kv_batch batch;
+    q4rdna_kv_append_desc d;
+    uint32_t kv_units;  // (sequence, block) places times kv heads
+    uint32_t q_units;   // workgroups that rotate q
+    uint32_t wide;      // rows of k, v, q, q_out can be read four elements at a time
+};
+hipError_t launch_append(const AppendArgs &a, hipStream_t stream);
+// Rows of q that one workgroup rotates.
+constexpr uint32_t kAppendQRows = 32;
+
+struct ReadArgs {
+    q4rdna_kv_cache cache;
+    q4rdna_kv_batch batch;
+    q4rdna_kv_rows k, v;
+    uint32_t dtype;
+    uint32_t units;
+};
+hipError_t launch_read(const ReadArgs &a, hipStream_t stream);
+
+// Places for the (sequence, block) pairs that a step touches.  Sequence i owns
+// the places from cu[i] / 64 + 2 i on: cu[i+1] / 64 - cu[i] / 64 + 2 of them,
+// enough for the blocks that its tokens touch, so no prefix sum is needed.
+inline uint64_t kv_places(const q4rdna_kv_batch &b) {
+    return b.cu_tokens == nullptr ? b.sequences : b.tokens / kKvBlock + 2ull * b.sequences;
+}
+
+struct AttendArgs {
+    q4rdna_kv_cache cache;
+    q4rdna_kv_batch batch;
+    q4rdna_kv_attend_desc d;
+    uint32_t group;       // query heads per kv head
+    uint32_t row_groups;  // row groups of the largest sequence
+    uint32_t splits;      // the most workgroups that share a row group
+    uint32_t wide;        // q rows can be read 16 bytes at a time
+    float *partials;      // [job][split][row][D], then max and sum [job][split][row][2]
+    uint32_t *arrived;    // [job], zero between launches
+};
+// Rows (query token, query head of the kv head) that one workgroup takes.
+uint32_t attend_few_rows(uint32_t rows);
+hipError_t launch_attend_few(const AttendArgs &a, uint32_t rows, hipStream_t stream);
+
+hipError_t launch_add_norm(const q4rdna_add_norm_desc &d, bool wide, uint32_t cus, hipStream_t stream);
+
+}  // namespace q4rdna

@@ -33,6 +33,12 @@ GLU_SWIGLU = 0
 MAX_BATCH = 8
 NOALLOC_SLOTS = 1 << 21
 
+F32 = 0
+F16 = 1
+BF16 = 2
+KV_BLOCK = 64
+NORM_MAX_WIDTH = 16384
+
 # Every symbol include/q4rdna.h declares.
 EXPORTS = (
     "q4rdna_abi_version", "q4rdna_last_error", "q4rdna_sidecar_inspect", "q4rdna_sidecar_open",
@@ -44,6 +50,7 @@ EXPORTS = (
     "q4rdna_plan_sweep", "q4rdna_plan_destroy",
     "q4rdna_plan_workgroups", "q4rdna_pack", "q4rdna_dequantize",
     "q4rdna_launch_count", "q4rdna_sidecar_hits", "q4rdna_report_stats",
+    "q4rdna_kv_append", "q4rdna_kv_attend", "q4rdna_kv_read", "q4rdna_add_norm",
 )
 
 
@@ -77,6 +84,44 @@ class GroupDesc(ctypes.Structure):
 class GemvDesc(ctypes.Structure):
     _fields_ = [("weight", Weight), ("gate_tiles", ctypes.c_void_p), ("x", ctypes.c_void_p),
                 ("add", ctypes.c_void_p), ("y", ctypes.c_void_p)]
+
+
+class CacheDesc(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("open", ctypes.c_void_p),
+                ("open_scales", ctypes.c_void_p), ("faults", ctypes.c_void_p), ("page_count", ctypes.c_uint32),
+                ("slot_count", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("device", ctypes.c_int32), ("reserved", ctypes.c_uint32)]
+
+
+class BatchDesc(ctypes.Structure):
+    _fields_ = [("past", ctypes.c_void_p), ("cu_tokens", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("slots", ctypes.c_void_p), ("sequences", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+                ("max_tokens", ctypes.c_uint32), ("table_width", ctypes.c_uint32)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class AppendDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("q_heads", ctypes.c_uint32), ("k", Rows), ("v", Rows), ("q", Rows),
+                ("q_out", Rows), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("positions", ctypes.c_uint32),
+                ("rotary", ctypes.c_uint32), ("interleaved", ctypes.c_uint32), ("eps", ctypes.c_float),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p)]
+
+
+class AttendDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("q_heads", ctypes.c_uint32), ("q", Rows), ("out", Rows),
+                ("lse", ctypes.c_void_p), ("scale", ctypes.c_float), ("window", ctypes.c_uint32)]
+
+
+class AddNormDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("width", ctypes.c_uint32),
+                ("scale", ctypes.c_float), ("eps", ctypes.c_float), ("reserved", ctypes.c_uint32),
+                ("residual", ctypes.c_void_p), ("y", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("h", ctypes.c_void_p), ("n", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+                ("y_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64), ("h_stride", ctypes.c_int64),
+                ("n_stride", ctypes.c_int64), ("post_weight", ctypes.c_void_p), ("weight", ctypes.c_void_p)]
 
 
 _lib = None
@@ -127,6 +172,11 @@ def load() -> ctypes.CDLL:
         "q4rdna_launch_count": (u64, []),
         "q4rdna_sidecar_hits": (u64, [vp, u32]),
         "q4rdna_report_stats": (None, []),
+        "q4rdna_kv_append": (i32, [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.POINTER(AppendDesc), vp]),
+        "q4rdna_kv_attend": (i32, [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.POINTER(AttendDesc), vp]),
+        "q4rdna_kv_read": (i32, [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), u32, ctypes.POINTER(Rows),
+                                 ctypes.POINTER(Rows), vp]),
+        "q4rdna_add_norm": (i32, [ctypes.POINTER(AddNormDesc), vp]),
     }
     for name, (res, args) in proto.items():
         fn = getattr(L, name)

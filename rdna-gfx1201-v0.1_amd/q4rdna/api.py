@@ -412,3 +412,287 @@ class Plan:
             self.close()
         except Exception:
             pass
+
+
+_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def _dtype(t: torch.dtype) -> int:
+    code = _DTYPES.get(t)
+    if code is None:
+        raise ValueError(f"dtype {t}: float32, float16 and bfloat16 are supported")
+    return code
+
+
+def _plain(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> int:
+    """The address of a contiguous tensor that the kernels read or write whole."""
+    if t.dtype != dtype or t.get_device() != device or not t.is_contiguous() or t.shape != shape:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(r: _lib.Rows, t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, heads: int, dim: int,
+          device: int) -> None:
+    """Describe activations [tokens, heads, dim] of any token and head strides."""
+    if t.dtype != dtype or t.get_device() != device or t.shape != (tokens, heads, dim):
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {(tokens, heads, dim)} on cuda:{device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    token_stride, head_stride, stride = t.stride()
+    if stride != 1:
+        raise ValueError(f"the numbers of a head of {name} must be contiguous")
+    r.data = t.data_ptr()
+    r.token_stride = token_stride
+    r.head_stride = head_stride
+
+
+def _no_overlap(t: torch.Tensor, name: str) -> None:
+    """An output whose rows share memory would be written by several rows at once."""
+    if not t.is_contiguous():
+        dims = sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1)
+        reach = 1
+        for st, n in dims:
+            if st < reach:
+                raise ValueError(f"rows of {name} overlap")
+            reach = st * (n - 1) + reach
+
+
+class KVBatch:
+    """The sequences of one step (q4rdna_kv_batch), shared by all layers' calls.
+
+    past [sequences], table [sequences, width] and, where given, cu_tokens
+    [sequences + 1] and slots [sequences] are int32 CUDA tensors, read when
+    the kernels run: a captured graph may be replayed after they were filled
+    anew.  Without cu_tokens every sequence has one token; with it max_tokens
+    (an int) bounds the tokens of a sequence.
+    """
+
+    def __init__(self, past: torch.Tensor, table: torch.Tensor, cu_tokens: torch.Tensor | None = None,
+                 slots: torch.Tensor | None = None, max_tokens: int = 1):
+        if not past.is_cuda or past.dim() != 1 or table.dim() != 2:
+            raise ValueError("past must be a CUDA tensor [sequences], table [sequences, width]")
+        device, n = past.get_device(), past.shape[0]
+        raw = _lib.BatchDesc()
+        raw.past = _plain(past, "past", torch.int32, (n,), device)
+        raw.table = _plain(table, "table", torch.int32, (n, table.shape[1]), device)
+        if cu_tokens is not None:
+            raw.cu_tokens = _plain(cu_tokens, "cu_tokens", torch.int32, (n + 1,), device)
+        elif max_tokens != 1:
+            raise ValueError("without cu_tokens every sequence has one token")
+        if slots is not None:
+            raw.slots = _plain(slots, "slots", torch.int32, (n,), device)
+        if max_tokens < 1:
+            raise ValueError("max_tokens must be at least 1")
+        raw.sequences = n
+        raw.max_tokens = max_tokens
+        raw.table_width = table.shape[1]
+        self.raw = raw
+        self._ref = ctypes.byref(raw)
+        self.device = device
+        self.sequences = n
+        self._keep = (past, table, cu_tokens, slots)
+
+    def _of(self, tokens: int):
+        """The descriptor for a call on `tokens` tokens."""
+        if self._keep[2] is None and tokens != self.sequences:
+            raise ValueError(f"{tokens} tokens for {self.sequences} sequences: without cu_tokens each has one")
+        self.raw.tokens = tokens
+        return self._ref
+
+
+class KVCache:
+    """A layer's paged key/value cache in 8 bits (q4rdna_kv_cache).
+
+    pages int8 [pages, kv_heads, 2, 64 * head_dim], scales float32 [pages,
+    kv_heads, 2], open int8 [slots, 2, kv_heads, 4, 64 * head_dim] and
+    open_scales float32 [slots, 2, kv_heads, 2, 64]; :meth:`empty` makes them.
+    The format, and what a page and a slot hold, is described in
+    include/q4rdna.h.
+    """
+
+    def __init__(self, pages: torch.Tensor, scales: torch.Tensor, open: torch.Tensor, open_scales: torch.Tensor):
+        if pages.dim() != 4 or open.dim() != 5 or not pages.is_cuda:
+            raise ValueError("pages must be a CUDA tensor [pages, kv_heads, 2, 64 * head_dim], open "
+                             "[slots, 2, kv_heads, 4, 64 * head_dim]")
+        device, (count, heads, _, size), slots = pages.get_device(), pages.shape, open.shape[0]
+        if size % _lib.KV_BLOCK:
+            raise ValueError("a block holds 64 * head_dim codes")
+        raw = _lib.CacheDesc()
+        raw.pages = _plain(pages, "pages", torch.int8, (count, heads, 2, size), device)
+        raw.scales = _plain(scales, "scales", torch.float32, (count, heads, 2), device)
+        raw.open = _plain(open, "open", torch.int8, (slots, 2, heads, 4, size), device)
+        raw.open_scales = _plain(open_scales, "open_scales", torch.float32, (slots, 2, heads, 2, _lib.KV_BLOCK), device)
+        self._faults = torch.zeros(1, dtype=torch.int32, device=pages.device)
+        raw.faults = self._faults.data_ptr()
+        raw.page_count, raw.slot_count, raw.kv_heads = count, slots, heads
+        raw.head_dim = size // _lib.KV_BLOCK
+        raw.device = device
+        self.raw = raw
+        self._ref = ctypes.byref(raw)
+        self.device = device
+        self.kv_heads = heads
+        self.head_dim = raw.head_dim
+        self.pages, self.scales, self.open, self.open_scales = pages, scales, open, open_scales
+
+    @classmethod
+    def empty(cls, pages: int, slots: int, kv_heads: int, head_dim: int, device: int = 0) -> "KVCache":
+        dev = torch.device("cuda", device)
+        size = _lib.KV_BLOCK * head_dim
+        return cls(torch.zeros((pages, kv_heads, 2, size), dtype=torch.int8, device=dev),
+                   torch.zeros((pages, kv_heads, 2), dtype=torch.float32, device=dev),
+                   torch.zeros((slots, 2, kv_heads, 4, size), dtype=torch.int8, device=dev),
+                   torch.zeros((slots, 2, kv_heads, 2, _lib.KV_BLOCK), dtype=torch.float32, device=dev))
+
+    def faults(self) -> int:
+        """How often the kernels refused a batch entry (waits for the device)."""
+        return int(self._faults.item())
+
+    def _step(self, batch: KVBatch, tokens: int):
+        if batch.device != self.device:
+            raise ValueError(f"the batch lives on cuda:{batch.device}, the cache on cuda:{self.device}")
+        return batch._of(tokens)
+
+    def append(self, batch: KVBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
+               q_out: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+               interleaved: bool = False, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+               eps: float = 1e-6, stream: int | None = None) -> torch.Tensor | None:
+        """Append the step's k and v [tokens, kv_heads, head_dim]; returns q
+        [tokens, q_heads, head_dim] normalised and rotated (q_norm, k_norm
+        [head_dim]; cos, sin [positions, rotary / 2], float32)."""
+        if k.dim() != 3:
+            raise ValueError("k must be [tokens, kv_heads, head_dim]")
+        tokens, heads, dim, device = k.shape[0], self.kv_heads, self.head_dim, self.device
+        step = self._step(batch, tokens)
+        d = _lib.AppendDesc()
+        d.dtype = _dtype(k.dtype)
+        _rows(d.k, k, "k", k.dtype, tokens, heads, dim, device)
+        _rows(d.v, v, "v", k.dtype, tokens, heads, dim, device)
+        if q is not None:
+            if q.dim() != 3:
+                raise ValueError("q must be [tokens, q_heads, head_dim]")
+            _rows(d.q, q, "q", k.dtype, tokens, q.shape[1], dim, device)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            _rows(d.q_out, q_out, "q_out", k.dtype, tokens, q.shape[1], dim, device)
+            _no_overlap(q_out, "q_out")
+            d.q_heads = q.shape[1]
+        elif q_out is not None or q_norm is not None:
+            raise ValueError("q_out or q_norm without q")
+        if cos is not None:
+            if cos.dim() != 2 or sin is None:
+                raise ValueError("cos and sin must be [positions, rotary / 2]")
+            d.cos = _plain(cos, "cos", torch.float32, cos.shape, device)
+            d.sin = _plain(sin, "sin", torch.float32, cos.shape, device)
+            d.positions, d.rotary = cos.shape[0], 2 * cos.shape[1]
+        elif sin is not None:
+            raise ValueError("sin without cos")
+        d.interleaved = interleaved
+        d.eps = eps
+        if q_norm is not None:
+            d.q_norm = _plain(q_norm, "q_norm", torch.float32, (dim,), device)
+        if k_norm is not None:
+            d.k_norm = _plain(k_norm, "k_norm", torch.float32, (dim,), device)
+        s = _raw_stream(device) if stream is None else stream
+        check(load().q4rdna_kv_append(self._ref, step, ctypes.byref(d), s))
+        return q_out
+
+    def attend(self, batch: KVBatch, q: torch.Tensor, out: torch.Tensor | None = None, scale: float | None = None,
+               window: int = 0, lse: bool | torch.Tensor = False, stream: int | None = None):
+        """Attention of the step's q [tokens, q_heads, head_dim] over the cache,
+        after :meth:`append` of the same batch.  scale None: head_dim ** -0.5.
+        window > 0: the last `window` tokens only.  lse True (or a float32
+        tensor [tokens, q_heads]): returns (out, lse)."""
+        if q.dim() != 3:
+            raise ValueError("q must be [tokens, q_heads, head_dim]")
+        tokens, heads, dim = q.shape
+        step = self._step(batch, tokens)
+        d = _lib.AttendDesc()
+        d.dtype = _dtype(q.dtype)
+        d.q_heads = heads
+        _rows(d.q, q, "q", q.dtype, tokens, heads, self.head_dim, self.device)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _rows(d.out, out, "out", q.dtype, tokens, heads, self.head_dim, self.device)
+        _no_overlap(out, "out")
+        if lse is True:
+            lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+        if lse is not False:
+            d.lse = _plain(lse, "lse", torch.float32, (tokens, heads), self.device)
+        d.scale = self.head_dim ** -0.5 if scale is None else scale
+        if window < 0:
+            raise ValueError("window must not be negative")
+        d.window = window
+        s = _raw_stream(self.device) if stream is None else stream
+        check(load().q4rdna_kv_attend(self._ref, step, ctypes.byref(d), s))
+        return out if lse is False else (out, lse)
+
+    def read(self, batch: KVBatch, tokens: int, dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None,
+             v: torch.Tensor | None = None, stream: int | None = None):
+        """(k, v) [tokens, kv_heads, head_dim]: the batch's tokens (past[i] on,
+        up to the sequence's length) as numbers."""
+        shape, device = (tokens, self.kv_heads, self.head_dim), torch.device("cuda", self.device)
+        step = self._step(batch, tokens)
+        rows = _lib.Rows(), _lib.Rows()
+        k = torch.empty(shape, dtype=dtype, device=device) if k is None else k
+        v = torch.empty(shape, dtype=dtype, device=device) if v is None else v
+        for r, t, name in ((rows[0], k, "k"), (rows[1], v, "v")):
+            _rows(r, t, name, dtype, *shape, self.device)
+            _no_overlap(t, name)
+        s = _raw_stream(self.device) if stream is None else stream
+        check(load().q4rdna_kv_read(self._ref, step, _dtype(dtype), ctypes.byref(rows[0]), ctypes.byref(rows[1]), s))
+        return k, v
+
+
+def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tensor | None, *,
+             post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+             eps: float = 1e-6, h: torch.Tensor | None = None, n: torch.Tensor | None = None,
+             stream: int | None = None):
+    """(h, n): h = residual + scale * gate * post(y), n = rms(h) * weight.
+
+    residual, y, h and n are [rows, width] (any row stride) of one dtype; gate
+    is [width] or [rows, width]; weight and post_weight are float32 [width].
+    y None: h is residual itself and is not written.  weight None: no n.
+    post_weight None: y as it is.  h and n may be given (h may be residual or
+    y, n may be y)."""
+    if residual.dim() != 2 or not residual.is_cuda:
+        raise ValueError("residual must be a CUDA tensor [rows, width]")
+    device, shape, dtype = residual.get_device(), residual.shape, residual.dtype
+    width = shape[1]
+    d = _lib.AddNormDesc()
+    d.dtype = _dtype(dtype)
+    d.rows, d.width = shape
+    d.scale, d.eps = scale, eps
+
+    def matrix(t, name):
+        if t.dtype != dtype or t.get_device() != device or t.shape != shape or t.stride(1) != 1 and width > 1:
+            raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} with contiguous rows on cuda:{device}")
+        return t.data_ptr(), t.stride(0)
+
+    d.residual, d.residual_stride = matrix(residual, "residual")
+    if y is not None:
+        d.y, d.y_stride = matrix(y, "y")
+        if h is None:
+            h = torch.empty(shape, dtype=dtype, device=residual.device)
+        d.h, d.h_stride = matrix(h, "h")
+        _no_overlap(h, "h")
+        if gate is not None:
+            if gate.dim() == 1:
+                d.gate = _plain(gate, "gate", dtype, (width,), device)
+            else:
+                d.gate, d.gate_stride = matrix(gate, "gate")
+        if post_weight is not None:
+            d.post_weight = _plain(post_weight, "post_weight", torch.float32, (width,), device)
+    elif gate is not None or post_weight is not None or h is not None:
+        raise ValueError("gate, post_weight or h without y")
+    if weight is not None:
+        if n is None:
+            n = torch.empty(shape, dtype=dtype, device=residual.device)
+        d.n, d.n_stride = matrix(n, "n")
+        _no_overlap(n, "n")
+        d.weight = _plain(weight, "weight", torch.float32, (width,), device)
+    elif n is not None:
+        raise ValueError("n without a weight")
+    with torch.cuda.device(device):
+        s = _raw_stream(device) if stream is None else stream
+        check(load().q4rdna_add_norm(ctypes.byref(d), s))
+    return (residual if h is None else h), n
