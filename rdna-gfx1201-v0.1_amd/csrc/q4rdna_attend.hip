@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, D * QT <= 128 ? 2 : 1) void attend_few_kernel(
     }
     const int rows = s.count * static_cast<int>(a.group);
     const int first_row = row_group * ROWS;
-    if (first_row >= rows) return;
+    if (first_row >= rows || static_cast<uint32_t>(rows) > a.few_rows) return;
 
     // Blocks that some row of the group sees.
     const int last_row = min(first_row + ROWS, rows) - 1;

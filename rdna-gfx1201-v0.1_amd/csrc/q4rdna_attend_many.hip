@@ -1,0 +1,474 @@
+// Attention over the 8-bit paged cache for many rows (q4rdna_kv_attend on
+// prompts): attend_many_kernel.
+//
+// A workgroup takes 128 rows (query token, query head of one kv head), 32 per
+// wave, and walks the blocks they see.  Each block's int8 codes are loaded once
+// per workgroup, become fp16 on their way into LDS (exact: |code| <= 127), and
+// are multiplied by 32x32x16 fp16 matrix instructions:
+//
+//  * S^T = K q^T, then O^T += V^T p^T.  A lane holds one row of q: its scores
+//    (32 of a block's 64; lane ^ 32 has the others) come out of the first
+//    product in the registers that the second takes as its operand, since V^T
+//    is laid into LDS in that order of tokens.  The row's maximum, sum and
+//    rescaling are the lane's own, with one exchange between the halves.
+//  * q is scaled by a power of two per row, so fp16 and bf16 rows are exact in
+//    fp16; the weights are rounded to fp16 (11 bits), finer than the output's
+//    rounding.  fp32 rows take two fp16 parts of q and of the weights each
+//    (SPLIT = 2, 22 bits) and twice the products, which keeps fp32's accuracy.
+//  * V's scale per block goes into the weights relative to the largest scale so
+//    far, so the accumulators are rescaled only when that or the row's maximum
+//    grows; the maximum is followed lazily, by steps of at least 2^8.
+//  * The open block's two planes are two tiles: 256 * high is exact in fp16.
+//
+// Row groups are split over several workgroups along the blocks when there are
+// too few of them; the last to arrive joins the parts in a fixed order.
+#include "q4rdna_layer_device.h"
+
+namespace q4rdna {
+namespace {
+
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kLazy = 8.0f;    // the maximum may trail by this much (base 2)
+constexpr float kWeight = 7.0f;  // weights are 2^7 p, at most 2^15, within fp16's range
+constexpr int kRowsMany = kAttendManyRows;
+
+// LDS tiles of a block in fp16: K [64 tokens][D + 8], V^T [D][64 + 8].  Rows
+// are 272 (144) and 144 bytes: 16 lanes' 16-byte reads of 16 rows cover all
+// 64 banks once.
+template <int D>
+struct ManyTile {
+    _Float16 k[kKvBlock * (D + 8)];
+    _Float16 v[D * (kKvBlock + 8)];
+};
+
+// Four codes as fp16: 0x6400 | (code + 128) is 1024 + code + 128.
+__device__ __forceinline__ void codes_to_half(uint32_t w, h16x2 &lo, h16x2 &hi) {
+    const uint32_t u = w ^ 0x80808080u;
+    const h16x2 bias = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    lo = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias;
+    hi = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias;
+}
+template <bool HIGH>
+__device__ __forceinline__ void piece_to_lds(_Float16 *at, i32x4 piece) {
+    h16x2 x[8];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) codes_to_half(static_cast<uint32_t>(piece[w]), x[2 * w], x[2 * w + 1]);
+    if (HIGH) {
+        const h16x2 f = {static_cast<_Float16>(256.0f), static_cast<_Float16>(256.0f)};
+#pragma unroll
+        for (int w = 0; w < 8; ++w) x[w] *= f;
+    }
+    h16x8 a, b;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        a[e] = x[e / 2][e % 2];
+        b[e] = x[4 + e / 2][e % 2];
+    }
+    *reinterpret_cast<h16x8 *>(at) = a;
+    *reinterpret_cast<h16x8 *>(at + 8) = b;
+}
+// A block's pieces `tid`, `tid + 256`, ... of K and V.
+template <int D>
+struct Raw {
+    i32x4 k[D / 64], v[D / 64];
+};
+template <int D>
+__device__ __forceinline__ void load_raw(Raw<D> &r, const int8_t *k, const int8_t *v) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        r.k[i] = load16(k + 16 * (threadIdx.x + 256 * i));
+        r.v[i] = load16(v + 16 * (threadIdx.x + 256 * i));
+    }
+}
+template <bool HIGH, int D>
+__device__ __forceinline__ void stage_raw(ManyTile<D> &t, const Raw<D> &r) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const int piece = threadIdx.x + 256 * i, c = piece % 16, g = piece / 16 % 4;
+        const int token = piece / (64 * (D / 64)) * 16 + c, number = piece / 64 % (D / 64) * 64 + g * 16;
+        piece_to_lds<HIGH>(t.k + token * (D + 8) + number, r.k[i]);
+        // Row d: [half of the wave][product][8 tokens]; a piece is one half's two products.
+        piece_to_lds<HIGH>(t.v + (piece / 64 * 16 + c) * (kKvBlock + 8) + (g & 1) * 32 + (g >> 1) * 16, r.v[i]);
+    }
+}
+
+template <int D, int SPLIT>
+struct ManyState {
+    h16x8 q[SPLIT][D / 16];
+    float q_scale;    // base-2 score = q_scale * (k scale) * product
+    int position;     // of the lane's row
+    float m, l;       // the maximum that the weights refer to; the lane's part of the sum, in units of 2^-7
+    float v_ref;      // accumulators are in units of 2^-7 v_ref
+    f32x16 o[D / 32];
+};
+
+// One block from LDS.  OPEN: two tiles (256 * high, low), scales per token
+// (kt, vt); otherwise k_scale and v_scale.
+template <bool OPEN, bool MASKED, int D, int SPLIT>
+__device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTile<D> *tile, float k_scale, float v_scale,
+                                           const float *token_scales, int start, uint32_t window) {
+    const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            const h16x8 a = *reinterpret_cast<const h16x8 *>(tile[0].k + (32 * t + column) * (D + 8) + 16 * k + 8 * half);
+#pragma unroll
+            for (int x = 0; x < SPLIT; ++x) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, st.q[x][k], s[t], 0, 0, 0);
+            if (OPEN) {
+                const h16x8 b = *reinterpret_cast<const h16x8 *>(tile[1].k + (32 * t + column) * (D + 8) + 16 * k + 8 * half);
+#pragma unroll
+                for (int x = 0; x < SPLIT; ++x) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, st.q[x][k], s[t], 0, 0, 0);
+            }
+        }
+    }
+    float ratio[8][4];  // OPEN: V's token scales
+    if (OPEN) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const f32x4 kt = *(gptr_f32x4)(uintptr_t)(token_scales + 8 * x + 4 * half);
+            const f32x4 vt = *(gptr_f32x4)(uintptr_t)(token_scales + kKvBlock + 8 * x + 4 * half);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                s[x / 4][4 * (x % 4) + b] *= kt[b];
+                ratio[x][b] = vt[b];
+            }
+        }
+    }
+    // Token of s[t][i]: 32 t + 8 (i / 4) + 4 half + i % 4.
+    uint32_t hidden = 0;
+    if (MASKED) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int token = start + 32 * t + 8 * (i / 4) + 4 * half + i % 4;
+                const bool seen = token <= st.position &&
+                                  (window == 0 || static_cast<uint32_t>(st.position - token) < window);
+                if (!seen) {
+                    hidden |= 1u << (16 * t + i);
+                    s[t][i] = kNegInf;
+                }
+            }
+    }
+    const float f = OPEN ? st.q_scale : st.q_scale * k_scale;
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+    top = max_xor32(top);
+    const bool none = MASKED && top == kNegInf;
+    const float now = none ? kNegInf : top * f;
+
+    // V's scale relative to the largest one so far; one that is not finite
+    // makes the seen weights NaN and leaves the reference alone.
+    float v_ref = st.v_ref;
+    if (OPEN) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const bool seen = !(hidden >> (4 * x + b) & 1u);
+                if (seen && ratio[x][b] < __builtin_inff()) v_ref = fmaxf(v_ref, ratio[x][b]);
+            }
+        // One reference for the whole wave: it belongs to every row's accumulators.
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) v_ref = fmaxf(v_ref, __shfl_xor(v_ref, d));
+        v_ref = max_xor32(v_ref);
+    } else if (v_scale < __builtin_inff()) {
+        v_ref = fmaxf(v_ref, v_scale);
+    }
+    const bool grown = now > st.m + kLazy || (st.m == kNegInf && now != kNegInf);
+    if (__builtin_amdgcn_ballot_w64(grown || v_ref != st.v_ref) != 0) {
+        const float m = grown ? now : st.m;
+        const float alpha = grown ? __builtin_amdgcn_exp2f(st.m - m) : 1.0f;  // 0 from -inf
+        const float beta = v_ref > 0.0f ? st.v_ref / v_ref : 1.0f;
+        st.l *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) st.o[d] *= alpha * beta;
+        st.m = m;
+        st.v_ref = v_ref;
+    }
+    const float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m);
+    const float to_ref = v_ref > 0.0f ? 1.0f / v_ref : 0.0f;
+    const float r = OPEN ? 0.0f : v_scale < __builtin_inff() ? v_scale * to_ref : __builtin_nanf("");
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool seen = !MASKED || !(hidden >> (16 * t + i) & 1u);
+            float p = __builtin_amdgcn_exp2f(fmaf(s[t][i], f, shift));
+            p = seen ? p : 0.0f;
+            sum += p;
+            float w = r;
+            if (OPEN) {
+                const float vt = ratio[4 * t + i / 4][i % 4];
+                w = vt < __builtin_inff() ? vt * to_ref : __builtin_nanf("");
+            }
+            s[t][i] = seen ? p * w : 0.0f;
+        }
+    st.l += sum;
+    // Products 2 parity + pair: tokens 16 a + 8 parity + 4 half + b, a = 2 pair, 2 pair + 1.
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        h16x8 p[SPLIT];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int a = 2 * (x & 1) + e / 4, eight = 2 * a + (x >> 1);
+            const float w = s[eight / 4][4 * (eight % 4) + e % 4];
+            p[0][e] = static_cast<_Float16>(w);
+            if (SPLIT == 2) p[SPLIT - 1][e] = static_cast<_Float16>(w - static_cast<float>(p[0][e]));
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+            const int at = (32 * d + column) * (kKvBlock + 8) + 32 * half + 8 * x;
+            const h16x8 a = *reinterpret_cast<const h16x8 *>(tile[0].v + at);
+#pragma unroll
+            for (int y = 0; y < SPLIT; ++y) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[y], st.o[d], 0, 0, 0);
+            if (OPEN) {
+                const h16x8 b = *reinterpret_cast<const h16x8 *>(tile[1].v + at);
+#pragma unroll
+                for (int y = 0; y < SPLIT; ++y) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, p[y], st.o[d], 0, 0, 0);
+            }
+        }
+    }
+}
+
+template <int D, int SPLIT, typename T>
+__device__ __forceinline__ void load_q_many(ManyState<D, SPLIT> &st, const AttendArgs &a, const Seq &s, uint32_t head, int row,
+                                            bool live) {
+    const int half = (threadIdx.x & 63) >> 5;
+    const int token = live ? row / static_cast<int>(a.group) : 0;
+    const uint32_t h = head * a.group + (live ? row - token * a.group : 0);
+    st.position = s.past + token;
+    const T *p = static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(s.first + token) * a.d.q.token_stride +
+                 h * a.d.q.head_stride + 8 * half;
+    float x[D / 16][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+        load_floats<T, 8>(p + 16 * k, a.wide != 0, x[k]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
+    }
+    top = __float_as_uint(max_xor32(__uint_as_float(min(top, 0x7f800000u))));  // NaN as infinity
+    const bool finite = top < 0x7f800000u;
+    // The largest number of the row to 2^13 .. 2^14: small ones stay normal in fp16.
+    const int up = finite && top != 0 ? 14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = finite ? __builtin_amdgcn_ldexpf(x[k][e], up) : 0.0f;
+            st.q[0][k][e] = static_cast<_Float16>(v);
+            if (SPLIT == 2) st.q[SPLIT - 1][k][e] = static_cast<_Float16>(v - static_cast<float>(st.q[0][k][e]));
+        }
+    st.q_scale = finite ? __builtin_amdgcn_ldexpf(a.d.scale * kLog2e, -up) : __builtin_nanf("");
+    st.m = kNegInf;
+    st.l = 0.0f;
+    st.v_ref = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[d][i] = 0.0f;
+}
+
+template <int D, int SPLIT, typename T>
+__global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a) {
+    __shared__ __align__(16) ManyTile<D> tiles[2];
+    __shared__ uint32_t ticket;
+    const int tid = threadIdx.x, lane = tid & 63, column = lane & 31, half = lane >> 5, wave = wave_id();
+    const uint32_t heads = a.cache.kv_heads;
+    // Neighbouring workgroups take different heads: with eight of them, each
+    // XCD's L2 holds one head's cache.  Late rows, which see most, go first.
+    const uint32_t head = blockIdx.x % heads, place = gridDim.x / heads - 1 - blockIdx.x / heads;
+
+    // The sequence and the rows of the place: sequence i has the places from
+    // cu[i] * group / 128 + i on (attend_many_places).
+    uint32_t seq = 0, base = 0;
+    {
+        auto first_place = [&](uint32_t i) {
+            return static_cast<int64_t>(a.batch.cu_tokens ? a.batch.cu_tokens[i] : static_cast<int>(i)) * a.group / kRowsMany + i;
+        };
+        uint32_t lo = 0, hi = a.batch.sequences;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (first_place(mid) <= static_cast<int64_t>(place)) lo = mid; else hi = mid;
+        }
+        seq = lo;
+        const int64_t f = first_place(lo);
+        base = f < 0 || f > place ? place : static_cast<uint32_t>(f);
+    }
+    const Seq s = seq_of(a.batch, a.cache, seq);
+    if (!s.ok) {
+        if (head == 0 && place == base && blockIdx.y == 0 && tid == 0) count_fault(a.cache);
+        return;
+    }
+    const int rows = s.count * static_cast<int>(a.group);
+    const int64_t first_row64 = static_cast<int64_t>(place - base) * kRowsMany;
+    if (first_row64 >= rows || static_cast<uint32_t>(rows) <= a.few_rows) return;
+    const int first_row = static_cast<int>(first_row64);
+    const int last_row = min(first_row + kRowsMany, rows) - 1;
+    const int group = static_cast<int>(a.group), block_size = static_cast<int>(kKvBlock);
+    const int first_position = s.past + first_row / group, end = s.past + last_row / group + 1;
+    const int begin = a.d.window != 0 && static_cast<uint32_t>(first_position) >= a.d.window
+                          ? first_position - static_cast<int>(a.d.window) + 1 : 0;
+    const int block0 = begin / block_size, blocks = (end + block_size - 1) / block_size - block0;
+    const int splits = min(static_cast<int>(a.splits), (blocks + 1) / 2);
+    const int split = blockIdx.y;
+    if (split >= splits) return;
+    const int from = block0 + static_cast<int>(static_cast<int64_t>(split) * blocks / splits);
+    const int to = block0 + static_cast<int>(static_cast<int64_t>(split + 1) * blocks / splits);
+    // The open block, where this workgroup has it, comes last.
+    const bool has_open = s.length % block_size != 0 && to - 1 == s.length / block_size;
+    const int to_full = has_open ? to - 1 : to;
+
+    // This wave's rows.
+    const int row = first_row + 32 * wave + column;
+    ManyState<D, SPLIT> st;
+    load_q_many<D, SPLIT, T>(st, a, s, head, row, row < rows);
+    const int wave_first = s.past + min(first_row + 32 * wave, rows - 1) / group;
+    const int wave_last = s.past + min(first_row + 32 * wave + 31, rows - 1) / group;
+
+    const int32_t *table = a.batch.table + static_cast<size_t>(seq) * a.batch.table_width;
+    constexpr size_t kPlane = kKvBlock * D;
+    Raw<D> raw;
+    f32x2 scale_next;
+    auto load = [&](int b) {
+        int page = __builtin_amdgcn_readfirstlane(table[b]);
+        float bad = 0.0f;
+        if (static_cast<uint32_t>(page) >= a.cache.page_count) {
+            if (tid == 0) count_fault(a.cache);
+            page = 0;
+            bad = __builtin_nanf("");
+        }
+        const int8_t *t = a.cache.pages + page_tile(a.cache, page, head);
+        load_raw<D>(raw, t, t + kPlane);
+        scale_next = *(gptr_f32x2)(uintptr_t)(a.cache.scales + (static_cast<size_t>(page) * heads + head) * 2);
+        scale_next += bad;
+    };
+    if (from < to_full) {
+        load(from);
+        stage_raw<false, D>(tiles[0], raw);
+    }
+    __syncthreads();
+    for (int b = from; b < to_full; ++b) {
+        const int buffer = (b - from) & 1, start = b * block_size;
+        const f32x2 scale = scale_next;
+        if (b + 1 < to_full) load(b + 1);
+        const bool away = start > wave_last ||
+                          (a.d.window != 0 && wave_first - (start + block_size - 1) >= static_cast<int64_t>(a.d.window));
+        if (!away) {
+            const bool masked = start + block_size - 1 > wave_first ||
+                                (a.d.window != 0 && static_cast<uint32_t>(wave_last - start) >= a.d.window);
+            if (masked)
+                many_block<false, true, D, SPLIT>(st, &tiles[buffer], scale[0], scale[1], nullptr, start, a.d.window);
+            else
+                many_block<false, false, D, SPLIT>(st, &tiles[buffer], scale[0], scale[1], nullptr, start, a.d.window);
+        }
+        if (b + 1 < to_full) stage_raw<false, D>(tiles[buffer ^ 1], raw);
+        __syncthreads();
+    }
+    if (has_open) {
+        const int8_t *planes = a.cache.open + open_tile(a.cache, s.slot, to - 1, head);
+        load_raw<D>(raw, planes, planes + 2 * kPlane);
+        stage_raw<true, D>(tiles[0], raw);
+        load_raw<D>(raw, planes + kPlane, planes + 3 * kPlane);
+        stage_raw<false, D>(tiles[1], raw);
+        __syncthreads();
+        const int start = (to - 1) * block_size;
+        if (start <= wave_last)
+            many_block<true, true, D, SPLIT>(st, tiles, 0.0f, 0.0f,
+                                             a.cache.open_scales + open_scale_row(a.cache, s.slot, to - 1, head), start, a.d.window);
+    }
+
+    // The row's sum over both halves; results in units of one.
+    const float l = add_xor32(st.l);
+    const bool live = row < rows;
+    const int token = live ? row / group : 0;
+    const uint32_t h = head * a.group + (live ? row - token * group : 0);
+    const uint32_t job = place * heads + head;
+    if (splits == 1) {
+        if (!live) return;
+        const float inv = l == 0.0f ? 0.0f : st.v_ref / l;
+        T *out = static_cast<T *>(a.d.out.data) + static_cast<int64_t>(s.first + token) * a.d.out.token_stride + h * a.d.out.head_stride;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = st.o[d][4 * x + e] * inv;
+                store_floats<T, 4>(out + 32 * d + 8 * x + 4 * half, a.wide_out != 0, v);
+            }
+        if (a.d.lse != nullptr && half == 0)
+            a.d.lse[static_cast<size_t>(s.first + token) * a.d.q_heads + h] = (st.m + log2f(l) - kWeight) * (1.0f / kLog2e);
+        return;
+    }
+    const size_t jobs = gridDim.x;
+    float *stats = a.partials + jobs * a.splits * kRowsMany * D;
+    const size_t slot = (static_cast<size_t>(job) * a.splits + split) * kRowsMany + 32 * wave + column;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            store_agent(a.partials + slot * D + 32 * d + 8 * (i / 4) + 4 * half + i % 4, st.o[d][i] * st.v_ref);
+    if (half == 0) {
+        store_agent(stats + 2 * slot, st.m);
+        store_agent(stats + 2 * slot + 1, l);
+    }
+    wait_stores();
+    __syncthreads();
+    if (tid == 0) ticket = add_agent(a.arrived + job, 1u);
+    __syncthreads();
+    if (ticket != static_cast<uint32_t>(splits - 1)) return;
+    if (tid == 0) store_agent(a.arrived + job, 0u);
+    const size_t first_slot = static_cast<size_t>(job) * a.splits * kRowsMany;
+    for (int x = tid; x < (last_row - first_row + 1) * D; x += 256) {
+        const int r = x / D, d = x % D;
+        float m = kNegInf;
+        for (int i = 0; i < splits; ++i) m = fmaxf(m, load_agent(stats + 2 * (first_slot + i * kRowsMany + r)));
+        const float ref = m == kNegInf ? 0.0f : m;
+        float sum = 0.0f, o = 0.0f;
+        for (int i = 0; i < splits; ++i) {
+            const size_t at = first_slot + i * kRowsMany + r;
+            const float f = __builtin_amdgcn_exp2f(load_agent(stats + 2 * at) - ref);
+            sum += load_agent(stats + 2 * at + 1) * f;
+            o += load_agent(a.partials + at * D + d) * f;
+        }
+        const int tk = (first_row + r) / group;
+        const uint32_t hh = head * a.group + (first_row + r - tk * group);
+        static_cast<T *>(a.d.out.data)[static_cast<int64_t>(s.first + tk) * a.d.out.token_stride + hh * a.d.out.head_stride + d] =
+            static_cast<T>(sum == 0.0f ? 0.0f : o / sum);
+        if (d == 0 && a.d.lse != nullptr)
+            a.d.lse[static_cast<size_t>(s.first + tk) * a.d.q_heads + hh] = (m + log2f(sum) - kWeight) * (1.0f / kLog2e);
+    }
+}
+
+}  // namespace
+
+uint64_t attend_many_places(const q4rdna_kv_batch &b, uint32_t group) {
+    return static_cast<uint64_t>(b.tokens) * group / kRowsMany + b.sequences;
+}
+
+hipError_t launch_attend_many(const AttendArgs &a, uint32_t places, hipStream_t stream) {
+    const dim3 grid(places * a.cache.kv_heads, a.splits);
+    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(a); };
+    if (a.cache.head_dim == 64)
+        a.d.dtype == Q4RDNA_F32 ? go(attend_many_kernel<64, 2, float>) : a.d.dtype == Q4RDNA_F16 ? go(attend_many_kernel<64, 1, _Float16>) : go(attend_many_kernel<64, 1, __bf16>);
+    else
+        a.d.dtype == Q4RDNA_F32 ? go(attend_many_kernel<128, 2, float>) : a.d.dtype == Q4RDNA_F16 ? go(attend_many_kernel<128, 1, _Float16>) : go(attend_many_kernel<128, 1, __bf16>);
+    return hipGetLastError();
+}
+
+}  // namespace q4rdna

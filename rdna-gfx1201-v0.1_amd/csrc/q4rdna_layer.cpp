@@ -207,6 +207,20 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     return launched(q4rdna::launch_append(a, static_cast<hipStream_t>(stream)), "kv_append");
 }
 
+// Sequences of up to so many rows per kv head go to attend_few_kernel.
+constexpr uint32_t kFewRows = 64;
+
+int take_scratch(q4rdna::AttendArgs &a, size_t jobs, uint32_t rows, hipStream_t stream) {
+    a.partials = nullptr;
+    a.arrived = nullptr;
+    if (a.splits == 1) return Q4RDNA_OK;
+    Scratch s;
+    const int rc = get_scratch(a.cache.device, stream, jobs * a.splits * rows * (a.cache.head_dim + 2), jobs, &s);
+    a.partials = s.partials;
+    a.arrived = s.arrived;
+    return rc;
+}
+
 int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4rdna_kv_attend_desc *desc, void *stream) {
     int rc;
     if ((rc = check_cache(cache)) != Q4RDNA_OK || (rc = check_batch(batch)) != Q4RDNA_OK) return rc;
@@ -223,30 +237,43 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     a.batch = *batch;
     a.d = *desc;
     a.group = desc->q_heads / cache->kv_heads;
-    const uint64_t most_rows = static_cast<uint64_t>(std::min(batch->max_tokens, batch->tokens)) * a.group;
-    const uint32_t rows = q4rdna::attend_few_rows(static_cast<uint32_t>(std::min<uint64_t>(most_rows, 1u << 30)));
-    const uint64_t row_groups = (most_rows + rows - 1) / rows;
-    if (row_groups * cache->kv_heads > 65535)
-        return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of a sequence are too many for one call", batch->max_tokens);
-    a.row_groups = static_cast<uint32_t>(row_groups);
     a.wide = wide_rows(desc->q, desc->dtype, 16 / size_of(desc->dtype));
+    a.wide_out = wide_rows(desc->out, desc->dtype, 4);
+    // The most rows (query token, query head) per kv head that a sequence has.
+    const uint64_t most_rows = static_cast<uint64_t>(std::min(batch->max_tokens, batch->tokens)) * a.group;
+    const bool many = most_rows > kFewRows;
+    const uint64_t places = q4rdna::attend_many_places(*batch, a.group);
+    if (most_rows > 0x3fffffffu || places * cache->kv_heads > 0x7fffffffu)
+        return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of %u query heads are too many for one call", batch->tokens, desc->q_heads);
     if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
-    // Enough workgroups for four per CU, no more than a block for each wave.
-    const uint64_t jobs = row_groups * cache->kv_heads * batch->sequences;
+    const uint32_t cus = cu_count(cache->device);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
     const uint64_t most_blocks = desc->window == 0 ? batch->table_width
                                                    : std::min<uint64_t>(batch->table_width, (static_cast<uint64_t>(desc->window) + batch->max_tokens) / q4rdna::kKvBlock + 2);
-    uint64_t splits = 4ull * cu_count(cache->device) / jobs;
-    splits = std::min(splits, (most_blocks + 3) / 4);
-    a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 256)));
-    if (a.splits > 1) {
-        Scratch s;
-        const size_t slots = jobs * a.splits * rows;
-        if ((rc = get_scratch(cache->device, static_cast<hipStream_t>(stream), slots * (cache->head_dim + 2), jobs, &s)) != Q4RDNA_OK)
+    // Sequences of few rows; a single one goes by the bound alone.
+    if (!many || batch->sequences > 1) {
+        a.few_rows = many ? kFewRows : 0x7fffffffu;
+        const uint32_t most = static_cast<uint32_t>(many ? kFewRows : most_rows), rows = q4rdna::attend_few_rows(most);
+        a.row_groups = (most + rows - 1) / rows;
+        // Enough workgroups for four per CU, no more than a block for each wave.
+        const uint64_t jobs = static_cast<uint64_t>(a.row_groups) * cache->kv_heads * batch->sequences;
+        const uint64_t splits = std::min<uint64_t>(4ull * cus / jobs, (most_blocks + 3) / 4);
+        a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 256)));
+        if ((rc = take_scratch(a, jobs, rows, s)) != Q4RDNA_OK ||
+            (rc = launched(q4rdna::launch_attend_few(a, rows, s), "kv_attend")) != Q4RDNA_OK)
             return rc;
-        a.partials = s.partials;
-        a.arrived = s.arrived;
     }
-    return launched(q4rdna::launch_attend_few(a, rows, static_cast<hipStream_t>(stream)), "kv_attend");
+    if (many) {
+        a.few_rows = batch->sequences > 1 ? kFewRows : 0;
+        // Two workgroups fit a CU: split until they are there.
+        const uint64_t jobs = places * cache->kv_heads;
+        const uint64_t splits = std::min<uint64_t>(2ull * cus / jobs, (most_blocks + 1) / 2);
+        a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 64)));
+        if ((rc = take_scratch(a, jobs, q4rdna::kAttendManyRows, s)) != Q4RDNA_OK ||
+            (rc = launched(q4rdna::launch_attend_many(a, static_cast<uint32_t>(places), s), "kv_attend")) != Q4RDNA_OK)
+            return rc;
+    }
+    return Q4RDNA_OK;
 }
 
 int read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dtype, const q4rdna_kv_rows *k,

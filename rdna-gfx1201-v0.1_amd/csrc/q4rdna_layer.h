@@ -54,13 +54,21 @@ struct AttendArgs {
     uint32_t group;       // query heads per kv head
     uint32_t row_groups;  // row groups of the largest sequence
     uint32_t splits;      // the most workgroups that share a row group
+    uint32_t few_rows;    // sequences of up to so many rows belong to attend_few_kernel, the others to
+                          // attend_many_kernel
     uint32_t wide;        // q rows can be read 16 bytes at a time
+    uint32_t wide_out;    // out rows can be written four elements at a time
     float *partials;      // [job][split][row][D], then max and sum [job][split][row][2]
     uint32_t *arrived;    // [job], zero between launches
 };
 // Rows (query token, query head of the kv head) that one workgroup takes.
 uint32_t attend_few_rows(uint32_t rows);
 hipError_t launch_attend_few(const AttendArgs &a, uint32_t rows, hipStream_t stream);
+
+// Row groups of 128 (attend_many_kernel) that the step's sequences may have.
+constexpr uint32_t kAttendManyRows = 128;
+uint64_t attend_many_places(const q4rdna_kv_batch &b, uint32_t group);
+hipError_t launch_attend_many(const AttendArgs &a, uint32_t places, hipStream_t stream);
 
 hipError_t launch_add_norm(const q4rdna_add_norm_desc &d, bool wide, uint32_t cus, hipStream_t stream);
 
