@@ -210,12 +210,17 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
 // Sequences of up to so many rows per kv head go to attend_few_kernel.
 constexpr uint32_t kFewRows = 64;
 
-int take_scratch(q4rdna::AttendArgs &a, size_t jobs, uint32_t rows, hipStream_t stream) {
+// Up to so many sequences the blocks are dealt by their lengths; more of them
+// fill the card by themselves.
+constexpr uint32_t kDealtSequences = 1024;
+
+// Room for partial results of `rows` rows, and arrival counters of `jobs` row groups.
+int take_scratch(q4rdna::AttendArgs &a, size_t rows, size_t jobs, hipStream_t stream) {
     a.partials = nullptr;
     a.arrived = nullptr;
     if (a.splits == 1) return Q4RDNA_OK;
     Scratch s;
-    const int rc = get_scratch(a.cache.device, stream, jobs * a.splits * rows * (a.cache.head_dim + 2), jobs, &s);
+    const int rc = get_scratch(a.cache.device, stream, rows * (a.cache.head_dim + 2), jobs, &s);
     a.partials = s.partials;
     a.arrived = s.arrived;
     return rc;
@@ -255,12 +260,21 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
         a.few_rows = many ? kFewRows : 0x7fffffffu;
         const uint32_t most = static_cast<uint32_t>(many ? kFewRows : most_rows), rows = q4rdna::attend_few_rows(most);
         a.row_groups = (most + rows - 1) / rows;
-        // Enough workgroups for four per CU, no more than a block for each wave.
+        // The device deals the blocks to about `target` workgroups; each row
+        // group ends in one part that may be short.
         const uint64_t jobs = static_cast<uint64_t>(a.row_groups) * cache->kv_heads * batch->sequences;
-        const uint64_t splits = std::min<uint64_t>(4ull * cus / jobs, (most_blocks + 3) / 4);
-        a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 256)));
-        if ((rc = take_scratch(a, jobs, rows, s)) != Q4RDNA_OK ||
-            (rc = launched(q4rdna::launch_attend_few(a, rows, s), "kv_attend")) != Q4RDNA_OK)
+        // Few row groups are cut into many parts, which cost time to join: take
+        // one workgroup of eight waves per CU there, two of four waves elsewhere.
+        const uint32_t waves = jobs < cus / 8 ? 8 : 4;
+        a.target = 8 / waves * cus;
+        const uint64_t most_splits = (most_blocks + q4rdna::kAttendFewChunk - 1) / q4rdna::kAttendFewChunk;
+        const bool split = most_splits > 1 && batch->sequences <= kDealtSequences;
+        a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>(most_splits, q4rdna::kAttendFewSplits) : 1);
+        const uint64_t workgroups = split ? std::min(jobs + a.target, jobs * a.splits) : jobs;
+        if (workgroups > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences are too many for one call", batch->sequences);
+        a.workgroups = static_cast<uint32_t>(workgroups);
+        if ((rc = take_scratch(a, workgroups * rows, jobs, s)) != Q4RDNA_OK ||
+            (rc = launched(q4rdna::launch_attend_few(a, rows, waves, s), "kv_attend")) != Q4RDNA_OK)
             return rc;
     }
     if (many) {
@@ -269,7 +283,7 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
         const uint64_t jobs = places * cache->kv_heads;
         const uint64_t splits = std::min<uint64_t>(2ull * cus / jobs, (most_blocks + 1) / 2);
         a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 64)));
-        if ((rc = take_scratch(a, jobs, q4rdna::kAttendManyRows, s)) != Q4RDNA_OK ||
+        if ((rc = take_scratch(a, jobs * a.splits * q4rdna::kAttendManyRows, jobs, s)) != Q4RDNA_OK ||
             (rc = launched(q4rdna::launch_attend_many(a, static_cast<uint32_t>(places), s), "kv_attend")) != Q4RDNA_OK)
             return rc;
     }

@@ -54,16 +54,25 @@ struct AttendArgs {
     uint32_t group;       // query heads per kv head
     uint32_t row_groups;  // row groups of the largest sequence
     uint32_t splits;      // the most workgroups that share a row group
+    uint32_t target;      // attend_few_kernel: workgroups to deal the blocks to
+    uint32_t workgroups;  // attend_few_kernel: workgroups launched
     uint32_t few_rows;    // sequences of up to so many rows belong to attend_few_kernel, the others to
                           // attend_many_kernel
     uint32_t wide;        // q rows can be read 16 bytes at a time
     uint32_t wide_out;    // out rows can be written four elements at a time
-    float *partials;      // [job][split][row][D], then max and sum [job][split][row][2]
+    float *partials;      // of each workgroup (attend_few_kernel) or [job][split]: [row][D], then all the
+                          // maxima and sums, [row][2]
     uint32_t *arrived;    // [job], zero between launches
 };
+// The most workgroups that share a row group of attend_few_kernel.
+constexpr uint32_t kAttendFewSplits = 64;
+// Blocks that a part has at least: joining two parts takes as long as two or
+// three more blocks per wave.
+constexpr uint32_t kAttendFewChunk = 8;
 // Rows (query token, query head of the kv head) that one workgroup takes.
 uint32_t attend_few_rows(uint32_t rows);
-hipError_t launch_attend_few(const AttendArgs &a, uint32_t rows, hipStream_t stream);
+// waves: 4 or 8 per workgroup.
+hipError_t launch_attend_few(const AttendArgs &a, uint32_t rows, uint32_t waves, hipStream_t stream);
 
 // Row groups of 128 (attend_many_kernel) that the step's sequences may have.
 constexpr uint32_t kAttendManyRows = 128;

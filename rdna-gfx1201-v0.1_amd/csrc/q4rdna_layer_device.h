@@ -92,6 +92,13 @@ __device__ __forceinline__ float max_xor32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// Two floats at once, device scope (see load_agent).
+__device__ __forceinline__ f32x2 load_agent2(const float *p) {
+    typedef __attribute__((address_space(1))) const uint64_t *gptr_cu64;
+    const uint64_t v = __hip_atomic_load((gptr_cu64)(uintptr_t)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return __builtin_bit_cast(f32x2, v);
+}
+
 __device__ __forceinline__ void count_fault(const q4rdna_kv_cache &c) {
     if (c.faults != nullptr) atomicAdd(c.faults, 1u);
 }
