@@ -39,11 +39,19 @@ __device__ __forceinline__ Place place_of(int lane, uint32_t rotary, bool interl
 }
 
 template <typename T>
-__device__ __forceinline__ Row load_row(const T *row, const Place &p, bool wide) {
-    Row r;
+__device__ __forceinline__ void load_row(Row &r, const T *row, const Place &p, bool wide) {
     load_floats<T, 4>(row + p.a_at, wide, r.a);
     load_floats<T, 4>(row + p.b_at, wide, r.b);
-    return r;
+}
+// The lane's four cosines and sines at a position.
+struct Turn {
+    float c[4], s[4];
+};
+__device__ __forceinline__ void load_turn(Turn &t, const Place &p, const q4rdna_kv_append_desc &d, int position) {
+    if (!p.turned) return;
+    const size_t at = static_cast<size_t>(position) * (d.rotary / 2) + p.pair;
+    load_floats<float, 4>(d.cos + at, true, t.c);
+    load_floats<float, 4>(d.sin + at, true, t.s);
 }
 
 // The norm of a head's row and its rotation, each product and sum rounded by
@@ -64,28 +72,44 @@ __device__ __forceinline__ void norm_row(Row &r, const Place &p, const float *we
         r.b[e] = r.b[e] * inv * wb[e];
     }
 }
-__device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s) {
+// (By value throughout: references that differ between the two orders of pairs
+// would put the rows into scratch memory.)
+__device__ __forceinline__ f32x2 turn_pair(float a, float b, float c, float s) {
 #pragma clang fp contract(off)
-    const float x = a * c - b * s;
-    const float y = b * c + a * s;
-    a = x;
-    b = y;
+    return f32x2{a * c - b * s, b * c + a * s};
 }
-__device__ __forceinline__ void turn_row(Row &r, const Place &p, const float *cos, const float *sin, size_t at,
-                                         bool interleaved) {
+__device__ __forceinline__ void turn_row(Row &r, const Place &p, const Turn &t, bool interleaved) {
     if (!p.turned) return;
-    float c[4], s[4];
-    load_floats<float, 4>(cos + at + p.pair, true, c);
-    load_floats<float, 4>(sin + at + p.pair, true, s);
-    if (interleaved) {
-        turn_pair(r.a[0], r.a[1], c[0], s[0]);
-        turn_pair(r.a[2], r.a[3], c[1], s[1]);
-        turn_pair(r.b[0], r.b[1], c[2], s[2]);
-        turn_pair(r.b[2], r.b[3], c[3], s[3]);
-    } else {
+    // Pair i is (first[i], second[i]).
+    const float first[4] = {r.a[0], interleaved ? r.a[2] : r.a[1], interleaved ? r.b[0] : r.a[2], interleaved ? r.b[2] : r.a[3]};
+    const float second[4] = {interleaved ? r.a[1] : r.b[0], interleaved ? r.a[3] : r.b[1], interleaved ? r.b[1] : r.b[2], r.b[3]};
+    f32x2 x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) turn_pair(r.a[e], r.b[e], c[e], s[e]);
-    }
+    for (int i = 0; i < 4; ++i) x[i] = turn_pair(first[i], second[i], t.c[i], t.s[i]);
+    r.a[0] = x[0][0];
+    r.a[1] = interleaved ? x[0][1] : x[1][0];
+    r.a[2] = interleaved ? x[1][0] : x[2][0];
+    r.a[3] = interleaved ? x[1][1] : x[3][0];
+    r.b[0] = interleaved ? x[2][0] : x[0][1];
+    r.b[1] = interleaved ? x[2][1] : x[1][1];
+    r.b[2] = interleaved ? x[3][0] : x[2][1];
+    r.b[3] = x[3][1];
+}
+
+// The low bytes of four values, packed.
+__device__ __forceinline__ uint32_t pack4(int x0, int x1, int x2, int x3) {
+    const uint32_t lo = __builtin_amdgcn_perm(static_cast<uint32_t>(x1), static_cast<uint32_t>(x0), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(static_cast<uint32_t>(x3), static_cast<uint32_t>(x2), 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+// Four words of four bytes, transposed.
+__device__ __forceinline__ void transpose4(const uint32_t (&t)[4], uint32_t (&n)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(t[1], t[0], 0x05010400u), b = __builtin_amdgcn_perm(t[1], t[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(t[3], t[2], 0x05010400u), d = __builtin_amdgcn_perm(t[3], t[2], 0x07030602u);
+    n[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    n[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    n[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    n[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
 // Two planes of 16 codes from 16 shorts: low bytes as signed numbers, and what
@@ -149,37 +173,60 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
     const bool full = to == static_cast<int>(kKvBlock);
     const bool keep = block >= s.length / static_cast<int>(kKvBlock) - 1;
 
-    // Rows: the block's K rows, then its V rows, a group of D / 8 lanes each.
+    // Rows: the block's K rows, then its V rows, a group of D / 8 lanes each,
+    // kEach of them in flight.
+    constexpr int kEach = 4;
     const int lane = tid % kLanes;
     const bool interleaved = a.d.interleaved != 0;
-    for (int row = tid / kLanes; row < 2 * fresh; row += kRows) {
-        const bool is_v = row >= fresh;
-        const int t = from + (is_v ? row - fresh : row);
-        const size_t n = static_cast<size_t>(s.first) + (start + t - s.past);
-        const q4rdna_kv_rows &src = is_v ? a.d.v : a.d.k;
-        const T *p = static_cast<const T *>(src.data) + n * src.token_stride + head * src.head_stride;
-        const Place at = place_of<D>(lane, is_v ? 0 : a.d.rotary, interleaved);
-        Row r = load_row(p, at, a.wide != 0);
-        if (!is_v) {
-            if (a.d.k_norm != nullptr) norm_row<D>(r, at, a.d.k_norm, a.d.eps);
-            turn_row(r, at, a.d.cos, a.d.sin, static_cast<size_t>(start + t) * (a.d.rotary / 2), interleaved);
-        }
-        // The largest magnitude by its bits: infinities and NaN come out on top.
-        uint32_t top = 0;
+    for (int row0 = tid / kLanes; row0 < 2 * fresh; row0 += kEach * kRows) {
+        Row r[kEach];
+        Turn turn[kEach];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            top = max(top, max(__float_as_uint(r.a[e]) & 0x7fffffffu, __float_as_uint(r.b[e]) & 0x7fffffffu));
-        top = lanes_max<kLanes>(top);
-        const float largest = __uint_as_float(top);
-        const bool finite = top < 0x7f800000u, some = finite && largest >= kKvZero;
-        const float inv = some ? kKvCode16 / largest : 0.0f;
-        short *out = &st.code[is_v][t * kRow<D>];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            out[at.a_at + e] = some ? static_cast<short>(static_cast<int>(rintf(r.a[e] * inv))) : 0;
-            out[at.b_at + e] = some ? static_cast<short>(static_cast<int>(rintf(r.b[e] * inv))) : 0;
+        for (int x = 0; x < kEach; ++x) {
+            const int row = row0 + x * kRows;
+            if (row < 2 * fresh) {
+                const bool is_v = row >= fresh;
+                const int t = from + (is_v ? row - fresh : row);
+                const size_t n = static_cast<size_t>(s.first) + (start + t - s.past);
+                const void *data = is_v ? a.d.v.data : a.d.k.data;
+                const int64_t token_stride = is_v ? a.d.v.token_stride : a.d.k.token_stride;
+                const int64_t head_stride = is_v ? a.d.v.head_stride : a.d.k.head_stride;
+                const Place at = place_of<D>(lane, is_v ? 0 : a.d.rotary, interleaved);
+                load_row(r[x], static_cast<const T *>(data) + n * token_stride + head * head_stride, at,
+                         a.wide != 0);
+                load_turn(turn[x], at, a.d, start + t);
+            }
         }
-        if (lane == 0) st.scale[is_v][t] = some ? largest / kKvCode16 : finite ? 0.0f : __builtin_nanf("");
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const int row = row0 + x * kRows;
+            if (row < 2 * fresh) {
+                const bool is_v = row >= fresh;
+                const int t = from + (is_v ? row - fresh : row);
+                const Place at = place_of<D>(lane, is_v ? 0 : a.d.rotary, interleaved);
+                if (!is_v && a.d.k_norm != nullptr) norm_row<D>(r[x], at, a.d.k_norm, a.d.eps);
+                turn_row(r[x], at, turn[x], interleaved);
+                // The largest magnitude by its bits: infinities and NaN come out on top.
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    top = max(top, max(__float_as_uint(r[x].a[e]) & 0x7fffffffu, __float_as_uint(r[x].b[e]) & 0x7fffffffu));
+                top = lanes_max<kLanes>(top);
+                const float largest = __uint_as_float(top);
+                const bool finite = top < 0x7f800000u, some = finite && largest >= kKvZero;
+                const float inv = some ? kKvCode16 / largest : 0.0f;
+                s16x4 ca, cb;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ca[e] = some ? static_cast<short>(static_cast<int>(rintf(r[x].a[e] * inv))) : 0;
+                    cb[e] = some ? static_cast<short>(static_cast<int>(rintf(r[x].b[e] * inv))) : 0;
+                }
+                short *out = &st.code[is_v][t * kRow<D>];
+                *reinterpret_cast<s16x4 *>(out + at.a_at) = ca;
+                *reinterpret_cast<s16x4 *>(out + at.b_at) = cb;
+                if (lane == 0) st.scale[is_v][t] = some ? largest / kKvCode16 : finite ? 0.0f : __builtin_nanf("");
+            }
+        }
     }
 
     int8_t *planes = a.cache.open + open_tile(a.cache, s.slot, block, head);
@@ -274,27 +321,46 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
     }
     __syncthreads();
     int8_t *tile = a.cache.pages + page_tile(a.cache, page, head);
-    for (int piece = tid; piece < kPieces; piece += 256) {
-        i32x4 k, v;
-        const int t = k_token<D>(piece);
-        const short *row = &st.code[0][t * kRow<D> + k_number<D>(piece)];
-        const float r = st.ratio[0][t];
-        const int number = v_number(piece);
+    if (tid < 128) {
+        // K: 16 numbers of a token are a piece.
+        for (int piece = tid; piece < kPieces; piece += 128) {
+            const int t = k_token<D>(piece);
+            const s16x8 *row = reinterpret_cast<const s16x8 *>(&st.code[0][t * kRow<D> + k_number<D>(piece)]);
+            const float r = st.ratio[0][t];
+            i32x4 k;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            uint32_t kw = 0, vw = 0;
+            for (int w = 0; w < 4; ++w) {
+                const s16x8 c = row[w / 2];
+                int x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int vt = v_token(piece, 4 * w + e);
-                kw |= (static_cast<uint32_t>(static_cast<int>(rintf(row[4 * w + e] * r))) & 255u) << (8 * e);
-                vw |= (static_cast<uint32_t>(static_cast<int>(rintf(st.code[1][vt * kRow<D> + number] * st.ratio[1][vt]))) & 255u)
-                      << (8 * e);
+                for (int e = 0; e < 4; ++e) x[e] = static_cast<int>(rintf(c[4 * (w % 2) + e] * r));
+                k[w] = static_cast<int>(pack4(x[0], x[1], x[2], x[3]));
             }
-            k[w] = static_cast<int>(kw);
-            v[w] = static_cast<int>(vw);
+            store16(tile + 16 * piece, k);
         }
-        store16(tile + 16 * piece, k);
-        store16(tile + kPlane + 16 * piece, v);
+    } else {
+        // V: 16 tokens of each of four numbers, transposed four by four.
+        for (int x = tid - 128; x < D; x += 128) {
+            const int number = x % (D / 4) * 4, g = x / (D / 4);
+            i32x4 v[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t by_token[4], by_number[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int t = 16 * w + 4 * g + b;
+                    const s16x4 c = *reinterpret_cast<const s16x4 *>(&st.code[1][t * kRow<D> + number]);
+                    const float r = st.ratio[1][t];
+                    by_token[b] = pack4(static_cast<int>(rintf(c[0] * r)), static_cast<int>(rintf(c[1] * r)),
+                                        static_cast<int>(rintf(c[2] * r)), static_cast<int>(rintf(c[3] * r)));
+                }
+                transpose4(by_token, by_number);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) v[n][w] = static_cast<int>(by_number[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) store16(tile + kPlane + 16 * (v_piece(4 * g, number) + n), v[n]);
+        }
     }
 }
 
@@ -334,31 +400,53 @@ __device__ void append_place(const AppendArgs &a, uint32_t unit, AppendStage<D> 
     append_block<D, T>(a, s, i, head, block, st);
 }
 
-// kAppendQRows rows (token, query head) of q.
+// a.q_rows rows (token, query head) of q, kEach per group of D / 8 lanes in flight.
 template <int D, typename T>
 __device__ void turn_q(const AppendArgs &a, uint32_t unit) {
-    constexpr int kLanes = D / 8;
+    constexpr int kLanes = D / 8, kRows = 256 / kLanes, kEach = 4;
     const int lane = threadIdx.x % kLanes;
     const bool interleaved = a.d.interleaved != 0;
     const Place at = place_of<D>(lane, a.d.rotary, interleaved);
-    const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * a.d.q_heads;
-    for (uint32_t x = threadIdx.x / kLanes; x < kAppendQRows; x += 256 / kLanes) {
-        const uint64_t row = static_cast<uint64_t>(unit) * kAppendQRows + x;
-        if (row >= rows) return;
-        const uint32_t n = static_cast<uint32_t>(row / a.d.q_heads), head = static_cast<uint32_t>(row - static_cast<uint64_t>(n) * a.d.q_heads);
-        Row r = load_row(static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(n) * a.d.q.token_stride +
-                             head * a.d.q.head_stride, at, a.wide != 0);
-        const Seq s = seq_of(a.batch, a.cache, token_seq(a.batch, n));
-        const int position = s.past + static_cast<int>(n) - s.first;
-        if (!s.ok || static_cast<int>(n) < s.first || static_cast<int>(n) >= s.first + s.count ||
-            (a.d.rotary != 0 && static_cast<uint32_t>(s.length) > a.d.positions))
-            continue;  // its sequence is refused (and counted) as a whole
-        if (a.d.q_norm != nullptr) norm_row<D>(r, at, a.d.q_norm, a.d.eps);
-        turn_row(r, at, a.d.cos, a.d.sin, static_cast<size_t>(position) * (a.d.rotary / 2), interleaved);
-        T *out = static_cast<T *>(a.d.q_out.data) + static_cast<int64_t>(n) * a.d.q_out.token_stride +
-                 head * a.d.q_out.head_stride;
-        store_floats<T, 4>(out + at.a_at, a.wide != 0, r.a);
-        store_floats<T, 4>(out + at.b_at, a.wide != 0, r.b);
+    const uint32_t heads = a.d.q_heads;
+    const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * heads, row_first = static_cast<uint64_t>(unit) * a.q_rows;
+    // The workgroup's tokens are mostly of one sequence: the first one's.
+    const Seq s0 = seq_of(a.batch, a.cache, token_seq(a.batch, static_cast<uint32_t>(row_first / heads)));
+    for (uint32_t x0 = threadIdx.x / kLanes; x0 < a.q_rows; x0 += kEach * kRows) {
+        Row r[kEach];
+        Turn turn[kEach];
+        uint32_t n[kEach], head[kEach];
+        bool live[kEach];
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const uint64_t row = row_first + x0 + x * kRows;
+            live[x] = x0 + x * kRows < a.q_rows && row < rows;
+            n[x] = live[x] ? static_cast<uint32_t>(row / heads) : 0;
+            head[x] = live[x] ? static_cast<uint32_t>(row - static_cast<uint64_t>(n[x]) * heads) : 0;
+            if (live[x])
+                load_row(r[x], static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(n[x]) * a.d.q.token_stride +
+                                   head[x] * a.d.q.head_stride, at, a.wide != 0);
+        }
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            if (!live[x]) continue;
+            Seq s = s0;
+            if (!s.ok || static_cast<int>(n[x]) < s.first || static_cast<int>(n[x]) >= s.first + s.count)
+                s = seq_of(a.batch, a.cache, token_seq(a.batch, n[x]));
+            // A refused sequence's rows are not written (it is counted with its blocks).
+            live[x] = s.ok && static_cast<int>(n[x]) >= s.first && static_cast<int>(n[x]) < s.first + s.count &&
+                      (a.d.rotary == 0 || static_cast<uint32_t>(s.length) <= a.d.positions);
+            if (live[x]) load_turn(turn[x], at, a.d, s.past + static_cast<int>(n[x]) - s.first);
+        }
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            if (!live[x]) continue;
+            if (a.d.q_norm != nullptr) norm_row<D>(r[x], at, a.d.q_norm, a.d.eps);
+            turn_row(r[x], at, turn[x], interleaved);
+            T *out = static_cast<T *>(a.d.q_out.data) + static_cast<int64_t>(n[x]) * a.d.q_out.token_stride +
+                     head[x] * a.d.q_out.head_stride;
+            store_floats<T, 4>(out + at.a_at, a.wide != 0, r[x].a);
+            store_floats<T, 4>(out + at.b_at, a.wide != 0, r[x].b);
+        }
     }
 }
 
@@ -371,11 +459,15 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
         turn_q<D, T>(a, blockIdx.x - a.kv_units);
 }
 
+// Byte e of a word as a signed number.
+__device__ __forceinline__ int byte_of(uint32_t w, int e) { return static_cast<int8_t>(w >> (8 * e)); }
+
 // One (sequence, block, kv head): its tokens past .. length - 1 as numbers.
+// Half of the threads take K, a piece (16 numbers of a token) at a time, eight
+// lanes a token's row; the others V, 16 tokens of four numbers, which are
+// transposed four by four, so that lanes side by side write a row.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
-    constexpr int kPieces = kKvBlock * D / 16;
-    __shared__ float values[kKvBlock * (D + 1)];
     const uint32_t heads = a.cache.kv_heads;
     const uint32_t place = blockIdx.x / heads, head = blockIdx.x - place * heads;
     const int tid = threadIdx.x;
@@ -392,6 +484,7 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
     const int start = block * static_cast<int>(kKvBlock);
     const int from = max(s.past - start, 0), to = min(s.length - start, static_cast<int>(kKvBlock));
     const bool full = start + static_cast<int>(kKvBlock) <= s.length;
+    constexpr size_t kPlane = kKvBlock * D;
     const int8_t *tile;
     const float *scales;
     float bad = 0.0f;
@@ -408,31 +501,52 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
         tile = a.cache.open + open_tile(a.cache, s.slot, block, head);
         scales = a.cache.open_scales + open_scale_row(a.cache, s.slot, block, head);
     }
-    constexpr size_t kPlane = kKvBlock * D;
-    for (int which = 0; which < 2; ++which) {
-        const int8_t *high = tile + (full ? which : 2 * which) * kPlane;
-        __syncthreads();
-        for (int piece = tid; piece < kPieces; piece += 256) {
-            const i32x4 h = load16(high + 16 * piece);
-            i32x4 l = {0, 0, 0, 0};
-            if (!full) l = load16(high + kPlane + 16 * piece);
+    const int64_t row0 = static_cast<int64_t>(s.first) + (start - s.past);  // of the block's token 0
+    if (tid < 128) {
+        T *out = static_cast<T *>(a.k.data) + head * a.k.head_stride;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int t = which == 0 ? k_token<D>(piece) : v_token(piece, e);
-                const int number = which == 0 ? k_number<D>(piece) + e : v_number(piece);
-                const float x = full ? static_cast<float>(static_cast<int8_t>(static_cast<uint32_t>(h[e / 4]) >> (8 * (e % 4))))
-                                     : static_cast<float>(join16(h, l, e));
-                // An open block's scales past its length are not there.
-                if (t >= from && t < to) values[t * (D + 1) + number] = x * (full ? scales[which] + bad : scales[which * 64 + t]);
-            }
+        for (int x = tid; x < kKvBlock * D / 16; x += 128) {
+            const int t = x / (D / 16), number = x % (D / 16) * 16, piece = k_piece<D>(t, number);
+            if (t < from || t >= to) continue;
+            const i32x4 h = load16(tile + 16 * piece);
+            i32x4 l = {0, 0, 0, 0};
+            if (!full) l = load16(tile + kPlane + 16 * piece);
+            const float scale = full ? scales[0] + bad : scales[t], high = full ? 1.0f : 256.0f;
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                v[e] = (byte_of(h[e / 4], e % 4) * high + byte_of(l[e / 4], e % 4)) * scale;
+            store_floats<T, 16>(out + (row0 + t) * a.k.token_stride + number, a.wide != 0, v);
         }
-        __syncthreads();
-        const q4rdna_kv_rows &dst = which == 0 ? a.k : a.v;
-        for (int x = tid; x < (to - from) * D; x += 256) {
-            const int t = from + x / D, number = x % D;
-            const int64_t n = static_cast<int64_t>(s.first) + (start + t - s.past);
-            static_cast<T *>(dst.data)[n * dst.token_stride + head * dst.head_stride + number] =
-                static_cast<T>(values[t * (D + 1) + number]);
+    } else {
+        T *out = static_cast<T *>(a.v.data) + head * a.v.head_stride;
+        const int8_t *plane = tile + (full ? 1 : 2) * kPlane;
+        for (int x = tid - 128; x < D; x += 128) {
+            const int number = x % (D / 4) * 4, g = x / (D / 4), piece = v_piece(4 * g, number);
+            if (4 * g >= to || 4 * g + 51 < from) continue;
+            i32x4 h[4], l[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                h[n] = load16(plane + 16 * (piece + n));
+                l[n] = i32x4{0, 0, 0, 0};
+                if (!full) l[n] = load16(plane + kPlane + 16 * (piece + n));
+            }
+            const float high = full ? 1.0f : 256.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const f32x4 by_token = full ? f32x4{scales[1] + bad, scales[1] + bad, scales[1] + bad, scales[1] + bad}
+                                            : *(gptr_f32x4)(uintptr_t)(scales + 64 + 16 * w + 4 * g);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int t = 16 * w + 4 * g + b;
+                    if (t < from || t >= to) continue;
+                    float v[4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        v[n] = (byte_of(h[n][w], b) * high + byte_of(l[n][w], b)) * by_token[b];
+                    store_floats<T, 4>(out + (row0 + t) * a.v.token_stride + number, a.wide != 0, v);
+                }
+            }
         }
     }
 }

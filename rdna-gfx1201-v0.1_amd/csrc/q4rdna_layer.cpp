@@ -193,7 +193,11 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     if (!aligned(desc->q_norm, 16) || !aligned(desc->k_norm, 16))
         return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned norm weight");
     const uint64_t kv_units = q4rdna::kv_places(*batch) * cache->kv_heads;
-    const uint64_t q_units = (static_cast<uint64_t>(batch->tokens) * desc->q_heads + q4rdna::kAppendQRows - 1) / q4rdna::kAppendQRows;
+    // Few rows of q: one per lane group, so that many workgroups share the
+    // wait for them; many: eight.
+    const uint64_t all_rows = static_cast<uint64_t>(batch->tokens) * desc->q_heads;
+    const uint32_t q_rows = all_rows <= 32768 ? 2048 / cache->head_dim : 16384 / cache->head_dim;
+    const uint64_t q_units = (all_rows + q_rows - 1) / q_rows;
     if (kv_units + q_units > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
     if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
     q4rdna::AppendArgs a{};
@@ -202,6 +206,7 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     a.d = *desc;
     a.kv_units = static_cast<uint32_t>(kv_units);
     a.q_units = static_cast<uint32_t>(q_units);
+    a.q_rows = q_rows;
     a.wide = wide_rows(desc->k, desc->dtype, 4) && wide_rows(desc->v, desc->dtype, 4) &&
              (desc->q_heads == 0 || (wide_rows(desc->q, desc->dtype, 4) && wide_rows(desc->q_out, desc->dtype, 4)));
     return launched(q4rdna::launch_append(a, static_cast<hipStream_t>(stream)), "kv_append");
@@ -309,6 +314,7 @@ int read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dt
     a.v = *v;
     a.dtype = dtype;
     a.units = static_cast<uint32_t>(units);
+    a.wide = wide_rows(*k, dtype, 16 / size_of(dtype)) && wide_rows(*v, dtype, 16 / size_of(dtype));
     return launched(q4rdna::launch_read(a, static_cast<hipStream_t>(stream)), "kv_read");
 }
 

@@ -25,11 +25,10 @@ struct AppendArgs {
     q4rdna_kv_append_desc d;
     uint32_t kv_units;  // (sequence, block) places times kv heads
     uint32_t q_units;   // workgroups that rotate q
+    uint32_t q_rows;    // rows (token, query head) that each of them takes
     uint32_t wide;      // rows of k, v, q, q_out can be read four elements at a time
 };
 hipError_t launch_append(const AppendArgs &a, hipStream_t stream);
-// Rows of q that one workgroup rotates.
-constexpr uint32_t kAppendQRows = 32;
 
 struct ReadArgs {
     q4rdna_kv_cache cache;
@@ -37,6 +36,7 @@ struct ReadArgs {
     q4rdna_kv_rows k, v;
     uint32_t dtype;
     uint32_t units;
+    uint32_t wide;      // k and v rows can be written 16 bytes at a time
 };
 hipError_t launch_read(const ReadArgs &a, hipStream_t stream);
 

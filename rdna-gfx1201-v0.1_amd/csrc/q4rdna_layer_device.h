@@ -7,6 +7,7 @@
 
 namespace q4rdna {
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // 16 bytes of global memory.

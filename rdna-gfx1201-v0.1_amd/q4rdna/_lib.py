@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libq4rdna_gfx950.so"
@@ -124,6 +125,13 @@ class AddNormDesc(ctypes.Structure):
                 ("n_stride", ctypes.c_int64), ("post_weight", ctypes.c_void_p), ("weight", ctypes.c_void_p)]
 
 
+# The same structures as packers: one call fills a descriptor, where setting
+# each field of a ctypes structure takes longer than the kernel's launch.
+ROWS = struct.Struct("@Pqq")
+APPEND = struct.Struct("@2I Pqq Pqq Pqq Pqq 2P 3If 2P")
+ATTEND = struct.Struct("@2I Pqq Pqq P f I")
+ADD_NORM = struct.Struct("@3I2fI 5P 5q 2P")
+
 _lib = None
 
 
@@ -172,11 +180,10 @@ def load() -> ctypes.CDLL:
         "q4rdna_launch_count": (u64, []),
         "q4rdna_sidecar_hits": (u64, [vp, u32]),
         "q4rdna_report_stats": (None, []),
-        "q4rdna_kv_append": (i32, [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.POINTER(AppendDesc), vp]),
-        "q4rdna_kv_attend": (i32, [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), ctypes.POINTER(AttendDesc), vp]),
-        "q4rdna_kv_read": (i32, [ctypes.POINTER(CacheDesc), ctypes.POINTER(BatchDesc), u32, ctypes.POINTER(Rows),
-                                 ctypes.POINTER(Rows), vp]),
-        "q4rdna_add_norm": (i32, [ctypes.POINTER(AddNormDesc), vp]),
+        "q4rdna_kv_append": (i32, [vp, vp, vp, vp]),
+        "q4rdna_kv_attend": (i32, [vp, vp, vp, vp]),
+        "q4rdna_kv_read": (i32, [vp, vp, u32, vp, vp, vp]),
+        "q4rdna_add_norm": (i32, [vp, vp]),
     }
     for name, (res, args) in proto.items():
         fn = getattr(L, name)

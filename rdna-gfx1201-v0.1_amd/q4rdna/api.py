@@ -432,18 +432,18 @@ def _plain(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device:
     return t.data_ptr()
 
 
-def _rows(r: _lib.Rows, t: torch.Tensor, name: str, dtype: torch.dtype, tokens: int, heads: int, dim: int,
-          device: int) -> None:
-    """Describe activations [tokens, heads, dim] of any token and head strides."""
-    if t.dtype != dtype or t.get_device() != device or t.shape != (tokens, heads, dim):
-        raise ValueError(f"{name} must be a {dtype} tensor of shape {(tokens, heads, dim)} on cuda:{device}, got "
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> tuple[int, int, int]:
+    """(address, token stride, head stride) of activations [tokens, heads, dim]."""
+    if t.dtype != dtype or t.get_device() != device or t.shape != shape:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{device}, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
     token_stride, head_stride, stride = t.stride()
     if stride != 1:
         raise ValueError(f"the numbers of a head of {name} must be contiguous")
-    r.data = t.data_ptr()
-    r.token_stride = token_stride
-    r.head_stride = head_stride
+    return t.data_ptr(), token_stride, head_stride
+
+
+_NO_ROWS = (0, 0, 0)
 
 
 def _no_overlap(t: torch.Tensor, name: str) -> None:
@@ -561,39 +561,41 @@ class KVCache:
         [head_dim]; cos, sin [positions, rotary / 2], float32)."""
         if k.dim() != 3:
             raise ValueError("k must be [tokens, kv_heads, head_dim]")
-        tokens, heads, dim, device = k.shape[0], self.kv_heads, self.head_dim, self.device
+        tokens, heads, dim, device, dtype = k.shape[0], self.kv_heads, self.head_dim, self.device, k.dtype
         step = self._step(batch, tokens)
-        d = _lib.AppendDesc()
-        d.dtype = _dtype(k.dtype)
-        _rows(d.k, k, "k", k.dtype, tokens, heads, dim, device)
-        _rows(d.v, v, "v", k.dtype, tokens, heads, dim, device)
+        shape = (tokens, heads, dim)
+        k_rows, v_rows = _rows(k, "k", dtype, shape, device), _rows(v, "v", dtype, shape, device)
+        q_rows = out_rows = _NO_ROWS
+        q_heads = 0
         if q is not None:
             if q.dim() != 3:
                 raise ValueError("q must be [tokens, q_heads, head_dim]")
-            _rows(d.q, q, "q", k.dtype, tokens, q.shape[1], dim, device)
+            q_heads = q.shape[1]
+            shape = (tokens, q_heads, dim)
+            q_rows = _rows(q, "q", dtype, shape, device)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            _rows(d.q_out, q_out, "q_out", k.dtype, tokens, q.shape[1], dim, device)
-            _no_overlap(q_out, "q_out")
-            d.q_heads = q.shape[1]
+                q_out = torch.empty_like(q)
+                out_rows = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+            else:
+                _no_overlap(q_out, "q_out")
+                out_rows = _rows(q_out, "q_out", dtype, shape, device)
         elif q_out is not None or q_norm is not None:
             raise ValueError("q_out or q_norm without q")
+        cos_at = sin_at = positions = rotary = 0
         if cos is not None:
             if cos.dim() != 2 or sin is None:
                 raise ValueError("cos and sin must be [positions, rotary / 2]")
-            d.cos = _plain(cos, "cos", torch.float32, cos.shape, device)
-            d.sin = _plain(sin, "sin", torch.float32, cos.shape, device)
-            d.positions, d.rotary = cos.shape[0], 2 * cos.shape[1]
+            cos_at = _plain(cos, "cos", torch.float32, cos.shape, device)
+            sin_at = _plain(sin, "sin", torch.float32, cos.shape, device)
+            positions, rotary = cos.shape[0], 2 * cos.shape[1]
         elif sin is not None:
             raise ValueError("sin without cos")
-        d.interleaved = interleaved
-        d.eps = eps
-        if q_norm is not None:
-            d.q_norm = _plain(q_norm, "q_norm", torch.float32, (dim,), device)
-        if k_norm is not None:
-            d.k_norm = _plain(k_norm, "k_norm", torch.float32, (dim,), device)
+        q_weight = 0 if q_norm is None else _plain(q_norm, "q_norm", torch.float32, (dim,), device)
+        k_weight = 0 if k_norm is None else _plain(k_norm, "k_norm", torch.float32, (dim,), device)
+        d = _lib.APPEND.pack(_dtype(dtype), q_heads, *k_rows, *v_rows, *q_rows, *out_rows, cos_at, sin_at, positions,
+                             rotary, interleaved, eps, q_weight, k_weight)
         s = _raw_stream(device) if stream is None else stream
-        check(load().q4rdna_kv_append(self._ref, step, ctypes.byref(d), s))
+        check(load().q4rdna_kv_append(self._ref, step, d, s))
         return q_out
 
     def attend(self, batch: KVBatch, q: torch.Tensor, out: torch.Tensor | None = None, scale: float | None = None,
@@ -604,42 +606,46 @@ class KVCache:
         tensor [tokens, q_heads]): returns (out, lse)."""
         if q.dim() != 3:
             raise ValueError("q must be [tokens, q_heads, head_dim]")
-        tokens, heads, dim = q.shape
+        shape, dtype, device = q.shape, q.dtype, self.device
+        tokens, heads, _ = shape
         step = self._step(batch, tokens)
-        d = _lib.AttendDesc()
-        d.dtype = _dtype(q.dtype)
-        d.q_heads = heads
-        _rows(d.q, q, "q", q.dtype, tokens, heads, self.head_dim, self.device)
+        shape = (tokens, heads, self.head_dim)
+        rows = _rows(q, "q", dtype, shape, device)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _rows(d.out, out, "out", q.dtype, tokens, heads, self.head_dim, self.device)
-        _no_overlap(out, "out")
+            out = torch.empty_like(q)
+            out_rows = out.data_ptr(), out.stride(0), out.stride(1)
+        else:
+            _no_overlap(out, "out")
+            out_rows = _rows(out, "out", dtype, shape, device)
         if lse is True:
             lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
-        if lse is not False:
-            d.lse = _plain(lse, "lse", torch.float32, (tokens, heads), self.device)
-        d.scale = self.head_dim ** -0.5 if scale is None else scale
         if window < 0:
             raise ValueError("window must not be negative")
-        d.window = window
-        s = _raw_stream(self.device) if stream is None else stream
-        check(load().q4rdna_kv_attend(self._ref, step, ctypes.byref(d), s))
+        d = _lib.ATTEND.pack(_dtype(dtype), heads, *rows, *out_rows,
+                             0 if lse is False else _plain(lse, "lse", torch.float32, (tokens, heads), device),
+                             self.head_dim ** -0.5 if scale is None else scale, window)
+        s = _raw_stream(device) if stream is None else stream
+        check(load().q4rdna_kv_attend(self._ref, step, d, s))
         return out if lse is False else (out, lse)
 
     def read(self, batch: KVBatch, tokens: int, dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None,
              v: torch.Tensor | None = None, stream: int | None = None):
         """(k, v) [tokens, kv_heads, head_dim]: the batch's tokens (past[i] on,
         up to the sequence's length) as numbers."""
-        shape, device = (tokens, self.kv_heads, self.head_dim), torch.device("cuda", self.device)
+        shape, device = (tokens, self.kv_heads, self.head_dim), self.device
         step = self._step(batch, tokens)
-        rows = _lib.Rows(), _lib.Rows()
-        k = torch.empty(shape, dtype=dtype, device=device) if k is None else k
-        v = torch.empty(shape, dtype=dtype, device=device) if v is None else v
-        for r, t, name in ((rows[0], k, "k"), (rows[1], v, "v")):
-            _rows(r, t, name, dtype, *shape, self.device)
-            _no_overlap(t, name)
-        s = _raw_stream(self.device) if stream is None else stream
-        check(load().q4rdna_kv_read(self._ref, step, _dtype(dtype), ctypes.byref(rows[0]), ctypes.byref(rows[1]), s))
+        rows = []
+        if k is None:
+            k = torch.empty(shape, dtype=dtype, device=self.pages.device)
+        else:
+            _no_overlap(k, "k")
+        if v is None:
+            v = torch.empty_like(k)
+        else:
+            _no_overlap(v, "v")
+        rows = [_lib.ROWS.pack(*_rows(t, name, dtype, shape, device)) for t, name in ((k, "k"), (v, "v"))]
+        s = _raw_stream(device) if stream is None else stream
+        check(load().q4rdna_kv_read(self._ref, step, _dtype(dtype), rows[0], rows[1], s))
         return k, v
 
 
@@ -658,41 +664,48 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
         raise ValueError("residual must be a CUDA tensor [rows, width]")
     device, shape, dtype = residual.get_device(), residual.shape, residual.dtype
     width = shape[1]
-    d = _lib.AddNormDesc()
-    d.dtype = _dtype(dtype)
-    d.rows, d.width = shape
-    d.scale, d.eps = scale, eps
 
     def matrix(t, name):
-        if t.dtype != dtype or t.get_device() != device or t.shape != shape or t.stride(1) != 1 and width > 1:
+        stride = t.stride()
+        if t.dtype != dtype or t.get_device() != device or t.shape != shape or stride[1] != 1 and width > 1:
             raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} with contiguous rows on cuda:{device}")
-        return t.data_ptr(), t.stride(0)
+        return t.data_ptr(), stride[0]
 
-    d.residual, d.residual_stride = matrix(residual, "residual")
+    r_at, r_stride = matrix(residual, "residual")
+    y_at = y_stride = gate_at = gate_stride = h_at = h_stride = n_at = n_stride = post_at = weight_at = 0
     if y is not None:
-        d.y, d.y_stride = matrix(y, "y")
+        y_at, y_stride = matrix(y, "y")
         if h is None:
-            h = torch.empty(shape, dtype=dtype, device=residual.device)
-        d.h, d.h_stride = matrix(h, "h")
-        _no_overlap(h, "h")
+            h = torch.empty_like(residual)
+            h_at, h_stride = h.data_ptr(), h.stride(0)
+        else:
+            _no_overlap(h, "h")
+            h_at, h_stride = matrix(h, "h")
         if gate is not None:
             if gate.dim() == 1:
-                d.gate = _plain(gate, "gate", dtype, (width,), device)
+                gate_at = _plain(gate, "gate", dtype, (width,), device)
             else:
-                d.gate, d.gate_stride = matrix(gate, "gate")
+                gate_at, gate_stride = matrix(gate, "gate")
         if post_weight is not None:
-            d.post_weight = _plain(post_weight, "post_weight", torch.float32, (width,), device)
+            post_at = _plain(post_weight, "post_weight", torch.float32, (width,), device)
     elif gate is not None or post_weight is not None or h is not None:
         raise ValueError("gate, post_weight or h without y")
     if weight is not None:
         if n is None:
-            n = torch.empty(shape, dtype=dtype, device=residual.device)
-        d.n, d.n_stride = matrix(n, "n")
-        _no_overlap(n, "n")
-        d.weight = _plain(weight, "weight", torch.float32, (width,), device)
+            n = torch.empty_like(residual)
+            n_at, n_stride = n.data_ptr(), n.stride(0)
+        else:
+            _no_overlap(n, "n")
+            n_at, n_stride = matrix(n, "n")
+        weight_at = _plain(weight, "weight", torch.float32, (width,), device)
     elif n is not None:
         raise ValueError("n without a weight")
-    with torch.cuda.device(device):
-        s = _raw_stream(device) if stream is None else stream
-        check(load().q4rdna_add_norm(ctypes.byref(d), s))
+    d = _lib.ADD_NORM.pack(_dtype(dtype), shape[0], width, scale, eps, 0, r_at, y_at, gate_at, h_at, n_at, r_stride,
+                           y_stride, gate_stride, h_stride, n_stride, post_at, weight_at)
+    s = _raw_stream(device) if stream is None else stream
+    if torch.cuda.current_device() == device:
+        check(load().q4rdna_add_norm(d, s))
+    else:
+        with torch.cuda.device(device):
+            check(load().q4rdna_add_norm(d, s))
     return (residual if h is None else h), n

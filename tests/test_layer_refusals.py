@@ -148,3 +148,6 @@ def test_structures_have_the_header_s_layout():
     assert ctypes.sizeof(_lib.CacheDesc) == 64 and ctypes.sizeof(_lib.BatchDesc) == 48 and ctypes.sizeof(_lib.Rows) == 24
     assert ctypes.sizeof(_lib.AppendDesc) == 152 and ctypes.sizeof(_lib.AttendDesc) == 72
     assert ctypes.sizeof(_lib.AddNormDesc) == 120
+    for packer, structure in ((_lib.ROWS, _lib.Rows), (_lib.APPEND, _lib.AppendDesc), (_lib.ATTEND, _lib.AttendDesc),
+                              (_lib.ADD_NORM, _lib.AddNormDesc)):
+        assert packer.size == ctypes.sizeof(structure)
