@@ -295,20 +295,12 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
 
     // The sequence and the rows of the place: sequence i has the places from
     // cu[i] * group / 128 + i on (attend_many_places).
-    uint32_t seq = 0, base = 0;
-    {
-        auto first_place = [&](uint32_t i) {
-            return static_cast<int64_t>(a.batch.cu_tokens ? a.batch.cu_tokens[i] : static_cast<int>(i)) * a.group / kRowsMany + i;
-        };
-        uint32_t lo = 0, hi = a.batch.sequences;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (first_place(mid) <= static_cast<int64_t>(place)) lo = mid; else hi = mid;
-        }
-        seq = lo;
-        const int64_t f = first_place(lo);
-        base = f < 0 || f > place ? place : static_cast<uint32_t>(f);
-    }
+    auto first_place = [&](uint32_t i) {
+        return static_cast<int64_t>(a.batch.cu_tokens ? a.batch.cu_tokens[i] : static_cast<int>(i)) * a.group / kRowsMany + i;
+    };
+    const uint32_t seq = __builtin_amdgcn_readfirstlane(last_not_past(a.batch.sequences, place, first_place));
+    const int64_t seq_place = first_place(seq);
+    const uint32_t base = seq_place < 0 || seq_place > place ? place : static_cast<uint32_t>(seq_place);
     const Seq s = seq_of(a.batch, a.cache, seq);
     if (!s.ok) {
         if (head == 0 && place == base && blockIdx.y == 0 && tid == 0) count_fault(a.cache);

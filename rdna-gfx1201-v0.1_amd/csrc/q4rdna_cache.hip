@@ -22,13 +22,13 @@ struct Place {
     int pair;     // the first of its four pairs
 };
 
-template <int D>
-__device__ __forceinline__ Place place_of(int lane, uint32_t rotary, bool interleaved) {
+template <bool INTERLEAVED>
+__device__ __forceinline__ Place place_of(int lane, uint32_t rotary) {
     const int half = static_cast<int>(rotary) / 2;
     Place p;
     p.pair = 4 * lane;
     p.turned = p.pair < half;  // rotary is a multiple of 8: a lane's pairs lie on one side
-    if (p.turned && !interleaved) {
+    if (p.turned && !INTERLEAVED) {
         p.a_at = p.pair;
         p.b_at = p.pair + half;
     } else {
@@ -54,46 +54,55 @@ __device__ __forceinline__ void load_turn(Turn &t, const Place &p, const q4rdna_
     load_floats<float, 4>(d.sin + at, true, t.s);
 }
 
-// The norm of a head's row and its rotation, each product and sum rounded by
-// itself (no contraction), as elementary fp32 operations give them.
+// The lane's norm weights, once per workgroup.
+struct Weights {
+    float a[4], b[4];
+};
+__device__ __forceinline__ void load_weights(Weights &w, const float *weight, const Place &p) {
+    if (weight == nullptr) return;
+    load_floats<float, 4>(weight + p.a_at, true, w.a);
+    load_floats<float, 4>(weight + p.b_at, true, w.b);
+}
 template <int D>
-__device__ __forceinline__ void norm_row(Row &r, const Place &p, const float *weight, float eps) {
+__device__ __forceinline__ void norm_row(Row &r, const Weights &w, float eps) {
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum += r.a[e] * r.a[e] + r.b[e] * r.b[e];
-    sum = lanes_sum<D / 8>(sum);
-    const float inv = 1.0f / sqrtf(sum * (1.0f / D) + eps);
-    float wa[4], wb[4];
-    load_floats<float, 4>(weight + p.a_at, true, wa);
-    load_floats<float, 4>(weight + p.b_at, true, wb);
+    const float inv = __builtin_amdgcn_rsqf(lanes_sum<D / 8>(sum) * (1.0f / D) + eps);  // to 1 ulp
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        r.a[e] = r.a[e] * inv * wa[e];
-        r.b[e] = r.b[e] * inv * wb[e];
+        r.a[e] = r.a[e] * inv * w.a[e];
+        r.b[e] = r.b[e] * inv * w.b[e];
     }
 }
-// (By value throughout: references that differ between the two orders of pairs
-// would put the rows into scratch memory.)
-__device__ __forceinline__ f32x2 turn_pair(float a, float b, float c, float s) {
-#pragma clang fp contract(off)
-    return f32x2{a * c - b * s, b * c + a * s};
+__device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s) {
+    const float x = a * c - b * s;
+    b = b * c + a * s;
+    a = x;
 }
-__device__ __forceinline__ void turn_row(Row &r, const Place &p, const Turn &t, bool interleaved) {
+template <bool INTERLEAVED>
+__device__ __forceinline__ void turn_row(Row &r, const Place &p, const Turn &t) {
     if (!p.turned) return;
-    // Pair i is (first[i], second[i]).
-    const float first[4] = {r.a[0], interleaved ? r.a[2] : r.a[1], interleaved ? r.b[0] : r.a[2], interleaved ? r.b[2] : r.a[3]};
-    const float second[4] = {interleaved ? r.a[1] : r.b[0], interleaved ? r.a[3] : r.b[1], interleaved ? r.b[1] : r.b[2], r.b[3]};
-    f32x2 x[4];
+    if (INTERLEAVED) {
+        turn_pair(r.a[0], r.a[1], t.c[0], t.s[0]);
+        turn_pair(r.a[2], r.a[3], t.c[1], t.s[1]);
+        turn_pair(r.b[0], r.b[1], t.c[2], t.s[2]);
+        turn_pair(r.b[2], r.b[3], t.c[3], t.s[3]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = turn_pair(first[i], second[i], t.c[i], t.s[i]);
-    r.a[0] = x[0][0];
-    r.a[1] = interleaved ? x[0][1] : x[1][0];
-    r.a[2] = interleaved ? x[1][0] : x[2][0];
-    r.a[3] = interleaved ? x[1][1] : x[3][0];
-    r.b[0] = interleaved ? x[2][0] : x[0][1];
-    r.b[1] = interleaved ? x[2][1] : x[1][1];
-    r.b[2] = interleaved ? x[3][0] : x[2][1];
-    r.b[3] = x[3][1];
+        for (int e = 0; e < 4; ++e) turn_pair(r.a[e], r.b[e], t.c[e], t.s[e]);
+    }
+}
+
+// x * f rounded to the nearest integer, as the low bits of a float's: the sum
+// with 1.5 * 2^23 has a last place of one.  For |x * f| < 2^22; a NaN gives 0
+// in its low bits.
+__device__ __forceinline__ uint32_t rounded(float x, float f) { return __float_as_uint(fmaf(x, f, 12582912.0f)); }
+// The low halves of four of them.
+__device__ __forceinline__ s16x4 pack_codes(const float (&x)[4], float f) {
+    const uint32_t w[2] = {__builtin_amdgcn_perm(rounded(x[1], f), rounded(x[0], f), 0x05040100u),
+                           __builtin_amdgcn_perm(rounded(x[3], f), rounded(x[2], f), 0x05040100u)};
+    return __builtin_bit_cast(s16x4, w);
 }
 
 // The low bytes of four values, packed.
@@ -112,22 +121,8 @@ __device__ __forceinline__ void transpose4(const uint32_t (&t)[4], uint32_t (&n)
     n[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-// Two planes of 16 codes from 16 shorts: low bytes as signed numbers, and what
-// is left.
-__device__ __forceinline__ void split16(const short (&v)[16], i32x4 &high, i32x4 &low) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        uint32_t h = 0, l = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int x = v[4 * w + e];
-            l |= (static_cast<uint32_t>(x) & 255u) << (8 * e);
-            h |= (static_cast<uint32_t>((x + 128) >> 8) & 255u) << (8 * e);
-        }
-        high[w] = static_cast<int>(h);
-        low[w] = static_cast<int>(l);
-    }
-}
+// A 16-bit code as 256 * high + low, low a signed byte.
+__device__ __forceinline__ int high_of(int v) { return (v + 128) >> 8; }
 __device__ __forceinline__ short join16(i32x4 high, i32x4 low, int e) {
     const int h = static_cast<int8_t>(static_cast<uint32_t>(high[e / 4]) >> (8 * (e % 4)));
     const int l = static_cast<int8_t>(static_cast<uint32_t>(low[e / 4]) >> (8 * (e % 4)));
@@ -162,7 +157,7 @@ struct AppendStage {
 
 // One (sequence, block, kv head): the step's tokens in the block to 16-bit codes
 // in LDS, then the open planes, and the page where the block is full.
-template <int D, typename T>
+template <int D, bool INTERLEAVED, typename T>
 __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint32_t head, int block, AppendStage<D> &st) {
     constexpr int kLanes = D / 8, kRows = 256 / kLanes, kPieces = kKvBlock * D / 16;
     const uint32_t heads = a.cache.kv_heads;
@@ -177,7 +172,8 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
     // kEach of them in flight.
     constexpr int kEach = 4;
     const int lane = tid % kLanes;
-    const bool interleaved = a.d.interleaved != 0;
+    Weights weights;
+    load_weights(weights, a.d.k_norm, place_of<INTERLEAVED>(lane, a.d.rotary));
     for (int row0 = tid / kLanes; row0 < 2 * fresh; row0 += kEach * kRows) {
         Row r[kEach];
         Turn turn[kEach];
@@ -191,7 +187,7 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 const void *data = is_v ? a.d.v.data : a.d.k.data;
                 const int64_t token_stride = is_v ? a.d.v.token_stride : a.d.k.token_stride;
                 const int64_t head_stride = is_v ? a.d.v.head_stride : a.d.k.head_stride;
-                const Place at = place_of<D>(lane, is_v ? 0 : a.d.rotary, interleaved);
+                const Place at = place_of<INTERLEAVED>(lane, is_v ? 0 : a.d.rotary);
                 load_row(r[x], static_cast<const T *>(data) + n * token_stride + head * head_stride, at,
                          a.wide != 0);
                 load_turn(turn[x], at, a.d, start + t);
@@ -203,9 +199,9 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
             if (row < 2 * fresh) {
                 const bool is_v = row >= fresh;
                 const int t = from + (is_v ? row - fresh : row);
-                const Place at = place_of<D>(lane, is_v ? 0 : a.d.rotary, interleaved);
-                if (!is_v && a.d.k_norm != nullptr) norm_row<D>(r[x], at, a.d.k_norm, a.d.eps);
-                turn_row(r[x], at, turn[x], interleaved);
+                const Place at = place_of<INTERLEAVED>(lane, is_v ? 0 : a.d.rotary);
+                if (!is_v && a.d.k_norm != nullptr) norm_row<D>(r[x], weights, a.d.eps);
+                turn_row<INTERLEAVED>(r[x], at, turn[x]);
                 // The largest magnitude by its bits: infinities and NaN come out on top.
                 uint32_t top = 0;
 #pragma unroll
@@ -214,17 +210,12 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 top = lanes_max<kLanes>(top);
                 const float largest = __uint_as_float(top);
                 const bool finite = top < 0x7f800000u, some = finite && largest >= kKvZero;
-                const float inv = some ? kKvCode16 / largest : 0.0f;
-                s16x4 ca, cb;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    ca[e] = some ? static_cast<short>(static_cast<int>(rintf(r[x].a[e] * inv))) : 0;
-                    cb[e] = some ? static_cast<short>(static_cast<int>(rintf(r[x].b[e] * inv))) : 0;
-                }
+                // Codes by a reciprocal of 1 ulp: they move by under 0.01 of a step.
+                const float inv = some ? kKvCode16 * __builtin_amdgcn_rcpf(largest) : 0.0f;
                 short *out = &st.code[is_v][t * kRow<D>];
-                *reinterpret_cast<s16x4 *>(out + at.a_at) = ca;
-                *reinterpret_cast<s16x4 *>(out + at.b_at) = cb;
-                if (lane == 0) st.scale[is_v][t] = some ? largest / kKvCode16 : finite ? 0.0f : __builtin_nanf("");
+                *reinterpret_cast<s16x4 *>(out + at.a_at) = pack_codes(r[x].a, inv);
+                *reinterpret_cast<s16x4 *>(out + at.b_at) = pack_codes(r[x].b, inv);
+                if (lane == 0) st.scale[is_v][t] = some ? largest * (1.0f / kKvCode16) : finite ? 0.0f : __builtin_nanf("");
             }
         }
     }
@@ -237,9 +228,12 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
             const int t = k_token<D>(piece);
             if (t < from) {
                 const i32x4 h = load16(planes + 16 * piece), l = load16(planes + kPlane + 16 * piece);
-                short *row = &st.code[0][t * kRow<D> + k_number<D>(piece)];
+                s16x8 *row = reinterpret_cast<s16x8 *>(&st.code[0][t * kRow<D> + k_number<D>(piece)]);
+                s16x8 c[2];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) row[e] = join16(h, l, e);
+                for (int e = 0; e < 16; ++e) c[e / 8][e % 8] = join16(h, l, e);
+                row[0] = c[0];
+                row[1] = c[1];
             }
             if (v_token(piece, 0) < from) {
                 const i32x4 h = load16(planes + 2 * kPlane + 16 * piece), l = load16(planes + 3 * kPlane + 16 * piece);
@@ -257,41 +251,66 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
         if (tid < 128 && tid % 64 >= from && tid % 64 < to) scales[tid] = st.scale[tid / 64][tid % 64];
         for (int x = tid; x < fresh * (D / 16); x += 256) {
             const int t = from + x / (D / 16), number = x % (D / 16) * 16;
-            short v[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = st.code[0][t * kRow<D> + number + e];
+            const s16x8 *row = reinterpret_cast<const s16x8 *>(&st.code[0][t * kRow<D> + number]);
+            const s16x8 c[2] = {row[0], row[1]};
             i32x4 h, l;
-            split16(v, h, l);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const s16x8 v = c[w / 2];
+                const int e = 4 * (w % 2);
+                h[w] = static_cast<int>(pack4(high_of(v[e]), high_of(v[e + 1]), high_of(v[e + 2]), high_of(v[e + 3])));
+                l[w] = static_cast<int>(pack4(v[e], v[e + 1], v[e + 2], v[e + 3]));
+            }
             const int at = 16 * k_piece<D>(t, number);
             store16(planes + at, h);
             store16(planes + kPlane + at, l);
         }
-        if (fresh < 16) {
+        int8_t *v_planes = planes + 2 * kPlane;
+        if (fresh < 16) {  // few tokens: their bytes
             for (int x = tid; x < fresh * D; x += 256) {
                 const int t = from + x / D, number = x % D;
                 const int v = st.code[1][t * kRow<D> + number];
                 const int at = 16 * v_piece(t, number) + v_byte(t);
-                planes[2 * kPlane + at] = static_cast<int8_t>((v + 128) >> 8);
-                planes[3 * kPlane + at] = static_cast<int8_t>(v);
+                v_planes[at] = static_cast<int8_t>(high_of(v));
+                v_planes[kPlane + at] = static_cast<int8_t>(v);
             }
         } else {
-            for (int piece = tid; piece < kPieces; piece += 256) {
-                short v[16];
-                const int number = v_number(piece);
+            // Whole pieces, 16 tokens of each of four numbers.  Tokens before
+            // `from` keep their bytes; what lies behind `to` is never read.
+            for (int x = tid; x < D; x += 256) {
+                const int number = x % (D / 4) * 4, g = x / (D / 4), at = 16 * v_piece(4 * g, number);
+                i32x4 h[4], l[4];
+                if (from > 4 * g) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = st.code[1][v_token(piece, e) * kRow<D> + number];
-                i32x4 h, l;
-                split16(v, h, l);
-                if (v_token(piece, 0) >= from && v_token(piece, 15) < to) {
-                    store16(planes + 2 * kPlane + 16 * piece, h);
-                    store16(planes + 3 * kPlane + 16 * piece, l);
-                } else {
+                    for (int n = 0; n < 4; ++n) {
+                        h[n] = load16(v_planes + at + 16 * n);
+                        l[n] = load16(v_planes + kPlane + at + 16 * n);
+                    }
+                }
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (v_token(piece, e) >= from && v_token(piece, e) < to) {
-                            planes[2 * kPlane + 16 * piece + e] = static_cast<int8_t>((v[e] + 128) >> 8);
-                            planes[3 * kPlane + 16 * piece + e] = static_cast<int8_t>(v[e]);
-                        }
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t ht[4], lt[4], hn[4], ln[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const s16x4 c = *reinterpret_cast<const s16x4 *>(&st.code[1][(16 * w + 4 * g + b) * kRow<D> + number]);
+                        ht[b] = pack4(high_of(c[0]), high_of(c[1]), high_of(c[2]), high_of(c[3]));
+                        lt[b] = pack4(c[0], c[1], c[2], c[3]);
+                    }
+                    transpose4(ht, hn);
+                    transpose4(lt, ln);
+                    const int kept = min(max(from - (16 * w + 4 * g), 0), 4);  // tokens of the word that were there
+                    const uint32_t mask = kept == 4 ? 0xffffffffu : (1u << (8 * kept)) - 1u;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const uint32_t oh = kept ? static_cast<uint32_t>(h[n][w]) : 0, ol = kept ? static_cast<uint32_t>(l[n][w]) : 0;
+                        h[n][w] = static_cast<int>((hn[n] & ~mask) | (oh & mask));
+                        l[n][w] = static_cast<int>((ln[n] & ~mask) | (ol & mask));
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    store16(v_planes + at + 16 * n, h[n]);
+                    store16(v_planes + kPlane + at + 16 * n, l[n]);
                 }
             }
         }
@@ -333,7 +352,7 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 const s16x8 c = row[w / 2];
                 int x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = static_cast<int>(rintf(c[4 * (w % 2) + e] * r));
+                for (int e = 0; e < 4; ++e) x[e] = static_cast<int>(rounded(c[4 * (w % 2) + e], r));
                 k[w] = static_cast<int>(pack4(x[0], x[1], x[2], x[3]));
             }
             store16(tile + 16 * piece, k);
@@ -351,8 +370,8 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                     const int t = 16 * w + 4 * g + b;
                     const s16x4 c = *reinterpret_cast<const s16x4 *>(&st.code[1][t * kRow<D> + number]);
                     const float r = st.ratio[1][t];
-                    by_token[b] = pack4(static_cast<int>(rintf(c[0] * r)), static_cast<int>(rintf(c[1] * r)),
-                                        static_cast<int>(rintf(c[2] * r)), static_cast<int>(rintf(c[3] * r)));
+                    by_token[b] = pack4(static_cast<int>(rounded(c[0], r)), static_cast<int>(rounded(c[1], r)),
+                                        static_cast<int>(rounded(c[2], r)), static_cast<int>(rounded(c[3], r)));
                 }
                 transpose4(by_token, by_number);
 #pragma unroll
@@ -365,7 +384,7 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
 }
 
 // The blocks of one place and kv head.
-template <int D, typename T>
+template <int D, bool INTERLEAVED, typename T>
 __device__ void append_place(const AppendArgs &a, uint32_t unit, AppendStage<D> &st) {
     const uint32_t place = unit / a.cache.kv_heads, head = unit - place * a.cache.kv_heads;
     uint32_t first_place;
@@ -393,35 +412,39 @@ __device__ void append_place(const AppendArgs &a, uint32_t unit, AppendStage<D> 
     if (owner != first) {
         if (block == first) return;
         if (block == owner) {
-            append_block<D, T>(a, s, i, head, first, st);
+            append_block<D, INTERLEAVED, T>(a, s, i, head, first, st);
             __syncthreads();
         }
     }
-    append_block<D, T>(a, s, i, head, block, st);
+    append_block<D, INTERLEAVED, T>(a, s, i, head, block, st);
 }
 
 // a.q_rows rows (token, query head) of q, kEach per group of D / 8 lanes in flight.
-template <int D, typename T>
+template <int D, bool INTERLEAVED, typename T>
 __device__ void turn_q(const AppendArgs &a, uint32_t unit) {
     constexpr int kLanes = D / 8, kRows = 256 / kLanes, kEach = 4;
     const int lane = threadIdx.x % kLanes;
-    const bool interleaved = a.d.interleaved != 0;
-    const Place at = place_of<D>(lane, a.d.rotary, interleaved);
+    const Place at = place_of<INTERLEAVED>(lane, a.d.rotary);
+    Weights weights;
+    load_weights(weights, a.d.q_norm, at);
     const uint32_t heads = a.d.q_heads;
+    // One long division per workgroup, short ones per row.
     const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * heads, row_first = static_cast<uint64_t>(unit) * a.q_rows;
+    const uint32_t n_first = static_cast<uint32_t>(row_first / heads), head_first = static_cast<uint32_t>(row_first % heads);
+    const uint32_t row_count = static_cast<uint32_t>(min(rows - row_first, static_cast<uint64_t>(a.q_rows)));
     // The workgroup's tokens are mostly of one sequence: the first one's.
-    const Seq s0 = seq_of(a.batch, a.cache, token_seq(a.batch, static_cast<uint32_t>(row_first / heads)));
-    for (uint32_t x0 = threadIdx.x / kLanes; x0 < a.q_rows; x0 += kEach * kRows) {
+    const Seq s0 = seq_of(a.batch, a.cache, wave_token_seq(a.batch, n_first));
+    for (uint32_t x0 = threadIdx.x / kLanes; x0 < row_count; x0 += kEach * kRows) {
         Row r[kEach];
         Turn turn[kEach];
         uint32_t n[kEach], head[kEach];
         bool live[kEach];
 #pragma unroll
         for (int x = 0; x < kEach; ++x) {
-            const uint64_t row = row_first + x0 + x * kRows;
-            live[x] = x0 + x * kRows < a.q_rows && row < rows;
-            n[x] = live[x] ? static_cast<uint32_t>(row / heads) : 0;
-            head[x] = live[x] ? static_cast<uint32_t>(row - static_cast<uint64_t>(n[x]) * heads) : 0;
+            live[x] = x0 + x * kRows < row_count;
+            const uint32_t local = head_first + (live[x] ? x0 + x * kRows : 0), token = div_split(local, heads, a.heads_magic);
+            n[x] = n_first + token;
+            head[x] = local - token * heads;
             if (live[x])
                 load_row(r[x], static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(n[x]) * a.d.q.token_stride +
                                    head[x] * a.d.q.head_stride, at, a.wide != 0);
@@ -440,8 +463,8 @@ __device__ void turn_q(const AppendArgs &a, uint32_t unit) {
 #pragma unroll
         for (int x = 0; x < kEach; ++x) {
             if (!live[x]) continue;
-            if (a.d.q_norm != nullptr) norm_row<D>(r[x], at, a.d.q_norm, a.d.eps);
-            turn_row(r[x], at, turn[x], interleaved);
+            if (a.d.q_norm != nullptr) norm_row<D>(r[x], weights, a.d.eps);
+            turn_row<INTERLEAVED>(r[x], at, turn[x]);
             T *out = static_cast<T *>(a.d.q_out.data) + static_cast<int64_t>(n[x]) * a.d.q_out.token_stride +
                      head[x] * a.d.q_out.head_stride;
             store_floats<T, 4>(out + at.a_at, a.wide != 0, r[x].a);
@@ -450,13 +473,17 @@ __device__ void turn_q(const AppendArgs &a, uint32_t unit) {
     }
 }
 
-template <int D, typename T>
+template <int D, bool INTERLEAVED, typename T>
 __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
     __shared__ AppendStage<D> stage;
-    if (blockIdx.x < a.kv_units)
-        append_place<D, T>(a, blockIdx.x, stage);
+    // The blocks' workgroups, which wait a lot, spread evenly among q's, which
+    // move the most bytes.
+    const uint64_t b = blockIdx.x;
+    const uint32_t before = static_cast<uint32_t>(b * a.kv_units / gridDim.x);
+    if (static_cast<uint32_t>((b + 1) * a.kv_units / gridDim.x) != before)
+        append_place<D, INTERLEAVED, T>(a, before, stage);
     else
-        turn_q<D, T>(a, blockIdx.x - a.kv_units);
+        turn_q<D, INTERLEAVED, T>(a, blockIdx.x - before);
 }
 
 // Byte e of a word as a signed number.
@@ -553,13 +580,19 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
 
 }  // namespace
 
+template <bool INTERLEAVED, typename T>
+static void launch_append_as(const AppendArgs &a, hipStream_t stream) {
+    auto go = [&](auto kernel) { kernel<<<a.kv_units + a.q_units, 256, 0, stream>>>(a); };
+    a.cache.head_dim == 64 ? go(append_kernel<64, INTERLEAVED, T>) : go(append_kernel<128, INTERLEAVED, T>);
+}
+template <typename T>
+static void launch_append_as(const AppendArgs &a, hipStream_t stream) {
+    a.d.interleaved != 0 ? launch_append_as<true, T>(a, stream) : launch_append_as<false, T>(a, stream);
+}
 hipError_t launch_append(const AppendArgs &a, hipStream_t stream) {
-    const uint32_t grid = a.kv_units + a.q_units;
-    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(a); };
-    if (a.cache.head_dim == 64)
-        a.d.dtype == Q4RDNA_F32 ? go(append_kernel<64, float>) : a.d.dtype == Q4RDNA_F16 ? go(append_kernel<64, _Float16>) : go(append_kernel<64, __bf16>);
-    else
-        a.d.dtype == Q4RDNA_F32 ? go(append_kernel<128, float>) : a.d.dtype == Q4RDNA_F16 ? go(append_kernel<128, _Float16>) : go(append_kernel<128, __bf16>);
+    if (a.d.dtype == Q4RDNA_F32) launch_append_as<float>(a, stream);
+    else if (a.d.dtype == Q4RDNA_F16) launch_append_as<_Float16>(a, stream);
+    else launch_append_as<__bf16>(a, stream);
     return hipGetLastError();
 }
 

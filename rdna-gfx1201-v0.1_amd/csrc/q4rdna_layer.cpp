@@ -99,7 +99,7 @@ int check_dtype(uint32_t dtype) {
 }
 
 int check_heads(uint32_t q_heads, uint32_t kv_heads) {
-    if (q_heads == 0 || q_heads % kv_heads != 0 || q_heads > 65536)
+    if (q_heads == 0 || q_heads % kv_heads != 0 || q_heads > 32768)
         return set_error(Q4RDNA_ERR_ARGUMENT, "%u query heads over %u kv heads", q_heads, kv_heads);
     return Q4RDNA_OK;
 }
@@ -207,6 +207,7 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     a.kv_units = static_cast<uint32_t>(kv_units);
     a.q_units = static_cast<uint32_t>(q_units);
     a.q_rows = q_rows;
+    a.heads_magic = desc->q_heads > 1 ? static_cast<uint32_t>(((1ull << 32) + desc->q_heads - 1) / desc->q_heads) : 0;
     a.wide = wide_rows(desc->k, desc->dtype, 4) && wide_rows(desc->v, desc->dtype, 4) &&
              (desc->q_heads == 0 || (wide_rows(desc->q, desc->dtype, 4) && wide_rows(desc->q_out, desc->dtype, 4)));
     return launched(q4rdna::launch_append(a, static_cast<hipStream_t>(stream)), "kv_append");

@@ -26,6 +26,7 @@ struct AppendArgs {
     uint32_t kv_units;  // (sequence, block) places times kv heads
     uint32_t q_units;   // workgroups that rotate q
     uint32_t q_rows;    // rows (token, query head) that each of them takes
+    uint32_t heads_magic;  // div_split's for q_heads
     uint32_t wide;      // rows of k, v, q, q_out can be read four elements at a time
 };
 hipError_t launch_append(const AppendArgs &a, hipStream_t stream);

@@ -128,27 +128,44 @@ __device__ __forceinline__ Seq seq_of(const q4rdna_kv_batch &b, const q4rdna_kv_
     return s;
 }
 
+// The last i in [0, n) with key(i) <= x, for ascending keys (0 if none): 64
+// keys a trip, a lane each.
+template <typename F>
+__device__ __forceinline__ uint32_t last_not_past(uint32_t n, int64_t x, F key) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0;
+    for (uint32_t step = n > 4096 ? 4096 : n > 64 ? 64 : 1;; step >>= 6) {
+        // lanes look at lo, lo + step, ...; the last that fits is the next lo
+        const uint32_t i = lo + lane * step;
+        const uint64_t fits = __builtin_amdgcn_ballot_w64(i < n && key(i) <= x);
+        // ascending keys give a run of ones; anything else still gives an index in range
+        lo += fits == 0 ? 0 : (63 - __builtin_clzll(fits)) * step;
+        if (step == 1) return lo;
+    }
+}
+
 // The sequence that owns `place` (kv_places): the last one whose first place
-// is not past it.
+// is not past it.  To be called by whole waves.
 __device__ __forceinline__ uint32_t place_seq(const q4rdna_kv_batch &b, uint32_t place, uint32_t *first_place) {
     if (b.cu_tokens == nullptr) {
         *first_place = place;
         return place;
     }
-    uint32_t lo = 0, hi = b.sequences;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (static_cast<int64_t>(b.cu_tokens[mid]) / kKvBlock + 2ll * mid <= static_cast<int64_t>(place))
-            lo = mid;
-        else
-            hi = mid;
-    }
-    const int64_t base = static_cast<int64_t>(b.cu_tokens[lo]) / kKvBlock + 2ll * lo;
+    auto key = [&](uint32_t i) { return static_cast<int64_t>(b.cu_tokens[i]) / kKvBlock + 2ll * i; };
+    const uint32_t i = __builtin_amdgcn_readfirstlane(last_not_past(b.sequences, place, key));
+    const int64_t base = key(i);
     *first_place = base < 0 || base > place ? place : static_cast<uint32_t>(base);
-    return lo;
+    return i;
 }
 
-// The sequence of token n of the step: the last one that starts at or before it.
+// The sequence of token n of the step: the last one that starts at or before
+// it.  To be called by whole waves, n the same in all lanes.
+__device__ __forceinline__ uint32_t wave_token_seq(const q4rdna_kv_batch &b, uint32_t n) {
+    if (b.cu_tokens == nullptr) return n;
+    return __builtin_amdgcn_readfirstlane(
+        last_not_past(b.sequences, n, [&](uint32_t i) { return static_cast<int64_t>(b.cu_tokens[i]); }));
+}
+// The same for each lane by itself.
 __device__ __forceinline__ uint32_t token_seq(const q4rdna_kv_batch &b, uint32_t n) {
     if (b.cu_tokens == nullptr) return n;
     uint32_t lo = 0, hi = b.sequences;
