@@ -48,10 +48,6 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v;
 }
 
-// Keeps the scheduler from moving instructions across: it would issue the
-// loads or products of many tiles ahead and run out of registers.
-__device__ __forceinline__ void tile_end() { __builtin_amdgcn_sched_barrier(0); }
-
 // Element `digit` (the lane's place in its quad) of the quad's sum of v.
 __device__ __forceinline__ float quad_sum_pick(f32x4 v, int digit) {
     const bool b0 = digit & 1, b1 = digit & 2;

@@ -107,11 +107,20 @@ struct ManyState {
     f32x16 o[D / 32];
 };
 
+// Bits of the tokens 8 x + b (bit 4 x + b, b < 4) that are at most `ahead`.
+__device__ __forceinline__ uint32_t first_tokens(int ahead) {
+    const int count = ahead < 0 ? 0 : ahead >= 63 ? 32 : ahead / 8 * 4 + min(ahead % 8 + 1, 4);
+    return count == 32 ? 0xffffffffu : (1u << count) - 1u;
+}
+__device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) {
+    return static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - i)) >> 31);
+}
+
 // One block from LDS.  OPEN: two tiles (256 * high, low), scales per token
 // (kt, vt); otherwise k_scale and v_scale.
-template <bool OPEN, bool MASKED, int D, int SPLIT>
+template <bool OPEN, int D, int SPLIT>
 __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTile<D> *tile, float k_scale, float v_scale,
-                                           const float *token_scales, int start, uint32_t window) {
+                                           const float *token_scales, int start, int length, uint32_t window, bool masked) {
     const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
     f32x16 s[2];
 #pragma unroll
@@ -129,34 +138,31 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
                 for (int x = 0; x < SPLIT; ++x) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, st.q[x][k], s[t], 0, 0, 0);
             }
         }
+        tile_end();
     }
-    float ratio[8][4];  // OPEN: V's token scales
     if (OPEN) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             const f32x4 kt = *(gptr_f32x4)(uintptr_t)(token_scales + 8 * x + 4 * half);
-            const f32x4 vt = *(gptr_f32x4)(uintptr_t)(token_scales + kKvBlock + 8 * x + 4 * half);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                s[x / 4][4 * (x % 4) + b] *= kt[b];
-                ratio[x][b] = vt[b];
-            }
+            for (int b = 0; b < 4; ++b) s[x / 4][4 * (x % 4) + b] *= kt[b];
         }
     }
     // Token of s[t][i]: 32 t + 8 (i / 4) + 4 half + i % 4.
-    uint32_t hidden = 0;
-    if (MASKED) {
+    // Of the lane's 32 tokens in this order, 8 x + b from start + 4 half on, the
+    // first few are at or before a position: bit masks, a word for each score
+    // (bit operations only; compares would take a pair of scalar registers each).
+    uint32_t seen = 0xffffffffu;
+    if (masked) {
+        const int ahead = st.position - start - 4 * half;
+        seen = first_tokens(ahead);
+        if (window != 0) seen &= ~first_tokens(static_cast<int>(max(static_cast<int64_t>(ahead) - window, static_cast<int64_t>(-1))));
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int token = start + 32 * t + 8 * (i / 4) + 4 * half + i % 4;
-                const bool seen = token <= st.position &&
-                                  (window == 0 || static_cast<uint32_t>(st.position - token) < window);
-                if (!seen) {
-                    hidden |= 1u << (16 * t + i);
-                    s[t][i] = kNegInf;
-                }
+                const uint32_t m = bit_mask(seen, 16 * t + i);
+                s[t][i] = __uint_as_float((__float_as_uint(s[t][i]) & m) | (__float_as_uint(kNegInf) & ~m));
             }
     }
     const float f = OPEN ? st.q_scale : st.q_scale * k_scale;
@@ -166,27 +172,22 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
     top = max_xor32(top);
-    const bool none = MASKED && top == kNegInf;
+    const bool none = top == kNegInf;
     const float now = none ? kNegInf : top * f;
 
     // V's scale relative to the largest one so far; one that is not finite
     // makes the seen weights NaN and leaves the reference alone.
-    float v_ref = st.v_ref;
-    if (OPEN) {
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const bool seen = !(hidden >> (4 * x + b) & 1u);
-                if (seen && ratio[x][b] < __builtin_inff()) v_ref = fmaxf(v_ref, ratio[x][b]);
-            }
-        // One reference for the whole wave: it belongs to every row's accumulators.
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) v_ref = fmaxf(v_ref, __shfl_xor(v_ref, d));
-        v_ref = max_xor32(v_ref);
-    } else if (v_scale < __builtin_inff()) {
-        v_ref = fmaxf(v_ref, v_scale);
+    float largest = v_scale;
+    if (OPEN) {  // of the block's tokens, one per lane
+        const float mine = token_scales[kKvBlock + lane];
+        largest = start + lane < length && mine < __builtin_inff() ? mine : 0.0f;
+        largest = fmaxf(largest, dpp<kDppXor1>(largest));
+        largest = fmaxf(largest, dpp<kDppXor2>(largest));
+        largest = fmaxf(largest, dpp<kDppMirror8>(largest));
+        largest = fmaxf(largest, dpp<kDppMirror16>(largest));
+        largest = max_xor32(max_xor16(largest));
     }
+    const float v_ref = largest < __builtin_inff() ? fmaxf(st.v_ref, largest) : st.v_ref;
     const bool grown = now > st.m + kLazy || (st.m == kNegInf && now != kNegInf);
     if (__builtin_amdgcn_ballot_w64(grown || v_ref != st.v_ref) != 0) {
         const float m = grown ? now : st.m;
@@ -201,23 +202,36 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
     const float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m);
     const float to_ref = v_ref > 0.0f ? 1.0f / v_ref : 0.0f;
     const float r = OPEN ? 0.0f : v_scale < __builtin_inff() ? v_scale * to_ref : __builtin_nanf("");
-    float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const bool seen = !MASKED || !(hidden >> (16 * t + i) & 1u);
-            float p = __builtin_amdgcn_exp2f(fmaf(s[t][i], f, shift));
-            p = seen ? p : 0.0f;
-            sum += p;
-            float w = r;
-            if (OPEN) {
-                const float vt = ratio[4 * t + i / 4][i % 4];
-                w = vt < __builtin_inff() ? vt * to_ref : __builtin_nanf("");
-            }
-            s[t][i] = seen ? p * w : 0.0f;
+        for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], f, shift));
+    auto hide = [&] {  // whatever f and the scales are
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = __uint_as_float(__float_as_uint(s[t][i]) & bit_mask(seen, 16 * t + i));
+    };
+    if (masked) hide();
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        f32x4 w = {r, r, r, r};
+        if (OPEN) {
+            const f32x4 vt = *(gptr_f32x4)(uintptr_t)(token_scales + kKvBlock + 8 * x + 4 * half);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) w[b] = vt[b] < __builtin_inff() ? vt[b] * to_ref : __builtin_nanf("");
         }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int i = 4 * (x % 4) + b;
+            sum += s[x / 4][i];
+            s[x / 4][i] *= w[b];
+        }
+    }
+    if (masked) hide();
     st.l += sum;
+    tile_end();
     // Products 2 parity + pair: tokens 16 a + 8 parity + 4 half + b, a = 2 pair, 2 pair + 1.
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -241,6 +255,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
                 for (int y = 0; y < SPLIT; ++y) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, p[y], st.o[d], 0, 0, 0);
             }
         }
+        tile_end();
     }
 }
 
@@ -363,10 +378,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         if (!away) {
             const bool masked = start + block_size - 1 > wave_first ||
                                 (a.d.window != 0 && static_cast<uint32_t>(wave_last - start) >= a.d.window);
-            if (masked)
-                many_block<false, true, D, SPLIT>(st, &tiles[buffer], scale[0], scale[1], nullptr, start, a.d.window);
-            else
-                many_block<false, false, D, SPLIT>(st, &tiles[buffer], scale[0], scale[1], nullptr, start, a.d.window);
+            many_block<false, D, SPLIT>(st, &tiles[buffer], scale[0], scale[1], nullptr, start, s.length, a.d.window, masked);
         }
         if (b + 1 < to_full) stage_raw<false, D>(tiles[buffer ^ 1], raw);
         __syncthreads();
@@ -380,8 +392,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         __syncthreads();
         const int start = (to - 1) * block_size;
         if (start <= wave_last)
-            many_block<true, true, D, SPLIT>(st, tiles, 0.0f, 0.0f,
-                                             a.cache.open_scales + open_scale_row(a.cache, s.slot, to - 1, head), start, a.d.window);
+            many_block<true, D, SPLIT>(st, tiles, 0.0f, 0.0f,
+                                       a.cache.open_scales + open_scale_row(a.cache, s.slot, to - 1, head), start, s.length,
+                                       a.d.window, true);
     }
 
     // The row's sum over both halves; results in units of one.

@@ -93,6 +93,10 @@ __device__ __forceinline__ float max_xor32(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// Keeps the scheduler from moving instructions across: it would issue the
+// loads or products of many tiles ahead and run out of registers.
+__device__ __forceinline__ void tile_end() { __builtin_amdgcn_sched_barrier(0); }
+
 // Two floats at once, device scope (see load_agent).
 __device__ __forceinline__ f32x2 load_agent2(const float *p) {
     typedef __attribute__((address_space(1))) const uint64_t *gptr_cu64;
