@@ -435,19 +435,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_few_kernel(const AttendA
     int pages = 0;
     FewTiles<D> tiles;
     f32x2 scale;
+    bool bad = false;
     const int8_t *tile = nullptr;
     auto next_tile = [&](int n) {
         if (n % 64 == 0 && n != 0) pages = table[min(from + wave + WAVES * (n + lane), to - 1)];
         int page = __builtin_amdgcn_readlane(pages, n % 64);
-        float bad = 0.0f;
-        if (static_cast<uint32_t>(page) >= a.cache.page_count) {
+        bad = static_cast<uint32_t>(page) >= a.cache.page_count;
+        if (bad) {
             if (lane == 0) count_fault(a.cache);
             page = 0;
-            bad = __builtin_nanf("");
         }
         tile = a.cache.pages + page_tile(a.cache, page, head);
         scale = *(gptr_f32x2)(uintptr_t)(a.cache.scales + (static_cast<size_t>(page) * a.cache.kv_heads + head) * 2);
-        scale += bad;
     };
     // q's loads go out with the table's and come back before the tiles.
     FewState<D, QT> st;
@@ -472,7 +471,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_few_kernel(const AttendA
         const int start = (from + wave + WAVES * n) * static_cast<int>(kKvBlock);
         const bool masked = start + static_cast<int>(kKvBlock) - 1 > first_position ||
                             (a.d.window != 0 && static_cast<uint32_t>(last_position - start) >= a.d.window);
-        const float k_scale = scale[0], v_scale = scale[1];
+        const float k_scale = bad ? __builtin_nanf("") : scale[0], v_scale = bad ? __builtin_nanf("") : scale[1];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
             float s4[4][4];

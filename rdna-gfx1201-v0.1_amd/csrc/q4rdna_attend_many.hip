@@ -199,9 +199,14 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         st.m = m;
         st.v_ref = v_ref;
     }
-    const float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m);
     const float to_ref = v_ref > 0.0f ? 1.0f / v_ref : 0.0f;
-    const float r = OPEN ? 0.0f : v_scale < __builtin_inff() ? v_scale * to_ref : __builtin_nanf("");
+    float r = OPEN ? 0.0f : v_scale < __builtin_inff() ? v_scale * to_ref : __builtin_nanf("");
+    float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m), per_r = 1.0f;
+    const bool folded = !OPEN && r > 0x1p-20f;
+    if (folded) {
+        shift += __builtin_amdgcn_logf(r);
+        per_r = 1.0f / r;
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -226,11 +231,18 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         for (int b = 0; b < 4; ++b) {
             const int i = 4 * (x % 4) + b;
             sum += s[x / 4][i];
-            s[x / 4][i] *= w[b];
+            if (OPEN) s[x / 4][i] *= w[b];
         }
     }
-    if (masked) hide();
-    st.l += sum;
+    if (!OPEN && !folded) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] *= r;
+        if (masked) hide();
+    }
+    if (OPEN) hide();
+    st.l += sum * per_r;
     tile_end();
     // Products 2 parity + pair: tokens 16 a + 8 parity + 4 half + b, a = 2 pair, 2 pair + 1.
 #pragma unroll
@@ -349,20 +361,23 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
 
     const int32_t *table = a.batch.table + static_cast<size_t>(seq) * a.batch.table_width;
     constexpr size_t kPlane = kKvBlock * D;
+    // Lane x keeps the page of the x-th of the next 64 blocks, so no load waits
+    // for another one inside the loop.
     Raw<D> raw;
     f32x2 scale_next;
+    bool bad_next;
+    int pages = 0;
     auto load = [&](int b) {
-        int page = __builtin_amdgcn_readfirstlane(table[b]);
-        float bad = 0.0f;
-        if (static_cast<uint32_t>(page) >= a.cache.page_count) {
+        if ((b - from) % 64 == 0) pages = table[min(b + lane, to - 1)];
+        int page = __builtin_amdgcn_readlane(pages, (b - from) % 64);
+        bad_next = static_cast<uint32_t>(page) >= a.cache.page_count;
+        if (bad_next) {
             if (tid == 0) count_fault(a.cache);
             page = 0;
-            bad = __builtin_nanf("");
         }
         const int8_t *t = a.cache.pages + page_tile(a.cache, page, head);
-        load_raw<D>(raw, t, t + kPlane);
         scale_next = *(gptr_f32x2)(uintptr_t)(a.cache.scales + (static_cast<size_t>(page) * heads + head) * 2);
-        scale_next += bad;
+        load_raw<D>(raw, t, t + kPlane);
     };
     if (from < to_full) {
         load(from);
@@ -371,7 +386,8 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     __syncthreads();
     for (int b = from; b < to_full; ++b) {
         const int buffer = (b - from) & 1, start = b * block_size;
-        const f32x2 scale = scale_next;
+        f32x2 scale = scale_next;
+        if (bad_next) scale[0] = scale[1] = __builtin_nanf("");
         if (b + 1 < to_full) load(b + 1);
         const bool away = start > wave_last ||
                           (a.d.window != 0 && wave_first - (start + block_size - 1) >= static_cast<int64_t>(a.d.window));
