@@ -343,7 +343,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const int begin = a.d.window != 0 && static_cast<uint32_t>(first_position) >= a.d.window
                           ? first_position - static_cast<int>(a.d.window) + 1 : 0;
     const int block0 = begin / block_size, blocks = (end + block_size - 1) / block_size - block0;
-    const int splits = min(static_cast<int>(a.splits), (blocks + 1) / 2);
+    // A part costs the joining workgroup about as long as a block costs a part:
+    // blocks / splits + splits is least at the root.
+    const int splits = min(static_cast<int>(a.splits), max(1, static_cast<int>(__builtin_amdgcn_sqrtf(static_cast<float>(blocks)))));
     const int split = blockIdx.y;
     if (split >= splits) return;
     const int from = block0 + static_cast<int>(static_cast<int64_t>(split) * blocks / splits);
@@ -419,61 +421,68 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const int token = live ? row / group : 0;
     const uint32_t h = head * a.group + (live ? row - token * group : 0);
     const uint32_t job = place * heads + head;
-    if (splits == 1) {
-        if (!live) return;
-        const float inv = l == 0.0f ? 0.0f : st.v_ref / l;
-        T *out = static_cast<T *>(a.d.out.data) + static_cast<int64_t>(s.first + token) * a.d.out.token_stride + h * a.d.out.head_stride;
+    // Parts lie as [number][row]: a lane's row, so neighbouring lanes side by side.
+    float m_row = st.m, l_row = l, unit = st.v_ref;
+    if (splits > 1) {
+        const size_t jobs = gridDim.x, first_slot = static_cast<size_t>(job) * a.splits;
+        float *stats = a.partials + jobs * a.splits * kRowsMany * D;
+        const int r = 32 * wave + column;
+        float *part = a.partials + (first_slot + split) * kRowsMany * D + r;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                float v[4];
+            for (int i = 0; i < 16; ++i)
+                store_agent(part + (32 * d + 8 * (i / 4) + 4 * half + i % 4) * kRowsMany, st.o[d][i] * st.v_ref);
+        if (half == 0) {
+            store_agent(stats + (first_slot + split) * 2 * kRowsMany + r, st.m);
+            store_agent(stats + (first_slot + split) * 2 * kRowsMany + kRowsMany + r, l);
+        }
+        wait_stores();
+        __syncthreads();
+        if (tid == 0) ticket = add_agent(a.arrived + job, 1u);
+        __syncthreads();
+        if (ticket != static_cast<uint32_t>(splits - 1)) return;
+        if (tid == 0) store_agent(a.arrived + job, 0u);
+        // The last to arrive reads all parts, its own too, in their order: the
+        // result does not depend on which one it was.
+        m_row = kNegInf;
+        for (int i = 0; i < splits; ++i) m_row = fmaxf(m_row, load_agent(stats + (first_slot + i) * 2 * kRowsMany + r));
+        const float ref = m_row == kNegInf ? 0.0f : m_row;
+        l_row = 0.0f;
+        unit = 1.0f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = st.o[d][4 * x + e] * inv;
-                store_floats<T, 4>(out + 32 * d + 8 * x + 4 * half, a.wide_out != 0, v);
-            }
-        if (a.d.lse != nullptr && half == 0)
-            a.d.lse[static_cast<size_t>(s.first + token) * a.d.q_heads + h] = (st.m + log2f(l) - kWeight) * (1.0f / kLog2e);
-        return;
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st.o[d][i] = 0.0f;
+        for (int y = 0; y < splits; ++y) {
+            const float f = __builtin_amdgcn_exp2f(load_agent(stats + (first_slot + y) * 2 * kRowsMany + r) - ref);
+            l_row += load_agent(stats + (first_slot + y) * 2 * kRowsMany + kRowsMany + r) * f;
+            const float *from_part = a.partials + (first_slot + y) * kRowsMany * D + r;
+            float v[D / 32][16];
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[d][i] = load_agent(from_part + (32 * d + 8 * (i / 4) + 4 * half + i % 4) * kRowsMany);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) st.o[d][i] = fmaf(v[d][i], f, st.o[d][i]);
+        }
     }
-    const size_t jobs = gridDim.x;
-    float *stats = a.partials + jobs * a.splits * kRowsMany * D;
-    const size_t slot = (static_cast<size_t>(job) * a.splits + split) * kRowsMany + 32 * wave + column;
+    if (!live) return;
+    const float inv = l_row == 0.0f ? 0.0f : unit / l_row;
+    T *out = static_cast<T *>(a.d.out.data) + static_cast<int64_t>(s.first + token) * a.d.out.token_stride + h * a.d.out.head_stride;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            store_agent(a.partials + slot * D + 32 * d + 8 * (i / 4) + 4 * half + i % 4, st.o[d][i] * st.v_ref);
-    if (half == 0) {
-        store_agent(stats + 2 * slot, st.m);
-        store_agent(stats + 2 * slot + 1, l);
-    }
-    wait_stores();
-    __syncthreads();
-    if (tid == 0) ticket = add_agent(a.arrived + job, 1u);
-    __syncthreads();
-    if (ticket != static_cast<uint32_t>(splits - 1)) return;
-    if (tid == 0) store_agent(a.arrived + job, 0u);
-    const size_t first_slot = static_cast<size_t>(job) * a.splits * kRowsMany;
-    for (int x = tid; x < (last_row - first_row + 1) * D; x += 256) {
-        const int r = x / D, d = x % D;
-        float m = kNegInf;
-        for (int i = 0; i < splits; ++i) m = fmaxf(m, load_agent(stats + 2 * (first_slot + i * kRowsMany + r)));
-        const float ref = m == kNegInf ? 0.0f : m;
-        float sum = 0.0f, o = 0.0f;
-        for (int i = 0; i < splits; ++i) {
-            const size_t at = first_slot + i * kRowsMany + r;
-            const float f = __builtin_amdgcn_exp2f(load_agent(stats + 2 * at) - ref);
-            sum += load_agent(stats + 2 * at + 1) * f;
-            o += load_agent(a.partials + at * D + d) * f;
+        for (int x = 0; x < 4; ++x) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = st.o[d][4 * x + e] * inv;
+            store_floats<T, 4>(out + 32 * d + 8 * x + 4 * half, a.wide_out != 0, v);
         }
-        const int tk = (first_row + r) / group;
-        const uint32_t hh = head * a.group + (first_row + r - tk * group);
-        static_cast<T *>(a.d.out.data)[static_cast<int64_t>(s.first + tk) * a.d.out.token_stride + hh * a.d.out.head_stride + d] =
-            static_cast<T>(sum == 0.0f ? 0.0f : o / sum);
-        if (d == 0 && a.d.lse != nullptr)
-            a.d.lse[static_cast<size_t>(s.first + tk) * a.d.q_heads + hh] = (m + log2f(sum) - kWeight) * (1.0f / kLog2e);
-    }
+    if (a.d.lse != nullptr && half == 0)
+        a.d.lse[static_cast<size_t>(s.first + token) * a.d.q_heads + h] = (m_row + log2f(l_row) - kWeight) * (1.0f / kLog2e);
 }
 
 }  // namespace
