@@ -92,16 +92,40 @@ __device__ __forceinline__ i32x4 few_scores(const FewState<D, QT> &st, const i32
     return c;
 }
 
-// Whether the lane's row at `position` sees token t.
-__device__ __forceinline__ bool sees(int position, int t, uint32_t window) {
-    return t <= position && (window == 0 || static_cast<uint32_t>(position - t) < window);
+// Bits 4 t + i of the tokens 16 t + i (t, i < 4) that are at most `ahead`.
+__device__ __forceinline__ uint32_t first_tokens(int ahead) {
+    const int count = ahead < 0 ? 0 : ahead >= 51 ? 16 : ahead / 16 * 4 + min(ahead % 16 + 1, 4);
+    return (1u << count) - 1u;
+}
+// The lane's tokens of the block from `start` on that its row sees: bit 4 t + i
+// is token start + 16 t + 4 group + i.
+__device__ __forceinline__ uint32_t seen_tokens(int position, int start, uint32_t window) {
+    const int ahead = position - start - 4 * ((static_cast<int>(threadIdx.x) & 63) >> 4);
+    uint32_t seen = first_tokens(ahead);
+    if (window != 0) seen &= ~first_tokens(static_cast<int>(max(static_cast<int64_t>(ahead) - window, static_cast<int64_t>(-1))));
+    return seen;
+}
+// All ones where bit i is set.
+__device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) {
+    return static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - i)) >> 31);
+}
+// -inf where a bit is clear; bit operations, since compares would each hold a
+// pair of scalar registers.
+__device__ __forceinline__ void hide(float (&s)[4][4], uint32_t seen) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t m = bit_mask(seen, 4 * t + i);
+            s[t][i] = __uint_as_float((__float_as_uint(s[t][i]) & m) | (__float_as_uint(kNegInf) & ~m));
+        }
 }
 
 // The softmax of a block: s holds the lane's base-2 scores (-inf where hidden),
 // on return p * 2^30 relative to the block's maximum.  Updates the running
 // maximum and sum and rescales o; returns the block's factor relative to the
 // new maximum (with the 2^-30), zero where the row sees nothing of the block.
-template <int DT>
+template <int QT, int DT>
 __device__ __forceinline__ float softmax_block(float (&s)[4][4], float &m, float &l, f32x4 (&o)[DT]) {
     float top = s[0][0];
 #pragma unroll
@@ -124,8 +148,10 @@ __device__ __forceinline__ float softmax_block(float (&s)[4][4], float &m, float
         }
     l = l * alpha + sum * factor;
     m = next;
-    // The maximum seldom moves after the first blocks.
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+    // The maximum seldom moves after the first blocks.  (With two tiles the
+    // branch costs more than the products: the accumulators' copies across it
+    // would not fit the registers.)
+    if (QT > 1 || __builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= alpha;
     }
@@ -153,28 +179,26 @@ __device__ __forceinline__ void few_open_block(FewState<D, QT> &st, const int8_t
                                                uint32_t window) {
     constexpr size_t kPlane = kKvBlock * D;
     const int group = (threadIdx.x & 63) >> 4;
-    i32x4 high[D / 16], low[D / 16];
-    load_tiles<D>(high, planes);
-    load_tiles<D>(low, planes + kPlane);
-    float s[QT][4][4];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt)
+    for (int qt = 0; qt < QT; ++qt) {
+        i32x4 high[D / 16], low[D / 16];
+        load_tiles<D>(high, planes);
+        load_tiles<D>(low, planes + kPlane);
+        const uint32_t seen = seen_tokens(st.position[qt], start, window);
+        const float unit = st.weight * st.q_scale[qt];
+        float s[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const f32x4 ks = *(gptr_f32x4)(uintptr_t)(scales + 16 * t + 4 * group);
             const i32x4 h = few_scores(st, high, qt, t), l = few_scores(st, low, qt, t);
-            const float w = st.weight * st.q_scale[qt];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float c = fmaf(static_cast<float>(h[i]), 256.0f, static_cast<float>(l[i]));
-                s[qt][t][i] = sees(st.position[qt], start + 16 * t + 4 * group + i, window) ? quad_sum(c * w) * ks[i] : kNegInf;
-            }
+            for (int i = 0; i < 4; ++i)
+                s[t][i] = quad_sum(fmaf(static_cast<float>(h[i]), 256.0f, static_cast<float>(l[i])) * unit) * ks[i];
         }
-    tile_end();
-    load_tiles<D>(high, planes + 2 * kPlane);
-    load_tiles<D>(low, planes + 3 * kPlane);
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
+        hide(s, seen);
+        tile_end();
+        load_tiles<D>(high, planes + 2 * kPlane);
+        load_tiles<D>(low, planes + 3 * kPlane);
         f32x4 vs[4];
         float v_top = 0.0f, poison = 0.0f;
 #pragma unroll
@@ -182,26 +206,27 @@ __device__ __forceinline__ void few_open_block(FewState<D, QT> &st, const int8_t
             vs[t] = *(gptr_f32x4)(uintptr_t)(scales + 64 + 16 * t + 4 * group);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (!sees(st.position[qt], start + 16 * t + 4 * group + i, window)) vs[t][i] = 0.0f;
+                vs[t][i] = __uint_as_float(__float_as_uint(vs[t][i]) & bit_mask(seen, 4 * t + i));
                 v_top = fmaxf(v_top, vs[t][i]);
                 poison += vs[t][i] - vs[t][i];  // NaN where a seen scale is not finite
             }
         }
         v_top = max_xor32(max_xor16(v_top));
         poison = add_xor32(add_xor16(poison));
-        const float factor = softmax_block(s[qt], st.m[qt], st.l[qt], st.o[qt]);
+        const float factor = softmax_block<QT>(s, st.m[qt], st.l[qt], st.o[qt]);
         const float inv = v_top > 0.0f ? 1.0f / v_top : 0.0f;
         i32x4 p;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             int x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = static_cast<int>(s[qt][t][i] * (vs[t][i] * inv));
+            for (int i = 0; i < 4; ++i) x[i] = static_cast<int>(s[t][i] * (vs[t][i] * inv));
             p[t] = digits4(x[0], x[1], x[2], x[3], st.pick);
         }
         const float w = v_top * factor * st.weight + poison;
         add_values<D>(st.o[qt], high, p, 256.0f * w);
         add_values<D>(st.o[qt], low, p, w);
+        tile_end();
     }
 }
 
@@ -488,14 +513,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_few_kernel(const AttendA
                 load_tiles<D>(tiles.a, tile);
             }
             tile_end();
-            if (masked) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!sees(st.position[qt], start + 16 * t + 4 * group + i, a.d.window)) s4[t][i] = kNegInf;
-            }
-            const float factor = softmax_block(s4, st.m[qt], st.l[qt], st.o[qt]);
+            if (masked) hide(s4, seen_tokens(st.position[qt], start, a.d.window));
+            const float factor = softmax_block<QT>(s4, st.m[qt], st.l[qt], st.o[qt]);
             i32x4 p;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
