@@ -487,17 +487,21 @@ class KVBatch:
         raw.max_tokens = max_tokens
         raw.table_width = table.shape[1]
         self.raw = raw
-        self._ref = ctypes.byref(raw)
         self.device = device
         self.sequences = n
         self._keep = (past, table, cu_tokens, slots)
 
     def _of(self, tokens: int):
-        """The descriptor for a call on `tokens` tokens."""
-        if self._keep[2] is None and tokens != self.sequences:
-            raise ValueError(f"{tokens} tokens for {self.sequences} sequences: without cu_tokens each has one")
-        self.raw.tokens = tokens
-        return self._ref
+        """The descriptor for a call on `tokens` tokens: a new one where the last
+        call had another count (that call may still be using its own)."""
+        raw = self.raw
+        if raw.tokens != tokens:
+            if self._keep[2] is None and tokens != self.sequences:
+                raise ValueError(f"{tokens} tokens for {self.sequences} sequences: without cu_tokens each has one")
+            raw = _lib.BatchDesc.from_buffer_copy(raw)
+            raw.tokens = tokens
+            self.raw = raw
+        return ctypes.byref(raw)
 
 
 class KVCache:
@@ -619,8 +623,8 @@ class KVCache:
             out_rows = _rows(out, "out", dtype, shape, device)
         if lse is True:
             lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
-        if window < 0:
-            raise ValueError("window must not be negative")
+        if not 0 <= window < 1 << 32:
+            raise ValueError("window must not be negative (or reach 2^32)")
         d = _lib.ATTEND.pack(_dtype(dtype), heads, *rows, *out_rows,
                              0 if lse is False else _plain(lse, "lse", torch.float32, (tokens, heads), device),
                              self.head_dim ** -0.5 if scale is None else scale, window)

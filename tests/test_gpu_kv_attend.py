@@ -297,3 +297,90 @@ def test_a_prompt_s_row_equals_the_single_token(cuda):
     single = cache.attend(step([n - 1], [1], table), q[n - 1:])
     # two results within the bound of `check`, sum |q k| / 8 under 16
     assert (single[0] - whole[n - 1]).abs().max() <= 4 * 2.0 ** -24 * (16 * 16 + 16) * v.abs().max()
+
+
+@pytest.mark.parametrize("sequences,cu", [(70, False), (70, True), (130, True), (1100, False), (4200, True)])
+def test_many_sequences(cuda, sequences, cu):
+    """More sequences than a wave has lanes, than are dealt by length, and than
+    two steps of the search over them reach; some long ones among them."""
+    kv_heads, dim, group = 1, 64, 2
+    r = np.random.RandomState(sequences)
+    counts = [int(c) for c in r.randint(0, 3, sequences)] if cu else [1] * sequences
+    counts[-1] = 1
+    past = [int(p) for p in r.randint(0, 90, sequences)]
+    past[sequences // 2], past[3] = 1500, 700
+    lengths = [p + c for p, c in zip(past, counts)]
+    cache, table, slots = filled(kv_heads, dim, lengths, 30)
+    q = normal((sum(counts), kv_heads * group, dim), "f32", 31)
+    batch = step(past, counts, table, slots)
+    out = cache.attend(batch, q)
+    every = list(range(sequences)) if sequences < 200 else sorted({0, 1, 3, sequences // 2, sequences - 1, *r.randint(0, sequences, 40)})
+    at = np.concatenate([[0], np.cumsum(counts)])
+    for i in every:
+        if counts[i]:
+            rows = slice(int(at[i]), int(at[i + 1]))
+            check(cache, table[i:i + 1], slots[i:i + 1], past[i:i + 1], counts[i:i + 1], q[rows], out[rows], "f32")
+    assert cache.faults() == 0
+
+
+def test_a_prompt_among_single_tokens(cuda):
+    """Both kernels in one call: long and short sequences take their own."""
+    past, counts = [300, 0, 20, 511, 64], [1, 150, 1, 2, 70]
+    cache, table, slots = filled(2, 128, [p + c for p, c in zip(past, counts)], 32)
+    q = normal((sum(counts), 8, 128), "bf16", 33)
+    batch = step(past, counts, table, slots)
+    out, lse = cache.attend(batch, q, lse=True)
+    check(cache, table, slots, past, counts, q, out, "bf16", lse)
+    assert torch.equal(cache.attend(batch, q), out) and cache.faults() == 0
+
+
+def test_the_batch_s_limit_may_be_generous(cuda):
+    """max_tokens far above what the sequences have."""
+    from q4rdna import api
+    past, counts = [100, 3], [2, 1]
+    cache, table, slots = filled(1, 64, [102, 4], 34)
+    q = normal((3, 2, 64), "f32", 35)
+    batch = api.KVBatch(ints(past), table, cu_tokens=ints([0, 2, 3]), slots=ints(slots), max_tokens=4000)
+    check(cache, table, slots, past, counts, q, cache.attend(batch, q), "f32")
+
+
+def test_refusals_of_the_python_calls(cuda):
+    from q4rdna import api
+    cache, table, slots = filled(2, 64, [70], 36)
+    batch = step([69], [1], table, slots)
+    q = normal((1, 4, 64), "f32", 37)
+    for bad in (q[0], q.double(), q.cpu(), q[:, :, :32], q.transpose(1, 2), normal((2, 4, 64), "f32", 38)):
+        with pytest.raises(ValueError):
+            cache.attend(batch, bad)
+    with pytest.raises(ValueError):
+        cache.attend(batch, q, window=-1)
+    with pytest.raises(ValueError):
+        cache.attend(batch, q, out=torch.empty((1, 1, 64), device="cuda").expand(1, 4, 64))
+    with pytest.raises(ValueError):
+        cache.attend(batch, q, lse=torch.empty((4, 1), device="cuda"))
+    with pytest.raises(api.Q4RdnaError):
+        cache.attend(batch, normal((1, 3, 64), "f32", 39))
+    with pytest.raises(ValueError):
+        api.KVBatch(ints([0]).long(), table)
+    with pytest.raises(ValueError):
+        api.KVBatch(ints([0, 1]), table)
+    with pytest.raises(ValueError):
+        api.KVBatch(ints([0]), table, max_tokens=4)
+    with pytest.raises(ValueError):
+        api.KVCache(cache.pages, cache.scales[:-1], cache.open, cache.open_scales)
+    k = normal((1, 2, 64), "f32", 40)
+    with pytest.raises(ValueError):
+        cache.append(batch, k, k.half())
+    with pytest.raises(ValueError):
+        cache.append(batch, k, k, q_out=q)
+    with pytest.raises(ValueError):
+        cache.append(batch, k, k, sin=k[0])
+    with pytest.raises(ValueError):
+        cache.read(batch, 2)
+    with pytest.raises(ValueError):
+        api.add_norm(k[0], k[0].half(), None)
+    with pytest.raises(ValueError):
+        api.add_norm(k[0], None, None, gate=k[0])
+    with pytest.raises(ValueError):
+        api.add_norm(k[0], k[0], torch.ones(63, device="cuda"))
+    assert cache.faults() == 0

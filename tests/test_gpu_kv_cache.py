@@ -308,3 +308,37 @@ def test_pages_past_four_gigabytes(cuda):
     for head in (0, 15):
         want, _, _ = R.attend(f64(q)[:, head], f64(got[0])[:, head], f64(got[1])[:, head], range(64), dim ** -0.5, 0)
         assert np.abs(f64(out)[:, head] - want).max() <= 2.0 ** -8 * np.abs(want).max() + 2.0 ** -10 * np.abs(f64(got[1])).max()
+
+
+@pytest.mark.parametrize("sequences", [100, 4300])
+def test_ragged_steps_of_many_sequences(cuda, sequences):
+    """Places are found among more sequences than one trip of the search sees:
+    appended raggedly and read back."""
+    kv_heads, dim = 1, 64
+    r = np.random.RandomState(sequences)
+    counts = [int(c) for c in r.randint(0, 4, sequences)]
+    counts[7] = 150
+    past = [0] * sequences
+    rows = [[i, sequences + i, 2 * sequences + i] for i in range(sequences)]
+    cache = make_cache(kv_heads, dim, 3 * sequences, sequences)
+    table = ints(rows)
+    total = sum(counts)
+    q, k, v = normal((total, 3, dim), "f32", 50), normal((total, kv_heads, dim), "f32", 51), normal((total, kv_heads, dim), "f32", 52)
+    cos, sin = rotary_table(160, dim)
+    batch = step(past, counts, table)
+    q_out = cache.append(batch, k, v, q=q, cos=cos, sin=sin)
+    got = cache.read(batch, total)
+    assert cache.faults() == 0
+    position = np.concatenate([np.arange(c) for c in counts])
+    c, s = f64(cos), f64(sin)
+    want_q = np.stack([R.rotate(f64(q[n]), p, c, s, False) for n, p in enumerate(position)])
+    want_k = np.stack([R.rotate(f64(k[n]), p, c, s, False) for n, p in enumerate(position)])
+    assert np.abs(f64(q_out) - want_q).max() <= 2.0 ** -20 * np.abs(want_q).max()
+    # 8-bit steps in the one sequence's full blocks, 16-bit steps elsewhere
+    first = sum(counts[:7])
+    full = np.zeros(total, dtype=bool)
+    full[first:first + 128] = True
+    for x, want in ((got[0], want_k), (got[1], f64(v))):
+        err, top = np.abs(f64(x) - want).max(axis=(1, 2)), np.abs(want).max()
+        assert (err[full] <= top * (0.5 / 127 + 0.5 / R.CODE16 + 2.0 ** -20)).all()
+        assert (err[~full] <= top * (0.5 / R.CODE16 + 2.0 ** -20)).all()
