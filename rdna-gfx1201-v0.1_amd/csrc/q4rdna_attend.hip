@@ -121,10 +121,14 @@ __device__ __forceinline__ void hide(float (&s)[4][4], uint32_t seen) {
         }
 }
 
+// A weight in [0, 1] as 30-bit fixed point.  (A 2^30 inside the exponential
+// would cost its argument four bits.)
+__device__ __forceinline__ int fixed30(float p) { return static_cast<int>(p * 0x1p30f); }
+
 // The softmax of a block: s holds the lane's base-2 scores (-inf where hidden),
-// on return p * 2^30 relative to the block's maximum.  Updates the running
-// maximum and sum and rescales o; returns the block's factor relative to the
-// new maximum (with the 2^-30), zero where the row sees nothing of the block.
+// on return p relative to the block's maximum.  Updates the running maximum and
+// sum and rescales o; returns the block's factor relative to the new maximum,
+// zero where the row sees nothing of the block.
 template <int QT, int DT>
 __device__ __forceinline__ float softmax_block(float (&s)[4][4], float &m, float &l, f32x4 (&o)[DT]) {
     float top = s[0][0];
@@ -136,14 +140,14 @@ __device__ __forceinline__ float softmax_block(float (&s)[4][4], float &m, float
     const float next = fmaxf(m, top);
     const float ref = next == kNegInf ? 0.0f : next;
     const float alpha = __builtin_amdgcn_exp2f(m - ref);
-    const float factor = __builtin_amdgcn_exp2f(top - ref) * 0x1p-30f;
-    const float shift = 30.0f - (top == kNegInf ? 0.0f : top);
+    const float factor = __builtin_amdgcn_exp2f(top - ref);
+    const float shift = top == kNegInf ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            s[t][i] = __builtin_amdgcn_exp2f(s[t][i] + shift);
+            s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - shift);
             sum += s[t][i];
         }
     l = l * alpha + sum * factor;
@@ -220,10 +224,10 @@ __device__ __forceinline__ void few_open_block(FewState<D, QT> &st, const int8_t
         for (int t = 0; t < 4; ++t) {
             int x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = static_cast<int>(s[t][i] * (vs[t][i] * inv));
+            for (int i = 0; i < 4; ++i) x[i] = fixed30(s[t][i] * (vs[t][i] * inv));
             p[t] = digits4(x[0], x[1], x[2], x[3], st.pick);
         }
-        const float w = v_top * factor * st.weight + poison;
+        const float w = v_top * factor * (st.weight * 0x1p-30f) + poison;
         add_values<D>(st.o[qt], high, p, 256.0f * w);
         add_values<D>(st.o[qt], low, p, w);
         tile_end();
@@ -518,10 +522,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_few_kernel(const AttendA
             i32x4 p;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                p[t] = digits4(static_cast<int>(s4[t][0]), static_cast<int>(s4[t][1]), static_cast<int>(s4[t][2]),
-                               static_cast<int>(s4[t][3]), st.pick);
+                p[t] = digits4(fixed30(s4[t][0]), fixed30(s4[t][1]), fixed30(s4[t][2]), fixed30(s4[t][3]), st.pick);
             // A row that sees nothing of the block takes nothing of it, a NaN scale included.
-            const float wv = masked && factor == 0.0f ? 0.0f : v_scale * factor * st.weight;
+            const float wv = masked && factor == 0.0f ? 0.0f : v_scale * factor * (st.weight * 0x1p-30f);
             tile_end();
             add_values<D>(st.o[qt], tiles.b, p, wv);
         }
