@@ -390,7 +390,9 @@ __device__ __forceinline__ FewItem find_item(const AttendArgs &a, uint32_t x) {
         w = work_of<ROWS>(a, i + lane);
         all += wave_total(static_cast<uint64_t>(w.jobs) * w.blocks);
     }
-    uint32_t chunk = static_cast<uint32_t>(max((all + a.target - 1) / a.target, static_cast<uint64_t>(kMinChunk)));
+    const uint64_t share = all + a.target - 1;
+    uint32_t chunk = share >> 32 == 0 ? static_cast<uint32_t>(share) / a.target : static_cast<uint32_t>(share / a.target);
+    chunk = max(chunk, kMinChunk);
     // A short last part wastes a workgroup's place: take larger ones until all
     // of them run at once, if they can.
     if (a.batch.sequences <= 64) {
@@ -451,8 +453,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_few_kernel(const AttendA
     const Span span = span_of(a, s.past, first_row, last_row);
     const int splits = min(it.splits, (span.blocks + WAVES - 1) / WAVES), split = it.split;
     if (split >= splits) return;
-    const int from = span.block0 + static_cast<int>(static_cast<int64_t>(split) * span.blocks / splits);
-    const int to = span.block0 + static_cast<int>(static_cast<int64_t>(split + 1) * span.blocks / splits);
+    const int from = span.block0 + static_cast<int>(mul_div(split, span.blocks, splits));
+    const int to = span.block0 + static_cast<int>(mul_div(split + 1, span.blocks, splits));
     const int open_block = s.length % static_cast<int>(kKvBlock) != 0 ? s.length / static_cast<int>(kKvBlock) : -1;
 
     // The wave's blocks: from + wave, from + wave + WAVES, ...  Lane x keeps

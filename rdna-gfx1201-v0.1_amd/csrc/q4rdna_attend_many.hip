@@ -348,8 +348,8 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const int splits = min(static_cast<int>(a.splits), max(1, static_cast<int>(__builtin_amdgcn_sqrtf(static_cast<float>(blocks)))));
     const int split = blockIdx.y;
     if (split >= splits) return;
-    const int from = block0 + static_cast<int>(static_cast<int64_t>(split) * blocks / splits);
-    const int to = block0 + static_cast<int>(static_cast<int64_t>(split + 1) * blocks / splits);
+    const int from = block0 + static_cast<int>(mul_div(split, blocks, splits));
+    const int to = block0 + static_cast<int>(mul_div(split + 1, blocks, splits));
     // The open block, where this workgroup has it, comes last.
     const bool has_open = s.length % block_size != 0 && to - 1 == s.length / block_size;
     const int to_full = has_open ? to - 1 : to;

@@ -428,9 +428,10 @@ __device__ void turn_q(const AppendArgs &a, uint32_t unit) {
     Weights weights;
     load_weights(weights, a.d.q_norm, at);
     const uint32_t heads = a.d.q_heads;
-    // One long division per workgroup, short ones per row.
+    // One division per workgroup, a multiplication per row.
     const uint64_t rows = static_cast<uint64_t>(a.batch.tokens) * heads, row_first = static_cast<uint64_t>(unit) * a.q_rows;
-    const uint32_t n_first = static_cast<uint32_t>(row_first / heads), head_first = static_cast<uint32_t>(row_first % heads);
+    const uint32_t n_first = mul_div(unit, a.q_rows, heads);
+    const uint32_t head_first = static_cast<uint32_t>(row_first - static_cast<uint64_t>(n_first) * heads);
     const uint32_t row_count = static_cast<uint32_t>(min(rows - row_first, static_cast<uint64_t>(a.q_rows)));
     // The workgroup's tokens are mostly of one sequence: the first one's.
     const Seq s0 = seq_of(a.batch, a.cache, wave_token_seq(a.batch, n_first));
@@ -478,9 +479,8 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
     __shared__ AppendStage<D> stage;
     // The blocks' workgroups, which wait a lot, spread evenly among q's, which
     // move the most bytes.
-    const uint64_t b = blockIdx.x;
-    const uint32_t before = static_cast<uint32_t>(b * a.kv_units / gridDim.x);
-    if (static_cast<uint32_t>((b + 1) * a.kv_units / gridDim.x) != before)
+    const uint32_t before = mul_div(blockIdx.x, a.kv_units, gridDim.x);
+    if (mul_div(blockIdx.x + 1, a.kv_units, gridDim.x) != before)
         append_place<D, INTERLEAVED, T>(a, before, stage);
     else
         turn_q<D, INTERLEAVED, T>(a, blockIdx.x - before);
