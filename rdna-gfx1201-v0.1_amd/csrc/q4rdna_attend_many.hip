@@ -99,7 +99,7 @@ __device__ __forceinline__ void stage_raw(ManyTile<D> &t, const Raw<D> &r) {
 
 template <int D, int SPLIT>
 struct ManyState {
-    h16x8 q[SPLIT][D / 16];
+    h16x8 q[D / 16][SPLIT];
     float q_scale;    // base-2 score = q_scale * (k scale) * product
     int position;     // of the lane's row
     float m, l;       // the maximum that the weights refer to; the lane's part of the sum, in units of 2^-7
@@ -121,24 +121,38 @@ __device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) {
 template <bool OPEN, int D, int SPLIT>
 __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTile<D> *tile, float k_scale, float v_scale,
                                            const float *token_scales, int start, int length, uint32_t window, bool masked) {
+    constexpr int KF = D / 16, VF = D / 32;  // fragments per product's tile
     const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
+    const int k_at = column * (D + 8) + 8 * half, v_at = column * (kKvBlock + 8) + 32 * half;
+    // The tile's fragments in the order of their use, the first DEPTH of them
+    // under way: the registers of each are refilled once its product is issued.
+    constexpr int ALL = 2 * KF + 4 * VF, DEPTH = SPLIT == 1 ? KF : KF / 2;
+    const auto fragment = [&](int y, int j) {
+        const _Float16 *k = tile[y].k + k_at + j / KF * 32 * (D + 8) + j % KF * 16;
+        const _Float16 *v = tile[y].v + v_at + (j - 2 * KF) % VF * 32 * (kKvBlock + 8) + (j - 2 * KF) / VF * 8;
+        return *reinterpret_cast<const h16x8 *>(j < 2 * KF ? k : v);
+    };
+    h16x8 f[DEPTH];
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) f[j] = fragment(0, j);
+    const auto use = [&](int j, const h16x8 (&operand)[SPLIT], f32x16 &sum) {
+#pragma unroll
+        for (int x = 0; x < SPLIT; ++x) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[j % DEPTH], operand[x], sum, 0, 0, 0);
+        if (j + DEPTH < ALL) f[j % DEPTH] = fragment(0, j + DEPTH);
+        tile_end();
+        if (OPEN) {
+            const h16x8 low = fragment(1, j);
+#pragma unroll
+            for (int x = 0; x < SPLIT; ++x) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(low, operand[x], sum, 0, 0, 0);
+        }
+    };
     f32x16 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            const h16x8 a = *reinterpret_cast<const h16x8 *>(tile[0].k + (32 * t + column) * (D + 8) + 16 * k + 8 * half);
-#pragma unroll
-            for (int x = 0; x < SPLIT; ++x) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, st.q[x][k], s[t], 0, 0, 0);
-            if (OPEN) {
-                const h16x8 b = *reinterpret_cast<const h16x8 *>(tile[1].k + (32 * t + column) * (D + 8) + 16 * k + 8 * half);
-#pragma unroll
-                for (int x = 0; x < SPLIT; ++x) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, st.q[x][k], s[t], 0, 0, 0);
-            }
-        }
-        tile_end();
+        for (int k = 0; k < KF; ++k) use(t * KF + k, st.q[k], s[t]);
     }
     if (OPEN) {
 #pragma unroll
@@ -165,7 +179,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
                 s[t][i] = __uint_as_float((__float_as_uint(s[t][i]) & m) | (__float_as_uint(kNegInf) & ~m));
             }
     }
-    const float f = OPEN ? st.q_scale : st.q_scale * k_scale;
+    const float unit = OPEN ? st.q_scale : st.q_scale * k_scale;
     float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -173,7 +187,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
     top = max_xor32(top);
     const bool none = top == kNegInf;
-    const float now = none ? kNegInf : top * f;
+    const float now = none ? kNegInf : top * unit;
 
     // V's scale relative to the largest one so far; one that is not finite
     // makes the seen weights NaN and leaves the reference alone.
@@ -188,7 +202,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         largest = max_xor32(max_xor16(largest));
     }
     const float v_ref = largest < __builtin_inff() ? fmaxf(st.v_ref, largest) : st.v_ref;
-    const bool grown = now > st.m + kLazy || (st.m == kNegInf && now != kNegInf);
+    const bool grown = now > st.m + kLazy;
     if (__builtin_amdgcn_ballot_w64(grown || v_ref != st.v_ref) != 0) {
         const float m = grown ? now : st.m;
         const float alpha = grown ? __builtin_amdgcn_exp2f(st.m - m) : 1.0f;  // 0 from -inf
@@ -199,19 +213,20 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         st.m = m;
         st.v_ref = v_ref;
     }
-    const float to_ref = v_ref > 0.0f ? 1.0f / v_ref : 0.0f;
-    float r = OPEN ? 0.0f : v_scale < __builtin_inff() ? v_scale * to_ref : __builtin_nanf("");
+    // A full block's ratio goes into the exponent (and comes out of the sum);
+    // under 2^-90 of the largest scale it might as well be that.
+    const float to_ref = v_ref > 0.0f ? __builtin_amdgcn_rcpf(v_ref) : 0.0f;
     float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m), per_r = 1.0f;
-    const bool folded = !OPEN && r > 0x1p-20f;
-    if (folded) {
+    if (!OPEN) {
+        const float r = v_scale < __builtin_inff() ? fmaxf(v_scale * to_ref, 0x1p-90f) : __builtin_nanf("");
         shift += __builtin_amdgcn_logf(r);
-        per_r = 1.0f / r;
+        per_r = __builtin_amdgcn_rcpf(r);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], f, shift));
-    auto hide = [&] {  // whatever f and the scales are
+        for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unit, shift));
+    auto hide = [&] {  // whatever the unit and the scales are
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -221,7 +236,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
     float sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-        f32x4 w = {r, r, r, r};
+        f32x4 w;
         if (OPEN) {
             const f32x4 vt = *(gptr_f32x4)(uintptr_t)(token_scales + kKvBlock + 8 * x + 4 * half);
 #pragma unroll
@@ -233,13 +248,6 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
             sum += s[x / 4][i];
             if (OPEN) s[x / 4][i] *= w[b];
         }
-    }
-    if (!OPEN && !folded) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][i] *= r;
-        if (masked) hide();
     }
     if (OPEN) hide();
     st.l += sum * per_r;
@@ -256,18 +264,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
             if (SPLIT == 2) p[SPLIT - 1][e] = static_cast<_Float16>(w - static_cast<float>(p[0][e]));
         }
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) {
-            const int at = (32 * d + column) * (kKvBlock + 8) + 32 * half + 8 * x;
-            const h16x8 a = *reinterpret_cast<const h16x8 *>(tile[0].v + at);
-#pragma unroll
-            for (int y = 0; y < SPLIT; ++y) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[y], st.o[d], 0, 0, 0);
-            if (OPEN) {
-                const h16x8 b = *reinterpret_cast<const h16x8 *>(tile[1].v + at);
-#pragma unroll
-                for (int y = 0; y < SPLIT; ++y) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, p[y], st.o[d], 0, 0, 0);
-            }
-        }
-        tile_end();
+        for (int d = 0; d < VF; ++d) use(2 * KF + x * VF + d, p, st.o[d]);
     }
 }
 
@@ -297,8 +294,8 @@ __device__ __forceinline__ void load_q_many(ManyState<D, SPLIT> &st, const Atten
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float v = finite ? __builtin_amdgcn_ldexpf(x[k][e], up) : 0.0f;
-            st.q[0][k][e] = static_cast<_Float16>(v);
-            if (SPLIT == 2) st.q[SPLIT - 1][k][e] = static_cast<_Float16>(v - static_cast<float>(st.q[0][k][e]));
+            st.q[k][0][e] = static_cast<_Float16>(v);
+            if (SPLIT == 2) st.q[k][SPLIT - 1][e] = static_cast<_Float16>(v - static_cast<float>(st.q[k][0][e]));
         }
     st.q_scale = finite ? __builtin_amdgcn_ldexpf(a.d.scale * kLog2e, -up) : __builtin_nanf("");
     st.m = kNegInf;
@@ -317,8 +314,13 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const int tid = threadIdx.x, lane = tid & 63, column = lane & 31, half = lane >> 5, wave = wave_id();
     const uint32_t heads = a.cache.kv_heads;
     // Neighbouring workgroups take different heads: with eight of them, each
-    // XCD's L2 holds one head's cache.  Late rows, which see most, go first.
-    const uint32_t head = blockIdx.x % heads, place = gridDim.x / heads - 1 - blockIdx.x / heads;
+    // XCD's L2 holds one head's cache.  Late rows, which see most, go first;
+    // the second workgroup of each CU comes in the opposite order, so that the
+    // longest ones share their CU with the shortest.
+    const uint32_t head = blockIdx.x % heads, units = gridDim.x / heads;
+    uint32_t unit = blockIdx.x / heads;
+    if (unit >= a.cu_units && unit < 2 * a.cu_units) unit = a.cu_units + min(2 * a.cu_units, units) - 1 - unit;
+    const uint32_t late = unit / a.splits, place = units / a.splits - 1 - late;
 
     // The sequence and the rows of the place: sequence i has the places from
     // cu[i] * group / 128 + i on (attend_many_places).
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const uint32_t base = seq_place < 0 || seq_place > place ? place : static_cast<uint32_t>(seq_place);
     const Seq s = seq_of(a.batch, a.cache, seq);
     if (!s.ok) {
-        if (head == 0 && place == base && blockIdx.y == 0 && tid == 0) count_fault(a.cache);
+        if (head == 0 && place == base && unit == late * a.splits && tid == 0) count_fault(a.cache);
         return;
     }
     const int rows = s.count * static_cast<int>(a.group);
@@ -346,7 +348,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     // A part costs the joining workgroup about as long as a block costs a part:
     // blocks / splits + splits is least at the root.
     const int splits = min(static_cast<int>(a.splits), max(1, static_cast<int>(__builtin_amdgcn_sqrtf(static_cast<float>(blocks)))));
-    const int split = blockIdx.y;
+    const int split = static_cast<int>(unit - late * a.splits);
     if (split >= splits) return;
     const int from = block0 + static_cast<int>(mul_div(split, blocks, splits));
     const int to = block0 + static_cast<int>(mul_div(split + 1, blocks, splits));
@@ -422,10 +424,10 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const uint32_t h = head * a.group + (live ? row - token * group : 0);
     const uint32_t job = place * heads + head;
     // Parts lie as [number][row]: a lane's row, so neighbouring lanes side by side.
-    float m_row = st.m, l_row = l, unit = st.v_ref;
+    float m_row = st.m, l_row = l, o_unit = st.v_ref;
     if (splits > 1) {
-        const size_t jobs = gridDim.x, first_slot = static_cast<size_t>(job) * a.splits;
-        float *stats = a.partials + jobs * a.splits * kRowsMany * D;
+        const size_t first_slot = static_cast<size_t>(job) * a.splits;
+        float *stats = a.partials + static_cast<size_t>(gridDim.x) * kRowsMany * D;
         const int r = 32 * wave + column;
         float *part = a.partials + (first_slot + split) * kRowsMany * D + r;
 #pragma unroll
@@ -449,7 +451,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         for (int i = 0; i < splits; ++i) m_row = fmaxf(m_row, load_agent(stats + (first_slot + i) * 2 * kRowsMany + r));
         const float ref = m_row == kNegInf ? 0.0f : m_row;
         l_row = 0.0f;
-        unit = 1.0f;
+        o_unit = 1.0f;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -470,7 +472,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         }
     }
     if (!live) return;
-    const float inv = l_row == 0.0f ? 0.0f : unit / l_row;
+    const float inv = l_row == 0.0f ? 0.0f : o_unit / l_row;
     T *out = static_cast<T *>(a.d.out.data) + static_cast<int64_t>(s.first + token) * a.d.out.token_stride + h * a.d.out.head_stride;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -492,7 +494,7 @@ uint64_t attend_many_places(const q4rdna_kv_batch &b, uint32_t group) {
 }
 
 hipError_t launch_attend_many(const AttendArgs &a, uint32_t places, hipStream_t stream) {
-    const dim3 grid(places * a.cache.kv_heads, a.splits);
+    const uint32_t grid = places * a.cache.kv_heads * a.splits;
     auto go = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(a); };
     if (a.cache.head_dim == 64)
         a.d.dtype == Q4RDNA_F32 ? go(attend_many_kernel<64, 2, float>) : a.d.dtype == Q4RDNA_F16 ? go(attend_many_kernel<64, 1, _Float16>) : go(attend_many_kernel<64, 1, __bf16>);

@@ -289,6 +289,7 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
         const uint64_t jobs = places * cache->kv_heads;
         const uint64_t splits = std::min<uint64_t>(2ull * cus / jobs, (most_blocks + 1) / 2);
         a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 64)));
+        a.cu_units = std::max(1u, cus / cache->kv_heads);
         if ((rc = take_scratch(a, jobs * a.splits * q4rdna::kAttendManyRows, jobs, s)) != Q4RDNA_OK ||
             (rc = launched(q4rdna::launch_attend_many(a, static_cast<uint32_t>(places), s), "kv_attend")) != Q4RDNA_OK)
             return rc;

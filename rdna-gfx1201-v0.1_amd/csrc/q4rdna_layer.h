@@ -57,6 +57,7 @@ struct AttendArgs {
     uint32_t splits;      // the most workgroups that share a row group
     uint32_t target;      // attend_few_kernel: workgroups to deal the blocks to
     uint32_t workgroups;  // attend_few_kernel: workgroups launched
+    uint32_t cu_units;    // attend_many_kernel: workgroups per head when every CU has one
     uint32_t few_rows;    // sequences of up to so many rows belong to attend_few_kernel, the others to
                           // attend_many_kernel
     uint32_t wide;        // q rows can be read 16 bytes at a time
