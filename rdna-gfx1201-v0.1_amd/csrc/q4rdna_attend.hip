@@ -29,7 +29,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr int kMaxSplits = kAttendFewSplits;
-constexpr uint32_t kMinChunk = kAttendFewChunk;
 
 // Four int32 values as balanced base-256 digits: byte d of (x + 0x808080) ^
 // 0x808080 is digit d in [-128, 127].  Returns byte `digit` of each, packed;
@@ -42,7 +41,12 @@ __device__ __forceinline__ int digits4(int x0, int x1, int x2, int x3, uint32_t 
     return static_cast<int>(__builtin_amdgcn_perm(hi, lo, 0x05040100u));
 }
 
+// The sum over a quad, the same bits in its four lanes: they hold the digits of
+// one weight, and a last place between them would be a carry in one digit and
+// not in the next.  So no addition may be fused with the product before it,
+// which each lane would round differently.
 __device__ __forceinline__ float quad_sum(float v) {
+#pragma clang fp contract(off)
     v += dpp<kDppXor1>(v);
     v += dpp<kDppXor2>(v);
     return v;
@@ -343,7 +347,7 @@ __device__ __forceinline__ uint64_t wave_total(uint64_t v) {  // v < 2^42
 }
 
 // What a sequence's workgroups take: every row group of every head is cut into
-// parts of about `chunk` blocks, at least kMinChunk.
+// parts of about `chunk` blocks (parts_of).
 struct SeqWork {
     Seq s;
     uint32_t jobs, blocks;
@@ -363,10 +367,21 @@ __device__ __forceinline__ SeqWork work_of(const AttendArgs &a, uint32_t i) {
     return w;
 }
 
+// Parts of a row group.  Joining costs 3 us, and 0.1 us more per part; a wave's
+// block 2 us, up to where the memory is busy.  So up to kAttendWhole blocks are
+// one part, and longer rows have parts of 8, from kAttendLong blocks on of 16
+// blocks at least (a token behind, 8 and 16 at least: 1000 tokens 10.5, 9.4 us;
+// 4000 11.2, 13.3; 8000 13.1, 13.7; 16000 16.8, 15.5; 32 times 1000 tokens 20.2, 16.9).
+__device__ __forceinline__ uint32_t parts_of(uint32_t blocks, uint32_t chunk, uint32_t most) {
+    const uint32_t least = blocks <= kAttendWhole || blocks > kAttendLong ? 16 : 8;
+    chunk = max(chunk, least);
+    return min((blocks + chunk - 1) / chunk, most);
+}
+
 // The item of workgroup x.  The device knows the sequences' lengths and the
 // host does not, so the deal happens here: all blocks over `target` workgroups,
 // and a prefix sum over the sequences, 64 at a time, by every wave for itself.
-template <int ROWS, int WAVES>
+template <int ROWS>
 __device__ __forceinline__ FewItem find_item(const AttendArgs &a, uint32_t x) {
     FewItem it;
     it.seq = -1;
@@ -392,19 +407,18 @@ __device__ __forceinline__ FewItem find_item(const AttendArgs &a, uint32_t x) {
     }
     const uint64_t share = all + a.target - 1;
     uint32_t chunk = share >> 32 == 0 ? static_cast<uint32_t>(share) / a.target : static_cast<uint32_t>(share / a.target);
-    chunk = max(chunk, kMinChunk);
     // A short last part wastes a workgroup's place: take larger ones until all
     // of them run at once, if they can.
     if (a.batch.sequences <= 64) {
         const uint32_t jobs = __builtin_amdgcn_readlane(wave_scan(w.jobs), 63);
         while (jobs < a.target && static_cast<uint32_t>(__builtin_amdgcn_readlane(
-                                      wave_scan(w.jobs * min((w.blocks + chunk - 1) / chunk, a.splits)), 63)) > a.target)
+                                      wave_scan(w.jobs * parts_of(w.blocks, chunk, a.splits)), 63)) > a.target)
             chunk += chunk / 8 + 1;
     }
     uint32_t base = 0;
     for (uint32_t i = 0; i < a.batch.sequences; i += 64) {
         if (a.batch.sequences > 64) w = work_of<ROWS>(a, i + lane);
-        const uint32_t parts = min((w.blocks + chunk - 1) / chunk, a.splits), end = base + wave_scan(w.jobs * parts);
+        const uint32_t parts = parts_of(w.blocks, chunk, a.splits), end = base + wave_scan(w.jobs * parts);
         const uint64_t later = __builtin_amdgcn_ballot_w64(end > x);
         if (later != 0) {
             const int owner = __builtin_ctzll(later);
@@ -439,7 +453,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_few_kernel(const AttendA
     __shared__ uint32_t ticket;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    const FewItem it = find_item<ROWS, WAVES>(a, blockIdx.x);
+    const FewItem it = find_item<ROWS>(a, blockIdx.x);
     if (blockIdx.x == 0)  // bad entries, once
         for (uint32_t i = tid; i < a.batch.sequences; i += kThreads)
             if (!seq_of(a.batch, a.cache, i).ok) count_fault(a.cache);

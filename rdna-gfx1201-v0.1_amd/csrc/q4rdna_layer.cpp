@@ -194,9 +194,11 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
         return set_error(Q4RDNA_ERR_ARGUMENT, "misaligned norm weight");
     const uint64_t kv_units = q4rdna::kv_places(*batch) * cache->kv_heads;
     // Few rows of q: one per lane group, so that many workgroups share the
-    // wait for them; many: eight.
+    // wait for them; many: eight, which divides the workgroup's fixed part (32
+    // bf16 heads of 128, one against eight: 32 tokens 6.7 and 7.1 us, 128
+    // tokens 10.4 and 10.4, 512 tokens 11.6 and 10.8, 2048 tokens 23.1 and 15.7).
     const uint64_t all_rows = static_cast<uint64_t>(batch->tokens) * desc->q_heads;
-    const uint32_t q_rows = all_rows <= 32768 ? 2048 / cache->head_dim : 16384 / cache->head_dim;
+    const uint32_t q_rows = all_rows <= 4096 ? 2048 / cache->head_dim : 16384 / cache->head_dim;
     const uint64_t q_units = (all_rows + q_rows - 1) / q_rows;
     if (kv_units + q_units > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
     if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
@@ -213,12 +215,33 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     return launched(q4rdna::launch_append(a, static_cast<hipStream_t>(stream)), "kv_append");
 }
 
-// Sequences of up to so many rows per kv head go to attend_few_kernel.
-constexpr uint32_t kFewRows = 64;
+// Sequences of up to so many rows (query token, query head) per kv head go to
+// attend_few_kernel, which reads the cache once per eight rows, the others to
+// attend_many_kernel, which reads it once per 128 and starts and joins slower.
+// Up to 32 rows the former is the faster one or within a tenth; beyond, while
+// its row groups all run at once and the blocks that they see are few.  The
+// lengths are on the device; the table's width and the window bound them.
+// bf16, 8 kv heads, us by the former and the latter:
+//   64 rows, one sequence behind 2000 tokens 17 and 26, 8000 28 and 42,
+//   30000 59 and 69; 8 sequences behind 500 19 and 27, 8000 108 and 76;
+//   16 sequences behind 500 36 and 28.
+//   128 rows, one sequence behind 2000 22 and 27, 8000 39 and 43, 30000 103 and
+//   72; 4 sequences behind 500 19 and 22, 8000 106 and 50.
+uint32_t few_rows(const q4rdna_kv_batch &b, uint32_t group, uint32_t kv_heads, uint64_t most_blocks, uint32_t cus) {
+    const auto small = [&](uint32_t rows, uint64_t blocks_per_cu) {
+        const uint64_t all = std::min(static_cast<uint64_t>(b.sequences) * rows, static_cast<uint64_t>(b.tokens) * group);
+        const uint64_t row_groups = (all + 7) / 8 * kv_heads;
+        return row_groups <= 2 * cus && row_groups * most_blocks <= blocks_per_cu * cus;
+    };
+    return small(128, 64) ? 128 : small(64, 128) ? 64 : 32;
+}
 
-// Up to so many sequences the blocks are dealt by their lengths; more of them
-// fill the card by themselves.
-constexpr uint32_t kDealtSequences = 1024;
+// Up to so many sequences the blocks are dealt by their lengths, by a scan of
+// all of them in every workgroup; more of them fill the card by themselves (a
+// token each of 8 heads, dealt and not, us: 200 of 64 to 4096 tokens 98 and 96,
+// 200 of which one has 16000 57 and 100; 400 198 and 178, 133 and 157; 800 420
+// and 309, 326 and 224).
+constexpr uint32_t kDealtSequences = 256;
 
 // Room for partial results of `rows` rows, and arrival counters of `jobs` row groups.
 int take_scratch(q4rdna::AttendArgs &a, size_t rows, size_t jobs, hipStream_t stream) {
@@ -252,7 +275,6 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     a.wide_out = wide_rows(desc->out, desc->dtype, 4);
     // The most rows (query token, query head) per kv head that a sequence has.
     const uint64_t most_rows = static_cast<uint64_t>(std::min(batch->max_tokens, batch->tokens)) * a.group;
-    const bool many = most_rows > kFewRows;
     const uint64_t places = q4rdna::attend_many_places(*batch, a.group);
     if (most_rows > 0x3fffffffu || places * cache->kv_heads > 0x7fffffffu)
         return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of %u query heads are too many for one call", batch->tokens, desc->q_heads);
@@ -261,20 +283,24 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const uint64_t most_blocks = desc->window == 0 ? batch->table_width
                                                    : std::min<uint64_t>(batch->table_width, (static_cast<uint64_t>(desc->window) + batch->max_tokens) / q4rdna::kKvBlock + 2);
+    const uint32_t few = few_rows(*batch, a.group, cache->kv_heads, most_blocks, cus);
+    const bool many = most_rows > few;
     // Sequences of few rows; a single one goes by the bound alone.
     if (!many || batch->sequences > 1) {
-        a.few_rows = many ? kFewRows : 0x7fffffffu;
-        const uint32_t most = static_cast<uint32_t>(many ? kFewRows : most_rows), rows = q4rdna::attend_few_rows(most);
+        a.few_rows = many ? few : 0x7fffffffu;
+        const uint32_t most = static_cast<uint32_t>(many ? few : most_rows), rows = q4rdna::attend_few_rows(most);
         a.row_groups = (most + rows - 1) / rows;
         // The device deals the blocks to about `target` workgroups; each row
         // group ends in one part that may be short.
         const uint64_t jobs = static_cast<uint64_t>(a.row_groups) * cache->kv_heads * batch->sequences;
         // Few row groups are cut into many parts, which cost time to join: take
-        // one workgroup of eight waves per CU there, two of four waves elsewhere.
+        // one workgroup of eight waves per CU there, two of four waves elsewhere
+        // (eight and four waves: one token behind 60000 30.7 and 33.1 us, 32
+        // ragged sequences of 100 to 8000 tokens 30.9 and 27.2 us).
         const uint32_t waves = jobs < cus / 8 ? 8 : 4;
         a.target = 8 / waves * cus;
-        const uint64_t most_splits = (most_blocks + q4rdna::kAttendFewChunk - 1) / q4rdna::kAttendFewChunk;
-        const bool split = most_splits > 1 && batch->sequences <= kDealtSequences;
+        const uint64_t most_splits = (most_blocks + 7) / 8;
+        const bool split = most_blocks > q4rdna::kAttendWhole && batch->sequences <= kDealtSequences;
         a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>(most_splits, q4rdna::kAttendFewSplits) : 1);
         const uint64_t workgroups = split ? std::min(jobs + a.target, jobs * a.splits) : jobs;
         if (workgroups > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences are too many for one call", batch->sequences);
@@ -284,7 +310,7 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
             return rc;
     }
     if (many) {
-        a.few_rows = batch->sequences > 1 ? kFewRows : 0;
+        a.few_rows = batch->sequences > 1 ? few : 0;
         // Two workgroups fit a CU: split until they are there.
         const uint64_t jobs = places * cache->kv_heads;
         const uint64_t splits = std::min<uint64_t>(2ull * cus / jobs, (most_blocks + 1) / 2);

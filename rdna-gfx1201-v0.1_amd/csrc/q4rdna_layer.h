@@ -68,9 +68,9 @@ struct AttendArgs {
 };
 // The most workgroups that share a row group of attend_few_kernel.
 constexpr uint32_t kAttendFewSplits = 64;
-// Blocks that a part has at least: joining two parts takes as long as two or
-// three more blocks per wave.
-constexpr uint32_t kAttendFewChunk = 8;
+// Up to so many blocks are not split, and more than so many are a long row.
+constexpr uint32_t kAttendWhole = 16;
+constexpr uint32_t kAttendLong = 160;
 // Rows (query token, query head of the kv head) that one workgroup takes.
 uint32_t attend_few_rows(uint32_t rows);
 // waves: 4 or 8 per workgroup.
