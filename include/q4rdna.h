@@ -383,7 +383,9 @@ typedef struct q4rdna_kv_cache {
  * (tokens outside the step's or more than max_tokens, past < 0, past + tokens
  * > 64 * table_width, a bad slot) is skipped, its results not written; a page
  * outside the cache is not written, and rows that need to read it come out as
- * NaN.  Each adds to *faults. */
+ * NaN.  Each adds to *faults.
+ * A call is made before the lengths are known: table_width bounds them, and a
+ * table no wider than the sequences may become is the faster one. */
 typedef struct q4rdna_kv_batch {
     const int32_t *past;      /* [sequences] */
     const int32_t *cu_tokens; /* [sequences + 1], ascending, or NULL */
