@@ -300,7 +300,8 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
         const uint32_t waves = jobs < cus / 8 ? 8 : 4;
         a.target = 8 / waves * cus;
         const uint64_t most_splits = (most_blocks + 7) / 8;
-        const bool split = most_blocks > q4rdna::kAttendWhole && batch->sequences <= kDealtSequences;
+        // (Nor are parts worth their scratch where row groups abound.)
+        const bool split = most_blocks > q4rdna::kAttendWhole && batch->sequences <= kDealtSequences && jobs <= 64ull * cus;
         a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>(most_splits, q4rdna::kAttendFewSplits) : 1);
         const uint64_t workgroups = split ? std::min(jobs + a.target, jobs * a.splits) : jobs;
         if (workgroups > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences are too many for one call", batch->sequences);

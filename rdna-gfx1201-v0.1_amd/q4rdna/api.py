@@ -464,11 +464,12 @@ class KVBatch:
     [sequences + 1] and slots [sequences] are int32 CUDA tensors, read when
     the kernels run: a captured graph may be replayed after they were filled
     anew.  Without cu_tokens every sequence has one token; with it max_tokens
-    (an int) bounds the tokens of a sequence.
+    (an int) bounds the tokens of a sequence, None where it is not known: a
+    bound lets short steps take faster paths.
     """
 
     def __init__(self, past: torch.Tensor, table: torch.Tensor, cu_tokens: torch.Tensor | None = None,
-                 slots: torch.Tensor | None = None, max_tokens: int = 1):
+                 slots: torch.Tensor | None = None, max_tokens: int | None = None):
         if not past.is_cuda or past.dim() != 1 or table.dim() != 2:
             raise ValueError("past must be a CUDA tensor [sequences], table [sequences, width]")
         device, n = past.get_device(), past.shape[0]
@@ -477,12 +478,16 @@ class KVBatch:
         raw.table = _plain(table, "table", torch.int32, (n, table.shape[1]), device)
         if cu_tokens is not None:
             raw.cu_tokens = _plain(cu_tokens, "cu_tokens", torch.int32, (n + 1,), device)
+            if max_tokens is None:
+                max_tokens = 0xffffffff  # the calls' tokens bound them
+        elif max_tokens is None:
+            max_tokens = 1
         elif max_tokens != 1:
             raise ValueError("without cu_tokens every sequence has one token")
         if slots is not None:
             raw.slots = _plain(slots, "slots", torch.int32, (n,), device)
-        if max_tokens < 1:
-            raise ValueError("max_tokens must be at least 1")
+        if not 1 <= max_tokens < 1 << 32:
+            raise ValueError("max_tokens must be at least 1 (and below 2^32)")
         raw.sequences = n
         raw.max_tokens = max_tokens
         raw.table_width = table.shape[1]

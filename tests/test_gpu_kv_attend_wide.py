@@ -99,3 +99,18 @@ def test_sequences_around_the_deal_s_limit(cuda, sequences):
     q = normal((sequences, 2, 64), "f32", 34)
     out, lse = cache.attend(step(past, [1] * sequences, table, slots), q, lse=True)
     narrow.check(cache, table, slots, past, [1] * sequences, q, out, "f32", lse)
+
+
+@pytest.mark.parametrize("kv_heads,sequences", [(1, 3), (32, 150)])
+def test_without_a_bound_on_the_tokens(cuda, kv_heads, sequences):
+    """max_tokens left out: the step's tokens bound every sequence's.  With 150
+    sequences of 32 kv heads the row groups are too many to be split."""
+    from q4rdna import api
+    past, counts = [1100, 0] + [1 + 5 * i % 70 for i in range(sequences - 2)], [5, 90] + [1] * (sequences - 2)
+    cache, table, slots = narrow.filled(kv_heads, 64, [p + c for p, c in zip(past, counts)], 37)
+    q = normal((sum(counts), kv_heads, 64), "f32", 38)
+    ends = torch.tensor([0] + counts, device="cuda").cumsum(0).int()
+    past_d, slots_d = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (past, slots))
+    out, lse = cache.attend(api.KVBatch(past_d, table, ends, slots_d), q, lse=True)
+    assert cache.faults() == 0
+    narrow.check(cache, table, slots, past, counts, q, out, "f32", lse)
