@@ -345,9 +345,11 @@ int q4rdna_dequantize(const q4rdna_weight *w, float *out, void *stream);
  * rint(code16 * (token scale / scale)): every number is rounded to 16 bits
  * once and to 8 bits once, so the cache's bytes do not depend on the chunks in
  * which the tokens arrive, and a full page never changes again (sequences may
- * share it).  A slot holds two blocks, used in turn: a sequence may be cut
- * back to any length >= 64 * (length / 64 - 1), its last full block included,
- * and be appended to from there, as long as no other sequence reads that page.
+ * share it).  A slot holds two blocks, used in turn: those of the greatest
+ * length m that the sequence has had and of the block before.  So tokens may be
+ * taken back to any length >= 64 * (m / 64 - 1), the last full block included,
+ * and the sequence be appended to from there, as long as no other one reads
+ * that page; cut back to length 0, or in a new slot, it starts afresh.
  *
  * The order of codes within a block of one head, 16 bytes per lane of a
  * 64-lane int8 matrix instruction:

@@ -73,12 +73,16 @@ __device__ __forceinline__ void load_weights(Weights &w, const float *weight, co
     load_floats<float, 4>(weight + p.a_at, true, w.a);
     load_floats<float, 4>(weight + p.b_at, true, w.b);
 }
+// Which products are fused is written out here and in turn_pair: the compiler
+// would choose anew for each copy of an unrolled loop, and the cache's bytes
+// would depend on a token's place in its step.
 template <int D>
 __device__ __forceinline__ void norm_row(Row &r, const Weights &w, float eps) {
+#pragma clang fp contract(off)
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum += r.a[e] * r.a[e] + r.b[e] * r.b[e];
-    const float inv = __builtin_amdgcn_rsqf(lanes_sum<D / 8>(sum) * (1.0f / D) + eps);  // to 1 ulp
+    for (int e = 0; e < 4; ++e) sum = fmaf(r.a[e], r.a[e], fmaf(r.b[e], r.b[e], sum));
+    const float inv = __builtin_amdgcn_rsqf(fmaf(lanes_sum<D / 8>(sum), 1.0f / D, eps));  // to 1 ulp
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         r.a[e] = r.a[e] * inv * w.a[e];
@@ -86,8 +90,10 @@ __device__ __forceinline__ void norm_row(Row &r, const Weights &w, float eps) {
     }
 }
 __device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s) {
-    const float x = a * c - b * s;
-    b = b * c + a * s;
+#pragma clang fp contract(off)
+    const float bs = b * s, as = a * s;
+    const float x = fmaf(a, c, -bs);
+    b = fmaf(b, c, as);
     a = x;
 }
 template <bool INTERLEAVED>
