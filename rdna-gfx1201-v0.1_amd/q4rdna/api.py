@@ -643,9 +643,8 @@ class KVCache:
         up to the sequence's length) as numbers."""
         shape, device = (tokens, self.kv_heads, self.head_dim), self.device
         step = self._step(batch, tokens)
-        rows = []
         if k is None:
-            k = torch.empty(shape, dtype=dtype, device=self.pages.device)
+            k = self.scales.new_empty(shape, dtype=dtype)
         else:
             _no_overlap(k, "k")
         if v is None:
