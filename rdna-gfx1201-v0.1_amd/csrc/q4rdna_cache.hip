@@ -185,8 +185,10 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
     const bool keep = block >= s.length / static_cast<int>(kKvBlock) - 1;
 
     // Rows: the block's K rows, then its V rows, a group of D / 8 lanes each,
-    // kEach of them in flight.
-    constexpr int kEach = 4;
+    // kEach of them in flight: an fp32 block's in one turn (four and eight:
+    // 128 tokens 10.5 and 9.7 us, 1024 14.7 and 12.9, one 4.0 and 4.1; bf16
+    // 128 10.4 and 10.1, 4096 24.1 and 24.5, one 3.8 and 4.0).
+    constexpr int kEach = sizeof(T) == 4 ? 8 : 4;
     const int lane = tid % kLanes;
     Weights weights;
     load_weights(weights, a.d.k_norm, place_of<INTERLEAVED>(lane, a.d.rotary));
@@ -435,10 +437,12 @@ __device__ void append_place(const AppendArgs &a, uint32_t unit, AppendStage<D> 
     append_block<D, INTERLEAVED, T>(a, s, i, head, block, st);
 }
 
-// a.q_rows rows (token, query head) of q, kEach per group of D / 8 lanes in flight.
+// a.q_rows rows (token, query head) of q, kEach per group of D / 8 lanes in
+// flight.  The waves of a CU are many here, and more rows each cost registers
+// (two, four and eight, fp32: 2048 tokens 18.1, 20.2 and 25.2 us).
 template <int D, bool INTERLEAVED, typename T>
 __device__ void turn_q(const AppendArgs &a, uint32_t unit) {
-    constexpr int kLanes = D / 8, kRows = 256 / kLanes, kEach = 4;
+    constexpr int kLanes = D / 8, kRows = 256 / kLanes, kEach = 2;
     const int lane = threadIdx.x % kLanes;
     const Place at = place_of<INTERLEAVED>(lane, a.d.rotary);
     Weights weights;

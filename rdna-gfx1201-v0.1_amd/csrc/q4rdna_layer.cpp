@@ -196,7 +196,7 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     // Few rows of q: one per lane group, so that many workgroups share the
     // wait for them; many: eight, which divides the workgroup's fixed part (32
     // bf16 heads of 128, one against eight: 32 tokens 6.7 and 7.1 us, 128
-    // tokens 10.4 and 10.4, 512 tokens 11.6 and 10.8, 2048 tokens 23.1 and 15.7).
+    // tokens 10.4 and 10.4, 512 tokens 11.6 and 10.8, 2048 tokens 23.1 and 15.4).
     const uint64_t all_rows = static_cast<uint64_t>(batch->tokens) * desc->q_heads;
     const uint32_t q_rows = all_rows <= 4096 ? 2048 / cache->head_dim : 16384 / cache->head_dim;
     const uint64_t q_units = (all_rows + q_rows - 1) / q_rows;
