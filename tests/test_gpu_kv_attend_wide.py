@@ -2,6 +2,10 @@
 what bounds the lengths when a call is made, so the same prompts go to the other
 of the two kernels here, and many sequences are dealt as if they could be long.
 The columns behind a sequence hold numbers that are no pages."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -114,3 +118,50 @@ def test_without_a_bound_on_the_tokens(cuda, kv_heads, sequences):
     out, lse = cache.attend(api.KVBatch(past_d, table, ends, slots_d), q, lse=True)
     assert cache.faults() == 0
     narrow.check(cache, table, slots, past, counts, q, out, "f32", lse)
+
+
+FIRST_CALL_CAPTURED = """
+import sys
+sys.path[:0] = sys.argv[1:3]
+import pytest, torch
+import test_gpu_kv_attend as narrow
+from q4rdna._lib import Q4RdnaError
+cache, table, slots = narrow.filled(1, 64, [3000], 39)
+batch = narrow.step([2999], [1], table, slots)
+q = narrow.normal((1, 2, 64), "f32", 40)
+out, count = torch.zeros_like(q), torch.zeros(1, device="cuda")
+stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    count += 1
+    with pytest.raises(Q4RdnaError, match="captured"):
+        cache.attend(batch, q, out=out)
+graph.replay()
+torch.cuda.synchronize()
+assert count.item() == 1 and (out == 0).all()
+want = cache.attend(batch, q)
+with torch.cuda.stream(stream):
+    cache.attend(batch, q, out=out)
+torch.cuda.synchronize()
+assert torch.equal(out, want)
+out.zero_()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    cache.attend(batch, q, out=out)
+for _ in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    out.zero_()
+print("captured")
+"""
+
+
+def test_a_first_call_under_capture_is_refused(cuda):
+    """In a fresh process, where no stream has scratch: the call that needs some
+    is refused under capture, the capture stays whole, and after one call outside
+    it the same call is captured."""
+    tests = os.path.dirname(os.path.abspath(__file__))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED, tests, os.path.dirname(tests)], capture_output=True,
+                         text=True, timeout=100)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
