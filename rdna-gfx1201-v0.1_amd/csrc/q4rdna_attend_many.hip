@@ -231,7 +231,8 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
     const float to_ref = v_ref > 0.0f ? __builtin_amdgcn_rcpf(v_ref) : 0.0f;
     float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m), per_r = 1.0f;
     if (!OPEN) {
-        const float r = v_scale < __builtin_inff() ? fmaxf(v_scale * to_ref, 0x1p-90f) : __builtin_nanf("");
+        // A row that sees nothing of the block adds zero to its sum, whatever the scale.
+        const float r = none ? 1.0f : v_scale < __builtin_inff() ? fmaxf(v_scale * to_ref, 0x1p-90f) : __builtin_nanf("");
         shift += __builtin_amdgcn_logf(r);
         per_r = __builtin_amdgcn_rcpf(r);
     }
