@@ -15,9 +15,11 @@
 //    fp16; the weights are rounded to fp16 (11 bits), finer than the output's
 //    rounding.  fp32 rows take two fp16 parts of q and of the weights each
 //    (SPLIT = 2, 22 bits) and twice the products, which keeps fp32's accuracy.
-//  * V's scale per block goes into the weights relative to the largest scale so
-//    far, so the accumulators are rescaled only when that or the row's maximum
-//    grows; the maximum is followed lazily, by steps of at least 2^8.
+//  * V's scale per block goes into the weights: they are relative to the largest
+//    product of a weight and a V scale that the row has had, not to the largest
+//    weight, so fp16's range is spent on what counts in the row's output, however
+//    far the blocks' scales lie apart.  That largest and the scores' maximum are
+//    the lane's own, followed lazily, by steps of at least 2^8.
 //  * The open block's two planes are two tiles: 256 * high is exact in fp16.
 //
 // Row groups are split over several workgroups along the blocks when there are
@@ -47,7 +49,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLazy = 8.0f;    // the maximum may trail by this much (base 2)
-constexpr float kWeight = 7.0f;  // weights are 2^7 p, at most 2^15, within fp16's range
+constexpr float kWeight = 7.0f;  // weights are 2^7 relative to their reference, at most 2^15, within fp16's range
+constexpr float kLeast = -90.0f; // a block's V scale counts as 2^-90 of the reference at least
 constexpr int kRowsMany = kAttendManyRows;
 
 // LDS tiles of a block in fp16: K [64 tokens][D + 8], V^T [D][64 + 8].  Rows
@@ -115,8 +118,8 @@ struct ManyState {
     h16x8 q[D / 16][SPLIT];
     float q_scale;    // base-2 score = q_scale * (k scale) * product
     int position;     // of the lane's row
-    float m, l;       // the maximum that the weights refer to; the lane's part of the sum, in units of 2^-7
-    float v_ref;      // accumulators are in units of 2^-7 v_ref
+    float m, l;       // the maximum that the sum refers to; the lane's part of the sum, in units of 2^(m - 7)
+    float e;          // a whole number, -inf while nothing was added: accumulators are in units of 2^(m + e - 7)
     f32x16 o[D / 32];
 };
 
@@ -127,6 +130,23 @@ __device__ __forceinline__ uint32_t first_tokens(int ahead) {
 }
 __device__ __forceinline__ uint32_t bit_mask(uint32_t bits, int i) {
     return static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - i)) >> 31);
+}
+
+// Moves the references where the row's next block needs it: m to its maximum
+// `now` and m + e to its largest weight times V scale, `top` (both base 2).
+template <int D, int SPLIT>
+__device__ __forceinline__ void refer(ManyState<D, SPLIT> &st, float now, float top) {
+    const bool grown = now > st.m + kLazy, more = top > st.m + st.e + kLazy;
+    if (__builtin_amdgcn_ballot_w64(grown || more) == 0) return;
+    if (!(grown || more)) return;
+    const float m = grown ? now : st.m, most = fmaxf(st.m + st.e, top);
+    const float e = most == kNegInf ? kNegInf : ceilf(most - m);
+    st.l *= __builtin_amdgcn_exp2f(st.m - m);  // 0 from -inf
+    const float f = st.e == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((st.m - m) + (st.e - e));  // (o is zero there)
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) st.o[d] *= f;
+    st.m = m;
+    st.e = e;
 }
 
 // One block from LDS.  OPEN: two tiles (256 * high, low), scales per token
@@ -202,10 +222,10 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
     const bool none = top == kNegInf;
     const float now = none ? kNegInf : top * unit;
 
-    // V's scale relative to the largest one so far; one that is not finite
-    // makes the seen weights NaN and leaves the reference alone.
+    // The block's scale of V, 2^(v_exp + v_log); in the open block the largest
+    // one of its tokens, one per lane.
     float largest = v_scale;
-    if (OPEN) {  // of the block's tokens, one per lane
+    if (OPEN) {
         const float mine = token_scales[kKvBlock + lane];
         largest = start + lane < length && mine < __builtin_inff() ? mine : 0.0f;
         largest = fmaxf(largest, dpp<kDppXor1>(largest));
@@ -214,28 +234,14 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         largest = fmaxf(largest, dpp<kDppMirror16>(largest));
         largest = max_xor32(max_xor16(largest));
     }
-    const float v_ref = largest < __builtin_inff() ? fmaxf(st.v_ref, largest) : st.v_ref;
-    const bool grown = now > st.m + kLazy;
-    if (__builtin_amdgcn_ballot_w64(grown || v_ref != st.v_ref) != 0) {
-        const float m = grown ? now : st.m;
-        const float alpha = grown ? __builtin_amdgcn_exp2f(st.m - m) : 1.0f;  // 0 from -inf
-        const float beta = v_ref > 0.0f ? st.v_ref / v_ref : 1.0f;
-        st.l *= alpha;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) st.o[d] *= alpha * beta;
-        st.m = m;
-        st.v_ref = v_ref;
-    }
-    // A full block's ratio goes into the exponent (and comes out of the sum);
-    // under 2^-90 of the largest scale it might as well be that.
-    const float to_ref = v_ref > 0.0f ? __builtin_amdgcn_rcpf(v_ref) : 0.0f;
-    float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m), per_r = 1.0f;
-    if (!OPEN) {
-        // A row that sees nothing of the block adds zero to its sum, whatever the scale.
-        const float r = none ? 1.0f : v_scale < __builtin_inff() ? fmaxf(v_scale * to_ref, 0x1p-90f) : __builtin_nanf("");
-        shift += __builtin_amdgcn_logf(r);
-        per_r = __builtin_amdgcn_rcpf(r);
-    }
+    const bool finite = largest < __builtin_inff();
+    const float v_exp = static_cast<float>(__builtin_amdgcn_frexp_expf(largest));
+    const float v_log = finite ? __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(largest)) : __builtin_nanf("");
+    refer(st, now, now + (v_exp + v_log));
+    // The scale goes into the exponent, and comes out of the sum.
+    const float ratio = none ? 0.0f : finite ? fmaxf(v_log + (v_exp - st.e), kLeast) : __builtin_nanf("");
+    const float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m) + ratio;
+    const float per_ratio = __builtin_amdgcn_exp2f(-ratio);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -247,6 +253,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
             for (int i = 0; i < 16; ++i) s[t][i] = __uint_as_float(__float_as_uint(s[t][i]) & bit_mask(seen, 16 * t + i));
     };
     if (masked) hide();
+    const float to_largest = OPEN && largest > 0.0f ? __builtin_amdgcn_rcpf(largest) : 0.0f;
     float sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
@@ -254,7 +261,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         if (OPEN) {
             const f32x4 vt = *(gptr_f32x4)(uintptr_t)(token_scales + kKvBlock + 8 * x + 4 * half);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) w[b] = vt[b] < __builtin_inff() ? vt[b] * to_ref : __builtin_nanf("");
+            for (int b = 0; b < 4; ++b) w[b] = vt[b] < __builtin_inff() ? vt[b] * to_largest : __builtin_nanf("");
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -264,7 +271,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
         }
     }
     if (OPEN) hide();
-    st.l += sum * per_r;
+    st.l += sum * per_ratio;
     tile_end();
     // Products 2 parity + pair: tokens 16 a + 8 parity + 4 half + b, a = 2 pair, 2 pair + 1.
 #pragma unroll
@@ -314,7 +321,7 @@ __device__ __forceinline__ void load_q_many(ManyState<D, SPLIT> &st, const Atten
     st.q_scale = finite ? __builtin_amdgcn_ldexpf(a.d.scale * kLog2e, -up) : __builtin_nanf("");
     st.m = kNegInf;
     st.l = 0.0f;
-    st.v_ref = 0.0f;
+    st.e = kNegInf;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -439,7 +446,8 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const uint32_t h = head * a.group + (live ? row - token * group : 0);
     const uint32_t job = place * heads + head;
     // Parts lie as [number][row]: a lane's row, so neighbouring lanes side by side.
-    float m_row = st.m, l_row = l, o_unit = st.v_ref;
+    // The result's unit is 2^(factor's logarithm + up).
+    float m_row = st.m, l_row = l, factor = 1.0f, up = st.e;
     if (splits > 1) {
         const size_t first_slot = static_cast<size_t>(job) * a.splits;
         float *stats = a.partials + static_cast<size_t>(gridDim.x) * kRowsMany * D;
@@ -449,10 +457,12 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                store_agent(part + (32 * d + 8 * (i / 4) + 4 * half + i % 4) * kRowsMany, st.o[d][i] * st.v_ref);
+                store_agent(part + (32 * d + 8 * (i / 4) + 4 * half + i % 4) * kRowsMany, st.o[d][i]);
+        float *stat = stats + first_slot * 3 * kRowsMany + r;  // of part i: m, l and e at i * 3 * kRowsMany
         if (half == 0) {
-            store_agent(stats + (first_slot + split) * 2 * kRowsMany + r, st.m);
-            store_agent(stats + (first_slot + split) * 2 * kRowsMany + kRowsMany + r, l);
+            store_agent(stat + split * 3 * kRowsMany, st.m);
+            store_agent(stat + split * 3 * kRowsMany + kRowsMany, l);
+            store_agent(stat + split * 3 * kRowsMany + 2 * kRowsMany, st.e);
         }
         wait_stores();
         __syncthreads();
@@ -463,17 +473,26 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         // The last to arrive reads all parts, its own too, in their order: the
         // result does not depend on which one it was.
         m_row = kNegInf;
-        for (int i = 0; i < splits; ++i) m_row = fmaxf(m_row, load_agent(stats + (first_slot + i) * 2 * kRowsMany + r));
+        up = kNegInf;
+        float m_up = 0.0f;  // the part with the largest unit has m_up and up
+        for (int i = 0; i < splits; ++i) {
+            const float m = load_agent(stat + i * 3 * kRowsMany), e = load_agent(stat + i * 3 * kRowsMany + 2 * kRowsMany);
+            m_row = fmaxf(m_row, m);
+            if (m + e > m_up + up) {
+                m_up = m;
+                up = e;
+            }
+        }
         const float ref = m_row == kNegInf ? 0.0f : m_row;
         l_row = 0.0f;
-        o_unit = 1.0f;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) st.o[d][i] = 0.0f;
         for (int y = 0; y < splits; ++y) {
-            const float f = __builtin_amdgcn_exp2f(load_agent(stats + (first_slot + y) * 2 * kRowsMany + r) - ref);
-            l_row += load_agent(stats + (first_slot + y) * 2 * kRowsMany + kRowsMany + r) * f;
+            const float m = load_agent(stat + y * 3 * kRowsMany), e = load_agent(stat + y * 3 * kRowsMany + 2 * kRowsMany);
+            l_row += load_agent(stat + y * 3 * kRowsMany + kRowsMany) * __builtin_amdgcn_exp2f(m - ref);
+            const float f = e == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((m - m_up) + (e - up));  // (such a part is zero)
             const float *from_part = a.partials + (first_slot + y) * kRowsMany * D + r;
             float v[D / 32][16];
 #pragma unroll
@@ -485,9 +504,15 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) st.o[d][i] = fmaf(v[d][i], f, st.o[d][i]);
         }
+        if (up != kNegInf) {  // m_up <= m_row: the difference's whole part goes to `up`
+            const float whole = rintf(m_up - m_row);
+            factor = __builtin_amdgcn_exp2f((m_up - m_row) - whole);
+            up += whole;
+        }
     }
     if (!live) return;
-    const float inv = l_row == 0.0f ? 0.0f : o_unit / l_row;
+    const float inv = l_row == 0.0f ? 0.0f : factor / l_row;
+    const int places = static_cast<int>(fminf(fmaxf(up, -400.0f), 400.0f));
     T *out = static_cast<T *>(a.d.out.data) + static_cast<int64_t>(s.first + token) * a.d.out.token_stride + h * a.d.out.head_stride;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -495,7 +520,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         for (int x = 0; x < 4; ++x) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = st.o[d][4 * x + e] * inv;
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(st.o[d][4 * x + e] * inv, places);
             store_floats<T, 4>(out + 32 * d + 8 * x + 4 * half, a.wide_out != 0, v);
         }
     if (a.d.lse != nullptr && half == 0)

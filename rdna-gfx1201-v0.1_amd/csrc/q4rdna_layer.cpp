@@ -243,13 +243,14 @@ uint32_t few_rows(const q4rdna_kv_batch &b, uint32_t group, uint32_t kv_heads, u
 // and 309, 326 and 224).
 constexpr uint32_t kDealtSequences = 256;
 
-// Room for partial results of `rows` rows, and arrival counters of `jobs` row groups.
-int take_scratch(q4rdna::AttendArgs &a, size_t rows, size_t jobs, hipStream_t stream) {
+// Room for partial results of `rows` rows with `stats` numbers beside each, and
+// arrival counters of `jobs` row groups.
+int take_scratch(q4rdna::AttendArgs &a, size_t rows, size_t stats, size_t jobs, hipStream_t stream) {
     a.partials = nullptr;
     a.arrived = nullptr;
     if (a.splits == 1) return Q4RDNA_OK;
     Scratch s;
-    const int rc = get_scratch(a.cache.device, stream, rows * (a.cache.head_dim + 2), jobs, &s);
+    const int rc = get_scratch(a.cache.device, stream, rows * (a.cache.head_dim + stats), jobs, &s);
     a.partials = s.partials;
     a.arrived = s.arrived;
     return rc;
@@ -306,7 +307,7 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
         const uint64_t workgroups = split ? std::min(jobs + a.target, jobs * a.splits) : jobs;
         if (workgroups > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences are too many for one call", batch->sequences);
         a.workgroups = static_cast<uint32_t>(workgroups);
-        if ((rc = take_scratch(a, workgroups * rows, jobs, s)) != Q4RDNA_OK ||
+        if ((rc = take_scratch(a, workgroups * rows, 2, jobs, s)) != Q4RDNA_OK ||
             (rc = launched(q4rdna::launch_attend_few(a, rows, waves, s), "kv_attend")) != Q4RDNA_OK)
             return rc;
     }
@@ -317,7 +318,7 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
         const uint64_t splits = std::min<uint64_t>(2ull * cus / jobs, (most_blocks + 1) / 2);
         a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 64)));
         a.cu_units = std::max(1u, cus / cache->kv_heads);
-        if ((rc = take_scratch(a, jobs * a.splits * q4rdna::kAttendManyRows, jobs, s)) != Q4RDNA_OK ||
+        if ((rc = take_scratch(a, jobs * a.splits * q4rdna::kAttendManyRows, 3, jobs, s)) != Q4RDNA_OK ||
             (rc = launched(q4rdna::launch_attend_many(a, static_cast<uint32_t>(places), s), "kv_attend")) != Q4RDNA_OK)
             return rc;
     }

@@ -62,8 +62,9 @@ struct AttendArgs {
                           // attend_many_kernel
     uint32_t wide;        // q rows can be read 16 bytes at a time
     uint32_t wide_out;    // out rows can be written four elements at a time
-    float *partials;      // of each workgroup (attend_few_kernel) or [job][split]: [row][D], then all the
-                          // maxima and sums, [row][2]
+    float *partials;      // of each workgroup (attend_few_kernel): [row][D], then all the maxima and sums,
+                          // [row][2]; of [job][split] (attend_many_kernel): [D][row], then all the
+                          // maxima, sums and units, [3][row]
     uint32_t *arrived;    // [job], zero between launches
 };
 // The most workgroups that share a row group of attend_few_kernel.
