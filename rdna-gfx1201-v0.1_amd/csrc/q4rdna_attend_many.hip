@@ -20,7 +20,10 @@
 //    weight, so fp16's range is spent on what counts in the row's output, however
 //    far the blocks' scales lie apart.  That largest and the scores' maximum are
 //    the lane's own, followed lazily, by steps of at least 2^8.
-//  * The open block's two planes are two tiles: 256 * high is exact in fp16.
+//  * The open block's two planes are two tiles, high and low / 256, both exact in
+//    fp16; so its codes are as large as a full block's, and its scales 256 times
+//    the tokens' own.  Its weights refer to the largest product of a weight and a
+//    scale among the tokens that the row sees.
 //
 // Row groups are split over several workgroups along the blocks when there are
 // too few of them; the last to arrive joins the parts in a fixed order.
@@ -69,13 +72,13 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, h16x2 &lo, h16x2 &hi) 
     lo = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias;
     hi = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias;
 }
-template <bool HIGH>
+template <bool LOW>
 __device__ __forceinline__ void piece_to_lds(_Float16 *at, i32x4 piece) {
     h16x2 x[8];
 #pragma unroll
     for (int w = 0; w < 4; ++w) codes_to_half(static_cast<uint32_t>(piece[w]), x[2 * w], x[2 * w + 1]);
-    if (HIGH) {
-        const h16x2 f = {static_cast<_Float16>(256.0f), static_cast<_Float16>(256.0f)};
+    if (LOW) {
+        const h16x2 f = {static_cast<_Float16>(0x1p-8f), static_cast<_Float16>(0x1p-8f)};
 #pragma unroll
         for (int w = 0; w < 8; ++w) x[w] *= f;
     }
@@ -101,15 +104,15 @@ __device__ __forceinline__ void load_raw(Raw<D> &r, const int8_t *k, const int8_
         r.v[i] = load16(v + 16 * (threadIdx.x + 256 * i));
     }
 }
-template <bool HIGH, int D>
+template <bool LOW, int D>
 __device__ __forceinline__ void stage_raw(ManyTile<D> &t, const Raw<D> &r) {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
         const int piece = threadIdx.x + 256 * i, c = piece % 16, g = piece / 16 % 4;
         const int token = piece / (64 * (D / 64)) * 16 + c, number = piece / 64 % (D / 64) * 64 + g * 16;
-        piece_to_lds<HIGH>(t.k + token * (D + 8) + number, r.k[i]);
+        piece_to_lds<LOW>(t.k + token * (D + 8) + number, r.k[i]);
         // Row d: [half of the wave][product][8 tokens]; a piece is one half's two products.
-        piece_to_lds<HIGH>(t.v + (piece / 64 * 16 + c) * (kKvBlock + 8) + (g & 1) * 32 + (g >> 1) * 16, r.v[i]);
+        piece_to_lds<LOW>(t.v + (piece / 64 * 16 + c) * (kKvBlock + 8) + (g & 1) * 32 + (g >> 1) * 16, r.v[i]);
     }
 }
 
@@ -149,11 +152,11 @@ __device__ __forceinline__ void refer(ManyState<D, SPLIT> &st, float now, float 
     st.e = e;
 }
 
-// One block from LDS.  OPEN: two tiles (256 * high, low), scales per token
-// (kt, vt); otherwise k_scale and v_scale.
+// One block from LDS.  OPEN: two tiles (high, low / 256), scales per token (kt,
+// vt, of 16-bit codes); otherwise k_scale and v_scale.
 template <bool OPEN, int D, int SPLIT>
 __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTile<D> *tile, float k_scale, float v_scale,
-                                           const float *token_scales, int start, int length, uint32_t window, bool masked) {
+                                           const float *token_scales, int start, uint32_t window, bool masked) {
     constexpr int KF = D / 16, VF = D / 32;  // fragments per product's tile
     const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
     const int k_at = column * (D + 8) + 8 * half, v_at = column * (kKvBlock + 8) + 32 * half;
@@ -212,7 +215,7 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
                 s[t][i] = __uint_as_float((__float_as_uint(s[t][i]) & m) | (__float_as_uint(kNegInf) & ~m));
             }
     }
-    const float unit = OPEN ? st.q_scale : st.q_scale * k_scale;
+    const float unit = OPEN ? 256.0f * st.q_scale : st.q_scale * k_scale;
     float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -222,56 +225,60 @@ __device__ __forceinline__ void many_block(ManyState<D, SPLIT> &st, const ManyTi
     const bool none = top == kNegInf;
     const float now = none ? kNegInf : top * unit;
 
-    // The block's scale of V, 2^(v_exp + v_log); in the open block the largest
-    // one of its tokens, one per lane.
-    float largest = v_scale;
-    if (OPEN) {
-        const float mine = token_scales[kKvBlock + lane];
-        largest = start + lane < length && mine < __builtin_inff() ? mine : 0.0f;
-        largest = fmaxf(largest, dpp<kDppXor1>(largest));
-        largest = fmaxf(largest, dpp<kDppXor2>(largest));
-        largest = fmaxf(largest, dpp<kDppMirror8>(largest));
-        largest = fmaxf(largest, dpp<kDppMirror16>(largest));
-        largest = max_xor32(max_xor16(largest));
-    }
-    const bool finite = largest < __builtin_inff();
-    const float v_exp = static_cast<float>(__builtin_amdgcn_frexp_expf(largest));
-    const float v_log = finite ? __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(largest)) : __builtin_nanf("");
-    refer(st, now, now + (v_exp + v_log));
-    // The scale goes into the exponent, and comes out of the sum.
-    const float ratio = none ? 0.0f : finite ? fmaxf(v_log + (v_exp - st.e), kLeast) : __builtin_nanf("");
-    const float shift = kWeight - (st.m == kNegInf ? 0.0f : st.m) + ratio;
-    const float per_ratio = __builtin_amdgcn_exp2f(-ratio);
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unit, shift));
     auto hide = [&] {  // whatever the unit and the scales are
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[t][i] = __uint_as_float(__float_as_uint(s[t][i]) & bit_mask(seen, 16 * t + i));
     };
-    if (masked) hide();
-    const float to_largest = OPEN && largest > 0.0f ? __builtin_amdgcn_rcpf(largest) : 0.0f;
-    float sum = 0.0f;
+    const auto exponentials = [&](float shift) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-        f32x4 w;
-        if (OPEN) {
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unit, shift));
+        if (masked) hide();
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += s[t][i];
+        return sum;
+    };
+    if (OPEN) {
+        // Weights of 2^8 at most times the scales, under 2^114, in fp32; the
+        // largest of them is what the row refers to.
+        const float m = now > st.m + kLazy ? now : st.m;
+        const float sum = exponentials(m == kNegInf ? 0.0f : -m);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
             const f32x4 vt = *(gptr_f32x4)(uintptr_t)(token_scales + kKvBlock + 8 * x + 4 * half);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) w[b] = vt[b] < __builtin_inff() ? vt[b] * to_largest : __builtin_nanf("");
+            for (int b = 0; b < 4; ++b) s[x / 4][4 * (x % 4) + b] *= vt[b] + (vt[b] - vt[b]);  // an infinite scale is made NaN
         }
+        hide();
+        float most = 0.0f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int i = 4 * (x % 4) + b;
-            sum += s[x / 4][i];
-            if (OPEN) s[x / 4][i] *= w[b];
-        }
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
+        refer(st, now, m + __builtin_amdgcn_logf(max_xor32(most)) + 8.0f);
+        st.l += __builtin_amdgcn_ldexpf(sum, static_cast<int>(kWeight));
+        // From units of 2^(m + 8) to the accumulators'.
+        const int up = st.e == kNegInf ? 0 : 8 + static_cast<int>(kWeight) - static_cast<int>(st.e);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_ldexpf(s[t][i], up);
+    } else {
+        // The block's scale of V, 2^(v_exp + v_log), goes into the exponent, and comes out of the sum.
+        const bool finite = v_scale < __builtin_inff();
+        const float v_exp = static_cast<float>(__builtin_amdgcn_frexp_expf(v_scale));
+        const float v_log = finite ? __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(v_scale)) : __builtin_nanf("");
+        refer(st, now, now + (v_exp + v_log));
+        const float ratio = none ? 0.0f : finite ? fmaxf(v_log + (v_exp - st.e), kLeast) : __builtin_nanf("");
+        const float sum = exponentials(kWeight - (st.m == kNegInf ? 0.0f : st.m) + ratio);
+        st.l += sum * __builtin_amdgcn_exp2f(-ratio);
     }
-    if (OPEN) hide();
-    st.l += sum * per_ratio;
     tile_end();
     // Products 2 parity + pair: tokens 16 a + 8 parity + 4 half + b, a = 2 pair, 2 pair + 1.
 #pragma unroll
@@ -420,7 +427,7 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
         if (!away) {
             const bool masked = start + block_size - 1 > wave_first ||
                                 (a.d.window != 0 && static_cast<uint32_t>(wave_last - start) >= a.d.window);
-            many_block<false, D, SPLIT>(st, &tiles[buffer], scale[0], scale[1], nullptr, start, s.length, a.d.window, masked);
+            many_block<false, D, SPLIT>(st, &tiles[buffer], scale[0], scale[1], nullptr, start, a.d.window, masked);
         }
         if (b + 1 < to_full) stage_raw<false, D>(tiles[buffer ^ 1], raw);
         __syncthreads();
@@ -428,14 +435,14 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     if (has_open) {
         const int8_t *planes = a.cache.open + open_tile(a.cache, s.slot, to - 1, head);
         load_raw<D>(raw, planes, planes + 2 * kPlane);
-        stage_raw<true, D>(tiles[0], raw);
+        stage_raw<false, D>(tiles[0], raw);
         load_raw<D>(raw, planes + kPlane, planes + 3 * kPlane);
-        stage_raw<false, D>(tiles[1], raw);
+        stage_raw<true, D>(tiles[1], raw);
         __syncthreads();
         const int start = (to - 1) * block_size;
         if (start <= wave_last)
             many_block<true, D, SPLIT>(st, tiles, 0.0f, 0.0f,
-                                       a.cache.open_scales + open_scale_row(a.cache, s.slot, to - 1, head), start, s.length,
+                                       a.cache.open_scales + open_scale_row(a.cache, s.slot, to - 1, head), start,
                                        a.d.window, true);
     }
 
