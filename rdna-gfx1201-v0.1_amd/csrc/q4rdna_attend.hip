@@ -194,8 +194,8 @@ __device__ __forceinline__ void add_values(f32x4 (&o)[D / 16], const i32x4 (&v)[
 }
 
 // The open block: codes in two planes, scales per token.  K's token scales
-// multiply the scores; V's are folded into the weights, relative to the
-// largest of them.
+// multiply the scores; V's are folded into the weights, which become fixed point
+// relative to the largest product of the two that the row sees.
 template <int D, int QT>
 __device__ __forceinline__ void few_open_block(FewState<D, QT> &st, const int8_t *planes, const float *scales, int start,
                                                uint32_t window) {
@@ -221,31 +221,31 @@ __device__ __forceinline__ void few_open_block(FewState<D, QT> &st, const int8_t
         tile_end();
         load_tiles<D>(high, planes + 2 * kPlane);
         load_tiles<D>(low, planes + 3 * kPlane);
-        f32x4 vs[4];
-        float v_top = 0.0f, poison = 0.0f;
+        const float factor = softmax_block<QT>(s, st.m[qt], st.l[qt], st.o[qt]);
+        float most = 0.0f, poison = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            vs[t] = *(gptr_f32x4)(uintptr_t)(scales + 64 + 16 * t + 4 * group);
+            const f32x4 vs = *(gptr_f32x4)(uintptr_t)(scales + 64 + 16 * t + 4 * group);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                vs[t][i] = __uint_as_float(__float_as_uint(vs[t][i]) & bit_mask(seen, 4 * t + i));
-                v_top = fmaxf(v_top, vs[t][i]);
-                poison += vs[t][i] - vs[t][i];  // NaN where a seen scale is not finite
+                const float scale = __uint_as_float(__float_as_uint(vs[i]) & bit_mask(seen, 4 * t + i));
+                poison += scale - scale;  // NaN where a seen scale is not finite
+                s[t][i] *= scale;
+                most = fmaxf(most, s[t][i]);
             }
         }
-        v_top = max_xor32(max_xor16(v_top));
+        most = max_xor32(max_xor16(most));
         poison = add_xor32(add_xor16(poison));
-        const float factor = softmax_block<QT>(s, st.m[qt], st.l[qt], st.o[qt]);
-        const float inv = v_top > 0.0f ? 1.0f / v_top : 0.0f;
+        const float inv = most >= 0x1p-126f ? 1.0f / most : 0.0f;  // (32512 of less is under 1e-30, which reads as zero)
         i32x4 p;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             int x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = fixed30(s[t][i] * (vs[t][i] * inv));
+            for (int i = 0; i < 4; ++i) x[i] = fixed30(s[t][i] * inv);
             p[t] = digits4(x[0], x[1], x[2], x[3], st.pick);
         }
-        const float w = v_top * factor * (st.weight * 0x1p-30f) + poison;
+        const float w = most * factor * (st.weight * 0x1p-30f) + poison;
         add_values<D>(st.o[qt], high, p, 256.0f * w);
         add_values<D>(st.o[qt], low, p, w);
         tile_end();
