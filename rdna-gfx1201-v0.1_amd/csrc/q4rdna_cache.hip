@@ -228,8 +228,9 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 top = lanes_max<kLanes>(top);
                 const float largest = __uint_as_float(top);
                 const bool finite = top < 0x7f800000u, some = finite && largest >= kKvZero;
-                // Codes by a reciprocal of 1 ulp: they move by under 0.01 of a step.
-                const float inv = some ? kKvCode16 * __builtin_amdgcn_rcpf(largest) : 0.0f;
+                // A full division: from 2^126 on the reciprocal alone would be
+                // subnormal, which the bare instruction gives as zero.
+                const float inv = some ? kKvCode16 / largest : 0.0f;
                 short *out = &st.code[is_v][t * kRow<D>];
                 *reinterpret_cast<s16x4 *>(out + at.a_at) = pack_codes(r[x].a, inv);
                 *reinterpret_cast<s16x4 *>(out + at.b_at) = pack_codes(r[x].b, inv);
