@@ -82,7 +82,7 @@ __device__ __forceinline__ void norm_row(Row &r, const Weights &w, float eps) {
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum = fmaf(r.a[e], r.a[e], fmaf(r.b[e], r.b[e], sum));
-    const float inv = __builtin_amdgcn_rsqf(fmaf(lanes_sum<D / 8>(sum), 1.0f / D, eps));  // to 1 ulp
+    const float inv = inverse_root(fmaf(lanes_sum<D / 8>(sum), 1.0f / D, eps));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         r.a[e] = r.a[e] * inv * w.a[e];

@@ -4,8 +4,12 @@
 //
 // One pass over memory: a workgroup keeps its row in registers between the two
 // sums (mean y^2, then mean h^2), so every input is read once and every output
-// written once.  Sums and products are in fp32; the weights stay fp32, since
-// models keep them so and they come from the L2.
+// written once.  Products are in fp32; the sums of squares go on in 64 bits from
+// four numbers on, so the factor does not depend on the order of the sum, which
+// differs between aligned and unaligned rows.  That costs small calls a tenth of a
+// microsecond (77 rows of 1111 in fp16, both norms: 3.6 us, with fp32 sums 3.5; 64
+// rows of 8192 4.1 and 3.75).  The weights stay fp32, since models keep them so and
+// they come from the L2.
 //
 // Many rows are bound by the memory: 8192 rows of 4096 in bf16 (residual and y
 // in, h and n out, 268 MB) take 39 us where the inputs are in the Infinity
@@ -16,25 +20,90 @@
 namespace q4rdna {
 namespace {
 
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t low = dpp<CTRL>(static_cast<uint32_t>(b)), high = dpp<CTRL>(static_cast<uint32_t>(b >> 32));
+    return __builtin_bit_cast(double, high << 32 | low);
+}
+// v + v of lane ^ 16 and of lane ^ 32.
+__device__ __forceinline__ double sum_rows(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const auto low = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(b), static_cast<uint32_t>(b), false, false);
+    const auto high = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(b >> 32), static_cast<uint32_t>(b >> 32), false, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(high[0]) << 32 | low[0]) +
+           __builtin_bit_cast(double, static_cast<uint64_t>(high[1]) << 32 | low[1]);
+}
+__device__ __forceinline__ double sum_halves(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const auto low = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(b), static_cast<uint32_t>(b), false, false);
+    const auto high = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(b >> 32), static_cast<uint32_t>(b >> 32), false, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(high[0]) << 32 | low[0]) +
+           __builtin_bit_cast(double, static_cast<uint64_t>(high[1]) << 32 | low[1]);
+}
+
 // The workgroup's sum of v; `slots` is the caller's own for each sum, so one
 // barrier is enough.
 template <int NT>
-__device__ __forceinline__ float block_sum(float v, float *slots) {
-    v = lanes_sum<16>(v);
-    v = add_xor32(add_xor16(v));
+__device__ __forceinline__ double block_sum(double v, double *slots) {
+    static_assert(NT == 64 || NT == 256 || NT == 512 || NT == 1024, "a sum over 4, 8 or 16 lanes joins the waves");
+    v += dpp64<kDppXor1>(v);
+    v += dpp64<kDppXor2>(v);
+    v += dpp64<kDppMirror8>(v);
+    v += dpp64<kDppMirror16>(v);
+    v = sum_halves(sum_rows(v));
     if (NT == 64) return v;
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
     __syncthreads();
-    float sum = 0.0f;
+    v = slots[threadIdx.x % (NT / 64)];
+    v += dpp64<kDppXor1>(v);
+    v += dpp64<kDppXor2>(v);
+    if (NT >= 512) v += dpp64<kDppMirror8>(v);
+    if (NT >= 1024) v += dpp64<kDppMirror16>(v);
+    return v;
+}
+// The sum of a thread's squares: four neighbours in fp32, in one order whether
+// they lie in a thread or, one each, in a quad of lanes (which each get a quarter
+// of it); those sums in 64 bits.
+template <int CH, int VEC>
+__device__ __forceinline__ double squares(const float (&x)[CH][VEC]) {
+#pragma clang fp contract(off)
+    double sum = 0.0;
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) sum += slots[w];
-    return sum;
+    for (int c = 0; c < CH; ++c) {
+        if (VEC == 1) {
+            float four = x[c][0] * x[c][0];
+            four += dpp<kDppXor1>(four);
+            four += dpp<kDppXor2>(four);
+            sum += four;
+        } else {
+#pragma unroll
+            for (int e = 0; e + 3 < VEC; e += 4) {
+                const float a = x[c][e] * x[c][e] + x[c][e + 1] * x[c][e + 1];
+                const float b = x[c][e + 2] * x[c][e + 2] + x[c][e + 3] * x[c][e + 3];
+                sum += a + b;
+            }
+        }
+    }
+    return VEC == 1 ? 0.25 * sum : sum;
+}
+
+// The norm's factor, 1 / sqrt(sum / width + eps), rounded once: the sum is in 64
+// bits and so is the step of Newton's iteration on the instruction's result (1
+// ulp).  A mean square outside fp32's normal range keeps that result: zero above
+// it, infinity below.
+__device__ __forceinline__ float norm_factor(double sum, double per_width, float eps) {
+    const double x = fma(sum, per_width, static_cast<double>(eps));
+    const float y = __builtin_amdgcn_rsqf(static_cast<float>(x));
+    const double y64 = y;
+    const float rest = static_cast<float>(fma(-x * y64, y64, 1.0));
+    return y > 0.0f && y < __builtin_inff() ? fmaf(0.5f * y, rest, y) : y;
 }
 
 // NT threads a row, CH runs of VEC numbers per thread.
 template <typename T, int VEC, int NT, int CH>
-__global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc d) {
-    __shared__ float slots[2][NT / 64];
+__global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc d, double per_width) {
+    __shared__ double slots[2][NT / 64];
     const uint32_t row = blockIdx.x;
     const T *res = static_cast<const T *>(d.residual) + row * d.residual_stride;
     const uint32_t width = d.width;
@@ -64,13 +133,8 @@ __global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc
             }
         }
         if (d.post_weight != nullptr) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) sum += y[c][e] * y[c][e];
-            sum = block_sum<NT>(sum, slots[0]);
-            const float inv = 1.0f / sqrtf(sum / static_cast<float>(width) + d.eps);
+            const double sum = block_sum<NT>(squares(y), slots[0]);
+            const float inv = norm_factor(sum, per_width, d.eps);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const uint32_t at = (c * NT + threadIdx.x) * VEC;
@@ -109,17 +173,8 @@ __global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc
         }
     }
     if (d.n == nullptr) return;
-    float sum = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        const uint32_t at = (c * NT + threadIdx.x) * VEC;
-        if (at < width) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) sum += h[c][e] * h[c][e];
-        }
-    }
-    sum = block_sum<NT>(sum, slots[1]);
-    const float inv = 1.0f / sqrtf(sum / static_cast<float>(width) + d.eps);
+    const double sum = block_sum<NT>(squares(h), slots[1]);
+    const float inv = norm_factor(sum, per_width, d.eps);
     T *out = static_cast<T *>(d.n) + row * d.n_stride;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -136,7 +191,7 @@ __global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc
 
 template <typename T, int VEC>
 hipError_t launch(const q4rdna_add_norm_desc &d, uint32_t cus, hipStream_t stream) {
-    auto go = [&](auto kernel, uint32_t threads) { kernel<<<d.rows, threads, 0, stream>>>(d); };
+    auto go = [&](auto kernel, uint32_t threads) { kernel<<<d.rows, threads, 0, stream>>>(d, 1.0 / d.width); };
     const uint32_t runs = (d.width + VEC - 1) / VEC;  // per row
     // A run per thread is the shortest chain, and up to 512 threads the faster
     // one at any number of rows (fp16/bf16 rows of 4096, against two runs in
