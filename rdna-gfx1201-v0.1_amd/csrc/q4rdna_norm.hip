@@ -89,15 +89,19 @@ __device__ __forceinline__ double squares(const float (&x)[CH][VEC]) {
 }
 
 // The norm's factor, 1 / sqrt(sum / width + eps), rounded once: the sum is in 64
-// bits and so is the step of Newton's iteration on the instruction's result (1
-// ulp).  A mean square outside fp32's normal range keeps that result: zero above
-// it, infinity below.
+// bits and so is the remainder of the step of Newton's iteration on the
+// instruction's result (1 ulp).  The instruction takes no subnormal number, so
+// small ones are scaled by 2^128; above fp32's range it gives zero, and infinity
+// for zero.
 __device__ __forceinline__ float norm_factor(double sum, double per_width, float eps) {
-    const double x = fma(sum, per_width, static_cast<double>(eps));
+    const double mean = fma(sum, per_width, static_cast<double>(eps));
+    const bool tiny = mean < 0x1p-100;
+    const double x = tiny ? mean * 0x1p128 : mean;
     const float y = __builtin_amdgcn_rsqf(static_cast<float>(x));
     const double y64 = y;
     const float rest = static_cast<float>(fma(-x * y64, y64, 1.0));
-    return y > 0.0f && y < __builtin_inff() ? fmaf(0.5f * y, rest, y) : y;
+    const float root = y > 0.0f && y < __builtin_inff() ? fmaf(0.5f * y, rest, y) : y;
+    return tiny ? root * 0x1p64f : root;
 }
 
 // NT threads a row, CH runs of VEC numbers per thread.

@@ -62,3 +62,16 @@ def test_rows_whose_squares_pass_fp32_s_range(cuda):
     for n in (api.add_norm(x, None, one, eps=1e-6)[1],
               cache.append(step([0], [4], ints([[0]])), k, k, q=x[:, None], q_norm=one, eps=1e-6)[:, 0]):
         assert (n[0] == 0).all() and (n[1] == 0).all() and (n[3] == 1).all()
+
+
+def test_rows_whose_squares_are_subnormal(cuda):
+    from q4rdna import api
+    x = torch.full((3, 64), 2.0 ** -70, device="cuda")
+    x[1] *= -0.5
+    x[2, 1:] = 0
+    one = torch.ones(64, device="cuda")
+    want = f64(x) / np.sqrt(np.mean(f64(x) ** 2, axis=-1, keepdims=True))  # powers of two
+    cache, k = make_cache(1, 64, 1, 1), torch.zeros((3, 1, 64), device="cuda")
+    for n in (api.add_norm(x, None, one, eps=0.0)[1], api.add_norm(torch.zeros_like(x), x, None, post_weight=one, eps=0.0)[0],
+              cache.append(step([0], [3], ints([[0]])), k, k, q=x[:, None], q_norm=one, eps=0.0)[:, 0]):
+        assert np.array_equal(f64(n), want)
