@@ -446,6 +446,14 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: 
 _NO_ROWS = (0, 0, 0)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new tensor for an output of t's shape, its rows' numbers contiguous.
+    (torch lays it out in the order of t's strides, which puts the numbers
+    elsewhere where t's rows overlap, as a sliding window's do.)"""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _no_overlap(t: torch.Tensor, name: str) -> None:
     """An output whose rows share memory would be written by several rows at once."""
     if not t.is_contiguous():
@@ -583,7 +591,7 @@ class KVCache:
             shape = (tokens, q_heads, dim)
             q_rows = _rows(q, "q", dtype, shape, device)
             if q_out is None:
-                q_out = torch.empty_like(q)
+                q_out = _like(q)
                 out_rows = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
             else:
                 _no_overlap(q_out, "q_out")
@@ -621,7 +629,7 @@ class KVCache:
         shape = (tokens, heads, self.head_dim)
         rows = _rows(q, "q", dtype, shape, device)
         if out is None:
-            out = torch.empty_like(q)
+            out = _like(q)
             out_rows = out.data_ptr(), out.stride(0), out.stride(1)
         else:
             _no_overlap(out, "out")
@@ -648,7 +656,7 @@ class KVCache:
         else:
             _no_overlap(k, "k")
         if v is None:
-            v = torch.empty_like(k)
+            v = _like(k)
         else:
             _no_overlap(v, "v")
         rows = [_lib.ROWS.pack(*_rows(t, name, dtype, shape, device)) for t, name in ((k, "k"), (v, "v"))]
@@ -684,7 +692,7 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
     if y is not None:
         y_at, y_stride = matrix(y, "y")
         if h is None:
-            h = torch.empty_like(residual)
+            h = _like(residual)
             h_at, h_stride = h.data_ptr(), h.stride(0)
         else:
             _no_overlap(h, "h")
@@ -700,7 +708,7 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
         raise ValueError("gate, post_weight or h without y")
     if weight is not None:
         if n is None:
-            n = torch.empty_like(residual)
+            n = _like(residual)
             n_at, n_stride = n.data_ptr(), n.stride(0)
         else:
             _no_overlap(n, "n")
