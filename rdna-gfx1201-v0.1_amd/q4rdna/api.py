@@ -4,7 +4,9 @@ Mirrors the reference's entry points (source/q4rdna.cuh:5-24): each GEMV
 call returns True when it launched and False when the call is not
 applicable (the reference's ``return false``: nothing was launched and the
 caller should use its own path).  Errors raise :class:`Q4RdnaError`.
-Launches are asynchronous on torch's current stream of the tensors' device.
+Launches are asynchronous on torch's current stream of the tensors' device, or
+on the stream whose handle is given as ``stream``; outputs that a call allocates
+belong to the stream that it launches on.
 """
 from __future__ import annotations
 
@@ -38,6 +40,15 @@ def _stream(device: torch.device | int | None = None) -> int:
     if isinstance(device, torch.device):
         device = device.index
     return _raw_stream(torch.cuda.current_device() if device is None else device)
+
+
+def _on_stream(stream: int, device: int):
+    """A context in which torch's current stream of the device is the one with
+    this handle: a call that allocates its outputs does so there, since memory
+    of another stream may still be in use by what is queued on that one."""
+    if stream == 0:  # a handle of 0 would stand for a new stream
+        return torch.cuda.stream(torch.cuda.default_stream(device))
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -122,6 +133,9 @@ def mul_mat(w: QWeight, x: torch.Tensor, y: torch.Tensor | None = None, stream: 
     """y = W x.  Returns y, or None when the call is not applicable."""
     x = _f32_vec(x, "x")
     if y is None:
+        if stream is not None:
+            with _on_stream(stream, x.get_device()):
+                return mul_mat(w, x)
         y = torch.empty(w.rows, dtype=torch.float32, device=x.device)
     _f32_vec(y, "y")
     device = w.raw.device
@@ -138,6 +152,9 @@ def mul_mat_add(w: QWeight, x: torch.Tensor, add: torch.Tensor, y: torch.Tensor 
     x = _f32_vec(x, "x")
     add = _f32_vec(add, "add")
     if y is None:
+        if stream is not None:
+            with _on_stream(stream, x.get_device()):
+                return mul_mat_add(w, x, add)
         y = torch.empty(w.rows, dtype=torch.float32, device=x.device)
     _f32_vec(y, "y")
     device = w.raw.device
@@ -155,6 +172,9 @@ def mul_mat_glu(up: QWeight, gate: QWeight, x: torch.Tensor, y: torch.Tensor | N
     """y = (W_up x) * silu(W_gate x).  Returns y, or None when not applicable."""
     x = _f32_vec(x, "x")
     if y is None:
+        if stream is not None:
+            with _on_stream(stream, x.get_device()):
+                return mul_mat_glu(up, gate, x, glu_op=glu_op)
         y = torch.empty(up.rows, dtype=torch.float32, device=x.device)
     _f32_vec(y, "y")
     device = up.raw.device
@@ -244,6 +264,9 @@ def pack(w: torch.Tensor, algorithm: int = ALGO_SIDECAR, out: torch.Tensor | Non
         raise ValueError("w must be a contiguous 2-D float32 CUDA tensor")
     rows, cols = w.shape
     if out is None:
+        if stream is not None:
+            with _on_stream(stream, w.get_device()):
+                return pack(w, algorithm)
         out = torch.empty(packed_size(rows, cols), dtype=torch.uint8, device=w.device)
     # The library sees only out's address: a short, mistyped or misplaced
     # buffer would be written past its end on the GPU.
@@ -261,6 +284,9 @@ def pack(w: torch.Tensor, algorithm: int = ALGO_SIDECAR, out: torch.Tensor | Non
 def dequantize(w: QWeight, out: torch.Tensor | None = None, stream: int | None = None) -> torch.Tensor:
     """fp32 [rows, cols] = scale * code (the exact product)."""
     if out is None:
+        if stream is not None:
+            with _on_stream(stream, w.device):
+                return dequantize(w)
         out = torch.empty((w.rows, w.cols), dtype=torch.float32, device=torch.device("cuda", w.device))
     _f32_buf(out, "out", w.rows * w.cols, w.device)
     s = _raw_stream(out.get_device()) if stream is None else stream
@@ -578,6 +604,9 @@ class KVCache:
         [head_dim]; cos, sin [positions, rotary / 2], float32)."""
         if k.dim() != 3:
             raise ValueError("k must be [tokens, kv_heads, head_dim]")
+        if stream is not None and q is not None and q_out is None:
+            with _on_stream(stream, self.device):
+                return self.append(batch, k, v, q, None, cos, sin, interleaved, q_norm, k_norm, eps)
         tokens, heads, dim, device, dtype = k.shape[0], self.kv_heads, self.head_dim, self.device, k.dtype
         step = self._step(batch, tokens)
         shape = (tokens, heads, dim)
@@ -623,6 +652,9 @@ class KVCache:
         tensor [tokens, q_heads]): returns (out, lse)."""
         if q.dim() != 3:
             raise ValueError("q must be [tokens, q_heads, head_dim]")
+        if stream is not None and (out is None or lse is True):
+            with _on_stream(stream, self.device):
+                return self.attend(batch, q, out, scale, window, lse)
         shape, dtype, device = q.shape, q.dtype, self.device
         tokens, heads, _ = shape
         step = self._step(batch, tokens)
@@ -650,6 +682,9 @@ class KVCache:
         """(k, v) [tokens, kv_heads, head_dim]: the batch's tokens (past[i] on,
         up to the sequence's length) as numbers."""
         shape, device = (tokens, self.kv_heads, self.head_dim), self.device
+        if stream is not None and (k is None or v is None):
+            with _on_stream(stream, device):
+                return self.read(batch, tokens, dtype, k, v)
         step = self._step(batch, tokens)
         if k is None:
             k = self.scales.new_empty(shape, dtype=dtype)
@@ -680,6 +715,9 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
         raise ValueError("residual must be a CUDA tensor [rows, width]")
     device, shape, dtype = residual.get_device(), residual.shape, residual.dtype
     width = shape[1]
+    if stream is not None and (y is not None and h is None or weight is not None and n is None):
+        with _on_stream(stream, device):
+            return add_norm(residual, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps, h=h, n=n)
 
     def matrix(t, name):
         stride = t.stride()
