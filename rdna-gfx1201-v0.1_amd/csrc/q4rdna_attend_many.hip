@@ -361,7 +361,8 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(const AttendArgs a)
     const uint32_t base = seq_place < 0 || seq_place > place ? place : static_cast<uint32_t>(seq_place);
     const Seq s = seq_of(a.batch, a.cache, seq);
     if (!s.ok) {
-        if (head == 0 && place == base && unit == late * a.splits && tid == 0) count_fault(a.cache);
+        // (With several sequences attend_few_kernel, which is launched too, counts them all.)
+        if (a.few_rows == 0 && head == 0 && place == base && unit == late * a.splits && tid == 0) count_fault(a.cache);
         return;
     }
     const int rows = s.count * static_cast<int>(a.group);
