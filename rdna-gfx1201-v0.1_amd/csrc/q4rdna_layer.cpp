@@ -374,7 +374,7 @@ int add_norm(const q4rdna_add_norm_desc *desc, void *stream) {
     if (d.h == d.n) return set_error(Q4RDNA_ERR_ARGUMENT, "h and n are one buffer");
     for (int o = 3; o < 5; ++o)
         for (int i = 0; i < 3; ++i)
-            if (buffers[o] != nullptr && buffers[o] == buffers[i] && (strides[o] != strides[i] || (i == 2 && d.rows > 1)))
+            if (d.rows > 1 && buffers[o] != nullptr && buffers[o] == buffers[i] && (strides[o] != strides[i] || i == 2))
                 return set_error(Q4RDNA_ERR_ARGUMENT, "an output over an input with another stride, or over the gate");
     int device = 0;
     if (hipGetDevice(&device) != hipSuccess) return set_error(Q4RDNA_ERR_HIP, "no current device");

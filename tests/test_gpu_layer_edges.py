@@ -19,3 +19,15 @@ def test_a_refused_sequence_counts_once(cuda):
                 before = cache.faults()
                 cache.attend(step(other, counts, table, at), q)
                 assert cache.faults() == before + 1
+
+
+def test_one_row_in_place_under_another_stride(cuda):
+    """A single row has no stride to agree on."""
+    from q4rdna import api
+    base, y, w = normal((4, 300), "f32", 72), normal((1, 100), "f32", 73), torch.ones(100, device="cuda")
+    x = base[1:2, :100]
+    want = api.add_norm(x, y, w)
+    h = base[1, :100].unsqueeze(0)
+    assert h.data_ptr() == x.data_ptr() and h.stride() != x.stride()
+    got = api.add_norm(x, y, w, h=h)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(x, want[0])
