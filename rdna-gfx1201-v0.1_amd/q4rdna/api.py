@@ -754,6 +754,8 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
         weight_at = _plain(weight, "weight", torch.float32, (width,), device)
     elif n is not None:
         raise ValueError("n without a weight")
+    if width == 0:
+        return (residual if h is None else h), n
     d = _lib.ADD_NORM.pack(_dtype(dtype), shape[0], width, scale, eps, 0, r_at, y_at, gate_at, h_at, n_at, r_stride,
                            y_stride, gate_stride, h_stride, n_stride, post_at, weight_at)
     s = _raw_stream(device) if stream is None else stream

@@ -31,3 +31,12 @@ def test_one_row_in_place_under_another_stride(cuda):
     assert h.data_ptr() == x.data_ptr() and h.stride() != x.stride()
     got = api.add_norm(x, y, w, h=h)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(x, want[0])
+
+
+@pytest.mark.parametrize("shape", [(3, 0), (0, 0), (0, 64)])
+def test_rows_without_numbers(cuda, shape):
+    from q4rdna import api
+    x, one = torch.empty(shape, device="cuda"), torch.ones(shape[1], device="cuda")
+    for y, gate in ((None, None), (torch.empty(shape, device="cuda"), None), (torch.empty(shape, device="cuda"), one)):
+        h, n = api.add_norm(x, y, one, gate=gate)
+        assert h.shape == n.shape == shape
