@@ -275,7 +275,7 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     a.wide = wide_rows(desc->q, desc->dtype, 16 / size_of(desc->dtype));
     a.wide_out = wide_rows(desc->out, desc->dtype, 4);
     // The most rows (query token, query head) per kv head that a sequence has.
-    const uint64_t most_rows = static_cast<uint64_t>(std::min(batch->max_tokens, batch->tokens)) * a.group;
+    const uint64_t most_tokens = std::min(batch->max_tokens, batch->tokens), most_rows = most_tokens * a.group;
     const uint64_t places = q4rdna::attend_many_places(*batch, a.group);
     if (most_rows > 0x3fffffffu || places * cache->kv_heads > 0x7fffffffu)
         return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of %u query heads are too many for one call", batch->tokens, desc->q_heads);
@@ -283,7 +283,7 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     const uint32_t cus = cu_count(cache->device);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const uint64_t most_blocks = desc->window == 0 ? batch->table_width
-                                                   : std::min<uint64_t>(batch->table_width, (static_cast<uint64_t>(desc->window) + batch->max_tokens) / q4rdna::kKvBlock + 2);
+                                                   : std::min<uint64_t>(batch->table_width, (desc->window + most_tokens) / q4rdna::kKvBlock + 2);
     const uint32_t few = few_rows(*batch, a.group, cache->kv_heads, most_blocks, cus);
     const bool many = most_rows > few;
     // Sequences of few rows; a single one goes by the bound alone.

@@ -40,3 +40,20 @@ def test_rows_without_numbers(cuda, shape):
     for y, gate in ((None, None), (torch.empty(shape, device="cuda"), None), (torch.empty(shape, device="cuda"), one)):
         h, n = api.add_norm(x, y, one, gate=gate)
         assert h.shape == n.shape == shape
+
+
+@pytest.mark.parametrize("tokens,window", [(16, 100), (32, 7), (9, 1000)])
+def test_a_window_bounds_the_blocks_without_max_tokens(cuda, tokens, window):
+    """One sequence under a table far wider than it is long: the step's tokens
+    bound its own as max_tokens does, and both calls take the same path."""
+    from q4rdna import api
+    length = 1300
+    cache, table, slots = filled(8, 64, [length], 74)
+    wide = torch.full((1, 5000), -7, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    past, cu = ints([length - tokens]), ints([0, tokens])
+    q = normal((tokens, 32, 64), "f32", 75)
+    want = cache.attend(api.KVBatch(past, wide, cu, ints(slots), max_tokens=tokens), q, window=window)
+    got = cache.attend(api.KVBatch(past, wide, cu, ints(slots)), q, window=window)
+    check(cache, wide, slots, [length - tokens], [tokens], q, got, "f32", window=window)
+    assert torch.equal(got, want)
