@@ -43,6 +43,9 @@ int check_device(int device) {
     return Q4RDNA_OK;
 }
 
+// HIP launches fewer than 2^32 threads.
+constexpr uint64_t most_workgroups(uint32_t threads) { return 0xffffffffu / threads; }
+
 // Compute units per device, looked up once.
 std::atomic<uint32_t> g_cus[64];
 
@@ -200,7 +203,7 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     const uint64_t all_rows = static_cast<uint64_t>(batch->tokens) * desc->q_heads;
     const uint32_t q_rows = all_rows <= 4096 ? 2048 / cache->head_dim : 16384 / cache->head_dim;
     const uint64_t q_units = (all_rows + q_rows - 1) / q_rows;
-    if (kv_units + q_units > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
+    if (kv_units + q_units > most_workgroups(256)) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
     if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
     q4rdna::AppendArgs a{};
     a.cache = *cache;
@@ -243,19 +246,6 @@ uint32_t few_rows(const q4rdna_kv_batch &b, uint32_t group, uint32_t kv_heads, u
 // and 309, 326 and 224).
 constexpr uint32_t kDealtSequences = 256;
 
-// Room for partial results of `rows` rows with `stats` numbers beside each, and
-// arrival counters of `jobs` row groups.
-int take_scratch(q4rdna::AttendArgs &a, size_t rows, size_t stats, size_t jobs, hipStream_t stream) {
-    a.partials = nullptr;
-    a.arrived = nullptr;
-    if (a.splits == 1) return Q4RDNA_OK;
-    Scratch s;
-    const int rc = get_scratch(a.cache.device, stream, rows * (a.cache.head_dim + stats), jobs, &s);
-    a.partials = s.partials;
-    a.arrived = s.arrived;
-    return rc;
-}
-
 int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4rdna_kv_attend_desc *desc, void *stream) {
     int rc;
     if ((rc = check_cache(cache)) != Q4RDNA_OK || (rc = check_batch(batch)) != Q4RDNA_OK) return rc;
@@ -276,53 +266,68 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     a.wide_out = wide_rows(desc->out, desc->dtype, 4);
     // The most rows (query token, query head) per kv head that a sequence has.
     const uint64_t most_tokens = std::min(batch->max_tokens, batch->tokens), most_rows = most_tokens * a.group;
-    const uint64_t places = q4rdna::attend_many_places(*batch, a.group);
-    if (most_rows > 0x3fffffffu || places * cache->kv_heads > 0x7fffffffu)
-        return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of %u query heads are too many for one call", batch->tokens, desc->q_heads);
-    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    const uint64_t places = q4rdna::attend_many_places(*batch, a.group), many_jobs = places * cache->kv_heads;
     const uint32_t cus = cu_count(cache->device);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     const uint64_t most_blocks = desc->window == 0 ? batch->table_width
                                                    : std::min<uint64_t>(batch->table_width, (desc->window + most_tokens) / q4rdna::kKvBlock + 2);
     const uint32_t few = few_rows(*batch, a.group, cache->kv_heads, most_blocks, cus);
     const bool many = most_rows > few;
+    if (most_rows > 0x3fffffffu || (many && many_jobs > most_workgroups(256)))
+        return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens of %u query heads are too many for one call", batch->tokens, desc->q_heads);
+    // Both launches are planned and their scratch is there before the first of
+    // them, so a call that is refused has launched nothing.
+    size_t floats = 0, jobs = 0;  // room for the parts' rows and the statistics beside them; row groups
+    q4rdna::AttendArgs f = a, m = a;
     // Sequences of few rows; a single one goes by the bound alone.
+    uint32_t rows = 0, waves = 0;
     if (!many || batch->sequences > 1) {
-        a.few_rows = many ? few : 0x7fffffffu;
-        const uint32_t most = static_cast<uint32_t>(many ? few : most_rows), rows = q4rdna::attend_few_rows(most);
-        a.row_groups = (most + rows - 1) / rows;
+        f.few_rows = many ? few : 0x7fffffffu;
+        const uint32_t most = static_cast<uint32_t>(many ? few : most_rows);
+        rows = q4rdna::attend_few_rows(most);
+        f.row_groups = (most + rows - 1) / rows;
         // The device deals the blocks to about `target` workgroups; each row
         // group ends in one part that may be short.
-        const uint64_t jobs = static_cast<uint64_t>(a.row_groups) * cache->kv_heads * batch->sequences;
+        const uint64_t few_jobs = static_cast<uint64_t>(f.row_groups) * cache->kv_heads * batch->sequences;
         // Few row groups are cut into many parts, which cost time to join: take
         // one workgroup of eight waves per CU there, two of four waves elsewhere
         // (eight and four waves: one token behind 60000 30.7 and 33.1 us, 32
         // ragged sequences of 100 to 8000 tokens 30.9 and 27.2 us).
-        const uint32_t waves = jobs < cus / 8 ? 8 : 4;
-        a.target = 8 / waves * cus;
+        waves = few_jobs < cus / 8 ? 8 : 4;
+        f.target = 8 / waves * cus;
         const uint64_t most_splits = (most_blocks + 7) / 8;
         // (Nor are parts worth their scratch where row groups abound.)
-        const bool split = most_blocks > q4rdna::kAttendWhole && batch->sequences <= kDealtSequences && jobs <= 64ull * cus;
-        a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>(most_splits, q4rdna::kAttendFewSplits) : 1);
-        const uint64_t workgroups = split ? std::min(jobs + a.target, jobs * a.splits) : jobs;
-        if (workgroups > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences are too many for one call", batch->sequences);
-        a.workgroups = static_cast<uint32_t>(workgroups);
-        if ((rc = take_scratch(a, workgroups * rows, 2, jobs, s)) != Q4RDNA_OK ||
-            (rc = launched(q4rdna::launch_attend_few(a, rows, waves, s), "kv_attend")) != Q4RDNA_OK)
-            return rc;
+        const bool split = most_blocks > q4rdna::kAttendWhole && batch->sequences <= kDealtSequences && few_jobs <= 64ull * cus;
+        f.splits = static_cast<uint32_t>(split ? std::min<uint64_t>(most_splits, q4rdna::kAttendFewSplits) : 1);
+        const uint64_t workgroups = split ? std::min(few_jobs + f.target, few_jobs * f.splits) : few_jobs;
+        if (workgroups > most_workgroups(64 * waves))
+            return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences of %u kv heads are too many for one call", batch->sequences, cache->kv_heads);
+        f.workgroups = static_cast<uint32_t>(workgroups);
+        if (f.splits > 1) {
+            floats = workgroups * rows * (cache->head_dim + 2);
+            jobs = few_jobs;
+        }
     }
     if (many) {
-        a.few_rows = batch->sequences > 1 ? few : 0;
+        m.few_rows = batch->sequences > 1 ? few : 0;
         // Two workgroups fit a CU: split until they are there.
-        const uint64_t jobs = places * cache->kv_heads;
-        const uint64_t splits = std::min<uint64_t>(2ull * cus / jobs, (most_blocks + 1) / 2);
-        a.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 64)));
-        a.cu_units = std::max(1u, cus / cache->kv_heads);
-        if ((rc = take_scratch(a, jobs * a.splits * q4rdna::kAttendManyRows, 3, jobs, s)) != Q4RDNA_OK ||
-            (rc = launched(q4rdna::launch_attend_many(a, static_cast<uint32_t>(places), s), "kv_attend")) != Q4RDNA_OK)
-            return rc;
+        const uint64_t splits = std::min<uint64_t>(2ull * cus / many_jobs, (most_blocks + 1) / 2);
+        m.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(splits, 64)));
+        m.cu_units = std::max(1u, cus / cache->kv_heads);
+        if (m.splits > 1) {
+            floats = std::max<size_t>(floats, many_jobs * m.splits * q4rdna::kAttendManyRows * (cache->head_dim + 3));
+            jobs = std::max<size_t>(jobs, many_jobs);
+        }
     }
-    return Q4RDNA_OK;
+    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (jobs != 0) {
+        Scratch scratch;
+        if ((rc = get_scratch(cache->device, s, floats, jobs, &scratch)) != Q4RDNA_OK) return rc;
+        f.partials = m.partials = scratch.partials;
+        f.arrived = m.arrived = scratch.arrived;
+    }
+    if (rows != 0 && (rc = launched(q4rdna::launch_attend_few(f, rows, waves, s), "kv_attend")) != Q4RDNA_OK) return rc;
+    return many ? launched(q4rdna::launch_attend_many(m, static_cast<uint32_t>(places), s), "kv_attend") : Q4RDNA_OK;
 }
 
 int read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dtype, const q4rdna_kv_rows *k,
@@ -335,7 +340,7 @@ int read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dt
         (rc = check_rows(*v, dtype, "v")) != Q4RDNA_OK)
         return rc;
     const uint64_t units = q4rdna::kv_places(*batch) * cache->kv_heads;
-    if (units > 0x7fffffffu) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
+    if (units > most_workgroups(256)) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
     if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
     q4rdna::ReadArgs a{};
     a.cache = *cache;

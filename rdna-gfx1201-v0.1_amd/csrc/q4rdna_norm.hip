@@ -17,6 +17,8 @@
 // Few rows are bound by the launch and one trip to memory: 2.4 us for one row.
 #include "q4rdna_layer_device.h"
 
+#include <algorithm>
+
 namespace q4rdna {
 namespace {
 
@@ -193,9 +195,31 @@ __global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc
     }
 }
 
+// A matrix from one of its rows on.
+template <typename T>
+const void *from_row(const void *p, int64_t stride, uint32_t row) {
+    return p == nullptr ? p : static_cast<const T *>(p) + row * stride;
+}
+template <typename T>
+void *from_row(void *p, int64_t stride, uint32_t row) {
+    return p == nullptr ? p : static_cast<T *>(p) + row * stride;
+}
+
 template <typename T, int VEC>
 hipError_t launch(const q4rdna_add_norm_desc &d, uint32_t cus, hipStream_t stream) {
-    auto go = [&](auto kernel, uint32_t threads) { kernel<<<d.rows, threads, 0, stream>>>(d, 1.0 / d.width); };
+    // A launch holds fewer than 2^32 threads: more rows go in several.
+    auto go = [&](auto kernel, uint32_t threads) {
+        q4rdna_add_norm_desc part = d;
+        for (uint32_t row = 0; row < d.rows; row += part.rows) {
+            part.rows = std::min(d.rows - row, 0xffffffffu / threads);
+            part.residual = from_row<T>(d.residual, d.residual_stride, row);
+            part.y = from_row<T>(d.y, d.y_stride, row);
+            part.gate = from_row<T>(d.gate, d.gate_stride, row);
+            part.h = from_row<T>(d.h, d.h_stride, row);
+            part.n = from_row<T>(d.n, d.n_stride, row);
+            kernel<<<part.rows, threads, 0, stream>>>(part, 1.0 / d.width);
+        }
+    };
     const uint32_t runs = (d.width + VEC - 1) / VEC;  // per row
     // A run per thread is the shortest chain, and up to 512 threads the faster
     // one at any number of rows (fp16/bf16 rows of 4096, against two runs in

@@ -57,3 +57,18 @@ def test_a_window_bounds_the_blocks_without_max_tokens(cuda, tokens, window):
     got = cache.attend(api.KVBatch(past, wide, cu, ints(slots)), q, window=window)
     check(cache, wide, slots, [length - tokens], [tokens], q, got, "f32", window=window)
     assert torch.equal(got, want)
+
+
+def test_more_rows_than_one_launch_holds(cuda):
+    """2^26 and a few rows of 64 threads are over 2^32 threads."""
+    from q4rdna import api
+    rows = 2 ** 26 + 70
+    x = torch.randint(-3, 4, (rows, 1), device="cuda", generator=torch.Generator("cuda").manual_seed(80)).half()
+    y = torch.ones_like(x)
+    h, n = api.add_norm(x, y, torch.ones(1, device="cuda"), scale=0.5, eps=0.25)
+    assert torch.equal(h, x + 0.5)
+    # n = h / sqrt(h^2 + 1/4): one rounding to fp16, and fp32's before it
+    at = torch.cat([torch.arange(1000), torch.arange(rows - 1000, rows), torch.arange(2 ** 26 - 500, 2 ** 26 + 70)]).cuda()
+    want = h[at].double() / (h[at].double() ** 2 + 0.25).sqrt()
+    assert ((n[at].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -20).all()
+    assert (n.float() - h.float() / (h.float() ** 2 + 0.25).sqrt()).abs().max() <= 2.0 ** -10
