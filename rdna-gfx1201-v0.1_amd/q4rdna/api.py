@@ -472,12 +472,11 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: 
 _NO_ROWS = (0, 0, 0)
 
 
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """A new tensor for an output of t's shape, its rows' numbers contiguous.
-    (torch lays it out in the order of t's strides, which puts the numbers
-    elsewhere where t's rows overlap, as a sliding window's do.)"""
-    out = torch.empty_like(t)
-    return out if out.stride(-1) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
+def _packed_like(t: torch.Tensor) -> torch.Tensor:
+    """What the calls allocate for an output where torch.empty_like, which lays
+    a tensor out in the order of t's strides, would put the numbers of a row
+    apart: t's rows overlap, as a sliding window's do."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _no_overlap(t: torch.Tensor, name: str) -> None:
@@ -620,8 +619,12 @@ class KVCache:
             shape = (tokens, q_heads, dim)
             q_rows = _rows(q, "q", dtype, shape, device)
             if q_out is None:
-                q_out = _like(q)
-                out_rows = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+                q_out = torch.empty_like(q)
+                token_stride, head_stride, stride = q_out.stride()
+                if stride != 1:
+                    q_out = _packed_like(q)
+                    token_stride, head_stride, _ = q_out.stride()
+                out_rows = q_out.data_ptr(), token_stride, head_stride
             else:
                 _no_overlap(q_out, "q_out")
                 out_rows = _rows(q_out, "q_out", dtype, shape, device)
@@ -661,8 +664,12 @@ class KVCache:
         shape = (tokens, heads, self.head_dim)
         rows = _rows(q, "q", dtype, shape, device)
         if out is None:
-            out = _like(q)
-            out_rows = out.data_ptr(), out.stride(0), out.stride(1)
+            out = torch.empty_like(q)
+            token_stride, head_stride, stride = out.stride()
+            if stride != 1:
+                out = _packed_like(q)
+                token_stride, head_stride, _ = out.stride()
+            out_rows = out.data_ptr(), token_stride, head_stride
         else:
             _no_overlap(out, "out")
             out_rows = _rows(out, "out", dtype, shape, device)
@@ -691,7 +698,9 @@ class KVCache:
         else:
             _no_overlap(k, "k")
         if v is None:
-            v = _like(k)
+            v = torch.empty_like(k)
+            if v.stride(2) != 1:
+                v = _packed_like(k)
         else:
             _no_overlap(v, "v")
         rows = [_lib.ROWS.pack(*_rows(t, name, dtype, shape, device)) for t, name in ((k, "k"), (v, "v"))]
@@ -730,8 +739,12 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
     if y is not None:
         y_at, y_stride = matrix(y, "y")
         if h is None:
-            h = _like(residual)
-            h_at, h_stride = h.data_ptr(), h.stride(0)
+            h = torch.empty_like(residual)
+            h_stride, stride = h.stride()
+            if stride != 1:
+                h = _packed_like(residual)
+                h_stride = width
+            h_at = h.data_ptr()
         else:
             _no_overlap(h, "h")
             h_at, h_stride = matrix(h, "h")
@@ -746,8 +759,12 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
         raise ValueError("gate, post_weight or h without y")
     if weight is not None:
         if n is None:
-            n = _like(residual)
-            n_at, n_stride = n.data_ptr(), n.stride(0)
+            n = torch.empty_like(residual)
+            n_stride, stride = n.stride()
+            if stride != 1:
+                n = _packed_like(residual)
+                n_stride = width
+            n_at = n.data_ptr()
         else:
             _no_overlap(n, "n")
             n_at, n_stride = matrix(n, "n")
