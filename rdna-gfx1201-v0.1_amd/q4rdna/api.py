@@ -6,7 +6,8 @@ applicable (the reference's ``return false``: nothing was launched and the
 caller should use its own path).  Errors raise :class:`Q4RdnaError`.
 Launches are asynchronous on torch's current stream of the tensors' device, or
 on the stream whose handle is given as ``stream``; outputs that a call allocates
-belong to the stream that it launches on.
+belong to the stream that it launches on.  All are forms for inference: none
+has a backward.
 """
 from __future__ import annotations
 
@@ -450,8 +451,17 @@ def _dtype(t: torch.dtype) -> int:
     return code
 
 
+def _no_gradient(name: str) -> None:
+    """For a tensor that requires a gradient: the calls have no backward, and
+    their results would silently be constants to torch."""
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which this call cannot give: use torch.no_grad() or detach it")
+
+
 def _plain(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> int:
     """The address of a contiguous tensor that the kernels read or write whole."""
+    if t.requires_grad:
+        _no_gradient(name)
     if t.dtype != dtype or t.get_device() != device or not t.is_contiguous() or t.shape != shape:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{device}, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
@@ -460,6 +470,8 @@ def _plain(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device:
 
 def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: int) -> tuple[int, int, int]:
     """(address, token stride, head stride) of activations [tokens, heads, dim]."""
+    if t.requires_grad:
+        _no_gradient(name)
     if t.dtype != dtype or t.get_device() != device or t.shape != shape:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on cuda:{device}, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
@@ -729,6 +741,8 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
             return add_norm(residual, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps, h=h, n=n)
 
     def matrix(t, name):
+        if t.requires_grad:
+            _no_gradient(name)
         stride = t.stride()
         if t.dtype != dtype or t.get_device() != device or t.shape != shape or stride[1] != 1 and width > 1:
             raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} with contiguous rows on cuda:{device}")

@@ -72,3 +72,25 @@ def test_more_rows_than_one_launch_holds(cuda):
     want = h[at].double() / (h[at].double() ** 2 + 0.25).sqrt()
     assert ((n[at].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -20).all()
     assert (n.float() - h.float() / (h.float() ** 2 + 0.25).sqrt()).abs().max() <= 2.0 ** -10
+
+
+def test_inputs_that_require_gradients_are_refused(cuda):
+    """The calls have no backward: where torch would record one they say so."""
+    from q4rdna import api
+    cache, table, slots = filled(2, 64, [70], 76)
+    batch = step([69], [1], table, slots)
+    q, k = normal((1, 4, 64), "f32", 77), normal((1, 2, 64), "f32", 78)
+    w, x = torch.ones(64, device="cuda"), normal((3, 64), "f32", 79)
+    wants = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda: cache.attend(batch, wants(q)), lambda: cache.append(batch, wants(k), k), lambda: cache.append(batch, k, wants(k)),
+             lambda: cache.append(batch, k, k, q=wants(q)), lambda: cache.append(batch, k, k, q=q, q_norm=wants(w)),
+             lambda: cache.append(batch, k, k, k_norm=wants(w)),
+             lambda: api.add_norm(wants(x), x, w), lambda: api.add_norm(x, wants(x), w), lambda: api.add_norm(x, x, wants(w)),
+             lambda: api.add_norm(x, x, w, post_weight=wants(w)), lambda: api.add_norm(x, x, w, gate=wants(w))]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
