@@ -369,7 +369,7 @@ typedef struct q4rdna_kv_cache {
     uint32_t slot_count;
     uint32_t kv_heads;
     uint32_t head_dim;    /* 64 or 128 */
-    int32_t device;
+    int32_t device;       /* of the buffers: the calls run there, whatever the current device is */
     uint32_t reserved;
 } q4rdna_kv_cache;
 

@@ -36,12 +36,30 @@ int launched(hipError_t e, const char *what) {
     return e == hipSuccess ? Q4RDNA_OK : set_error(Q4RDNA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
-int check_device(int device) {
-    int current = -1;
-    if (hipGetDevice(&current) != hipSuccess || current != device)
-        return set_error(Q4RDNA_ERR_ARGUMENT, "the cache lives on device %d, the current device is %d", device, current);
-    return Q4RDNA_OK;
-}
+// A call runs on the cache's device, whatever the calling thread's current one,
+// which it gets back.
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&saved_) != hipSuccess) saved_ = -1;
+        if (saved_ == device) return;
+        switched_ = hipSetDevice(device) == hipSuccess;
+        if (!switched_) {
+            (void)hipGetLastError();
+            status_ = set_error(Q4RDNA_ERR_ARGUMENT, "the cache lives on device %d, which cannot be used", device);
+        }
+    }
+    ~OnDevice() {
+        if (switched_ && saved_ >= 0) (void)hipSetDevice(saved_);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+    int status() const { return status_; }
+
+private:
+    int saved_ = -1, status_ = Q4RDNA_OK;
+    bool switched_ = false;
+};
 
 // HIP launches fewer than 2^32 threads.
 constexpr uint64_t most_workgroups(uint32_t threads) { return 0xffffffffu / threads; }
@@ -54,7 +72,10 @@ uint32_t cu_count(int device) {
     uint32_t n = g_cus[device].load(std::memory_order_relaxed);
     if (n != 0) return n;
     int v = 0;
-    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || v <= 0) v = 256;
+    if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || v <= 0) {
+        (void)hipGetLastError();
+        return 256;
+    }
     g_cus[device].store(static_cast<uint32_t>(v), std::memory_order_relaxed);
     return static_cast<uint32_t>(v);
 }
@@ -204,7 +225,8 @@ int append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     const uint32_t q_rows = all_rows <= 4096 ? 2048 / cache->head_dim : 16384 / cache->head_dim;
     const uint64_t q_units = (all_rows + q_rows - 1) / q_rows;
     if (kv_units + q_units > most_workgroups(256)) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
-    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    const OnDevice device(cache->device);
+    if (device.status() != Q4RDNA_OK) return device.status();
     q4rdna::AppendArgs a{};
     a.cache = *cache;
     a.batch = *batch;
@@ -318,7 +340,8 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
             jobs = std::max<size_t>(jobs, many_jobs);
         }
     }
-    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    const OnDevice device(cache->device);
+    if (device.status() != Q4RDNA_OK) return device.status();
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (jobs != 0) {
         Scratch scratch;
@@ -341,7 +364,8 @@ int read(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, uint32_t dt
         return rc;
     const uint64_t units = q4rdna::kv_places(*batch) * cache->kv_heads;
     if (units > most_workgroups(256)) return set_error(Q4RDNA_ERR_ARGUMENT, "%u tokens are too many for one call", batch->tokens);
-    if ((rc = check_device(cache->device)) != Q4RDNA_OK) return rc;
+    const OnDevice device(cache->device);
+    if (device.status() != Q4RDNA_OK) return device.status();
     q4rdna::ReadArgs a{};
     a.cache = *cache;
     a.batch = *batch;
