@@ -114,6 +114,20 @@ __device__ __forceinline__ void turn_row(Row &r, const Place &p, const Turn &t) 
 // with 1.5 * 2^23 has a last place of one.  For |x * f| < 2^22; a NaN gives 0
 // in its low bits.
 __device__ __forceinline__ uint32_t rounded(float x, float f) { return __float_as_uint(fmaf(x, f, 12582912.0f)); }
+// The same with the product rounded first.  Where the exact product lies midway
+// between two integers, which numbers of few bits often meet, a factor that is off
+// by a last place would decide; rounded, it is midway again and goes to the even one.
+__device__ __forceinline__ uint32_t rounded_twice(float x, float f) {
+#pragma clang fp contract(off)
+    const float y = x * f;
+    return __float_as_uint(y + 12582912.0f);
+}
+// largest / 32512, rounded once: the product with the reciprocal and its remainder.
+// (At fp32's very end it is rounded down, for the largest code times it to be finite.)
+__device__ __forceinline__ float token_scale(float largest) {
+    const float per = 1.0f / kKvCode16, q = largest * per;
+    return fminf(fmaf(fmaf(-q, kKvCode16, largest), per, q), 0x1.0204060000000p+113f);
+}
 // The low halves of four of them.
 __device__ __forceinline__ s16x4 pack_codes(const float (&x)[4], float f) {
     const uint32_t w[2] = {__builtin_amdgcn_perm(rounded(x[1], f), rounded(x[0], f), 0x05040100u),
@@ -234,7 +248,7 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 short *out = &st.code[is_v][t * kRow<D>];
                 *reinterpret_cast<s16x4 *>(out + at.a_at) = pack_codes(r[x].a, inv);
                 *reinterpret_cast<s16x4 *>(out + at.b_at) = pack_codes(r[x].b, inv);
-                if (lane == 0) st.scale[is_v][t] = some ? largest * (1.0f / kKvCode16) : finite ? 0.0f : __builtin_nanf("");
+                if (lane == 0) st.scale[is_v][t] = some ? token_scale(largest) : finite ? 0.0f : __builtin_nanf("");
             }
         }
     }
@@ -371,7 +385,7 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 const s16x8 c = row[w / 2];
                 int x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = static_cast<int>(rounded(c[4 * (w % 2) + e], r));
+                for (int e = 0; e < 4; ++e) x[e] = static_cast<int>(rounded_twice(c[4 * (w % 2) + e], r));
                 k[w] = static_cast<int>(pack4(x[0], x[1], x[2], x[3]));
             }
             store16(tile + 16 * piece, k);
@@ -389,8 +403,8 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                     const int t = 16 * w + 4 * g + b;
                     const s16x4 c = *reinterpret_cast<const s16x4 *>(&st.code[1][t * kRow<D> + number]);
                     const float r = st.ratio[1][t];
-                    by_token[b] = pack4(static_cast<int>(rounded(c[0], r)), static_cast<int>(rounded(c[1], r)),
-                                        static_cast<int>(rounded(c[2], r)), static_cast<int>(rounded(c[3], r)));
+                    by_token[b] = pack4(static_cast<int>(rounded_twice(c[0], r)), static_cast<int>(rounded_twice(c[1], r)),
+                                        static_cast<int>(rounded_twice(c[2], r)), static_cast<int>(rounded_twice(c[3], r)));
                 }
                 transpose4(by_token, by_number);
 #pragma unroll

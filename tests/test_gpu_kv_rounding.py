@@ -1,4 +1,6 @@
 """The append's roundings, number by number."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
@@ -51,3 +53,39 @@ def test_codes_are_the_nearest_to_the_scaled_numbers(cuda, dtype, dim):
         got = np.zeros((64, kv_heads, dim))
         got[token, :, number] = (256 * o[0, 0, :, 2 * which] + o[0, 0, :, 2 * which + 1]).T
         assert np.array_equal(got[:length], want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_full_blocks_round_the_product_of_code_and_ratio(cuda, dtype):
+    """code8 = rint(fl(code16 * r)), r = fl(token scale / block scale), with token
+    scale = fl(largest / 32512) and block scale 256 times the largest of them:
+    each in fp32, bit by bit.  Numbers of few bits make many exact products lie
+    midway; rounded first, most of those go to the even code as they should."""
+    kv_heads, dim = 8, 128
+    cache = make_cache(kv_heads, dim, 1, 1)
+    k, v = normal((64, kv_heads, dim), dtype, 5, 2.0), normal((64, kv_heads, dim), dtype, 6)
+    cache.append(step([0], [64], ints([[0]])), k, v)
+    snap = snapshot(cache)
+    wrong = {"once": 0, "fused": 0}
+    for which, x in ((0, k), (1, v)):
+        x = x.float().cpu().numpy()
+        largest = np.abs(x).max(axis=-1, keepdims=True)
+        code = np.rint(x.astype(np.float64) * (np.float32(R.CODE16) / largest).astype(np.float64))
+        scale = largest / np.float32(R.CODE16)
+        whole = np.float32(256) * scale.max(axis=0, keepdims=True)
+        ratio = scale / whole
+        want = np.rint(code.astype(np.float32) * ratio)
+        token, number = R.codes(which, dim)
+        got = np.zeros((64, kv_heads, dim))
+        got[token, :, number] = snap["pages"][0, :, which].T
+        assert np.array_equal(snap["scales"][0, :, which], whole[0, :, 0]) and np.array_equal(got, want)
+        b = largest.max(axis=0, keepdims=True)
+        exact = np.array([[[nearest(c, l, t) for c in row] for row, l, t in zip(rows, ls[:, 0], b[0, :, 0])] for rows, ls in zip(code, largest)])
+        wrong["once"] += int((want != exact).sum())
+        wrong["fused"] += int((np.rint(code * ratio.astype(np.float64)) != exact).sum())
+    assert wrong["once"] <= wrong["fused"]
+
+
+def nearest(code, largest, top):
+    """rint(code * largest / (256 * top)) of exact numbers, ties to the even."""
+    return round(Fraction(int(code)) * Fraction(float(largest)) / (256 * Fraction(float(top))))
