@@ -511,6 +511,12 @@ class KVBatch:
     anew.  Without cu_tokens every sequence has one token; with it max_tokens
     (an int) bounds the tokens of a sequence, None where it is not known: a
     bound lets short steps take faster paths.
+
+    The kernels refuse a sequence whose entries are out of range, and pages
+    outside the cache, and count them in :meth:`KVCache.faults`.  A refused
+    sequence's rows of an output are not written, nor are rows behind
+    cu_tokens[-1]: in an output that a call allocated they hold whatever was in
+    that memory.
     """
 
     def __init__(self, past: torch.Tensor, table: torch.Tensor, cu_tokens: torch.Tensor | None = None,
@@ -537,6 +543,7 @@ class KVBatch:
         raw.max_tokens = max_tokens
         raw.table_width = table.shape[1]
         self.raw = raw
+        self._call = -1, None  # the last call's tokens and descriptor
         self.device = device
         self.sequences = n
         self._keep = (past, table, cu_tokens, slots)
@@ -544,14 +551,15 @@ class KVBatch:
     def _of(self, tokens: int):
         """The descriptor for a call on `tokens` tokens: a new one where the last
         call had another count (that call may still be using its own)."""
-        raw = self.raw
-        if raw.tokens != tokens:
+        held, step = self._call
+        if held != tokens:
             if self._keep[2] is None and tokens != self.sequences:
                 raise ValueError(f"{tokens} tokens for {self.sequences} sequences: without cu_tokens each has one")
-            raw = _lib.BatchDesc.from_buffer_copy(raw)
+            raw = _lib.BatchDesc.from_buffer_copy(self.raw)
             raw.tokens = tokens
-            self.raw = raw
-        return ctypes.byref(raw)
+            step = ctypes.byref(raw)
+            self._call = tokens, step
+        return step
 
 
 class KVCache:
@@ -612,7 +620,8 @@ class KVCache:
                eps: float = 1e-6, stream: int | None = None) -> torch.Tensor | None:
         """Append the step's k and v [tokens, kv_heads, head_dim]; returns q
         [tokens, q_heads, head_dim] normalised and rotated (q_norm, k_norm
-        [head_dim]; cos, sin [positions, rotary / 2], float32)."""
+        [head_dim]; cos, sin [positions, rotary / 2], float32).  Rows of a
+        refused sequence are not written (see :class:`KVBatch`)."""
         if k.dim() != 3:
             raise ValueError("k must be [tokens, kv_heads, head_dim]")
         if stream is not None and q is not None and q_out is None:
@@ -644,11 +653,12 @@ class KVCache:
             raise ValueError("q_out or q_norm without q")
         cos_at = sin_at = positions = rotary = 0
         if cos is not None:
-            if cos.dim() != 2 or sin is None:
+            table = cos.shape
+            if len(table) != 2 or sin is None:
                 raise ValueError("cos and sin must be [positions, rotary / 2]")
-            cos_at = _plain(cos, "cos", torch.float32, cos.shape, device)
-            sin_at = _plain(sin, "sin", torch.float32, cos.shape, device)
-            positions, rotary = cos.shape[0], 2 * cos.shape[1]
+            cos_at = _plain(cos, "cos", torch.float32, table, device)
+            sin_at = _plain(sin, "sin", torch.float32, table, device)
+            positions, rotary = table[0], 2 * table[1]
         elif sin is not None:
             raise ValueError("sin without cos")
         q_weight = 0 if q_norm is None else _plain(q_norm, "q_norm", torch.float32, (dim,), device)
@@ -664,7 +674,8 @@ class KVCache:
         """Attention of the step's q [tokens, q_heads, head_dim] over the cache,
         after :meth:`append` of the same batch.  scale None: head_dim ** -0.5.
         window > 0: the last `window` tokens only.  lse True (or a float32
-        tensor [tokens, q_heads]): returns (out, lse)."""
+        tensor [tokens, q_heads]): returns (out, lse).  Rows of a refused
+        sequence are not written (see :class:`KVBatch`)."""
         if q.dim() != 3:
             raise ValueError("q must be [tokens, q_heads, head_dim]")
         if stream is not None and (out is None or lse is True):
@@ -699,7 +710,8 @@ class KVCache:
     def read(self, batch: KVBatch, tokens: int, dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None,
              v: torch.Tensor | None = None, stream: int | None = None):
         """(k, v) [tokens, kv_heads, head_dim]: the batch's tokens (past[i] on,
-        up to the sequence's length) as numbers."""
+        up to the sequence's length) as numbers.  Rows of a refused sequence
+        are not written (see :class:`KVBatch`)."""
         shape, device = (tokens, self.kv_heads, self.head_dim), self.device
         if stream is not None and (k is None or v is None):
             with _on_stream(stream, device):
