@@ -99,6 +99,8 @@ class Decoder:
 
     def prompt(self, tokens: list[int]) -> torch.Tensor:
         """Append a prompt, up to eight tokens a step; the last token's logits."""
+        if not tokens:
+            raise ValueError("an empty prompt")
         for at in range(0, len(tokens), 8):
             ids = torch.tensor(tokens[at:at + 8], device=self.device)
             n = len(ids)
@@ -112,33 +114,35 @@ class Decoder:
 
     def decode(self, logits: torch.Tensor, count: int) -> tuple[list[int], float]:
         """Decode greedily from the given logits: (tokens, seconds a step).  The
-        step is captured once; the sequence's length, the token and the logits
-        live in tensors that the graph reads and writes."""
+        model's step is captured once; the sequence's length, the token and the
+        logits live in tensors that the graph reads and writes."""
         if self.length + count > self.max_tokens:
             raise ValueError(f"more than {self.max_tokens} tokens")
+        if count == 0:
+            return [], 0.0
         batch = api.KVBatch(self.past, self.table)
         token = logits.argmax().reshape(1)
 
         def step():
-            out = self.forward(self.embedding[token], batch)
-            token.copy_(out[0].argmax().reshape(1))
+            return self.forward(self.embedding[token], batch)[0]
 
         stream = torch.cuda.Stream(self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
-        saved = token.clone()
         with torch.cuda.stream(stream):
             step()  # every shape once on this stream: scratch grows here, not in the capture
-            token.copy_(saved)
         torch.cuda.current_stream(self.device).wait_stream(stream)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
-            step()
+            logits = step()
         chosen = []
         torch.cuda.synchronize(self.device)
         began = time.perf_counter()
         for _ in range(count):
             chosen.append(token.clone())
             graph.replay()
+            # Outside the graph: torch's argmax over many logits sets memory
+            # that it counts in, and such a node must not be replayed.
+            token.copy_(logits.argmax())
             self.past += 1
         torch.cuda.synchronize(self.device)
         spent = (time.perf_counter() - began) / count
