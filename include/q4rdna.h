@@ -342,7 +342,7 @@ int q4rdna_dequantize(const q4rdna_weight *w, float *out, void *stream);
  * 16-bit codes, as two int8 planes (256 * high + low, |code| <= 32512), and an
  * fp32 scale per token and head (absmax / 32512).  When a block fills, its
  * scale becomes 256 * the largest of its tokens' scales and each code
- * rint(code16 * (token scale / scale)): every number is rounded to 16 bits
+ * rint(code16 * (token scale / scale)), in fp32: every number is rounded to 16 bits
  * once and to 8 bits once, so the cache's bytes do not depend on the chunks in
  * which the tokens arrive, and a full page never changes again (sequences may
  * share it).  A slot holds two blocks, used in turn: those of the greatest

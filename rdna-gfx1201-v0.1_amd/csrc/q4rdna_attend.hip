@@ -28,8 +28,10 @@
 // numbers, 266 MB) take 54.5 us, 4.9 TB/s: 2 us to deal the blocks, 5 until the
 // first tiles arrive, 37 at 7.2 TB/s, a plain read's rate, then waiting for the
 // slowest workgroups and the join.  Eight query heads a kv head take 65 us.
-// With a short cache the chain of dependent loads (lengths, page, codes) is
-// what is left: 6.3 us behind 17 tokens.
+// A row group is cut into 64 parts at most (one trip joins them), so a single
+// sequence of one to three kv heads leaves CUs idle.  With a short cache the chain
+// of dependent loads (lengths, page, codes, the open block's V behind its softmax)
+// is what is left: 6.4 us behind 17 tokens.
 //
 // Eight or four waves a workgroup and two waves per SIMD, 185 registers each
 // (256 for eight rows): both operands of a block and its accumulators stay in

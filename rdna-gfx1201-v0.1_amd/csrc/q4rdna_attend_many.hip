@@ -12,9 +12,13 @@
 //    is laid into LDS in that order of tokens.  The row's maximum, sum and
 //    rescaling are the lane's own, with one exchange between the halves.
 //  * q is scaled by a power of two per row, so fp16 and bf16 rows are exact in
-//    fp16; the weights are rounded to fp16 (11 bits), finer than the output's
-//    rounding.  fp32 rows take two fp16 parts of q and of the weights each
-//    (SPLIT = 2, 22 bits) and twice the products, which keeps fp32's accuracy.
+//    fp16.  Their weights are rounded to fp16 (11 bits), which the matrix
+//    instruction needs, while their sum keeps them whole: each weight is off by as
+//    much as an fp16 output is rounded by, an eighth of a bf16 output's rounding,
+//    and the errors of many weights average out.  fp32 rows take two fp16 parts of
+//    q and of the weights each (SPLIT = 2, 22 bits) and twice the products: the
+//    error is half of that of a plain fp32 softmax and product (5.7e-7 and 1.1e-6
+//    of the output at 2047 tokens).
 //  * V's scale per block goes into the weights: they are relative to the largest
 //    product of a weight and a V scale that the row has had, not to the largest
 //    weight, so fp16's range is spent on what counts in the row's output, however
@@ -29,9 +33,9 @@
 // too few of them; the last to arrive joins the parts in a fixed order.
 //
 // 2048 tokens behind 6100 (bf16, 8 kv heads of four query heads of 128 numbers)
-// take 267 us, 0.9 PFLOP/s where a large matrix product of the library reaches
-// 1.2; 2047 tokens from the start in fp32, twice the products, 86 us.  Two
-// workgroups share a CU (72 KB of LDS, 240 registers).  The matrix unit is busy
+// take 271 us, 0.9 PFLOP/s where a large matrix product of the library reaches
+// 1.2; 2047 tokens from the start in fp32, twice the products, 88 us.  Two
+// workgroups share a CU (72 KB of LDS, 241 to 255 registers).  The matrix unit is busy
 // 37 % of the time, the vector unit 54 %, the LDS 28 % without bank conflicts:
 // a wave's products and its softmax follow each other, and two waves per SIMD
 // overlap in part; one alone takes 1.5 us a block, two 2.15.  Of a block's 1500

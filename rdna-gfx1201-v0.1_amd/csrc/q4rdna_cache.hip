@@ -6,10 +6,12 @@
 // one kv head, K and V: it needs all of a block's scales when the block fills,
 // and LDS turns rows of numbers into the pages' order and writes whole 16-byte
 // pieces.  7873 tokens of six prompts (bf16, 8 kv heads, 32 heads of q with norm
-// and rotation, 177 MB) take 54 us, 3.3 TB/s of the 5.2 that a copy reaches; the
-// vector unit is busy 36 % of the time, the rest is waiting for a block's rows.
-// Reading them back (48 MB) takes 14 us.  One token takes 4.3 us and 64
-// sequences' tokens 9.2 us, where some fill their blocks: a block that closes is
+// and rotation, 177 MB) take 55 us, 3.2 TB/s of the 5.2 that a copy reaches: the
+// vector unit is busy 36 % of the time, the rest is waiting for rows, with the
+// four workgroups that the stage's 36 KB lets a CU have, those of q among them,
+// which use none of it.  Reading them back (48 MB) takes 14 us, for the same
+// reason: a workgroup's loads, then its stores.  One token takes 4.4 us and 64
+// sequences' tokens 9.3 us, where some fill their blocks: a block that closes is
 // a chain of loads (lengths, open planes, page) with LDS round trips between.
 #include "q4rdna_layer_device.h"
 
