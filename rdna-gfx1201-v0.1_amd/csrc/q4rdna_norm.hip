@@ -4,12 +4,12 @@
 //
 // One pass over memory: a workgroup keeps its row in registers between the two
 // sums (mean y^2, then mean h^2), so every input is read once and every output
-// written once.  Products are in fp32; the sums of squares go on in 64 bits from
-// four numbers on, so the factor does not depend on the order of the sum, which
-// differs between aligned and unaligned rows.  That costs small calls a tenth of a
-// microsecond (77 rows of 1111 in fp16, both norms: 3.6 us, with fp32 sums 3.5; 64
-// rows of 8192 4.1 and 3.75).  The weights stay fp32, since models keep them so and
-// they come from the L2.
+// written once.  Products are in fp32, sums of squares in fp32 over 64 neighbours, as
+// one tree of pairs, and in 64 bits from there on: so the factor does not depend on
+// how many numbers a thread takes, which differs between aligned and unaligned rows.
+// With 1024 threads a row the 64 bits cost a few percent (64 rows of 8192 in fp16,
+// both norms: 3.9 us, in fp32 alone 3.75; 77 rows of 1111 3.4 and 3.5).  The weights
+// stay fp32, since models keep them so and they come from the L2.
 //
 // Many rows are bound by the memory: 8192 rows of 4096 in bf16 (residual and y
 // in, h and n out, 268 MB) take 39 us where the inputs are in the Infinity
@@ -44,50 +44,66 @@ __device__ __forceinline__ double sum_halves(double v) {
            __builtin_bit_cast(double, static_cast<uint64_t>(high[1]) << 32 | low[1]);
 }
 
-// The workgroup's sum of v; `slots` is the caller's own for each sum, so one
-// barrier is enough.
+// The sums of four v over the wave's rows of 16 lanes, v[i] in row i: two sums for
+// each swap.  Its pairs are those of add_xor32(add_xor16(v)).
+__device__ __forceinline__ float sum_rows4(float v0, float v1, float v2, float v3) {
+    const auto p01 = __builtin_amdgcn_permlane16_swap(__float_as_uint(v0), __float_as_uint(v1), false, false);
+    const auto p23 = __builtin_amdgcn_permlane16_swap(__float_as_uint(v2), __float_as_uint(v3), false, false);
+    const float s01 = __uint_as_float(p01[0]) + __uint_as_float(p01[1]);
+    const float s23 = __uint_as_float(p23[0]) + __uint_as_float(p23[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(s01), __float_as_uint(s23), false, false);
+    return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+
+// The wave's sum of squares of VEC numbers a lane in CH runs: 64 neighbours in
+// fp32, always as the same tree of pairs, whether eight, four or one of them lie in
+// a lane; the sums of 64 in 64 bits.
+template <int CH, int VEC>
+__device__ __forceinline__ double wave_squares(const float (&x)[CH][VEC]) {
+#pragma clang fp contract(off)
+    static_assert(VEC == 1 || VEC == 4 || VEC == 8);
+    float v[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        float tree[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) tree[e] = x[c][e] * x[c][e];
+#pragma unroll
+        for (int step = 1; step < VEC; step *= 2)
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2 * step) tree[e] += tree[e + step];
+        v[c] = tree[0];
+        v[c] += dpp<kDppXor1>(v[c]);
+        v[c] += dpp<kDppXor2>(v[c]);
+        v[c] += dpp<kDppMirror8>(v[c]);
+        if (VEC < 8) v[c] += dpp<kDppMirror16>(v[c]);
+    }
+    double sum = 0.0;
+    if constexpr (VEC == 1 && CH % 4 == 0) {
+#pragma unroll
+        for (int c = 0; c < CH; c += 4) sum += sum_rows4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) sum += VEC == 1 ? add_xor32(add_xor16(v[c])) : v[c];
+        if (VEC == 1) return sum;
+        if (VEC == 8) sum += dpp64<kDppMirror16>(sum);
+    }
+    return sum_halves(sum_rows(sum));
+}
+
+// The workgroup's sum of v, the same in each wave's lanes; `slots` is the caller's
+// own for each sum, so one barrier is enough.
 template <int NT>
 __device__ __forceinline__ double block_sum(double v, double *slots) {
-    static_assert(NT == 64 || NT == 256 || NT == 512 || NT == 1024, "a sum over 4, 8 or 16 lanes joins the waves");
-    v += dpp64<kDppXor1>(v);
-    v += dpp64<kDppXor2>(v);
-    v += dpp64<kDppMirror8>(v);
-    v += dpp64<kDppMirror16>(v);
-    v = sum_halves(sum_rows(v));
+    static_assert(NT == 64 || NT == 256 || NT == 512 || NT == 1024, "one, two or four lanes with four waves' sums each");
     if (NT == 64) return v;
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = slots[threadIdx.x % (NT / 64)];
-    v += dpp64<kDppXor1>(v);
-    v += dpp64<kDppXor2>(v);
-    if (NT >= 512) v += dpp64<kDppMirror8>(v);
-    if (NT >= 1024) v += dpp64<kDppMirror16>(v);
+    const double *mine = slots + threadIdx.x % (NT / 256 ? NT / 256 : 1) * 4;
+    v = (mine[0] + mine[1]) + (mine[2] + mine[3]);
+    if (NT >= 512) v += dpp64<kDppXor1>(v);
+    if (NT >= 1024) v += dpp64<kDppXor2>(v);
     return v;
-}
-// The sum of a thread's squares: four neighbours in fp32, in one order whether
-// they lie in a thread or, one each, in a quad of lanes (which each get a quarter
-// of it); those sums in 64 bits.
-template <int CH, int VEC>
-__device__ __forceinline__ double squares(const float (&x)[CH][VEC]) {
-#pragma clang fp contract(off)
-    double sum = 0.0;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        if (VEC == 1) {
-            float four = x[c][0] * x[c][0];
-            four += dpp<kDppXor1>(four);
-            four += dpp<kDppXor2>(four);
-            sum += four;
-        } else {
-#pragma unroll
-            for (int e = 0; e + 3 < VEC; e += 4) {
-                const float a = x[c][e] * x[c][e] + x[c][e + 1] * x[c][e + 1];
-                const float b = x[c][e + 2] * x[c][e + 2] + x[c][e + 3] * x[c][e + 3];
-                sum += a + b;
-            }
-        }
-    }
-    return VEC == 1 ? 0.25 * sum : sum;
 }
 
 // The norm's factor, 1 / sqrt(sum / width + eps), rounded once: the sum is in 64
@@ -109,7 +125,7 @@ __device__ __forceinline__ float norm_factor(double sum, double per_width, float
 // NT threads a row, CH runs of VEC numbers per thread.
 template <typename T, int VEC, int NT, int CH>
 __global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc d, double per_width) {
-    __shared__ double slots[2][NT / 64];
+    __shared__ __align__(16) double slots[2][NT / 64];
     const uint32_t row = blockIdx.x;
     const T *res = static_cast<const T *>(d.residual) + row * d.residual_stride;
     const uint32_t width = d.width;
@@ -139,7 +155,7 @@ __global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc
             }
         }
         if (d.post_weight != nullptr) {
-            const double sum = block_sum<NT>(squares(y), slots[0]);
+            const double sum = block_sum<NT>(wave_squares(y), slots[0]);
             const float inv = norm_factor(sum, per_width, d.eps);
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -179,7 +195,7 @@ __global__ __launch_bounds__(NT) void add_norm_kernel(const q4rdna_add_norm_desc
         }
     }
     if (d.n == nullptr) return;
-    const double sum = block_sum<NT>(squares(h), slots[1]);
+    const double sum = block_sum<NT>(wave_squares(h), slots[1]);
     const float inv = norm_factor(sum, per_width, d.eps);
     T *out = static_cast<T *>(d.n) + row * d.n_stride;
 #pragma unroll

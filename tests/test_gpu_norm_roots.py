@@ -75,3 +75,16 @@ def test_rows_whose_squares_are_subnormal(cuda):
     for n in (api.add_norm(x, None, one, eps=0.0)[1], api.add_norm(torch.zeros_like(x), x, None, post_weight=one, eps=0.0)[0],
               cache.append(step([0], [3], ints([[0]])), k, k, q=x[:, None], q_norm=one, eps=0.0)[:, 0]):
         assert np.array_equal(f64(n), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("rows,width", [(9, 64), (50, 264), (600, 1032), (40, 3000), (700, 5000), (5, 8192), (3, 16384)])
+def test_aligned_and_unaligned_rows_give_the_same_bits(cuda, dtype, rows, width):
+    """A row's factor does not depend on how many numbers a thread takes."""
+    from q4rdna import api
+    x, y = (torch.randn((rows, width), device="cuda").to(dtype) for _ in range(2))
+    one = torch.ones(width, device="cuda")
+    shifted = [torch.empty(rows * width + 1, dtype=dtype, device="cuda")[1:].view(rows, width).copy_(t) for t in (x, y)]
+    assert shifted[0].data_ptr() % 16 != 0
+    for a, b in zip(api.add_norm(x, y, one, post_weight=one), api.add_norm(*shifted, one, post_weight=one)):
+        assert torch.equal(a, b)
