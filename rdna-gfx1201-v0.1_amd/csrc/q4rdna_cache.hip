@@ -84,7 +84,7 @@ __device__ __forceinline__ void norm_row(Row &r, const Weights &w, float eps) {
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum = fmaf(r.a[e], r.a[e], fmaf(r.b[e], r.b[e], sum));
-    const float inv = inverse_root(fmaf(lanes_sum<D / 8>(sum), 1.0f / D, eps));
+    const float inv = inverse_root(fmaf(lanes_sum<D / 8>(sum), 1.0f / D, eps), eps);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         r.a[e] = r.a[e] * inv * w.a[e];
@@ -123,6 +123,17 @@ __device__ __forceinline__ uint32_t rounded_twice(float x, float f) {
 #pragma clang fp contract(off)
     const float y = x * f;
     return __float_as_uint(y + 12582912.0f);
+}
+// 32512 / largest, rounded once, for 1e-30 and more: a quarter of both, since the
+// reciprocal of a number above 2^126 would be subnormal, which the instruction
+// gives as zero; its refined reciprocal, the quotient and that one's remainder.
+__device__ __forceinline__ float code_factor(float largest) {
+#pragma clang fp contract(off)
+    const float b = 0.25f * largest, a = 0.25f * kKvCode16;
+    float y = __builtin_amdgcn_rcpf(b);
+    y = fmaf(fmaf(-b, y, 1.0f), y, y);
+    const float q = a * y;
+    return fmaf(fmaf(-b, q, a), y, q);
 }
 // largest / 32512, rounded once: the product with the reciprocal and its remainder.
 // (At fp32's very end it is rounded down, for the largest code times it to be finite.)
@@ -244,9 +255,7 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 top = lanes_max<kLanes>(top);
                 const float largest = __uint_as_float(top);
                 const bool finite = top < 0x7f800000u, some = finite && largest >= kKvZero;
-                // A full division: from 2^126 on the reciprocal alone would be
-                // subnormal, which the bare instruction gives as zero.
-                const float inv = some ? kKvCode16 / largest : 0.0f;
+                const float inv = some ? code_factor(largest) : 0.0f;
                 short *out = &st.code[is_v][t * kRow<D>];
                 *reinterpret_cast<s16x4 *>(out + at.a_at) = pack_codes(r[x].a, inv);
                 *reinterpret_cast<s16x4 *>(out + at.b_at) = pack_codes(r[x].b, inv);

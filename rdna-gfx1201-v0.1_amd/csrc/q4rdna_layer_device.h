@@ -18,19 +18,19 @@ __device__ __forceinline__ uint32_t mul_div(uint32_t a, uint32_t b, uint32_t c) 
     return static_cast<uint32_t>(x / c);
 }
 
-// 1 / sqrt(x) rounded once: one step of Newton's iteration on the instruction's
-// result (1 ulp), with the exact remainder 1 - x y^2 of two products and their
-// errors.  The instruction takes no subnormal x, so small ones are scaled by
-// 2^64; zeros, infinities and NaN keep its result.
-__device__ __forceinline__ float inverse_root(float x) {
+// 1 / sqrt(x) rounded once, x >= `least`: one step of Newton's iteration on the
+// instruction's result (1 ulp), with the exact remainder 1 - x y^2 of two products
+// and their errors.  The instruction takes no subnormal x, so where there may be
+// one, small ones are scaled by 2^64; zeros, infinities and NaN keep its result.
+__device__ __forceinline__ float inverse_root(float x, float least) {
 #pragma clang fp contract(off)
-    const bool tiny = x < 0x1p-100f;
+    const bool tiny = least < 0x1p-100f && x < 0x1p-100f;
     const float s = tiny ? x * 0x1p64f : x;
     const float y = __builtin_amdgcn_rsqf(s);
     const float t = s * y;
     const float rest = fmaf(-fmaf(s, y, -t), y, fmaf(-t, y, 1.0f));
-    const float z = fmaf(0.5f * y, rest, y);
-    const float root = s > 0.0f && s < __builtin_inff() ? z : y;
+    constexpr int kPositiveNormal = 0x100;
+    const float root = __builtin_amdgcn_classf(s, kPositiveNormal) ? fmaf(0.5f * y, rest, y) : y;
     return tiny ? root * 0x1p32f : root;
 }
 
