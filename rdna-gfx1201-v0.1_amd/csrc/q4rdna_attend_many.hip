@@ -14,11 +14,12 @@
 //  * q is scaled by a power of two per row, so fp16 and bf16 rows are exact in
 //    fp16.  Their weights are rounded to fp16 (11 bits), which the matrix
 //    instruction needs, while their sum keeps them whole: each weight is off by as
-//    much as an fp16 output is rounded by, an eighth of a bf16 output's rounding,
-//    and the errors of many weights average out.  fp32 rows take two fp16 parts of
-//    q and of the weights each (SPLIT = 2, 22 bits) and twice the products: the
-//    error is half of that of a plain fp32 softmax and product (5.7e-7 and 1.1e-6
-//    of the output at 2047 tokens).
+//    much as an fp16 output is rounded by, an eighth of a bf16 output's rounding
+//    (2048 tokens behind 6100 in bf16: 8 % of the outputs are a last place off those
+//    of a plain fp32 form, the error against 64 bits is 1.67e-3, that one's 1.66e-3).
+//    fp32 rows take two fp16 parts of q and of the weights each (SPLIT = 2, 22 bits)
+//    and twice the products: the error is half of a plain fp32 form's (5.7e-7 and
+//    1.1e-6 of the output at 2047 tokens).
 //  * V's scale per block goes into the weights: they are relative to the largest
 //    product of a weight and a V scale that the row has had, not to the largest
 //    weight, so fp16's range is spent on what counts in the row's output, however
