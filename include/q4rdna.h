@@ -478,6 +478,141 @@ typedef struct q4rdna_add_norm_desc {
 } q4rdna_add_norm_desc;
 int q4rdna_add_norm(const q4rdna_add_norm_desc *desc, void *stream);
 
+/* ---- several continuations of a sequence ------------------------------------
+ * Drafted tokens verified together (a tree of them per sequence), beams, and
+ * sequences that fork.  No reference counterpart.  As above: asynchronous on
+ * `stream`, fp32, fp16 or bf16, sums in fp32 and more. */
+
+/* A sequence of a step has at most so many drafted tokens. */
+#define Q4RDNA_TREE_MAX 64
+
+/* Positions and ancestors of a step's drafted tokens, once for all layers.
+ * Sequence i has the step's tokens cu_tokens[i] .. (as in q4rdna_kv_batch; of
+ * which past, cu_tokens, sequences, tokens and max_tokens <= Q4RDNA_TREE_MAX
+ * are used).  parents[n] is the place among its sequence's tokens of token n's
+ * parent, which comes before it, or -1 for one that follows the last cached
+ * token.  seen[n]: bit j is set where the sequence's j-th token is n itself or
+ * above it.  positions[n] = past + the number of tokens above n.  A token whose
+ * parent is out of range, those below it, and the tokens of a sequence whose
+ * entries are out of range get position -1 and seen 0; tokens of no sequence
+ * are not written.  Runs on the current device. */
+int q4rdna_kv_tree(const q4rdna_kv_batch *batch, const int32_t *parents, int32_t *positions,
+                   uint64_t *seen, void *stream);
+
+/* Rows of q and k normalised and rotated as q4rdna_kv_append does it, bit for
+ * bit, by a position given for each token.  A position outside the `positions`
+ * rows of cos and sin makes the token's rows NaN.  q_out may be q and k_out k;
+ * other overlaps are not allowed.  q_heads or k_heads 0: no q or k.  rotary 0:
+ * no rotation, cos, sin and position are not read.  Runs on the current device. */
+typedef struct q4rdna_rotate_desc {
+    uint32_t dtype;           /* of q, k and the outputs */
+    uint32_t tokens;
+    uint32_t q_heads, k_heads; /* at most 32768 in all */
+    uint32_t head_dim;        /* 64 or 128 */
+    uint32_t positions;
+    uint32_t rotary;          /* a multiple of 8 up to head_dim */
+    uint32_t interleaved;
+    q4rdna_kv_rows q, k, q_out, k_out;
+    const int32_t *position;  /* [tokens] */
+    const float *cos, *sin;   /* [positions][rotary / 2], 16-byte aligned */
+    const float *q_norm, *k_norm; /* [head_dim], 16-byte aligned, or NULL */
+    float eps;
+    uint32_t reserved;
+} q4rdna_rotate_desc;
+int q4rdna_rotate(const q4rdna_rotate_desc *desc, void *stream);
+
+/* Attention of a step's drafted tokens over the cache and over each other.
+ * The drafted tokens are not in the cache: sequence i holds past[i] tokens
+ * there, and k and v have the drafted ones' rows (k normalised and rotated).
+ * Query token n of a sequence sees the cached tokens and the drafted ones j
+ * of its sequence whose bit j is set in seen[n] (q4rdna_kv_tree's, or any
+ * other mask):
+ *   out = softmax(scale * q . k) v over these, lse as in q4rdna_kv_attend.
+ * With window > 0 a drafted token stands at past - 1 + the number of bits in
+ * its seen (those of tokens that are there), and sees what lies less than
+ * `window` before it: cached tokens at t > p - window, drafted ones at
+ * p_j > p - window.
+ * A row that sees nothing is zero, its lse -inf.  A drafted token with a number
+ * of k (v) that is not finite makes every row that sees it NaN.
+ * The cache is read only; accepted tokens are appended by q4rdna_kv_append of
+ * their rows, with rotary 0.  max_tokens <= Q4RDNA_TREE_MAX.  Refusals on the
+ * device, and scratch, as for q4rdna_kv_attend. */
+typedef struct q4rdna_kv_tree_desc {
+    uint32_t dtype;           /* of q, k, v and out */
+    uint32_t q_heads;
+    q4rdna_kv_rows q, k, v, out;
+    const uint64_t *seen;     /* [tokens] */
+    float *lse;
+    float scale;
+    uint32_t window;
+} q4rdna_kv_tree_desc;
+int q4rdna_kv_attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
+                          const q4rdna_kv_tree_desc *desc, void *stream);
+
+/* The best continuations of groups of beams.  For each group, over its beams b
+ * and the tokens v of the vocabulary,
+ *   total[b][v] = scores[b] + logits[b][v] - log sum_u exp(logits[b][u])
+ * and the `count` largest of them, largest first: out_scores, out_rows (group *
+ * beams + b) and out_tokens, each [groups][count].  Totals are compared in 64
+ * bits, those of one row by their logits; equal ones go by row, then by token.
+ * scores NULL: zeros.  A beam has no continuation, all its totals are -inf, if
+ * its score is not finite, if all its logits are -inf or if one of them is NaN
+ * or +inf; such totals come behind all others.  Scratch as for
+ * q4rdna_kv_attend.  Runs on the current device. */
+#define Q4RDNA_BEAM_MAX_COUNT 128
+#define Q4RDNA_BEAM_MAX_BEAMS 1024
+typedef struct q4rdna_beam_desc {
+    uint32_t dtype;           /* of logits */
+    uint32_t groups;
+    uint32_t beams;           /* at most Q4RDNA_BEAM_MAX_BEAMS */
+    uint32_t vocab;           /* at most 2^24 */
+    uint32_t count;           /* 1 .. Q4RDNA_BEAM_MAX_COUNT, at most beams * vocab */
+    uint32_t reserved;
+    const void *logits;       /* rows of `vocab` contiguous numbers, strides in elements */
+    int64_t group_stride, beam_stride;
+    const float *scores;      /* [groups][beams] or NULL */
+    float *out_scores;
+    int32_t *out_rows, *out_tokens;
+} q4rdna_beam_desc;
+int q4rdna_beam_select(const q4rdna_beam_desc *desc, void *stream);
+
+/* Sequences that go on from others, in place.  Sequence i of the batch becomes
+ * a copy of what sequence parents[i] was: its length, its full pages, which the
+ * two share from then on, and its open blocks.  parents[i] = -1: sequence i is
+ * dropped, its length becomes 0.
+ *  - slots: the first sequence that goes on from a parent takes the parent's
+ *    slot, the others the slots of sequences that nobody goes on from, both in
+ *    ascending order, and the parent's open blocks are copied there: of a length
+ *    m the block m / 64 where it holds tokens, and the one before it.
+ *  - table: entries of full blocks come from the parent's row.  A page that is
+ *    then in no row's full blocks is free, but for those marked in `kept`, and
+ *    the entries of the blocks that the next `room` tokens of each sequence
+ *    (none of a dropped one) touch get free pages: the lowest numbers first, in
+ *    the order of sequences and blocks.  Other entries become -1, and so do those
+ *    that no page is left for, each of which adds to *faults.
+ * So `fork` with parents[i] = i gives out the pages for the next tokens, and a
+ * program that calls it before each step needs no allocator of its own.  Every
+ * sequence that holds pages of these caches has to be in the batch, or its
+ * pages in `kept`.  A parent that is out of range, or has a length or a slot
+ * that is, drops the sequence, and adds to *faults.  Two sequences may not share
+ * a slot.
+ * `caches` are the layers' caches, of one geometry (page_count, slot_count,
+ * kv_heads, head_dim, device), none of whose buffers may be another's; their
+ * pages are neither read nor written.  The batch's past, table and slots are
+ * written; cu_tokens, tokens and max_tokens are not used.  Scratch as for
+ * q4rdna_kv_attend. */
+#define Q4RDNA_FORK_MAX_SEQUENCES 4096
+typedef struct q4rdna_kv_fork_desc {
+    const int32_t *parents;   /* [sequences] */
+    int32_t *past, *table, *slots; /* as in q4rdna_kv_batch, not NULL */
+    const uint8_t *kept;      /* [page_count], non-zero: not free, or NULL */
+    uint32_t sequences;       /* at most Q4RDNA_FORK_MAX_SEQUENCES */
+    uint32_t table_width;
+    uint32_t room;
+    uint32_t reserved;
+} q4rdna_kv_fork_desc;
+int q4rdna_kv_fork(const q4rdna_kv_cache *caches, uint32_t count, const q4rdna_kv_fork_desc *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -342,20 +342,6 @@ __device__ __forceinline__ Span span_of(const AttendArgs &a, int past, int first
     return s;
 }
 
-// Inclusive sum over the wave's lanes up to this one: shifts within rows of 16
-// lanes, then the rows' last lanes into the rows after them.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
-    return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v = scan_step<0x111, 0xf>(v);
-    v = scan_step<0x112, 0xf>(v);
-    v = scan_step<0x114, 0xf>(v);
-    v = scan_step<0x118, 0xf>(v);
-    v = scan_step<0x142, 0xa>(v);
-    return scan_step<0x143, 0xc>(v);
-}
 __device__ __forceinline__ uint64_t wave_total(uint64_t v) {  // v < 2^42
     const uint32_t low = wave_scan(static_cast<uint32_t>(v & 0xffffu)), high = wave_scan(static_cast<uint32_t>(v >> 16));
     return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(high, 63))) << 16) +

@@ -14,6 +14,7 @@
 // sequences' tokens 9.3 us, where some fill their blocks: a block that closes is
 // a chain of loads (lengths, open planes, page) with LDS round trips between.
 #include "q4rdna_layer_device.h"
+#include "q4rdna_rotate_device.h"
 
 namespace q4rdna {
 namespace {
@@ -22,95 +23,6 @@ namespace {
 // shorts: the pad keeps rows 16-byte aligned and shifts them by four banks.
 template <int D>
 constexpr int kRow = D + 8;
-
-// One row of a head in the lanes of a group of D / 8: eight numbers per lane in
-// two runs of four, at a_at and b_at.
-struct Row {
-    float a[4], b[4];
-};
-struct Place {
-    int a_at, b_at;
-    bool turned;  // the lane's numbers are rotated
-    int pair;     // the first of its four pairs
-};
-
-template <bool INTERLEAVED>
-__device__ __forceinline__ Place place_of(int lane, uint32_t rotary) {
-    const int half = static_cast<int>(rotary) / 2;
-    Place p;
-    p.pair = 4 * lane;
-    p.turned = p.pair < half;  // rotary is a multiple of 8: a lane's pairs lie on one side
-    if (p.turned && !INTERLEAVED) {
-        p.a_at = p.pair;
-        p.b_at = p.pair + half;
-    } else {
-        p.a_at = 8 * lane;
-        p.b_at = 8 * lane + 4;
-    }
-    return p;
-}
-
-template <typename T>
-__device__ __forceinline__ void load_row(Row &r, const T *row, const Place &p, bool wide) {
-    load_floats<T, 4>(row + p.a_at, wide, r.a);
-    load_floats<T, 4>(row + p.b_at, wide, r.b);
-}
-// The lane's four cosines and sines at a position.
-struct Turn {
-    float c[4], s[4];
-};
-__device__ __forceinline__ void load_turn(Turn &t, const Place &p, const q4rdna_kv_append_desc &d, int position) {
-    if (!p.turned) return;
-    const size_t at = static_cast<size_t>(position) * (d.rotary / 2) + p.pair;
-    load_floats<float, 4>(d.cos + at, true, t.c);
-    load_floats<float, 4>(d.sin + at, true, t.s);
-}
-
-// The lane's norm weights, once per workgroup.
-struct Weights {
-    float a[4], b[4];
-};
-__device__ __forceinline__ void load_weights(Weights &w, const float *weight, const Place &p) {
-    if (weight == nullptr) return;
-    load_floats<float, 4>(weight + p.a_at, true, w.a);
-    load_floats<float, 4>(weight + p.b_at, true, w.b);
-}
-// Which products are fused is written out here and in turn_pair: the compiler
-// would choose anew for each copy of an unrolled loop, and the cache's bytes
-// would depend on a token's place in its step.
-template <int D>
-__device__ __forceinline__ void norm_row(Row &r, const Weights &w, float eps) {
-#pragma clang fp contract(off)
-    float sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum = fmaf(r.a[e], r.a[e], fmaf(r.b[e], r.b[e], sum));
-    const float inv = inverse_root(fmaf(lanes_sum<D / 8>(sum), 1.0f / D, eps), eps);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        r.a[e] = r.a[e] * inv * w.a[e];
-        r.b[e] = r.b[e] * inv * w.b[e];
-    }
-}
-__device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s) {
-#pragma clang fp contract(off)
-    const float bs = b * s, as = a * s;
-    const float x = fmaf(a, c, -bs);
-    b = fmaf(b, c, as);
-    a = x;
-}
-template <bool INTERLEAVED>
-__device__ __forceinline__ void turn_row(Row &r, const Place &p, const Turn &t) {
-    if (!p.turned) return;
-    if (INTERLEAVED) {
-        turn_pair(r.a[0], r.a[1], t.c[0], t.s[0]);
-        turn_pair(r.a[2], r.a[3], t.c[1], t.s[1]);
-        turn_pair(r.b[0], r.b[1], t.c[2], t.s[2]);
-        turn_pair(r.b[2], r.b[3], t.c[3], t.s[3]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) turn_pair(r.a[e], r.b[e], t.c[e], t.s[e]);
-    }
-}
 
 // x * f rounded to the nearest integer, as the low bits of a float's: the sum
 // with 1.5 * 2^23 has a last place of one.  For |x * f| < 2^22; a NaN gives 0
@@ -235,7 +147,7 @@ __device__ void append_block(const AppendArgs &a, const Seq &s, uint32_t i, uint
                 const Place at = place_of<INTERLEAVED>(lane, is_v ? 0 : a.d.rotary);
                 load_row(r[x], static_cast<const T *>(data) + n * token_stride + head * head_stride, at,
                          a.wide != 0);
-                load_turn(turn[x], at, a.d, start + t);
+                load_turn(turn[x], at, a.d.cos, a.d.sin, a.d.rotary, start + t);
             }
         }
 #pragma unroll
@@ -505,7 +417,7 @@ __device__ void turn_q(const AppendArgs &a, uint32_t unit) {
             // A refused sequence's rows are not written (it is counted with its blocks).
             live[x] = s.ok && static_cast<int>(n[x]) >= s.first && static_cast<int>(n[x]) < s.first + s.count &&
                       (a.d.rotary == 0 || static_cast<uint32_t>(s.length) <= a.d.positions);
-            if (live[x]) load_turn(turn[x], at, a.d, s.past + static_cast<int>(n[x]) - s.first);
+            if (live[x]) load_turn(turn[x], at, a.d.cos, a.d.sin, a.d.rotary, s.past + static_cast<int>(n[x]) - s.first);
         }
 #pragma unroll
         for (int x = 0; x < kEach; ++x) {

@@ -1,0 +1,237 @@
+// Sequences that go on from others (q4rdna_kv_fork).
+//
+// Two launches.  fork_plan_kernel, one workgroup, decides: each sequence's
+// parent, length and slot, which open blocks are copied, and which pages are
+// free, in the order in which they are given out.  fork_move_kernel carries it
+// out: a workgroup renames some columns of the table, all rows of which it has
+// read before it writes the first, and others copy open blocks, which is what
+// takes the time (2 us of planning and launching aside, a copy's rate).
+#include "q4rdna_layer_device.h"
+
+namespace q4rdna {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kBlock = static_cast<int>(kKvBlock);
+
+// Sum of v over the threads before this one; `all` receives that of all.
+__device__ __forceinline__ uint32_t threads_before(uint32_t v, uint32_t *totals, uint32_t *all) {
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const uint32_t upto = wave_scan(v);
+    __syncthreads();  // the totals of the call before have been read
+    if (lane == 63) totals[wave] = upto;
+    __syncthreads();
+    uint32_t before = 0, sum = 0;
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        const uint32_t t = totals[w];
+        before += w < wave ? t : 0;
+        sum += t;
+    }
+    *all = sum;
+    return before + upto - v;
+}
+
+// Blocks that the next `room` tokens behind `past` touch: from past / 64 up to
+// this one.
+__device__ __forceinline__ int room_end(const q4rdna_kv_fork_desc &d, int past) {
+    const uint64_t end = (static_cast<uint64_t>(past) + d.room + kBlock - 1) / kBlock;
+    return static_cast<int>(min(end, static_cast<uint64_t>(d.table_width)));
+}
+
+__global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs a) {
+    __shared__ int32_t parent[Q4RDNA_FORK_MAX_SEQUENCES], past[Q4RDNA_FORK_MAX_SEQUENCES];
+    __shared__ int32_t first[Q4RDNA_FORK_MAX_SEQUENCES];  // the first that goes on from a sequence
+    __shared__ int32_t vacant[Q4RDNA_FORK_MAX_SEQUENCES];  // slots of those that nobody goes on from
+    __shared__ uint32_t used[kForkPages / 32];
+    __shared__ uint32_t totals[kPlanThreads / 64], copies, longest;
+    const int tid = threadIdx.x, n = static_cast<int>(a.d.sequences), width = static_cast<int>(a.d.table_width);
+    const int words = static_cast<int>((a.page_count + 31) / 32);
+    const auto fault = [&] {
+        if (a.faults != nullptr) atomicAdd(a.faults, 1u);
+    };
+    for (int w = tid; w < words; w += kPlanThreads) used[w] = 0;
+    for (int i = tid; i < n; i += kPlanThreads) first[i] = n;
+    if (tid == 0) copies = longest = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kPlanThreads) {
+        int p = a.d.parents[i], length = 0;
+        if (p != -1) {
+            bool ok = static_cast<uint32_t>(p) < static_cast<uint32_t>(n);
+            if (ok) {
+                length = a.d.past[p];
+                ok = length >= 0 && length <= static_cast<int64_t>(width) * kBlock && static_cast<uint32_t>(a.d.slots[p]) < a.slot_count;
+            }
+            if (!ok) {
+                fault();
+                p = -1;
+                length = 0;
+            }
+        }
+        parent[i] = p;
+        past[i] = length;
+        if (p >= 0) atomicMin(&first[p], i);
+    }
+    __syncthreads();
+    uint32_t base = 0, all;
+    for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+        const int i = i0 + tid;
+        const bool none = i < n && first[i] == n;
+        const uint32_t at = base + threads_before(none, totals, &all);
+        if (none) vacant[at] = a.d.slots[i];
+        base += all;
+    }
+    __syncthreads();
+    uint32_t later = 0, given = 0;  // as many later children and dropped ones as vacant slots
+    for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+        const int i = i0 + tid;
+        int p = i < n ? parent[i] : -1, length = i < n ? past[i] : 0;
+        const bool moved = i < n && (p < 0 || first[p] != i);
+        const uint32_t at = later + threads_before(moved, totals, &all);
+        later += all;
+        const int from = p >= 0 ? a.d.slots[p] : 0, slot = moved ? vacant[at] : from;
+        if (p >= 0 && static_cast<uint32_t>(slot) >= a.slot_count) {
+            fault();
+            p = -1;
+            length = 0;
+        }
+        const int blocks = p >= 0 ? max(room_end(a.d, length) - length / kBlock, 0) : 0;
+        const uint32_t rank = given + threads_before(static_cast<uint32_t>(blocks), totals, &all);
+        given += all;
+        if (i < n) {
+            parent[i] = p;
+            past[i] = length;
+            a.moves[i] = ForkMove{p, length, slot, rank};
+            if (moved && length > 0) a.copies[atomicAdd(&copies, 1u)] = ForkCopy{from, slot, length};
+            if (length >= kBlock) atomicMax(&longest, static_cast<uint32_t>(length / kBlock));
+        }
+    }
+    __syncthreads();
+    // The pages of full blocks, kEach entries of a thread in flight.
+    constexpr int kEach = 8;
+    const uint32_t columns = longest;
+    const uint64_t entries = static_cast<uint64_t>(n) * columns;
+    for (uint64_t e0 = tid; e0 < entries; e0 += kEach * kPlanThreads) {
+        int page[kEach];
+#pragma unroll
+        for (int x = 0; x < kEach; ++x) {
+            const uint64_t e = e0 + static_cast<uint64_t>(x) * kPlanThreads;
+            page[x] = -1;
+            if (e < entries) {
+                const uint32_t i = entries >> 32 == 0 ? static_cast<uint32_t>(e) / columns : static_cast<uint32_t>(e / columns);
+                const int b = static_cast<int>(e - static_cast<uint64_t>(i) * columns);
+                if (b < past[i] / kBlock) page[x] = a.d.table[static_cast<size_t>(parent[i]) * width + b];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < kEach; ++x)
+            if (static_cast<uint32_t>(page[x]) < a.page_count) atomicOr(&used[page[x] / 32], 1u << (page[x] % 32));
+    }
+    if (a.d.kept != nullptr)
+        for (uint32_t p = tid; p < a.page_count; p += kPlanThreads)
+            if (a.d.kept[p] != 0) atomicOr(&used[p / 32], 1u << (p % 32));
+    __syncthreads();
+    uint32_t found = 0;
+    for (int w0 = 0; w0 < words && found < given; w0 += kPlanThreads) {
+        const int w = w0 + tid;
+        uint32_t open = w < words ? ~used[w] : 0;
+        if (w == words - 1 && a.page_count % 32 != 0) open &= (1u << (a.page_count % 32)) - 1u;
+        uint32_t at = found + threads_before(static_cast<uint32_t>(__builtin_popcount(open)), totals, &all);
+        found += all;
+        for (; open != 0 && at < given; open &= open - 1, ++at) a.free[at] = 32 * w + __builtin_ctz(open);
+    }
+    if (tid == 0) {
+        a.counts[0] = copies;
+        a.counts[1] = min(found, given);
+    }
+}
+
+__device__ __forceinline__ void move_table(const ForkArgs &a) {
+    constexpr int kEach = kForkEntries / 256;
+    const int tid = threadIdx.x, n = static_cast<int>(a.d.sequences), width = static_cast<int>(a.d.table_width);
+    const int columns = 1 << a.columns_log2, column0 = static_cast<int>(blockIdx.x << a.columns_log2);
+    const uint32_t given = a.counts[1];
+    int32_t entry[kEach];
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+        const int e = tid + 256 * x, i = e >> a.columns_log2, b = column0 + (e & (columns - 1));
+        entry[x] = -1;
+        if (i >= n || b >= width) continue;
+        const ForkMove m = a.moves[i];
+        const int full = m.past / kBlock;
+        if (m.parent < 0) continue;
+        if (b < full) {
+            entry[x] = a.d.table[static_cast<size_t>(m.parent) * width + b];
+        } else if (b < room_end(a.d, m.past)) {
+            const uint32_t rank = m.pages + (b - full);
+            if (rank < given) entry[x] = a.free[rank];
+            else if (a.faults != nullptr) atomicAdd(a.faults, 1u);
+        }
+    }
+    wait_stores();  // the loads too: all rows have been read
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+        const int e = tid + 256 * x, i = e >> a.columns_log2, b = column0 + (e & (columns - 1));
+        if (i < n && b < width) a.d.table[static_cast<size_t>(i) * width + b] = entry[x];
+    }
+    if (blockIdx.x == 0)
+        for (int i = tid; i < n; i += 256) {
+            const ForkMove m = a.moves[i];
+            a.d.past[i] = m.past;
+            a.d.slots[i] = m.slot;
+        }
+}
+
+// One head's planes and token scales of one block: 16 bytes of a thread, kEach
+// times.
+template <int D>
+__device__ __forceinline__ void copy_open(const ForkArgs &a, uint32_t unit) {
+    constexpr int kEach = 4 * kBlock * D / (16 * 256);
+    const int tid = threadIdx.x;
+    const uint32_t head = unit % a.kv_heads, rest = unit / a.kv_heads;
+    const uint32_t layer = rest / 2 % a.layers;
+    const ForkCopy c = a.copies[rest / 2 / a.layers];
+    // the open block, where it holds tokens, or the one before it
+    const int block = c.past / kBlock - static_cast<int>(rest % 2);
+    if (block < 0 || block * kBlock >= c.past) return;
+    const size_t from = (static_cast<size_t>(c.from) * 2 + (block & 1)) * a.kv_heads + head;
+    const size_t to = (static_cast<size_t>(c.to) * 2 + (block & 1)) * a.kv_heads + head;
+    constexpr size_t kPlanes = 4 * kBlock * D;
+    const int8_t *src = a.open[layer] + from * kPlanes + 16 * tid;
+    int8_t *dst = a.open[layer] + to * kPlanes + 16 * tid;
+    i32x4 v[kEach];
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) v[x] = load16(src + 4096 * x);
+    if (tid < 2 * kBlock / 4) {
+        const i32x4 s = load16(a.open_scales[layer] + from * 2 * kBlock + 4 * tid);
+        store16(a.open_scales[layer] + to * 2 * kBlock + 4 * tid, s);
+    }
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) store16(dst + 4096 * x, v[x]);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void fork_move_kernel(const ForkArgs a) {
+    if (blockIdx.x < a.table_units) {
+        move_table(a);
+        return;
+    }
+    const uint32_t copiers = gridDim.x - a.table_units;
+    const uint64_t units = static_cast<uint64_t>(a.counts[0]) * a.layers * 2 * a.kv_heads;  // fewer than 2^32
+    for (uint64_t u = blockIdx.x - a.table_units; u < units; u += copiers) copy_open<D>(a, static_cast<uint32_t>(u));
+}
+
+}  // namespace
+
+hipError_t launch_fork_plan(const ForkArgs &a, hipStream_t stream) {
+    fork_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t launch_fork_move(const ForkArgs &a, uint32_t copiers, hipStream_t stream) {
+    auto go = [&](auto kernel) { kernel<<<a.table_units + copiers, 256, 0, stream>>>(a); };
+    a.head_dim == 64 ? go(fork_move_kernel<64>) : go(fork_move_kernel<128>);
+    return hipGetLastError();
+}
+
+}  // namespace q4rdna

@@ -1,6 +1,8 @@
 // Internal interface of the decoder-layer operators: the kernels of
-// q4rdna_cache.hip (append, read), q4rdna_attend.hip and q4rdna_norm.hip, and
-// their entry points in q4rdna_layer.cpp.  Not part of the C ABI.
+// q4rdna_cache.hip (append, read), q4rdna_attend.hip and q4rdna_norm.hip, with
+// their entry points in q4rdna_layer.cpp, and those of q4rdna_draft.hip,
+// q4rdna_attend_tree.hip, q4rdna_beam.hip and q4rdna_fork.hip, with theirs in
+// q4rdna_branch.cpp.  Not part of the C ABI.
 #pragma once
 
 #include <hip/hip_runtime_api.h>
@@ -83,5 +85,83 @@ uint64_t attend_many_places(const q4rdna_kv_batch &b, uint32_t group);
 hipError_t launch_attend_many(const AttendArgs &a, uint32_t places, hipStream_t stream);
 
 hipError_t launch_add_norm(const q4rdna_add_norm_desc &d, bool wide, uint32_t cus, hipStream_t stream);
+
+constexpr uint32_t kTreeMax = Q4RDNA_TREE_MAX;
+hipError_t launch_tree(const q4rdna_kv_batch &batch, const int32_t *parents, int32_t *positions, uint64_t *seen,
+                       hipStream_t stream);
+
+struct RotateArgs {
+    q4rdna_rotate_desc d;
+    uint32_t heads;        // of q and k together
+    uint32_t heads_magic;  // div_split's
+    uint32_t rows;         // (token, head), fewer than 2^31
+    uint32_t unit_rows;    // that a workgroup takes
+    uint32_t wide;         // rows can be read and written four elements at a time
+};
+hipError_t launch_rotate(const RotateArgs &a, hipStream_t stream);
+
+struct TreeArgs {
+    q4rdna_kv_cache cache;
+    q4rdna_kv_batch batch;
+    q4rdna_kv_tree_desc d;
+    uint32_t group;       // query heads per kv head
+    uint32_t row_waves;   // 1, 2 or 4 of a workgroup's waves have rows of their own, 32 each: a row group
+    uint32_t row_groups;  // of the largest sequence
+    uint32_t splits;      // the most workgroups that share a row group
+    uint32_t least;       // units (cached blocks, the drafts) of a part, the least
+    uint32_t target;      // workgroups to deal the units to
+    uint32_t workgroups;  // launched
+    uint32_t wide;        // rows of q, k and v can be read 16 bytes at a time
+    uint32_t wide_out;    // out rows can be written four elements at a time
+    float *partials;      // of each workgroup: [row][D], then all the maxima, sums and units, [row][3]
+    uint32_t *arrived;    // [sequence][row group][head], zero between launches
+};
+hipError_t launch_attend_tree(const TreeArgs &a, hipStream_t stream);
+
+struct BeamArgs {
+    q4rdna_beam_desc d;
+    uint32_t each;      // numbers of a row that a thread takes: 4, 8, 16 or 32
+    uint32_t chunks;    // of 256 * each numbers, per row
+    uint64_t *tops;     // [group][count][beam][chunk]: ordered logit << 32 | ~token, 0: none
+    uint64_t *stats;    // [group][beam][chunk][2]: sum (double), max (float)
+    uint32_t *arrived;  // [group], zero between launches
+};
+hipError_t launch_beam(const BeamArgs &a, hipStream_t stream);
+
+// A sequence's new state, by the plan that fork_plan_kernel makes.
+struct ForkMove {
+    int32_t parent;  // -1: dropped
+    int32_t past;
+    int32_t slot;
+    uint32_t pages;  // of the pages given out, its first one's rank
+};
+struct ForkCopy {
+    int32_t from, to;  // slots
+    int32_t past;
+};
+// Layers whose open blocks one launch copies.
+constexpr uint32_t kForkLayers = 64;
+struct ForkArgs {
+    q4rdna_kv_fork_desc d;
+    uint32_t *faults;
+    uint32_t page_count, slot_count, kv_heads, head_dim;
+    ForkMove *moves;   // [sequences]
+    ForkCopy *copies;  // [sequences]
+    uint32_t *counts;  // copies, pages in `free`
+    int32_t *free;     // pages in the order in which they are given out
+    uint32_t columns_log2;  // of the table, that a workgroup takes
+    uint32_t table_units;
+    uint32_t layers;
+    int8_t *open[kForkLayers];
+    float *open_scales[kForkLayers];
+};
+// The most pages: their bits lie in LDS.
+constexpr uint32_t kForkPages = 1u << 18;
+// Entries of the table that a workgroup takes.
+constexpr uint32_t kForkEntries = 4096;
+hipError_t launch_fork_plan(const ForkArgs &a, hipStream_t stream);
+// a.table_units workgroups for the table, the lengths and the slots, and
+// `copiers` for the open blocks.
+hipError_t launch_fork_move(const ForkArgs &a, uint32_t copiers, hipStream_t stream);
 
 }  // namespace q4rdna

@@ -1,5 +1,5 @@
-// Device helpers of the decoder-layer kernels (q4rdna_cache.hip,
-// q4rdna_attend.hip, q4rdna_norm.hip).
+// Device helpers of the decoder-layer kernels (q4rdna_cache.hip and the others
+// that q4rdna_layer.h lists).
 #pragma once
 
 #include "q4rdna_device.h"
@@ -107,6 +107,20 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     v = max(v, dpp<kDppMirror8>(v));
     if (LANES == 16) v = max(v, dpp<kDppMirror16>(v));
     return v;
+}
+// Inclusive sum over the wave's lanes up to this one: shifts within rows of 16
+// lanes, then the rows' last lanes into the rows after them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+    return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = scan_step<0x111, 0xf>(v);
+    v = scan_step<0x112, 0xf>(v);
+    v = scan_step<0x114, 0xf>(v);
+    v = scan_step<0x118, 0xf>(v);
+    v = scan_step<0x142, 0xa>(v);
+    return scan_step<0x143, 0xc>(v);
 }
 __device__ __forceinline__ float max_xor16(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

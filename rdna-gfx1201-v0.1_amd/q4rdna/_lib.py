@@ -39,6 +39,10 @@ F16 = 1
 BF16 = 2
 KV_BLOCK = 64
 NORM_MAX_WIDTH = 16384
+TREE_MAX = 64
+BEAM_MAX_COUNT = 128
+BEAM_MAX_BEAMS = 1024
+FORK_MAX_SEQUENCES = 4096
 
 # Every symbol include/q4rdna.h declares.
 EXPORTS = (
@@ -52,6 +56,7 @@ EXPORTS = (
     "q4rdna_plan_workgroups", "q4rdna_pack", "q4rdna_dequantize",
     "q4rdna_launch_count", "q4rdna_sidecar_hits", "q4rdna_report_stats",
     "q4rdna_kv_append", "q4rdna_kv_attend", "q4rdna_kv_read", "q4rdna_add_norm",
+    "q4rdna_kv_tree", "q4rdna_rotate", "q4rdna_kv_attend_tree", "q4rdna_beam_select", "q4rdna_kv_fork",
 )
 
 
@@ -125,12 +130,45 @@ class AddNormDesc(ctypes.Structure):
                 ("n_stride", ctypes.c_int64), ("post_weight", ctypes.c_void_p), ("weight", ctypes.c_void_p)]
 
 
+class RotateDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("q_heads", ctypes.c_uint32),
+                ("k_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("positions", ctypes.c_uint32),
+                ("rotary", ctypes.c_uint32), ("interleaved", ctypes.c_uint32), ("q", Rows), ("k", Rows), ("q_out", Rows),
+                ("k_out", Rows), ("position", ctypes.c_void_p), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+                ("reserved", ctypes.c_uint32)]
+
+
+class TreeDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("q_heads", ctypes.c_uint32), ("q", Rows), ("k", Rows), ("v", Rows),
+                ("out", Rows), ("seen", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("scale", ctypes.c_float),
+                ("window", ctypes.c_uint32)]
+
+
+class BeamDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("groups", ctypes.c_uint32), ("beams", ctypes.c_uint32),
+                ("vocab", ctypes.c_uint32), ("count", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+                ("logits", ctypes.c_void_p), ("group_stride", ctypes.c_int64), ("beam_stride", ctypes.c_int64),
+                ("scores", ctypes.c_void_p), ("out_scores", ctypes.c_void_p), ("out_rows", ctypes.c_void_p),
+                ("out_tokens", ctypes.c_void_p)]
+
+
+class ForkDesc(ctypes.Structure):
+    _fields_ = [("parents", ctypes.c_void_p), ("past", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("slots", ctypes.c_void_p), ("kept", ctypes.c_void_p), ("sequences", ctypes.c_uint32),
+                ("table_width", ctypes.c_uint32), ("room", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
 # The same structures as packers: one call fills a descriptor, where setting
 # each field of a ctypes structure takes longer than the kernel's launch.
 ROWS = struct.Struct("@Pqq")
 APPEND = struct.Struct("@2I Pqq Pqq Pqq Pqq 2P 3If 2P")
 ATTEND = struct.Struct("@2I Pqq Pqq P f I")
 ADD_NORM = struct.Struct("@3I2fI 5P 5q 2P")
+ROTATE = struct.Struct("@8I Pqq Pqq Pqq Pqq 5P f I")
+TREE = struct.Struct("@2I Pqq Pqq Pqq Pqq 2P f I")
+BEAM = struct.Struct("@6I P 2q 4P")
+FORK = struct.Struct("@5P 4I")
 
 _lib = None
 
@@ -184,6 +222,11 @@ def load() -> ctypes.CDLL:
         "q4rdna_kv_attend": (i32, [vp, vp, vp, vp]),
         "q4rdna_kv_read": (i32, [vp, vp, u32, vp, vp, vp]),
         "q4rdna_add_norm": (i32, [vp, vp]),
+        "q4rdna_kv_tree": (i32, [vp, vp, vp, vp, vp]),
+        "q4rdna_rotate": (i32, [vp, vp]),
+        "q4rdna_kv_attend_tree": (i32, [vp, vp, vp, vp]),
+        "q4rdna_beam_select": (i32, [vp, vp]),
+        "q4rdna_kv_fork": (i32, [vp, u32, vp, vp]),
     }
     for name, (res, args) in proto.items():
         fn = getattr(L, name)

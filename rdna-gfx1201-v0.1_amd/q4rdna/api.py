@@ -491,6 +491,18 @@ def _packed_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _out_rows(out: torch.Tensor | None, name: str, like: torch.Tensor, device: int):
+    """(out, its rows): the one given, or a new one like the input."""
+    if out is None:
+        out = torch.empty_like(like)
+        if out.stride(2) != 1:
+            out = _packed_like(like)
+        token_stride, head_stride, _ = out.stride()
+        return out, (out.data_ptr(), token_stride, head_stride)
+    _no_overlap(out, name)
+    return out, _rows(out, name, like.dtype, like.shape, device)
+
+
 def _no_overlap(t: torch.Tensor, name: str) -> None:
     """An output whose rows share memory would be written by several rows at once."""
     if not t.is_contiguous():
@@ -548,6 +560,37 @@ class KVBatch:
         self.sequences = n
         self._keep = (past, table, cu_tokens, slots)
 
+    def fork(self, parents: torch.Tensor, caches: Sequence["KVCache"], room: int = 1, kept: torch.Tensor | None = None,
+             stream: int | None = None) -> None:
+        """Sequence i goes on from what sequence parents[i] (int32 [sequences],
+        -1: none) was; past, table and slots are changed in place, and so are
+        the open blocks in `caches`, all layers' (q4rdna_kv_fork).
+
+        Full pages are shared.  Entries for the next `room` tokens get pages
+        that no sequence of the batch holds (and that `kept`, bool or uint8
+        [pages], does not mark), so a program that forks before each step, with
+        parents[i] = i where nothing changes, needs no allocator of its own.
+        What is refused, and entries that no page is left for, count in the
+        first cache's faults()."""
+        past, table, _, slots = self._keep
+        if slots is None:
+            raise ValueError("a batch that forks needs its slots")
+        device, n, caches = self.device, self.sequences, tuple(caches)
+        if not caches:
+            raise ValueError("fork needs the layers' caches")
+        for cache in caches:
+            if cache.device != device:
+                raise ValueError(f"the batch lives on cuda:{device}, a cache on cuda:{cache.device}")
+        at = _plain(parents, "parents", torch.int32, (n,), device)
+        kept_at = 0
+        if kept is not None:
+            kept_at = _plain(kept, "kept", torch.uint8 if kept.dtype == torch.uint8 else torch.bool, (caches[0].pages.shape[0],), device)
+        if not 0 <= room < 1 << 31:
+            raise ValueError("room must not be negative (or reach 2^31)")
+        d = _lib.FORK.pack(at, past.data_ptr(), table.data_ptr(), slots.data_ptr(), kept_at, n, table.shape[1], room, 0)
+        s = _raw_stream(device) if stream is None else stream
+        check(load().q4rdna_kv_fork(b"".join([c._bytes for c in caches]), len(caches), d, s))
+
     def _of(self, tokens: int):
         """The descriptor for a call on `tokens` tokens: a new one where the last
         call had another count (that call may still be using its own)."""
@@ -591,6 +634,7 @@ class KVCache:
         raw.device = device
         self.raw = raw
         self._ref = ctypes.byref(raw)
+        self._bytes = bytes(raw)
         self.device = device
         self.kv_heads = heads
         self.head_dim = raw.head_dim
@@ -707,6 +751,43 @@ class KVCache:
         check(load().q4rdna_kv_attend(self._ref, step, d, s))
         return out if lse is False else (out, lse)
 
+    def attend_tree(self, batch: KVBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor,
+                    out: torch.Tensor | None = None, scale: float | None = None, window: int = 0,
+                    lse: bool | torch.Tensor = False, stream: int | None = None):
+        """Attention of the step's drafted tokens, q [tokens, q_heads, head_dim],
+        over the cache, which holds `past` tokens of each sequence and none of
+        these, and over each other: k and v [tokens, kv_heads, head_dim] are the
+        drafted tokens', k normalised and rotated (:func:`rotate`), and bit j of
+        seen[n] (int64 [tokens], :func:`tree`'s or any mask) is set where token n
+        sees the j-th drafted one of its sequence.  The cache does not change:
+        the rows of accepted tokens are appended afterwards, by :meth:`append`
+        without cos and sin.  The batch's max_tokens is 64 at most.  scale,
+        window, lse and refused sequences as for :meth:`attend`; with a window a
+        token stands at past - 1 + the number of drafted ones that it sees."""
+        if q.dim() != 3:
+            raise ValueError("q must be [tokens, q_heads, head_dim]")
+        if stream is not None and (out is None or lse is True):
+            with _on_stream(stream, self.device):
+                return self.attend_tree(batch, q, k, v, seen, out, scale, window, lse)
+        dtype, device = q.dtype, self.device
+        tokens, heads, _ = q.shape
+        step = self._step(batch, tokens)
+        shape, kv_shape = (tokens, heads, self.head_dim), (tokens, self.kv_heads, self.head_dim)
+        rows = _rows(q, "q", dtype, shape, device)
+        k_rows, v_rows = _rows(k, "k", dtype, kv_shape, device), _rows(v, "v", dtype, kv_shape, device)
+        out, out_rows = _out_rows(out, "out", q, device)
+        if lse is True:
+            lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+        if not 0 <= window < 1 << 32:
+            raise ValueError("window must not be negative (or reach 2^32)")
+        d = _lib.TREE.pack(_dtype(dtype), heads, *rows, *k_rows, *v_rows, *out_rows,
+                           _plain(seen, "seen", torch.int64, (tokens,), device),
+                           0 if lse is False else _plain(lse, "lse", torch.float32, (tokens, heads), device),
+                           self.head_dim ** -0.5 if scale is None else scale, window)
+        s = _raw_stream(device) if stream is None else stream
+        check(load().q4rdna_kv_attend_tree(self._ref, step, d, s))
+        return out if lse is False else (out, lse)
+
     def read(self, batch: KVBatch, tokens: int, dtype: torch.dtype = torch.float32, k: torch.Tensor | None = None,
              v: torch.Tensor | None = None, stream: int | None = None):
         """(k, v) [tokens, kv_heads, head_dim]: the batch's tokens (past[i] on,
@@ -808,3 +889,129 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
         with torch.cuda.device(device):
             check(load().q4rdna_add_norm(d, s))
     return (residual if h is None else h), n
+
+
+def _call(device: int, entry, *args) -> None:
+    """A call that runs on the current device, on its tensors' one."""
+    if torch.cuda.current_device() == device:
+        check(entry(*args))
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args))
+
+
+def tree(batch: KVBatch, parents: torch.Tensor, positions: torch.Tensor | None = None, seen: torch.Tensor | None = None,
+         stream: int | None = None):
+    """(positions, seen) of a step's drafted tokens, once for all layers
+    (q4rdna_kv_tree): parents (int32 [tokens]) holds each token's parent among
+    its sequence's tokens, which comes before it, or -1 for one that follows
+    the last cached token.  positions (int32) is past + the tokens above it,
+    seen (int64) has a bit for each of them and for itself.  A token whose
+    parent is out of range, and what lies below it, gets position -1 and seen
+    0.  The batch's max_tokens is 64 at most."""
+    device = batch.device
+    if stream is not None and (positions is None or seen is None):
+        with _on_stream(stream, device):
+            return tree(batch, parents, positions, seen)
+    shape = parents.shape
+    if len(shape) != 1:
+        raise ValueError("parents must be [tokens]")
+    at = _plain(parents, "parents", torch.int32, shape, device)
+    step = batch._of(shape[0])
+    if positions is None:
+        positions = torch.empty_like(parents)
+    if seen is None:
+        seen = torch.empty_like(parents, dtype=torch.int64)
+    to = _plain(positions, "positions", torch.int32, shape, device), _plain(seen, "seen", torch.int64, shape, device)
+    s = _raw_stream(device) if stream is None else stream
+    _call(device, load().q4rdna_kv_tree, step, at, *to, s)
+    return positions, seen
+
+
+def rotate(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor | None, cos: torch.Tensor | None = None,
+           sin: torch.Tensor | None = None, *, interleaved: bool = False, q_norm: torch.Tensor | None = None,
+           k_norm: torch.Tensor | None = None, eps: float = 1e-6, q_out: torch.Tensor | None = None,
+           k_out: torch.Tensor | None = None, stream: int | None = None):
+    """(q, k) normalised and rotated as :meth:`KVCache.append` does it, bit for
+    bit, by positions (int32 [tokens]) of each token: q [tokens, q_heads,
+    head_dim] and k [tokens, kv_heads, head_dim], either of which may be None;
+    q_norm, k_norm [head_dim] and cos, sin [positions, rotary / 2] float32.  A
+    position outside cos and sin makes the token's rows NaN.  Without cos and
+    sin nothing is rotated.  q_out may be q and k_out k."""
+    first = k if q is None else q
+    if first is None or first.dim() != 3 or not first.is_cuda:
+        raise ValueError("q or k must be a CUDA tensor [tokens, heads, head_dim]")
+    device, dtype = first.get_device(), first.dtype
+    tokens, _, dim = first.shape
+    if stream is not None and (q is not None and q_out is None or k is not None and k_out is None):
+        with _on_stream(stream, device):
+            return rotate(q, k, positions, cos, sin, interleaved=interleaved, q_norm=q_norm, k_norm=k_norm, eps=eps,
+                          q_out=q_out, k_out=k_out)
+    rows, to, heads = [_NO_ROWS, _NO_ROWS], [_NO_ROWS, _NO_ROWS], [0, 0]
+    outs = [q_out, k_out]
+    for i, (x, name, norm) in enumerate(((q, "q", q_norm), (k, "k", k_norm))):
+        if x is None:
+            if outs[i] is not None or norm is not None:
+                raise ValueError(f"{name}_out or {name}_norm without {name}")
+            continue
+        if x.dim() != 3:
+            raise ValueError(f"{name} must be [tokens, heads, head_dim]")
+        heads[i] = x.shape[1]
+        rows[i] = _rows(x, name, dtype, (tokens, heads[i], dim), device)
+        outs[i], to[i] = _out_rows(outs[i], name + "_out", x, device)
+    at = cos_at = sin_at = table_rows = rotary = 0
+    if cos is not None:
+        table = cos.shape
+        if len(table) != 2 or sin is None or positions is None:
+            raise ValueError("cos and sin must be [positions, rotary / 2], with positions [tokens]")
+        at = _plain(positions, "positions", torch.int32, (tokens,), device)
+        cos_at = _plain(cos, "cos", torch.float32, table, device)
+        sin_at = _plain(sin, "sin", torch.float32, table, device)
+        table_rows, rotary = table[0], 2 * table[1]
+    elif sin is not None:
+        raise ValueError("sin without cos")
+    q_weight = 0 if q_norm is None else _plain(q_norm, "q_norm", torch.float32, (dim,), device)
+    k_weight = 0 if k_norm is None else _plain(k_norm, "k_norm", torch.float32, (dim,), device)
+    d = _lib.ROTATE.pack(_dtype(dtype), tokens, *heads, dim, table_rows, rotary, interleaved, *rows[0], *rows[1], *to[0], *to[1],
+                         at, cos_at, sin_at, q_weight, k_weight, eps, 0)
+    s = _raw_stream(device) if stream is None else stream
+    _call(device, load().q4rdna_rotate, d, s)
+    return tuple(outs)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor | None, count: int, out: tuple | None = None,
+                stream: int | None = None):
+    """(scores, rows, tokens), each [groups, count]: the best continuations of
+    each group's beams, largest first (q4rdna_beam_select).  logits [groups,
+    beams, vocab] (any strides of the rows), scores float32 [groups, beams] or
+    None for zeros; a continuation's total is its beam's score plus the
+    log-softmax of its beam's logits.  rows (int32) is group * beams + beam, what
+    :meth:`KVBatch.fork` takes for a batch of all groups' beams; tokens is
+    int32; out: these three, to be written.  Equal totals go by row, then by
+    token.  A beam whose score is not finite (such as -inf) or whose logits have
+    a NaN or +inf has no continuation: its totals are -inf, behind all others."""
+    if logits.dim() != 3 or not logits.is_cuda:
+        raise ValueError("logits must be a CUDA tensor [groups, beams, vocab]")
+    if logits.requires_grad:
+        _no_gradient("logits")
+    device, (groups, beams, vocab) = logits.get_device(), logits.shape
+    if stream is not None and out is None:
+        with _on_stream(stream, device):
+            return beam_select(logits, scores, count)
+    group_stride, beam_stride, stride = logits.stride()
+    if stride != 1 and vocab > 1:
+        raise ValueError("the logits of a row must be contiguous")
+    scores_at = 0 if scores is None else _plain(scores, "scores", torch.float32, (groups, beams), device)
+    if not 1 <= count <= min(_lib.BEAM_MAX_COUNT, beams * vocab):
+        raise ValueError(f"count is {count}: 1 to {_lib.BEAM_MAX_COUNT}, and no more than there are continuations")
+    shape = (groups, count)
+    if out is None:
+        ints = torch.empty((2, groups, count), dtype=torch.int32, device=logits.device)
+        out = torch.empty(shape, dtype=torch.float32, device=logits.device), ints[0], ints[1]
+    at = [_plain(t, name, dtype, shape, device) for t, name, dtype in zip(
+        out, ("out scores", "out rows", "out tokens"), (torch.float32, torch.int32, torch.int32), strict=True)]
+    d = _lib.BEAM.pack(_dtype(logits.dtype), groups, beams, vocab, count, 0, logits.data_ptr(), group_stride, beam_stride,
+                       scores_at, *at)
+    s = _raw_stream(device) if stream is None else stream
+    _call(device, load().q4rdna_beam_select, d, s)
+    return tuple(out)
