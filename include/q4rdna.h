@@ -554,13 +554,14 @@ int q4rdna_kv_attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *b
  *   total[b][v] = scores[b] + logits[b][v] - log sum_u exp(logits[b][u])
  * and the `count` largest of them, largest first: out_scores, out_rows (group *
  * beams + b) and out_tokens, each [groups][count].  Totals are compared in 64
- * bits, those of one row by their logits; equal ones go by row, then by token.
+ * bits; equal ones go by row, then by logit (totals that 64 bits cannot tell
+ * apart), then by token.
  * scores NULL: zeros.  A beam has no continuation, all its totals are -inf, if
  * its score is not finite, if all its logits are -inf or if one of them is NaN
  * or +inf; such totals come behind all others.  Scratch as for
  * q4rdna_kv_attend.  Runs on the current device. */
 #define Q4RDNA_BEAM_MAX_COUNT 128
-#define Q4RDNA_BEAM_MAX_BEAMS 1024
+#define Q4RDNA_BEAM_MAX_BEAMS 256
 typedef struct q4rdna_beam_desc {
     uint32_t dtype;           /* of logits */
     uint32_t groups;

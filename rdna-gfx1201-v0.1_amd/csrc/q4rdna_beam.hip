@@ -183,6 +183,13 @@ __device__ __forceinline__ void store_agent64(uint64_t *p, uint64_t v) {
     __hip_atomic_store((gptr_au64)(uintptr_t)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// A continuation: by its total, then by its row (lower first), its logit and its
+// token (lower first).
+__device__ __forceinline__ Item total_item(double total, uint32_t beam, uint32_t logit, uint32_t token) {
+    static_assert(Q4RDNA_BEAM_MAX_BEAMS == 1 << 8, "beam, logit and token (under 2^24) fill 64 bits");
+    return Item{ordered(total), static_cast<uint64_t>(255u - beam) << 56 | static_cast<uint64_t>(logit) << 24 | (~token & 0xffffffu)};
+}
+
 __device__ __forceinline__ bool alive(const q4rdna_beam_desc &d, uint32_t row) {
     return d.scores == nullptr || __builtin_fabsf(d.scores[row]) < __builtin_inff();
 }
@@ -282,10 +289,12 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
     __syncthreads();
     if (ticket != lists - 1) return;
     if (tid == 0) store_agent(a.arrived + group, 0u);
-    __shared__ double offset[Q4RDNA_BEAM_MAX_BEAMS];  // of a beam: its score less its log-sum-exp, or NaN
+    // A beam's log-sum-exp, NaN where it has no continuation, and its score.
+    __shared__ double beam_lse[Q4RDNA_BEAM_MAX_BEAMS];
+    __shared__ float beam_score[Q4RDNA_BEAM_MAX_BEAMS];
     for (uint32_t b = wave; b < a.d.beams; b += 4) {
         const uint32_t r = group * a.d.beams + b;
-        double o = __builtin_nan("");
+        double lse = __builtin_nan("");
         if (alive(a.d, r)) {
             float m = -__builtin_inff();
             for (uint32_t c = lane; c < a.chunks; c += 64)
@@ -305,10 +314,13 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
                 }
 #pragma unroll
                 for (int s = 32; s != 0; s >>= 1) sum += __shfl_xor(sum, s);
-                o = (a.d.scores == nullptr ? 0.0 : static_cast<double>(a.d.scores[r])) - (static_cast<double>(m) + log(sum));
+                lse = static_cast<double>(m) + log(sum);
             }
         }
-        if (lane == 0) offset[b] = o;
+        if (lane == 0) {
+            beam_lse[b] = lse;
+            beam_score[b] = a.d.scores == nullptr ? 0.0f : a.d.scores[r];
+        }
     }
     __syncthreads();
     // The lists' first items, then their second ones, and so on: the threads'
@@ -316,12 +328,12 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
     // at -inf.
     const auto item = [&](uint32_t r, uint32_t list) {
         const uint32_t b = list / a.chunks;
-        const double o = offset[b];
-        if (o != o) return list == b * a.chunks && r < a.d.vocab ? Item{ordered(-__builtin_inf()), ~(static_cast<uint64_t>(b) << 32 | r)} : Item{0, 0};
+        const double lse = beam_lse[b];
+        if (lse != lse) return list == b * a.chunks && r < a.d.vocab ? total_item(-__builtin_inf(), b, ordered(-__builtin_inff()), r) : Item{0, 0};
         const uint64_t top = load_agent64(tops + static_cast<size_t>(r) * lists + list);
         if (top == 0) return Item{0, 0};
-        const uint32_t token = ~static_cast<uint32_t>(top);
-        return Item{ordered(o + static_cast<double>(unordered(static_cast<uint32_t>(top >> 32)))), ~(static_cast<uint64_t>(b) << 32 | token)};
+        const uint32_t logit = static_cast<uint32_t>(top >> 32);
+        return total_item(static_cast<double>(beam_score[b]) + (static_cast<double>(unordered(logit)) - lse), b, logit, ~static_cast<uint32_t>(top));
     };
     const auto each = [&](auto f) {
         for (uint32_t i = tid; i < lists * count; i += kBeamThreads) {
@@ -337,8 +349,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
     select_first(select, count, mine, each, [&](uint32_t r, const Item &i) {
         const size_t at = static_cast<size_t>(group) * count + r;
         a.d.out_scores[at] = static_cast<float>(unordered(i.rank));
-        a.d.out_rows[at] = static_cast<int32_t>(group * a.d.beams + static_cast<uint32_t>(~i.place >> 32));
-        a.d.out_tokens[at] = static_cast<int32_t>(static_cast<uint32_t>(~i.place));
+        a.d.out_rows[at] = static_cast<int32_t>(group * a.d.beams + static_cast<uint32_t>(~i.place >> 56));
+        a.d.out_tokens[at] = static_cast<int32_t>(static_cast<uint32_t>(~i.place) & 0xffffffu);
     });
 }
 

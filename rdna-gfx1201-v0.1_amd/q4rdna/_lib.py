@@ -41,7 +41,7 @@ KV_BLOCK = 64
 NORM_MAX_WIDTH = 16384
 TREE_MAX = 64
 BEAM_MAX_COUNT = 128
-BEAM_MAX_BEAMS = 1024
+BEAM_MAX_BEAMS = 256
 FORK_MAX_SEQUENCES = 4096
 
 # Every symbol include/q4rdna.h declares.

@@ -988,7 +988,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor | None, count: int, o
     log-softmax of its beam's logits.  rows (int32) is group * beams + beam, what
     :meth:`KVBatch.fork` takes for a batch of all groups' beams; tokens is
     int32; out: these three, to be written.  Equal totals go by row, then by
-    token.  A beam whose score is not finite (such as -inf) or whose logits have
+    logit, then by token.  A beam whose score is not finite (such as -inf) or whose logits have
     a NaN or +inf has no continuation: its totals are -inf, behind all others."""
     if logits.dim() != 3 or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor [groups, beams, vocab]")
