@@ -11,9 +11,8 @@
 // Selection: threads' maxima, several threads' together, 64 or 128 in all; the
 // count-th largest of them is a bound that `count` items at least reach, and
 // few more.  These go to LDS and each counts how many are before it.  Equal
-// items are told apart by their place, so a bound always cuts; where more items
-// reach it than LDS takes, as in rows that are sorted, the bound is raised by
-// halving.
+// logits are told apart by their token, so a bound always cuts; where more items
+// reach it than LDS takes, the bound is raised by halving.
 #include "q4rdna_layer_device.h"
 
 namespace q4rdna {
@@ -21,6 +20,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kBeamThreads = 256;
+constexpr uint32_t kBeamWaves = kBeamPartials;
 constexpr uint32_t kHeld = 1024;  // items that LDS takes
 
 // Bits that order as the numbers do; both zeros are one.
@@ -28,151 +28,224 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t u = __float_as_uint(v + 0.0f);
     return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float unordered(uint32_t u) {
+__device__ __forceinline__ float unordered32(uint32_t u) {
     return __uint_as_float(u ^ (static_cast<uint32_t>(static_cast<int32_t>(~u) >> 31) | 0x80000000u));
 }
 __device__ __forceinline__ uint64_t ordered(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
     return u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | 0x8000000000000000ull);
 }
-__device__ __forceinline__ double unordered(uint64_t u) {
+__device__ __forceinline__ double unordered64(uint64_t u) {
     return __builtin_bit_cast(double, u ^ (static_cast<uint64_t>(static_cast<int64_t>(~u) >> 63) | 0x8000000000000000ull));
 }
 
-// What is selected: by `rank`, equal ones by `place`, larger first.  {0, 0}: no
-// item, behind all.
-struct Item {
-    uint64_t rank, place;
+// What is selected, larger first; zero: no item, behind all.
+//  Pick    an item of a chunk: ordered logit << 32 | ~token, no two alike.
+//  Total   a continuation: by its total, then by row, logit and token.
+struct Pick {
+    uint64_t key;
+    static constexpr int kParts = 1;
+    __device__ __forceinline__ uint64_t &part(int) { return key; }
+    __device__ __forceinline__ bool before(const Pick &o) const { return key > o.key; }
 };
-__device__ __forceinline__ bool before(const Item &a, const Item &b) {
-    return a.rank > b.rank || (a.rank == b.rank && a.place > b.place);
-}
+struct Total {
+    uint64_t key, place;
+    static constexpr int kParts = 2;
+    __device__ __forceinline__ uint64_t &part(int i) { return i == 0 ? key : place; }
+    __device__ __forceinline__ bool before(const Total &o) const { return key > o.key || (key == o.key && place > o.place); }
+};
 __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
     return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
 template <int CTRL>
-__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
-    return static_cast<uint64_t>(dpp<CTRL>(static_cast<uint32_t>(v >> 32))) << 32 | dpp<CTRL>(static_cast<uint32_t>(v));
-}
-template <int CTRL>
-__device__ __forceinline__ Item best_dpp(const Item &a) {
-    const Item b = {dpp64<CTRL>(a.rank), dpp64<CTRL>(a.place)};
-    return before(b, a) ? b : a;
+__device__ __forceinline__ uint64_t max_dpp(uint64_t v) {
+    const uint64_t o = static_cast<uint64_t>(dpp<CTRL>(static_cast<uint32_t>(v >> 32))) << 32 | dpp<CTRL>(static_cast<uint32_t>(v));
+    return o > v ? o : v;
 }
 
+template <typename Item>
 struct Select {
     Item held[kHeld];
-    Item group[128];
+    uint64_t group[128];
+    uint32_t ranks[4][128];
     uint32_t count;
 };
 
-// The `count` first items, count <= 128, in order: take(r, item) is called once
-// for each place r < count by some thread, with {0, 0} where there are fewer
-// items.  `mine` is the first of the thread's items, each(f) calls f with all of
-// them.  Every thread of the workgroup calls it.
-template <typename Each, typename Take>
-__device__ __forceinline__ void select_first(Select &s, uint32_t count, const Item &mine, Each each, Take take) {
-    const int tid = threadIdx.x, lane = tid & 63;
-    const bool pairs = count > 64;  // 128 groups of two threads, else 64 of four
-    Item g = best_dpp<kDppXor1>(mine);
-    if (!pairs) g = best_dpp<kDppXor2>(g);
+// A key that `count` of the workgroup's threads' largest keys, `mine`, taken
+// together by two (count > 64) or four threads, at least reach: the count-th of
+// them; 1 where fewer are not zero.
+template <typename Item>
+__device__ __forceinline__ uint64_t count_th(Select<Item> &s, uint32_t count, uint64_t mine) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const bool pairs = count > 64;
+    uint64_t g = max_dpp<kDppXor1>(mine);
+    if (!pairs) g = max_dpp<kDppXor2>(g);
     if (tid % (pairs ? 2 : 4) == 0) s.group[tid / (pairs ? 2 : 4)] = g;
-    if (tid == 0) s.count = 0;
     __syncthreads();
-    // Each wave finds the count-th group by itself: a lane has one or two and
-    // counts those before it.
-    Item bound;
-    {
-        const Item a = s.group[lane];
-        uint32_t a_rank = 0;
-        if (!pairs) {
-            for (int i = 0; i < 64; ++i) {
-                const Item o = {lane_value(a.rank, i), lane_value(a.place, i)};
-                a_rank += before(o, a) || (i < lane && o.rank == a.rank && o.place == a.place);
-            }
-            const uint64_t at = __builtin_amdgcn_ballot_w64(a_rank == count - 1);
-            const int owner = __builtin_ctzll(at | 1ull << 63);
-            bound = {lane_value(a.rank, owner), lane_value(a.place, owner)};
-        } else {
-            const Item b = s.group[lane + 64];
-            uint32_t b_rank = 0;
-            for (int i = 0; i < 64; ++i) {
-                const Item o = {lane_value(a.rank, i), lane_value(a.place, i)}, p = {lane_value(b.rank, i), lane_value(b.place, i)};
-                a_rank += before(o, a) || (i < lane && o.rank == a.rank && o.place == a.place);
-                a_rank += before(p, a);
-                b_rank += before(o, b) || (o.rank == b.rank && o.place == b.place);
-                b_rank += before(p, b) || (i < lane && p.rank == b.rank && p.place == b.place);
-            }
-            const uint64_t at = __builtin_amdgcn_ballot_w64(a_rank == count - 1), bt = __builtin_amdgcn_ballot_w64(b_rank == count - 1);
-            const int owner = __builtin_ctzll((at != 0 ? at : bt) | 1ull << 63);
-            bound = at != 0 ? Item{lane_value(a.rank, owner), lane_value(a.place, owner)}
-                            : Item{lane_value(b.rank, owner), lane_value(b.place, owner)};
-        }
+    // A lane has one or two keys and counts those that are before it, and above
+    // these, 2^16 each, those that are not behind it, a quarter in each wave.
+    const uint64_t a = s.group[lane], b = pairs ? s.group[lane + 64] : 0;
+    uint32_t a_rank = 0, b_rank = 0;
+    constexpr uint32_t kLeast = 1u << 16;
+#pragma unroll 4
+    for (int i = 16 * wave; i < 16 * wave + 16; ++i) {
+        const uint64_t o = lane_value(a, i);
+        a_rank += o > a ? 1 + kLeast : o == a ? kLeast : 0;
     }
-    if (bound.rank == 0) bound = {1, 0};  // fewer groups with items than `count`: all items
-    // How many reach a bound.
-    const auto reach = [&](const Item &at) {
-        uint32_t n = 0;
-        each([&](const Item &x) { n += !before(at, x); });
-        if (n != 0) atomicAdd(&s.count, n);
-        __syncthreads();
-        const uint32_t all = s.count;
-        __syncthreads();
-        if (tid == 0) s.count = 0;
-        __syncthreads();
-        return all;
+    if (pairs) {
+#pragma unroll 1
+        for (int i = 16 * wave; i < 16 * wave + 16; ++i) {
+            const uint64_t o = lane_value(a, i), p = lane_value(b, i);
+            a_rank += p > a ? 1 + kLeast : p == a ? kLeast : 0;
+            b_rank += (o > b ? 1 + kLeast : o == b ? kLeast : 0) + (p > b ? 1 + kLeast : p == b ? kLeast : 0);
+        }
+        s.ranks[wave][lane + 64] = b_rank;
+    }
+    s.ranks[wave][lane] = a_rank;
+    __syncthreads();
+    const auto found = [&](uint64_t key, int at) {
+        const uint32_t rank = s.ranks[0][at] + s.ranks[1][at] + s.ranks[2][at] + s.ranks[3][at];
+        const uint64_t here = __builtin_amdgcn_ballot_w64((rank & 0xffffu) < count && rank >> 16 >= count);
+        return here != 0 ? lane_value(key, __builtin_ctzll(here)) : 0;
     };
-    uint32_t n = reach(bound);
-    if (n > kHeld) {
-        // The largest rank that `count` items at least reach, then the same of the places: the
-        // bound is then the count-th item itself.
-        Item low = {bound.rank, 0}, high = {~0ull, 0};  // low is reached by enough, high is not
-        while (high.rank - low.rank > 1) {
-            const Item mid = {low.rank + (high.rank - low.rank) / 2, 0};
-            (reach(mid) >= count ? low : high) = mid;
-        }
-        high = {low.rank, ~0ull};
-        while (high.place - low.place > 1) {
-            const Item mid = {low.rank, low.place + (high.place - low.place) / 2};
-            (reach(mid) >= count ? low : high) = mid;
-        }
-        bound = low;
-    }
-    each([&](const Item &x) {
-        if (!before(bound, x)) s.held[atomicAdd(&s.count, 1u)] = x;
-    });
+    uint64_t key = found(a, lane);
+    if (pairs && key == 0) key = found(b, lane + 64);
+    return key != 0 ? key : 1;
+}
+
+// How many of the items that each(f) calls f with reach a bound: in `counter`,
+// which is zero before and after.
+template <typename Item, typename Each>
+__device__ __forceinline__ uint32_t reach(uint32_t *counter, const Item &bound, Each each) {
+    uint32_t n = 0;
+    each([&](const Item &x) { n += !bound.before(x); });
+    if (n != 0) atomicAdd(counter, n);
     __syncthreads();
-    n = s.count;
-    for (uint32_t i = tid; i < max(n, count); i += kBeamThreads) {
+    const uint32_t all = *counter;
+    __syncthreads();
+    if (threadIdx.x == 0) *counter = 0;
+    __syncthreads();
+    return all;
+}
+// Where more items reach a bound than LDS takes: the count-th item itself, by
+// halving its key and then its place.
+template <typename Item, typename Each>
+__device__ __forceinline__ Item count_th_item(uint32_t *counter, uint32_t count, Item bound, Each each) {
+    for (int part = 0; part < Item::kParts; ++part) {
+        uint64_t &low = bound.part(part);  // reached by enough
+        uint64_t high = ~0ull;             // not reached by enough
+        while (high - low > 1) {
+            Item mid = bound;
+            mid.part(part) = low + (high - low) / 2;
+            (reach(counter, mid, each) >= count ? low : high) = mid.part(part);
+        }
+    }
+    return bound;
+}
+
+// The `count` first of the `n` items in LDS, count <= 128, in order: take(r, item)
+// is called once for each place r < count by some thread, with zero where there
+// are fewer.
+template <typename Item, typename Take>
+__device__ __forceinline__ void take_first(const Select<Item> &s, uint32_t n, uint32_t count, Take take) {
+    for (uint32_t i = threadIdx.x; i < max(n, count); i += kBeamThreads) {
         if (i >= n) {
-            take(i, Item{0, 0});
+            take(i, Item{});
             continue;
         }
         const Item x = s.held[i];
         uint32_t r = 0;
-        for (uint32_t j = 0; j < n; ++j) r += before(s.held[j], x);
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; ++j) r += s.held[j].before(x);
         if (r < count) take(r, x);
     }
+}
+template <typename Item>
+__device__ __forceinline__ void hold(Select<Item> &s, const Item &bound, const Item &x) {
+    if (bound.before(x)) return;
+    const uint32_t at = atomicAdd(&s.count, 1u);
+    if (at < kHeld) s.held[at] = x;
+}
+// Sets the count of what is held to zero, between barriers.
+template <typename Item>
+__device__ __forceinline__ void let_go(Select<Item> &s) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
 }
-
-// What a chunk leaves: its items' logits (ordered) and tokens in `top`, and
-// max and sum; max NaN: the row has a NaN or +inf.
-struct ChunkStat {
-    double sum;  // of exp(logit - max)
-    float max;
-    uint32_t unused;
-};
-
-// N numbers of a row, of any alignment.
-template <typename T, int N>
-__device__ __forceinline__ void load_any(const T *p, float (&x)[N]) {
-    typedef T TV __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-    typedef __attribute__((address_space(1))) const TV *gptr;
-    const TV v = *(gptr)(uintptr_t)p;
+// The count afterwards, the same for all threads.
+template <typename Item>
+__device__ __forceinline__ uint32_t held_count(const Select<Item> &s) {
+    __syncthreads();
+    const uint32_t n = s.count;
+    __syncthreads();
+    return n;
+}
+// A thread's share of the first `n` items that are held.
+constexpr int kShare = static_cast<int>(kHeld) / kBeamThreads;
+__device__ __forceinline__ void share_of(const Select<Pick> &s, uint32_t n, Pick (&share)[kShare]) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = static_cast<float>(v[e]);
+    for (int i = 0; i < kShare; ++i) {
+        const uint32_t at = threadIdx.x + i * kBeamThreads;
+        share[i] = at < n ? s.held[at] : Pick{0};
+    }
+}
+// Of n <= kHeld items that are held, those that reach a higher bound, `count` at
+// least: how many.
+__device__ __forceinline__ uint32_t tighten(Select<Pick> &s, uint32_t count, uint32_t n, Pick &bound) {
+    Pick share[kShare];
+    share_of(s, n, share);
+    uint64_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) mine = max(mine, share[i].key);
+    let_go(s);
+    bound.key = max(bound.key, count_th(s, count, mine));
+#pragma unroll
+    for (int i = 0; i < kShare; ++i)
+        if (share[i].key != 0) hold(s, bound, share[i]);
+    return held_count(s);
+}
+
+// The sum over a wave, in every lane.
+template <int CTRL>
+__device__ __forceinline__ double add_dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return v + __builtin_bit_cast(double, static_cast<uint64_t>(dpp<CTRL>(static_cast<uint32_t>(u >> 32))) << 32 | dpp<CTRL>(static_cast<uint32_t>(u)));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = add_dpp<kDppMirror16>(add_dpp<kDppMirror8>(add_dpp<kDppXor2>(add_dpp<kDppXor1>(v))));
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    double row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[i] = __builtin_bit_cast(double, lane_value(u, 16 * i));
+    return (row[0] + row[1]) + (row[2] + row[3]);
+}
+// log x for x > 0 to 2^-39: of x = f 2^e, f in [1/2^.5, 2^.5), by the series of
+// 2 atanh((f - 1) / (f + 1)).
+__device__ __forceinline__ double log_of(double x) {
+    double f = __builtin_amdgcn_frexp_mant(x);
+    int e = __builtin_amdgcn_frexp_exp(x);
+    if (f < 0.70710678118654752) {
+        f += f;
+        --e;
+    }
+    const double s = (f - 1.0) / (f + 1.0), z = s * s;
+    double p = 1.0 / 13.0;
+    p = fma(p, z, 1.0 / 11.0);
+    p = fma(p, z, 1.0 / 9.0);
+    p = fma(p, z, 1.0 / 7.0);
+    p = fma(p, z, 1.0 / 5.0);
+    p = fma(p, z, 1.0 / 3.0);
+    p = fma(p, z, 1.0);
+    return fma(static_cast<double>(e), 0.69314718055994531, 2.0 * s * p);
+}
+__device__ __forceinline__ float wave_max(float m) {
+    m = fmaxf(m, dpp<kDppXor1>(m));
+    m = fmaxf(m, dpp<kDppXor2>(m));
+    m = fmaxf(m, dpp<kDppMirror8>(m));
+    m = fmaxf(m, dpp<kDppMirror16>(m));
+    return max_xor32(max_xor16(m));
 }
 
 __device__ __forceinline__ uint64_t load_agent64(const uint64_t *p) {
@@ -185,101 +258,160 @@ __device__ __forceinline__ void store_agent64(uint64_t *p, uint64_t v) {
 
 // A continuation: by its total, then by its row (lower first), its logit and its
 // token (lower first).
-__device__ __forceinline__ Item total_item(double total, uint32_t beam, uint32_t logit, uint32_t token) {
+__device__ __forceinline__ Total total_item(double total, uint32_t beam, uint32_t logit, uint32_t token) {
     static_assert(Q4RDNA_BEAM_MAX_BEAMS == 1 << 8, "beam, logit and token (under 2^24) fill 64 bits");
-    return Item{ordered(total), static_cast<uint64_t>(255u - beam) << 56 | static_cast<uint64_t>(logit) << 24 | (~token & 0xffffffu)};
+    return Total{ordered(total), static_cast<uint64_t>(255u - beam) << 56 | static_cast<uint64_t>(logit) << 24 | (~token & 0xffffffu)};
 }
 
-__device__ __forceinline__ bool alive(const q4rdna_beam_desc &d, uint32_t row) {
-    return d.scores == nullptr || __builtin_fabsf(d.scores[row]) < __builtin_inff();
+// A trip's numbers: a thread has E, in vectors of 16 bytes, at any alignment.
+constexpr int E = kBeamTrip / kBeamThreads;
+constexpr uint32_t kTrip = kBeamTrip;
+template <typename T>
+constexpr int V = 16 / static_cast<int>(sizeof(T));
+template <typename T>
+__device__ __forceinline__ uint32_t token_of(uint32_t base, int e) {
+    return base + (e / V<T> * kBeamThreads + threadIdx.x) * V<T> + e % V<T>;
+}
+// A number of a row; under 2^24 of them, so 32 bits hold the offset.
+template <typename V>
+__device__ __forceinline__ V row_at(const void *row, uint32_t offset) {
+    typedef __attribute__((address_space(1))) const char *gptr_char;
+    typedef __attribute__((address_space(1))) const V *gptr;
+    return *(gptr)((gptr_char)(uintptr_t)row + offset);
+}
+// As they lie in memory; -inf behind the row's end.  (They become floats where
+// they are used: a conversion here would wait for them.)
+template <typename T>
+struct Trip {
+    typedef T TV __attribute__((ext_vector_type(V<T>), aligned(sizeof(T))));
+    TV v[E / V<T>];
+};
+template <typename T>
+__device__ __forceinline__ void load_trip(const T *p, uint32_t base, uint32_t vocab, Trip<T> &x) {
+    constexpr uint32_t kSize = sizeof(T);
+    if (base + kTrip <= vocab) {
+#pragma unroll
+        for (int j = 0; j < E / V<T>; ++j) x.v[j] = row_at<typename Trip<T>::TV>(p, kSize * token_of<T>(base, j * V<T>));
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t at = token_of<T>(base, e);
+            const T v = row_at<T>(p, kSize * min(at, vocab - 1));
+            x.v[e / V<T>][e % V<T>] = at < vocab ? v : static_cast<T>(-__builtin_inff());
+        }
+    }
 }
 
-template <int E, typename T>
+// Rows in which more logits of a trip reach the bound than LDS takes, as those
+// that rise from token to token: the bound becomes the count-th of the trip's and
+// of the `before` that were held.
+template <typename T>
+__device__ __noinline__ void overflown(Select<Pick> &s, const T *p, uint32_t base, uint32_t vocab, uint32_t before, uint32_t count,
+                                       Pick *bound) {
+    const uint32_t end = min(vocab - base, kTrip);
+    const auto trip = [&](auto f) {
+        for (uint32_t i = threadIdx.x; i < end; i += kBeamThreads) {
+            const float x = static_cast<float>(row_at<T>(p, sizeof(T) * (base + i)));
+            if (x == x) f(Pick{static_cast<uint64_t>(ordered(x)) << 32 | static_cast<uint32_t>(~(base + i))});
+        }
+    };
+    let_go(s);
+    *bound = count_th_item(&s.count, count, *bound, [&](auto f) {
+        trip(f);
+        for (uint32_t i = threadIdx.x; i < before; i += kBeamThreads) f(s.held[i]);
+    });
+    Pick share[kShare];
+    share_of(s, before, share);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kShare; ++i)
+        if (share[i].key != 0) hold(s, *bound, share[i]);
+    trip([&](const Pick &x) { hold(s, *bound, x); });
+}
+
+template <typename T>
 __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
-    constexpr int V = E * sizeof(T) < 16 ? E : 16 / static_cast<int>(sizeof(T));
-    __shared__ Select select;
-    __shared__ float wave_max[4];
-    __shared__ double wave_sum[4];
+    __shared__ union {
+        Select<Pick> chunk;
+        Select<Total> group;
+    } select;
     __shared__ uint32_t ticket;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
     const uint32_t group = row / a.d.beams, beam = row - group * a.d.beams, count = a.d.count;
     const uint32_t lists = a.d.beams * a.chunks;  // of a group
     uint64_t *tops = a.tops + static_cast<size_t>(group) * lists * count;
-    uint64_t *stats = a.stats + static_cast<size_t>(group) * lists * 2;
+    uint64_t *stats = a.stats + static_cast<size_t>(group) * lists * kBeamWaves * 2;
 
-    if (alive(a.d, row)) {
-        const T *p = static_cast<const T *>(a.d.logits) + group * a.d.group_stride + beam * a.d.beam_stride;
-        const uint32_t first = chunk * (kBeamThreads * E);
+    const T *p = static_cast<const T *>(a.d.logits) + group * a.d.group_stride + beam * a.d.beam_stride;
+    const uint32_t first = chunk * a.trips * kTrip, trips = min(a.trips, (a.d.vocab - first + kTrip - 1) / kTrip);
+    uint64_t *top = tops + static_cast<size_t>(beam) * a.chunks + chunk;
+    float m = -__builtin_inff();  // of the thread
+    double sum = 0.0;             // of its exponentials, relative to m
+    Trip<T> next;
+    Select<Pick> &s = select.chunk;
+    if (tid == 0) s.count = 0;
+    Pick bound = {0};
+    uint32_t n = 0;
+    for (uint32_t trip = 0; trip <= trips; ++trip) {  // a trip is loaded in the one before
         float x[E];
-        uint32_t valid = 0;  // bits of the thread's vectors' elements that are there
 #pragma unroll
-        for (int j = 0; j < E / V; ++j) {
-            const uint32_t at = first + (j * kBeamThreads + tid) * V;
-            float v[V];
-            if (at + V <= a.d.vocab) {
-                load_any<T, V>(p + at, v);
-                valid |= ((1u << V) - 1u) << (V * j);
-            } else {
+        for (int e = 0; e < E; ++e) x[e] = static_cast<float>(next.v[e / V<T>][e % V<T>]);
+        if (trip < trips) load_trip<T>(p, first + trip * kTrip, a.d.vocab, next);
+        if (trip == 0) continue;
+        const uint32_t base = first + (trip - 1) * kTrip;
+        // (The maximum leaves NaN out; the sum takes it in.)
+        float tops_of[E / 8], most = -__builtin_inff();
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    v[e] = 0.0f;
-                    if (at + e < a.d.vocab) {
-                        v[e] = static_cast<float>(p[at + e]);
-                        valid |= 1u << (V * j + e);
-                    }
-                }
-            }
+        for (int g = 0; g < E / 8; ++g) {
+            tops_of[g] = x[8 * g];
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[V * j + e] = v[e];
+            for (int e = 1; e < 8; ++e) tops_of[g] = fmaxf(tops_of[g], x[8 * g + e]);
+            most = fmaxf(most, tops_of[g]);
         }
-        // The maximum, with NaN and +inf as +inf.
-        float most = -__builtin_inff();
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (!(x[e] < __builtin_inff())) x[e] = __builtin_inff();
-            if (valid >> e & 1) most = fmaxf(most, x[e]);
-        }
-        // The thread's first item: of equal logits the lowest token.
-        Item mine = {0, 0};
-#pragma unroll
-        for (int e = E - 1; e >= 0; --e)
-            if ((valid >> e & 1) && x[e] == most)
-                mine = {static_cast<uint64_t>(ordered(x[e])), static_cast<uint64_t>(~(first + (e / V * kBeamThreads + tid) * V + e % V))};
-        float m = most;
-        m = fmaxf(m, dpp<kDppXor1>(m));
-        m = fmaxf(m, dpp<kDppXor2>(m));
-        m = fmaxf(m, dpp<kDppMirror8>(m));
-        m = fmaxf(m, dpp<kDppMirror16>(m));
-        m = max_xor32(max_xor16(m));
-        if (lane == 0) wave_max[wave] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
-        // Up to 32 exponentials in 32 bits, all sums of them in 64.
-        const float ref = m == -__builtin_inff() ? 0.0f : m;
+        const float now = fmaxf(m, most), ref = now == -__builtin_inff() ? 0.0f : now;
         float part = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (valid >> e & 1) part += __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e);
-        double sum = part;
+        for (int e = 0; e < E; ++e) part += __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e);
+        sum = sum * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + part;
+        m = now;
+        if (trip == 1) {
+            int best_at = 0;  // of equal logits the lowest token
 #pragma unroll
-        for (int s = 32; s != 0; s >>= 1) sum += __shfl_xor(sum, s);
-        if (lane == 0) wave_sum[wave] = sum;
-        uint64_t *top = tops + static_cast<size_t>(beam) * a.chunks + chunk;
-        select_first(select, count, mine,
-                     [&](auto f) {
-#pragma unroll
-                         for (int e = 0; e < E; ++e)
-                             if (valid >> e & 1)
-                                 f(Item{static_cast<uint64_t>(ordered(x[e])),
-                                        static_cast<uint64_t>(~(first + (e / V * kBeamThreads + tid) * V + e % V))});
-                     },
-                     [&](uint32_t r, const Item &i) { store_agent64(top + static_cast<size_t>(r) * lists, i.rank << 32 | static_cast<uint32_t>(i.place)); });
-        if (tid == 0) {
-            uint64_t *stat = stats + (static_cast<size_t>(beam) * a.chunks + chunk) * 2;
-            store_agent64(stat, __builtin_bit_cast(uint64_t, (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3])));
-            store_agent64(stat + 1, __float_as_uint(m));
+            for (int e = E - 1; e >= 0; --e) best_at = x[e] == most ? e : best_at;
+            bound.key = count_th(s, count, static_cast<uint64_t>(ordered(most)) << 32 | static_cast<uint32_t>(~token_of<T>(base, best_at)));
         }
+        const float least = unordered32(max(static_cast<uint32_t>(bound.key >> 32), ordered(-__builtin_inff())));
+#pragma unroll
+        for (int g = 0; g < E / 8; ++g)
+            if (__builtin_amdgcn_ballot_w64(!(tops_of[g] < least)) != 0) {
+#pragma unroll
+                for (int e = 8 * g; e < 8 * g + 8; ++e)
+                    if (x[e] >= least) hold(s, bound, Pick{static_cast<uint64_t>(ordered(x[e])) << 32 | static_cast<uint32_t>(~token_of<T>(base, e))});
+            }
+        const uint32_t before = n;
+        n = held_count(s);
+        if (n > kHeld) {
+            overflown<T>(s, p, base, a.d.vocab, before, count, &bound);
+            n = held_count(s);
+        } else if (n > (trip < trips ? kHeld / 2 : 2 * count + 64)) {
+            n = tighten(s, count, n, bound);
+        }
+    }
+    take_first(s, n, count, [&](uint32_t r, const Pick &i) {
+        const bool there = ~static_cast<uint32_t>(i.key) < a.d.vocab;
+        store_agent64(top + static_cast<size_t>(r) * lists, there ? i.key : 0);
+    });
+    // Each wave's sum by itself.  A NaN, and +inf less itself, have come through it:
+    // a maximum of +inf tells them.
+    float wave_most = wave_max(m);
+    const float wave_ref = wave_most == -__builtin_inff() ? 0.0f : wave_most;
+    const double all = wave_sum(sum * __builtin_amdgcn_exp2f((m - wave_ref) * kLog2e));
+    if (all != all) wave_most = __builtin_inff();
+    if (lane == 0) {
+        uint64_t *stat = stats + ((static_cast<size_t>(beam) * a.chunks + chunk) * kBeamWaves + wave) * 2;
+        store_agent64(stat, __builtin_bit_cast(uint64_t, all));
+        store_agent64(stat + 1, __float_as_uint(wave_most));
     }
 
     // The group's last workgroup goes on.
@@ -292,82 +424,115 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
     // A beam's log-sum-exp, NaN where it has no continuation, and its score.
     __shared__ double beam_lse[Q4RDNA_BEAM_MAX_BEAMS];
     __shared__ float beam_score[Q4RDNA_BEAM_MAX_BEAMS];
+    // A list to each thread, its first items to the first ones, and so on: the
+    // threads' maxima are near each other.  Where these are few a thread they
+    // stay in registers, and are under way while the sums are added up.
+    const uint32_t items = lists * count, width = 1u << (32 - __builtin_clz(max(lists, 2u) - 1));  // of a row of threads
+    constexpr int kKept = 4;
+    const bool few = width <= kBeamThreads && count <= kKept * (kBeamThreads / width);
+    const uint32_t my_list = tid & (width - 1), my_first = tid / width, my_step = kBeamThreads / width;
+    uint64_t kept[kKept];
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+        const uint32_t r = my_first + i * my_step;
+        kept[i] = few && my_list < lists && r < count ? load_agent64(tops + static_cast<size_t>(r) * lists + my_list) : 0;
+    }
+    const uint32_t parts = a.chunks * kBeamWaves;
     for (uint32_t b = wave; b < a.d.beams; b += 4) {
         const uint32_t r = group * a.d.beams + b;
-        double lse = __builtin_nan("");
-        if (alive(a.d, r)) {
-            float m = -__builtin_inff();
-            for (uint32_t c = lane; c < a.chunks; c += 64)
-                m = fmaxf(m, __uint_as_float(static_cast<uint32_t>(load_agent64(stats + (static_cast<size_t>(b) * a.chunks + c) * 2 + 1))));
-            m = fmaxf(m, dpp<kDppXor1>(m));
-            m = fmaxf(m, dpp<kDppXor2>(m));
-            m = fmaxf(m, dpp<kDppMirror8>(m));
-            m = fmaxf(m, dpp<kDppMirror16>(m));
-            m = max_xor32(max_xor16(m));
-            double sum = 0.0;
-            if (__builtin_fabsf(m) < __builtin_inff()) {
-                for (uint32_t c = lane; c < a.chunks; c += 64) {
-                    const uint64_t *stat = stats + (static_cast<size_t>(b) * a.chunks + c) * 2;
-                    const float cm = __uint_as_float(static_cast<uint32_t>(load_agent64(stat + 1)));
-                    const double cs = __builtin_bit_cast(double, load_agent64(stat));
-                    if (cm > -__builtin_inff()) sum += cs * exp(static_cast<double>(cm) - static_cast<double>(m));
-                }
+        const float score = a.d.scores == nullptr ? 0.0f : a.d.scores[r];
+        double lse = __builtin_nan(""), sum_of = 0.0;
+        float most_of = -__builtin_inff();  // what the lane's parts are relative to
+        constexpr int kParts = 4;           // of a lane, under way together
+#pragma unroll 1
+        for (uint32_t c0 = lane; c0 < parts; c0 += 64 * kParts) {
+            float most[kParts], now = most_of;
+            double sum[kParts];
 #pragma unroll
-                for (int s = 32; s != 0; s >>= 1) sum += __shfl_xor(sum, s);
-                lse = static_cast<double>(m) + log(sum);
+            for (int i = 0; i < kParts; ++i) {
+                const uint32_t c = c0 + 64 * i;
+                const uint64_t *stat = stats + (static_cast<size_t>(b) * parts + min(c, parts - 1)) * 2;
+                sum[i] = __builtin_bit_cast(double, load_agent64(stat));
+                most[i] = c < parts ? __uint_as_float(static_cast<uint32_t>(load_agent64(stat + 1))) : -__builtin_inff();
             }
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) now = fmaxf(now, most[i]);
+            const float to = now == -__builtin_inff() ? 0.0f : now;
+            sum_of *= __builtin_amdgcn_exp2f((most_of - to) * kLog2e);
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) sum_of += sum[i] * __builtin_amdgcn_exp2f((most[i] - to) * kLog2e);
+            most_of = now;
         }
+        const float m = wave_max(most_of);
+        if (__builtin_fabsf(score) < __builtin_inff() && __builtin_fabsf(m) < __builtin_inff())
+            lse = static_cast<double>(m) + log_of(wave_sum(sum_of * __builtin_amdgcn_exp2f((most_of - m) * kLog2e)));
         if (lane == 0) {
             beam_lse[b] = lse;
-            beam_score[b] = a.d.scores == nullptr ? 0.0f : a.d.scores[r];
+            beam_score[b] = score;
         }
     }
     __syncthreads();
-    // The lists' first items, then their second ones, and so on: the threads'
-    // maxima are near each other.  A dead beam's items are its first tokens, all
+    // The r-th of a list, of a beam.  A dead beam's items are its first tokens, all
     // at -inf.
-    const auto item = [&](uint32_t r, uint32_t list) {
-        const uint32_t b = list / a.chunks;
+    const auto item = [&](uint32_t r, uint32_t list, uint32_t b, uint64_t top) {
         const double lse = beam_lse[b];
-        if (lse != lse) return list == b * a.chunks && r < a.d.vocab ? total_item(-__builtin_inf(), b, ordered(-__builtin_inff()), r) : Item{0, 0};
-        const uint64_t top = load_agent64(tops + static_cast<size_t>(r) * lists + list);
-        if (top == 0) return Item{0, 0};
+        if (lse != lse) return list == b * a.chunks && r < min(count, a.d.vocab) ? total_item(-__builtin_inf(), b, ordered(-__builtin_inff()), r) : Total{0, 0};
+        if (top == 0) return Total{0, 0};
         const uint32_t logit = static_cast<uint32_t>(top >> 32);
-        return total_item(static_cast<double>(beam_score[b]) + (static_cast<double>(unordered(logit)) - lse), b, logit, ~static_cast<uint32_t>(top));
+        return total_item(static_cast<double>(beam_score[b]) + (static_cast<double>(unordered32(logit)) - lse), b, logit, ~static_cast<uint32_t>(top));
     };
-    const auto each = [&](auto f) {
-        for (uint32_t i = tid; i < lists * count; i += kBeamThreads) {
-            const uint32_t r = i / lists;
-            const Item x = item(r, i - r * lists);
-            if (x.rank != 0) f(x);
+    const auto take = [&](uint32_t r, const Total &t) {
+        const size_t at = static_cast<size_t>(group) * count + r;
+        a.d.out_scores[at] = static_cast<float>(unordered64(t.key));
+        a.d.out_rows[at] = static_cast<int32_t>(group * a.d.beams + static_cast<uint32_t>(~t.place >> 56));
+        a.d.out_tokens[at] = static_cast<int32_t>(static_cast<uint32_t>(~t.place) & 0xffffffu);
+    };
+    const auto every = [&](auto f) {
+#pragma unroll 1
+        for (uint32_t i = tid; i < items; i += kBeamThreads) {
+            const uint32_t r = i / lists, list = i - r * lists;
+            const Total t = item(r, list, list / a.chunks, load_agent64(tops + i));
+            if (t.key != 0) f(t);
         }
     };
-    Item mine = {0, 0};
-    each([&](const Item &x) {
-        if (before(x, mine)) mine = x;
-    });
-    select_first(select, count, mine, each, [&](uint32_t r, const Item &i) {
-        const size_t at = static_cast<size_t>(group) * count + r;
-        a.d.out_scores[at] = static_cast<float>(unordered(i.rank));
-        a.d.out_rows[at] = static_cast<int32_t>(group * a.d.beams + static_cast<uint32_t>(~i.place >> 56));
-        a.d.out_tokens[at] = static_cast<int32_t>(static_cast<uint32_t>(~i.place) & 0xffffffu);
-    });
+    Select<Total> &g = select.group;
+    if (tid == 0) g.count = 0;
+    uint64_t best = 0;
+    Total least = {0, 0};
+    if (few) {
+        Total t[kKept];
+        const uint32_t my_beam = min(my_list, lists - 1) / a.chunks;
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) {
+            t[i] = Total{0, 0};
+            if (i * my_step >= count) continue;
+            if (my_list < lists) t[i] = item(my_first + i * my_step, my_list, my_beam, kept[i]);
+            best = max(best, t[i].key);
+        }
+        least.key = count_th(g, count, best);
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+            if (i * my_step < count) hold(g, least, t[i]);
+    } else {
+        every([&](const Total &t) { best = max(best, t.key); });
+        least.key = count_th(g, count, best);
+        every([&](const Total &t) { hold(g, least, t); });
+    }
+    uint32_t found = held_count(g);
+    if (found > kHeld) {
+        let_go(g);
+        least = count_th_item(&g.count, count, least, every);
+        every([&](const Total &t) { hold(g, least, t); });
+        found = held_count(g);
+    }
+    take_first(g, found, count, take);
 }
 
 }  // namespace
 
-template <int E>
-static void launch_beam_as(const BeamArgs &a, hipStream_t stream) {
-    const auto go = [&](auto kernel) { kernel<<<a.d.groups * a.d.beams * a.chunks, kBeamThreads, 0, stream>>>(a); };
-    a.d.dtype == Q4RDNA_F32 ? go(beam_kernel<E, float>) : a.d.dtype == Q4RDNA_F16 ? go(beam_kernel<E, _Float16>) : go(beam_kernel<E, __bf16>);
-}
 hipError_t launch_beam(const BeamArgs &a, hipStream_t stream) {
-    switch (a.each) {
-        case 4: launch_beam_as<4>(a, stream); break;
-        case 8: launch_beam_as<8>(a, stream); break;
-        case 16: launch_beam_as<16>(a, stream); break;
-        default: launch_beam_as<32>(a, stream); break;
-    }
+    const auto go = [&](auto kernel) { kernel<<<a.d.groups * a.d.beams * a.chunks, kBeamThreads, 0, stream>>>(a); };
+    a.d.dtype == Q4RDNA_F32 ? go(beam_kernel<float>) : a.d.dtype == Q4RDNA_F16 ? go(beam_kernel<_Float16>) : go(beam_kernel<__bf16>);
     return hipGetLastError();
 }
 

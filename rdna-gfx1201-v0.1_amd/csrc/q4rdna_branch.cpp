@@ -152,16 +152,23 @@ int beam_select(const q4rdna_beam_desc *desc, void *stream) {
     if ((rc = current_device(&device)) != Q4RDNA_OK) return rc;
     BeamArgs a{};
     a.d = d;
-    // The shortest chunks that give every CU four workgroups at most.
+    // A trip costs a workgroup 0.8 us, its own start and end 4, and every chunk's
+    // items lengthen the join: up to three workgroups a CU, and up to 128 chunks of
+    // a group, a chunk is one trip (one, two and three trips: 4 rows of 151936 in
+    // fp32, 152 trips, 12.8, 12.2, 13.5 us; one row 8.6, 10.1, 10.5; 160 rows of
+    // 50257 in bf16, 2080 trips, 35.6, 23.6, 19.4, and 20.8 with four).
     const uint64_t rows = static_cast<uint64_t>(d.groups) * d.beams;
-    for (a.each = 4; a.each < 32; a.each *= 2)
-        if (rows * ((d.vocab + 256 * a.each - 1) / (256 * a.each)) <= 4ull * cu_count(device)) break;
-    a.chunks = (d.vocab + 256 * a.each - 1) / (256 * a.each);
+    const uint32_t row_trips = (d.vocab + kBeamTrip - 1) / kBeamTrip;
+    const uint64_t most = 3ull * cu_count(device);
+    a.trips = static_cast<uint32_t>(std::max<uint64_t>((rows * row_trips + most - 1) / most,
+                                                       (static_cast<uint64_t>(d.beams) * row_trips + 127) / 128));
+    a.trips = std::min(a.trips, row_trips);
+    a.chunks = (row_trips + a.trips - 1) / a.trips;
     const uint64_t lists = rows * a.chunks;
     if (lists > most_workgroups(256) || static_cast<uint64_t>(d.beams) * a.chunks * d.count > 0x7fffffffu)
         return set_error(Q4RDNA_ERR_ARGUMENT, "%u groups of %u beams are too many for one call", d.groups, d.beams);
     Scratch scratch;
-    if ((rc = get_scratch(device, static_cast<hipStream_t>(stream), 2 * lists * (d.count + 2), d.groups, &scratch)) != Q4RDNA_OK) return rc;
+    if ((rc = get_scratch(device, static_cast<hipStream_t>(stream), 2 * lists * (d.count + 2 * kBeamPartials), d.groups, &scratch)) != Q4RDNA_OK) return rc;
     a.tops = reinterpret_cast<uint64_t *>(scratch.partials);
     a.stats = a.tops + lists * d.count;
     a.arrived = scratch.arrived;

@@ -118,12 +118,14 @@ struct TreeArgs {
 };
 hipError_t launch_attend_tree(const TreeArgs &a, hipStream_t stream);
 
+constexpr uint32_t kBeamTrip = 4096;
+constexpr uint32_t kBeamPartials = 4;  // sums of a chunk, one of each wave
 struct BeamArgs {
     q4rdna_beam_desc d;
-    uint32_t each;      // numbers of a row that a thread takes: 4, 8, 16 or 32
-    uint32_t chunks;    // of 256 * each numbers, per row
+    uint32_t trips;     // of a workgroup, kBeamTrip numbers each
+    uint32_t chunks;    // of trips * kBeamTrip numbers, per row
     uint64_t *tops;     // [group][count][beam][chunk]: ordered logit << 32 | ~token, 0: none
-    uint64_t *stats;    // [group][beam][chunk][2]: sum (double), max (float)
+    uint64_t *stats;    // [group][beam][chunk][kBeamPartials][2]: sum (double), max (float)
     uint32_t *arrived;  // [group], zero between launches
 };
 hipError_t launch_beam(const BeamArgs &a, hipStream_t stream);
