@@ -10,16 +10,28 @@
 //    operands' worth when q has its numbers in the same order;
 //  * the 16 bytes that it loads of V are 16 tokens of one number, the tokens
 //    whose scores the lane holds after the first product.
-// So no wave waits for another before the end.  Up to 32 rows the workgroup's
-// four waves take different blocks, up to 64 two and two of them, and with more
-// rows each has its own 32 and they read the same blocks side by side.
+// A workgroup has one tile of 32 rows, and its four waves every fourth block of
+// it: no wave waits for another before the end, when their parts meet in LDS.
+// (Tiles of 128 rows, a wave per 32, read each block once rather than once a
+// tile, but left three waves idle where rows are few or odd, and parts four times
+// as large to join: 63 us rather than 56 for 32 sequences of 100 .. 8000 tokens,
+// 1 .. 24 drafts, 8 kv heads of 4 by 128.  The second read is the L2's.)
 //
 // The drafted tokens are one more block.  The workgroup lays their rows into LDS
 // in fp16, scaled by a power of two for each token, fp32 ones in two parts; a
 // row's mask is 64 bits.
 //
-// A sequence's blocks are split over workgroups, dealt by the sequences' lengths,
-// and joined by the last one to arrive, in a fixed order.
+// A tile's blocks are split over workgroups, dealt on the device by the
+// sequences' lengths, and joined in a fixed order by a second kernel.
+//
+// What bounds it: a wave's vector instructions, some 600 for a block of 64 tokens
+// (2048 codes into fp16, 2048 weights), a 16th as many matrix instructions; for
+// one sequence, the chain of dependent loads and the first fetch of the code.
+// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 13.0 us; 16 drafts
+// after 4001 17.2 us and 4.0 us the joining; bf16, the 32 sequences above (118 MB
+// of codes) 56.4 us and 4.9 us.
+#include <type_traits>
+
 #include "q4rdna_rows_device.h"
 
 namespace q4rdna {
@@ -29,26 +41,36 @@ constexpr int kWaves = 4, kTreeThreads = 64 * kWaves;
 constexpr int kBlock = static_cast<int>(kKvBlock);
 
 template <int D>
-struct TreeTile {  // as attend_many_kernel's
-    _Float16 k[kKvBlock * (D + 8)];
-    _Float16 v[D * (kKvBlock + 8)];
+struct TreeTile {
+    _Float16 k[kKvBlock * (D + 8)];  // rows of 272 (144) bytes: 16 lanes' 16-byte reads of 16 rows cover all banks once
+    _Float16 v[D * kKvBlock];        // V^T, see v_place
 };
+// Place of a row of V^T's numbers `at` and on (of 64, in the order of the lanes'
+// scores): its 16-byte pieces are turned by the row, so that 16 rows side by side
+// (the products') and 16 rows of every eighth (the staging's) lie in all banks.
+__device__ __forceinline__ int v_place(int row, int at) { return row * kBlock + (((at >> 3) ^ ((row >> 3) + row)) & 7) * 8 + (at & 7); }
 template <int D, int SPLIT>
 struct TreeStage {
     TreeTile<D> part[SPLIT];
     float k_scale[kKvBlock], v_scale[kKvBlock];
 };
+// Parts of one row joined: its maximum m, the accumulators' exponent e (a whole
+// number) and its sum l, in units of 2^(m - 7).
+struct Joined {
+    float m, l, e;
+};
 template <int D>
 struct TreeJoin {
     float o[kWaves][32][D + 4];
     float m[kWaves][32], l[kWaves][32], e[kWaves][32];
+    Joined joined[32];
 };
 
-// Rows of K and V of a block as they lie in memory.
+// K or V of a block as it lies in memory, 16 bytes of a lane each: of K
+// [32 tokens][32 numbers], of V [32 numbers][tokens with bit 3 clear, set].
 template <int D>
 struct TreeRaw {
-    i32x4 k[2][D / 32];  // [32 tokens][32 numbers]
-    i32x4 v[D / 32][2];  // [32 numbers][tokens with bit 3 clear, set]
+    i32x4 x[D / 16];
 };
 template <int D>
 __device__ __forceinline__ void load_k(TreeRaw<D> &r, const int8_t *tile) {
@@ -57,7 +79,7 @@ __device__ __forceinline__ void load_k(TreeRaw<D> &r, const int8_t *tile) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) r.k[t][x] = load16(p + t * (D / 64 * 2048) + x / 2 * 1024 + x % 2 * 512);
+        for (int x = 0; x < D / 32; ++x) r.x[t * (D / 32) + x] = load16(p + t * (D / 64 * 2048) + x / 2 * 1024 + x % 2 * 512);
 }
 template <int D>
 __device__ __forceinline__ void load_v(TreeRaw<D> &r, const int8_t *tile) {
@@ -66,7 +88,7 @@ __device__ __forceinline__ void load_v(TreeRaw<D> &r, const int8_t *tile) {
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) r.v[d][y] = load16(p + d * 2048 + y * 512);
+        for (int y = 0; y < 2; ++y) r.x[d * 2 + y] = load16(p + d * 2048 + y * 512);
 }
 // Half of 16 codes as fp16, times 2^-8 where they are low bytes.
 template <bool LOW>
@@ -85,26 +107,36 @@ __device__ __forceinline__ h16x8 half_piece(i32x4 piece, int half) {
     return r;
 }
 
+// Operands of the two products out of raw tiles.
+template <bool LOW, int D>
+__device__ __forceinline__ h16x8 k_fragment(const TreeRaw<D> &r, int t, int f) { return half_piece<LOW>(r.x[t * (D / 32) + f / 2], f % 2); }
+template <bool LOW, int D>
+__device__ __forceinline__ h16x8 v_fragment(const TreeRaw<D> &r, int d, int y, int pair) { return half_piece<LOW>(r.x[d * 2 + y], pair); }
+
 // s[t] += the products of K's fragments (32 tokens t, 16 numbers f) with the rows.
+// `more`: there are tokens in the second 32.
 template <int D, int SPLIT, typename K>
-__device__ __forceinline__ void add_scores(const ManyState<D, SPLIT> &st, f32x16 (&s)[2], K fragment) {
+__device__ __forceinline__ void add_scores(const ManyState<D, SPLIT> &st, f32x16 (&s)[2], K fragment, bool more = true) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+        if (t == 1 && !more) return;
 #pragma unroll
         for (int f = 0; f < D / 16; ++f) {
             const h16x8 k = fragment(t, f);
 #pragma unroll
             for (int x = 0; x < SPLIT; ++x) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, st.q[f][x], s[t], 0, 0, 0);
         }
+    }
 }
 // o += the products of V's fragments (32 numbers d; tokens 16 a + 8 y + 4 half + b,
 // a = 2 pair, 2 pair + 1) with the weights.
 template <int D, int SPLIT, typename V>
-__device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (&s)[2], V fragment) {
+__device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (&s)[2], V fragment, bool more = true) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int pair = 0; pair < 2; ++pair) {
+        if (pair == 1 && !more) return;
 #pragma unroll
-        for (int pair = 0; pair < 2; ++pair) {
+        for (int y = 0; y < 2; ++y) {
             h16x8 p[SPLIT];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -120,6 +152,7 @@ __device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (
                 for (int x = 0; x < SPLIT; ++x) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], st.o[d], 0, 0, 0);
             }
         }
+    }
 }
 __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
 #pragma unroll
@@ -127,23 +160,35 @@ __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
 }
+// All ones where bit i is set.  (As an instruction of its own: the compiler would
+// make a compare of it, and 32 of them would each hold a pair of scalar registers.)
+__device__ __forceinline__ uint32_t bit_ones(uint32_t bits, int i) { return static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), i, 1)); }
 // `instead` where a bit is clear.
 __device__ __forceinline__ void hide(f32x16 (&s)[2], uint32_t seen, float instead) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const uint32_t m = bit_mask(seen, 16 * t + i);
+            const uint32_t m = bit_ones(seen, 16 * t + i);
             s[t][i] = __uint_as_float((__float_as_uint(s[t][i]) & m) | (__float_as_uint(instead) & ~m));
         }
 }
+// The largest and the sum of the lane's 32 numbers, four chains of them side by side.
 __device__ __forceinline__ float largest(const f32x16 (&s)[2]) {
-    float top = s[0][0];
+    float top[4] = {s[0][0], s[0][8], s[1][0], s[1][8]};
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-    return max_xor32(top);
+        for (int i = 1; i < 8; ++i) top[x] = fmaxf(top[x], s[x / 2][8 * (x % 2) + i]);
+    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+__device__ __forceinline__ float total(const f32x16 (&s)[2]) {
+    float sum[4] = {s[0][0], s[0][8], s[1][0], s[1][8]};
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum[x] += s[x / 2][8 * (x % 2) + i];
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 // Scores to weights: s = 2^(s * unit + shift), zero where hidden; their sum.
 __device__ __forceinline__ float exponentials(f32x16 (&s)[2], float unit, float shift, uint32_t seen, bool masked) {
@@ -152,12 +197,7 @@ __device__ __forceinline__ float exponentials(f32x16 (&s)[2], float unit, float 
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unit, shift));
     if (masked) hide(s, seen, 0.0f);
-    float sum = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum += s[t][i];
-    return sum;
+    return total(s);
 }
 
 // The softmax of a full block: integer products to weights in the accumulators'
@@ -166,7 +206,7 @@ template <int D, int SPLIT>
 __device__ __forceinline__ void soften_block(ManyState<D, SPLIT> &st, f32x16 (&s)[2], float k_scale, float v_scale, uint32_t seen,
                                              bool masked) {
     if (masked) hide(s, seen, kNegInf);
-    const float unit = st.q_scale * k_scale, top = largest(s);
+    const float unit = st.q_scale * k_scale, top = max_xor32(largest(s));
     const bool none = top == kNegInf;
     const float now = none ? kNegInf : top * unit;
     // The block's scale of V, 2^(v_exp + v_log), goes into the exponent, and comes out of the sum.
@@ -189,7 +229,7 @@ __device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&
         for (int b = 0; b < 4; ++b) s[x / 4][4 * (x % 4) + b] *= kt[b];
     }
     hide(s, seen, kNegInf);
-    const float unit = __builtin_amdgcn_ldexpf(st.q_scale, unit_log), top = largest(s);
+    const float unit = __builtin_amdgcn_ldexpf(st.q_scale, unit_log), top = max_xor32(largest(s));
     const float now = top == kNegInf ? kNegInf : top * unit;
     // Weights of 2^8 at most times the scales, under 2^122, in fp32; the largest
     // of them is what the row refers to.
@@ -202,12 +242,7 @@ __device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&
         for (int b = 0; b < 4; ++b) s[x / 4][4 * (x % 4) + b] *= vt[b] + (vt[b] - vt[b]);  // an infinite scale is made NaN
     }
     hide(s, seen, 0.0f);
-    float most = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i]);
-    refer(st, now, m + __builtin_amdgcn_logf(max_xor32(most)) + static_cast<float>(unit_log));
+    refer(st, now, m + __builtin_amdgcn_logf(max_xor32(fmaxf(largest(s), 0.0f))) + static_cast<float>(unit_log));
     st.l += __builtin_amdgcn_ldexpf(sum, static_cast<int>(kWeight));
     // From units of 2^(m + unit_log) to the accumulators'.
     const int up = st.e == kNegInf ? 0 : unit_log + static_cast<int>(kWeight) - static_cast<int>(st.e);
@@ -217,20 +252,42 @@ __device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&
         for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_ldexpf(s[t][i], up);
 }
 
+// Numbers as they lie in memory, N side by side at any alignment: they become
+// floats where they are used, since a conversion waits for them.
+template <typename T, int N>
+struct Numbers {
+    typedef T TN __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    TN v;
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_numbers(Numbers<T, N> &x, const T *p) {
+    typedef __attribute__((address_space(1))) const typename Numbers<T, N>::TN *gptr;
+    x.v = *(gptr)(uintptr_t)p;
+}
+template <typename T>
+using Eight = Numbers<T, 8>;
+
 // Rows of q, the numbers of a fragment f in the order in which K's pieces have
 // them: 64 (f / 4) + 32 (f / 2 % 2) + 16 half + 8 (f % 2) and on.
 __device__ __forceinline__ int fragment_number(int f, int half) { return f / 4 * 64 + f / 2 % 2 * 32 + 16 * half + f % 2 * 8; }
-template <int D, int SPLIT, typename T>
-__device__ __forceinline__ void load_rows(ManyState<D, SPLIT> &st, const T *row, bool wide, float scale) {
+template <int D, typename T>
+__device__ __forceinline__ void load_query(Eight<T> (&x)[D / 16], const T *row) {
     const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int f = 0; f < D / 16; ++f) load_numbers(x[f], row + fragment_number(f, half));
+}
+template <int D, int SPLIT, typename T>
+__device__ __forceinline__ void set_query(ManyState<D, SPLIT> &st, const Eight<T> (&raw)[D / 16], float scale) {
     float x[D / 16][8];
+#pragma unroll
+    for (int f = 0; f < D / 16; ++f)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[f][e] = static_cast<float>(raw[f].v[e]);
     uint32_t top = 0;
 #pragma unroll
-    for (int f = 0; f < D / 16; ++f) {
-        load_floats<T, 8>(row + fragment_number(f, half), wide, x[f]);
+    for (int f = 0; f < D / 16; ++f)
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[f][e]) & 0x7fffffffu);
-    }
     top = __float_as_uint(max_xor32(__uint_as_float(min(top, 0x7f800000u))));  // NaN as infinity
     const bool finite = top < 0x7f800000u;
     // The largest number of the row to 2^13 .. 2^14: small ones stay normal in fp16.
@@ -255,34 +312,42 @@ __device__ __forceinline__ void load_rows(ManyState<D, SPLIT> &st, const T *row,
 
 // The drafted tokens' K and V into LDS: a thread takes eight numbers of four
 // tokens, D / 8 threads side by side a row.
-template <int D, int SPLIT, typename T>
-__device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const TreeArgs &a, int first, int count, uint32_t head) {
-    constexpr int kOctets = D / 8;
-    const int tid = threadIdx.x, octet = tid % kOctets, quad = tid / kOctets;
-    if (quad >= kBlock / 4) return;
-    float x[2][4][8];
+template <int D, typename T>
+struct DraftRows {
+    static constexpr int kOctets = D / 8;
+    Eight<T> raw[2][4];
+    __device__ __forceinline__ static int octet() { return threadIdx.x % kOctets; }
+    __device__ __forceinline__ static int quad() { return threadIdx.x / kOctets; }  // of 16 (the threads behind have none)
+};
+template <int D, typename T>
+__device__ __forceinline__ void load_drafts(DraftRows<D, T> &r, const TreeArgs &a, int first, int count, uint32_t head) {
+    const int quad = r.quad();
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         const q4rdna_kv_rows &rows = which == 0 ? a.d.k : a.d.v;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            if (4 * quad + b < count) {
-                load_floats<T, 8>(static_cast<const T *>(rows.data) + static_cast<int64_t>(first + 4 * quad + b) * rows.token_stride +
-                                      head * rows.head_stride + 8 * octet, a.wide != 0, x[which][b]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[which][b][e] = 0.0f;
-            }
+            // (Tokens behind the last one are that one, and seen by nobody.)
+            load_numbers(r.raw[which][b], static_cast<const T *>(rows.data) + static_cast<int64_t>(first + min(4 * quad + b, count - 1)) * rows.token_stride +
+                                              head * rows.head_stride + 8 * r.octet());
         }
     }
+}
+template <int D, int SPLIT, typename T>
+__device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const DraftRows<D, T> &r) {
+    const int octet = r.octet(), quad = r.quad();
+    if (quad >= kBlock / 4) return;
+    float x[2][4][8];
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[which][b][e] = static_cast<float>(r.raw[which][b].v[e]);
             uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[which][b][e]) & 0x7fffffffu);
-            top = lanes_max<kOctets>(top);
+            top = lanes_max<DraftRows<D, T>::kOctets>(top);
             const bool finite = top < 0x7f800000u;
             // The largest to 2^13 .. 2^14, but for numbers under 2^-96: the scale stays a normal number.
             const int up = finite && top != 0 ? min(14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 110) : 0;
@@ -314,7 +379,7 @@ __device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const T
                 v[b] = static_cast<_Float16>(x[1][b][e]);
                 x[1][b][e] -= static_cast<float>(v[b]);
             }
-            *reinterpret_cast<h16x4 *>(tile.v + (8 * octet + e) * (kBlock + 8) + at) = v;
+            *reinterpret_cast<h16x4 *>(tile.v + v_place(8 * octet + e, at)) = v;
         }
     }
 }
@@ -339,68 +404,75 @@ __device__ __forceinline__ int first_block(const TreeArgs &a, int past) {
     return a.d.window != 0 && static_cast<uint32_t>(past) > a.d.window ? (past - static_cast<int>(a.d.window)) / kBlock : 0;
 }
 
-// What a sequence's workgroups take: each row group of each head is cut into
+// What a sequence's workgroups take: each tile of 32 rows of each head is cut into
 // parts of about `chunk` of its units, the cached blocks and the drafts.
 struct TreeWork {
     Seq s;
     uint32_t jobs, units;
 };
-__device__ __forceinline__ TreeWork tree_work(const TreeArgs &a, uint32_t rows, uint32_t i) {
+__device__ __forceinline__ TreeWork tree_work(const TreeArgs &a, uint32_t i) {
     TreeWork w;
     w.jobs = w.units = 0;
     w.s = draft_seq(a, min(i, a.batch.sequences - 1));
     if (i >= a.batch.sequences || !w.s.ok || w.s.count == 0) return w;
-    w.jobs = (w.s.count * a.group + rows - 1) / rows * a.cache.kv_heads;
+    w.jobs = (w.s.count * a.group + kTreeRows - 1) / kTreeRows * a.cache.kv_heads;
     w.units = (w.s.past + kBlock - 1) / kBlock - first_block(a, w.s.past) + 1;
     return w;
 }
-__device__ __forceinline__ uint32_t tree_parts(const TreeArgs &a, uint32_t units, uint32_t chunk) {
-    chunk = max(chunk, a.least);
-    return min((units + chunk - 1) / chunk, a.splits);
+// (A part has a unit for every wave.)
+__device__ __forceinline__ uint32_t tree_parts(const TreeArgs &a, const TreeWork &w, uint32_t chunk) {
+    chunk = max(chunk, static_cast<uint32_t>(kWaves));
+    return min((w.units + chunk - 1) / chunk, a.splits);
 }
 
 struct TreeItem {
     int seq;  // -1: nothing
     Seq s;
-    uint32_t head, row_group;
+    uint32_t head, tile;
     int split, splits;
-    uint32_t first, step;  // workgroup of part 0; part i is `step` * i further on
+    uint32_t first;  // workgroup of part 0; part i is kv_heads * i further on
 };
 // The item of workgroup x: the device knows the lengths, the host does not, so
 // every wave adds up the sequences' parts, 64 at a time.
-__device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a, uint32_t rows, uint32_t x) {
+__device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a, uint32_t x) {
     TreeItem it;
     it.seq = -1;
     const int lane = threadIdx.x & 63;
     const uint32_t heads = a.cache.kv_heads;
-    if (a.splits == 1) {  // as many workgroups as there may be row groups
-        const uint32_t per = a.row_groups * heads;
+    if (a.splits == 1) {  // as many workgroups as there may be tiles
+        const uint32_t per = a.tiles * heads;
         it.seq = static_cast<int>(x / per);
         it.s = draft_seq(a, x / per);
-        it.row_group = x % per / heads;
+        it.tile = x % per / heads;
         it.head = x % heads;
         it.split = 0;
         it.splits = 1;
         it.first = x;
-        it.step = 1;
         return it;
     }
     TreeWork w;
     uint32_t all = 0;  // jobs * units, fewer than 2^32 by the host's bound
     for (uint32_t i = 0; i < a.batch.sequences; i += 64) {
-        w = tree_work(a, rows, i + lane);
+        w = tree_work(a, i + lane);
         all += __builtin_amdgcn_readlane(wave_scan(w.jobs * w.units), 63);
     }
-    const uint32_t chunk = (all - 1) / a.target + 1;
+    uint32_t chunk = (max(all, 1u) - 1) / a.target + 1;
+    // Larger parts until all of them run at once, if they can.
+    if (a.batch.sequences <= 64) {
+        const uint32_t jobs = __builtin_amdgcn_readlane(wave_scan(w.jobs), 63);
+        while (jobs < a.target &&
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(wave_scan(w.jobs * tree_parts(a, w, chunk)), 63)) > a.target)
+            chunk += chunk / 8 + 1;
+    }
     uint32_t base = 0;
     for (uint32_t i = 0; i < a.batch.sequences; i += 64) {
-        if (a.batch.sequences > 64) w = tree_work(a, rows, i + lane);
-        const uint32_t parts = tree_parts(a, w.units, chunk), end = base + wave_scan(w.jobs * parts);
+        if (a.batch.sequences > 64) w = tree_work(a, i + lane);
+        const uint32_t parts = tree_parts(a, w, chunk), end = base + wave_scan(w.jobs * parts);
         const uint64_t later = __builtin_amdgcn_ballot_w64(end > x);
         if (later != 0) {
             const int owner = __builtin_ctzll(later);
             const uint32_t mine = __builtin_amdgcn_readlane(parts, owner);
-            const uint32_t local = x - __builtin_amdgcn_readlane(end - w.jobs * parts, owner);  // (row group, part, head)
+            const uint32_t local = x - __builtin_amdgcn_readlane(end - w.jobs * parts, owner);  // (tile, part, head)
             it.seq = static_cast<int>(i) + owner;
             it.s.first = __builtin_amdgcn_readlane(w.s.first, owner);
             it.s.count = __builtin_amdgcn_readlane(w.s.count, owner);
@@ -410,9 +482,8 @@ __device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a, uint32_t r
             it.s.ok = true;
             it.head = local % heads;
             it.split = static_cast<int>(local / heads % mine);
-            it.row_group = local / heads / mine;
+            it.tile = local / heads / mine;
             it.splits = static_cast<int>(mine);
-            it.step = heads;
             it.first = x - it.split * heads;
             return it;
         }
@@ -421,39 +492,46 @@ __device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a, uint32_t r
     return it;
 }
 
-// Parts of one row joined: its maximum m, the accumulators' exponent e (a whole
-// number) and its sum l, in units of 2^(m - 7).
-struct Joined {
-    float m, l, e;
-};
-__device__ __forceinline__ float part_factor(const Joined &j, float m, float e) {  // (a part without e is zero, or NaN)
-    return e == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((m - j.m) + (e - j.e));
-}
-template <typename Stat>
-__device__ __forceinline__ Joined join(int parts, Stat stat) {
-    Joined j = {kNegInf, 0.0f, kNegInf};
-    for (int i = 0; i < parts; ++i) j.m = fmaxf(j.m, stat(i).m);
-    const float ref = j.m == kNegInf ? 0.0f : j.m;
-    for (int i = 0; i < parts; ++i) {
-        const Joined s = stat(i);
-        if (s.e != kNegInf) j.e = fmaxf(j.e, ceilf((s.m - ref) + s.e));
-        j.l += s.l * __builtin_amdgcn_exp2f(s.m - ref);
-    }
-    return j;
+// A part's e where the row's maximum is `ref`, and its factor in the row's unit e.
+// (A part without e is zero, or NaN.)
+__device__ __forceinline__ float shifted_unit(float ref, float m, float e) { return e == kNegInf ? kNegInf : ceilf((m - ref) + e); }
+__device__ __forceinline__ float part_factor(float ref, float row_e, float m, float e) {
+    return e == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((m - ref) + (e - row_e));
 }
 
-// RW of the four waves have different rows, 4 / RW different blocks.
-template <int D, int SPLIT, int RW, typename T>
+// Four numbers of a row.
+template <typename T>
+__device__ __forceinline__ void write_row(const TreeArgs &a, const Seq &s, uint32_t head, int row, int d, const Joined &w, f32x4 o) {
+    const int group = static_cast<int>(a.group), n = s.first + row / group;
+    const uint32_t to_head = head * a.group + row % group;
+    const float inv = w.l == 0.0f ? 0.0f : 1.0f / w.l;
+    const int places = static_cast<int>(fminf(fmaxf(w.e, -400.0f), 400.0f));
+    typedef __attribute__((address_space(1))) typename Numbers<T, 4>::TN *gptr;
+    typename Numbers<T, 4>::TN v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(__builtin_amdgcn_ldexpf(o[e] * inv, places));
+    *(gptr)(uintptr_t)(static_cast<T *>(a.d.out.data) + static_cast<int64_t>(n) * a.d.out.token_stride + to_head * a.d.out.head_stride + d) = v;
+    if (d == 0 && a.d.lse != nullptr)
+        a.d.lse[static_cast<size_t>(n) * a.d.q_heads + to_head] = (w.m + log2f(w.l) - kWeight) * (1.0f / kLog2e);
+}
+
+// The parts' results of workgroup x: [row][D], and behind all of these [m, l, e][row].
+template <int D>
+__device__ __forceinline__ float *part_rows(const TreeArgs &a, uint32_t x) { return a.partials + static_cast<size_t>(x) * kTreeRows * D; }
+template <int D>
+__device__ __forceinline__ float *part_stats(const TreeArgs &a, uint32_t x) {
+    return a.partials + static_cast<size_t>(a.workgroups) * kTreeRows * D + static_cast<size_t>(x) * kTreeRows * 3;
+}
+
+template <int D, int SPLIT, typename T>
 __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_kernel(const TreeArgs a) {
-    constexpr int BW = kWaves / RW, ROWS = 32 * RW;
     __shared__ __align__(16) union Shared {
         TreeStage<D, SPLIT> stage;
         TreeJoin<D> join;
     } shared;
-    __shared__ uint32_t ticket;
+    __shared__ __align__(16) float open_scales[kWaves][2 * kBlock];
     const int tid = threadIdx.x, lane = tid & 63, column = lane & 31, half = lane >> 5, wave = wave_id();
-    const int row_wave = wave % RW, block_wave = wave / RW;
-    const TreeItem it = find_tree_item(a, ROWS, blockIdx.x);
+    const TreeItem it = find_tree_item(a, blockIdx.x);
     if (blockIdx.x == 0)  // bad entries, once
         for (uint32_t i = tid; i < a.batch.sequences; i += kTreeThreads)
             if (!draft_seq(a, i).ok) count_fault(a.cache);
@@ -461,115 +539,97 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     const uint32_t head = it.head;
     const Seq &s = it.s;
     const int group = static_cast<int>(a.group), rows = s.count * group;
-    const int first_row = static_cast<int>(it.row_group) * ROWS;
+    const int first_row = static_cast<int>(it.tile * kTreeRows);
     if (first_row >= rows) return;
+    const int live_rows = min(static_cast<int>(kTreeRows), rows - first_row);
     // Units: the cached blocks from block0 on, full ones, then the open one, then the drafts.
     const int block0 = first_block(a, s.past), full_blocks = s.past / kBlock;
     const int units = (s.past + kBlock - 1) / kBlock - block0 + 1;
     const int splits = min(it.splits, units), split = it.split;
     if (split >= splits) return;
+    if (a.splits > 1 && split == 0 && tid == 0)
+        a.jobs[(static_cast<size_t>(it.seq) * a.tiles + it.tile) * a.cache.kv_heads + head] = TreeJob{it.first, static_cast<uint32_t>(splits)};
     const int from = block0 + static_cast<int>(mul_div(split, units, splits));
     const int to = block0 + static_cast<int>(mul_div(split + 1, units, splits));
     const int drafts = block0 + units - 1;
     const bool has_drafts = drafts < to;
-    const auto mine = [&](int unit) { return unit >= from && unit < to && (unit - from) % BW == block_wave; };
+    const auto mine = [&](int unit) { return unit >= from && unit < to && (unit - from) % kWaves == wave; };
 
-    // This wave's rows.
-    const int row = first_row + 32 * row_wave + column;
-    const bool live = row < rows;
-    const int token = live ? row / group : 0;
-    const uint32_t h = head * a.group + (live ? row - token * group : 0);
-    ManyState<D, SPLIT> st;
-
-    // The wave's full blocks: from + block_wave + BW n.  Lane x keeps the page of
-    // the x-th of the next 64.
+    // Everything that depends on the item alone is under way first.  The wave's
+    // full blocks: from + wave + 4 n.  Lane x keeps the page of the x-th of
+    // the next 64, -1 for a bad one.
     const int32_t *table = a.batch.table + static_cast<size_t>(it.seq) * a.batch.table_width;
-    const int start = from + block_wave, full_to = min(to, full_blocks);
-    const int full = full_to > start ? (full_to - start + BW - 1) / BW : 0;
-    constexpr size_t kPlane = kKvBlock * D;
-    TreeRaw<D> raw;
-    f32x2 scale_next = {0.0f, 0.0f};
-    bool bad_next = false;
+    const int start = from + wave, full_to = min(to, full_blocks);
+    const int full = full_to > start ? (full_to - start + kWaves - 1) / kWaves : 0;
+    const bool open_mine = s.past % kBlock != 0 && mine(full_blocks), drafts_mine = mine(drafts);
     int pages = 0;
+    if (full > 0) pages = table[min(start + kWaves * lane, full_to - 1)];
+    const int8_t *planes = a.cache.open + open_tile(a.cache, s.slot, full_blocks, head);
+    f32x2 open_scale = {0.0f, 0.0f};
+    if (open_mine) {
+        const float *scales = a.cache.open_scales + open_scale_row(a.cache, s.slot, full_blocks, head);
+        open_scale = f32x2{scales[lane], scales[kBlock + lane]};
+    }
+    Eight<T> query[D / 16];
+    const int row = first_row + column, token = row < rows ? row / group : 0;
+    load_query<D, T>(query, static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(s.first + token) * a.d.q.token_stride +
+                                (head * a.group + (row < rows ? row - token * group : 0)) * a.d.q.head_stride);
+    uint64_t seen = a.d.seen[s.first + token];  // of the drafts, by the lane's row
+    DraftRows<D, T> draft_rows;
+    if (has_drafts) load_drafts<D, T>(draft_rows, a, s.first, s.count, head);
+    tile_end();
+    constexpr size_t kPlane = kKvBlock * D;
+    const int8_t *head_pages = a.cache.pages + head * (2 * kPlane);
+    const float *head_scales = a.cache.scales + 2 * head;
+    const uint32_t page_bytes = a.cache.kv_heads * static_cast<uint32_t>(2 * kPlane), page_count = a.cache.page_count;
+    TreeRaw<D> ka, vb;  // K and V of a full block, or K's (V's) high and low bytes of the open one
+    f32x2 scale_next = {0.0f, 0.0f};
     const int8_t *tile = nullptr;
-    const auto next = [&](int n) {
-        if (n % 64 == 0) pages = table[min(start + BW * (n + lane), full_to - 1)];
-        int page = __builtin_amdgcn_readlane(pages, n % 64);
-        bad_next = static_cast<uint32_t>(page) >= a.cache.page_count;
-        if (bad_next) {
-            if (lane == 0) count_fault(a.cache);
-            page = 0;
+    const auto check_pages = [&](int n) {
+        if (static_cast<uint32_t>(pages) >= page_count) {
+            if (n + lane < full) count_fault(a.cache);
+            pages = -1;
         }
-        tile = a.cache.pages + page_tile(a.cache, page, head);
-        scale_next = *(gptr_f32x2)(uintptr_t)(a.cache.scales + (static_cast<size_t>(page) * a.cache.kv_heads + head) * 2);
     };
-    if (full > 0) next(0);
-    // What the row sees of the drafts, and where it stands.
-    const uint64_t there = s.count >= 64 ? ~0ull : (1ull << s.count) - 1;
-    uint64_t seen = a.d.seen[s.first + token] & there;
-    const int depth = __builtin_popcountll(seen);
-    load_rows<D, SPLIT, T>(st, static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(s.first + token) * a.d.q.token_stride +
-                                   h * a.d.q.head_stride, a.wide != 0, a.d.scale);
-    st.position = s.past - 1 + depth;
+    const auto next = [&](int n) {
+        if (n % 64 == 0 && n != 0) {
+            pages = table[min(start + kWaves * (n + lane), full_to - 1)];
+            check_pages(n);
+        }
+        const int page = __builtin_amdgcn_readlane(pages, n % 64), safe = max(page, 0);
+        tile = head_pages + static_cast<size_t>(static_cast<uint32_t>(safe)) * page_bytes;
+        scale_next = *(gptr_f32x2)(uintptr_t)(head_scales + static_cast<size_t>(static_cast<uint32_t>(safe)) * (2 * a.cache.kv_heads));
+        return page >= 0;
+    };
+    bool good_next = true;
     if (full > 0) {
-        load_k(raw, tile);
-        load_v(raw, tile + kPlane);
+        check_pages(0);
+        good_next = next(0);
+        load_k(ka, tile);
+        load_v(vb, tile + kPlane);
+    } else if (open_mine) {
+        load_k(ka, planes);
+        load_k(vb, planes + kPlane);
+    }
+    tile_end();
+    ManyState<D, SPLIT> st;
+    set_query<D, SPLIT, T>(st, query, a.d.scale);
+    const uint64_t there = s.count >= 64 ? ~0ull : (1ull << s.count) - 1;
+    seen &= there;
+    st.position = s.past - 1 + __builtin_popcountll(seen);
+    if (open_mine) {
+        open_scales[wave][lane] = open_scale[0];
+        open_scales[wave][kBlock + lane] = open_scale[1];
     }
     if (has_drafts) {  // the same for the whole workgroup
-        stage_drafts<D, SPLIT, T>(shared.stage, a, s.first, s.count, head);
+        stage_drafts<D, SPLIT, T>(shared.stage, draft_rows);
         __syncthreads();
     }
-    // Of the lane's 32 tokens of a block, in the order of its scores: those cached and within the window.
-    const auto seen_from = [&](int first) {
-        const int ahead = s.past - 1 - first - 4 * half;
-        uint32_t bits = first_tokens(ahead);
-        if (a.d.window != 0) {
-            const int64_t behind = static_cast<int64_t>(st.position) - first - 4 * half - a.d.window;
-            bits &= ~first_tokens(static_cast<int>(max(behind, static_cast<int64_t>(-1))));
-        }
-        return bits;
-    };
 
     f32x16 sc[2];
-    for (int n = 0; n < full; ++n) {
-        const int first = (start + BW * n) * kBlock;
-        const f32x2 scale = scale_next;
-        const float k_scale = bad_next ? __builtin_nanf("") : scale[0], v_scale = bad_next ? __builtin_nanf("") : scale[1];
-        // No row stands behind past + 63.
-        const bool masked = a.d.window != 0 && static_cast<int64_t>(s.past) + 63 - first >= static_cast<int64_t>(a.d.window);
-        clear(sc);
-        add_scores(st, sc, [&](int t, int f) { return half_piece<false>(raw.k[t][f / 2], f % 2); });
-        tile_end();
-        if (n + 1 < full) {
-            next(n + 1);
-            load_k(raw, tile);
-        }
-        tile_end();
-        soften_block(st, sc, k_scale, v_scale, masked ? seen_from(first) : 0xffffffffu, masked);
-        tile_end();
-        add_rows(st, sc, [&](int d, int y, int pair) { return half_piece<false>(raw.v[d][y], pair); });
-        tile_end();
-        if (n + 1 < full) load_v(raw, tile + kPlane);
-        tile_end();
-    }
-    if (s.past % kBlock != 0 && mine(full_blocks)) {
-        const int8_t *planes = a.cache.open + open_tile(a.cache, s.slot, full_blocks, head);
-        const float *scales = a.cache.open_scales + open_scale_row(a.cache, s.slot, full_blocks, head);
-        clear(sc);
-        load_k(raw, planes);
-        add_scores(st, sc, [&](int t, int f) { return half_piece<false>(raw.k[t][f / 2], f % 2); });
-        load_k(raw, planes + kPlane);
-        load_v(raw, planes + 2 * kPlane);
-        add_scores(st, sc, [&](int t, int f) { return half_piece<true>(raw.k[t][f / 2], f % 2); });
-        soften_tokens(st, sc, 8, seen_from(full_blocks * kBlock), [&](int which, int x) {
-            return *(gptr_f32x4)(uintptr_t)(scales + kBlock * which + 8 * x + 4 * half);
-        });
-        add_rows(st, sc, [&](int d, int y, int pair) { return half_piece<false>(raw.v[d][y], pair); });
-        load_v(raw, planes + 3 * kPlane);
-        add_rows(st, sc, [&](int d, int y, int pair) { return half_piece<true>(raw.v[d][y], pair); });
-    }
-    if (mine(drafts)) {
+    if (drafts_mine) {
         if (a.d.window != 0 && a.d.window < 64) {  // drafted tokens that lie too far above
+            const int depth = st.position - (s.past - 1);
             const int depths = __builtin_popcountll(a.d.seen[s.first + min(lane, s.count - 1)] & there);
             for (int j = 0; j < s.count; ++j)
                 if (__builtin_amdgcn_readlane(depths, j) + static_cast<int>(a.d.window) <= depth) seen &= ~(1ull << j);
@@ -582,109 +642,206 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
         for (int part = 0; part < SPLIT; ++part)
             add_scores(st, sc, [&](int t, int f) {
                 return *reinterpret_cast<const h16x8 *>(shared.stage.part[part].k + (32 * t + column) * (D + 8) + fragment_number(f, half));
-            });
+            }, s.count > 32);
         soften_tokens(st, sc, 0, bits, [&](int which, int x) {
             return *reinterpret_cast<const f32x4 *>((which == 0 ? shared.stage.k_scale : shared.stage.v_scale) + 8 * x + 4 * half);
         });
 #pragma unroll
         for (int part = 0; part < SPLIT; ++part)
             add_rows(st, sc, [&](int d, int y, int pair) {
-                return *reinterpret_cast<const h16x8 *>(shared.stage.part[part].v + (32 * d + column) * (kBlock + 8) + 32 * half + 16 * y + 8 * pair);
-            });
+                return *reinterpret_cast<const h16x8 *>(shared.stage.part[part].v + v_place(32 * d + column, 32 * half + 16 * y + 8 * pair));
+            }, s.count > 32);
+    }
+    // Of the lane's 32 tokens of a block, in the order of its scores: those cached and within the window.
+    const auto seen_from = [&](int first) {
+        const int ahead = s.past - 1 - first - 4 * half;
+        uint32_t bits = first_tokens(ahead);
+        if (a.d.window != 0) {
+            const int64_t behind = static_cast<int64_t>(st.position) - first - 4 * half - a.d.window;
+            bits &= ~first_tokens(static_cast<int>(max(behind, static_cast<int64_t>(-1))));
+        }
+        return bits;
+    };
+    // A full block; `masked` ones are the first of a window's.
+    const auto block = [&](int n, auto masked) {
+        const float nan = __builtin_nanf("");
+        const float k_scale = good_next ? scale_next[0] : nan, v_scale = good_next ? scale_next[1] : nan;
+        clear(sc);
+        add_scores(st, sc, [&](int t, int f) { return k_fragment<false>(ka, t, f); });
+        tile_end();
+        if (n + 1 < full) {
+            good_next = next(n + 1);
+            load_k(ka, tile);
+        } else if (open_mine) {
+            load_k(ka, planes);
+        }
+        tile_end();
+        soften_block(st, sc, k_scale, v_scale, masked ? seen_from((start + kWaves * n) * kBlock) : 0xffffffffu, masked);
+        tile_end();
+        add_rows(st, sc, [&](int d, int y, int pair) { return v_fragment<false>(vb, d, y, pair); });
+        tile_end();
+        if (n + 1 < full) load_v(vb, tile + kPlane);
+        else if (open_mine) load_k(vb, planes + kPlane);
+        tile_end();
+    };
+    int n = 0;
+    if (a.d.window != 0)  // no row stands behind past + 63
+        for (; n < full && static_cast<int64_t>(s.past) + 63 - (start + kWaves * n) * kBlock >= static_cast<int64_t>(a.d.window); ++n)
+            block(n, std::true_type());
+    for (; n < full; ++n) block(n, std::false_type());
+    if (open_mine) {
+        const bool more = s.past % kBlock > 32;
+        clear(sc);
+        add_scores(st, sc, [&](int t, int f) { return k_fragment<false>(ka, t, f); }, more);
+        add_scores(st, sc, [&](int t, int f) { return k_fragment<true>(vb, t, f); }, more);
+        tile_end();
+        load_v(ka, planes + 2 * kPlane);
+        load_v(vb, planes + 3 * kPlane);
+        tile_end();
+        soften_tokens(st, sc, 8, seen_from(full_blocks * kBlock), [&](int which, int x) {
+            return *reinterpret_cast<const f32x4 *>(&open_scales[wave][kBlock * which + 8 * x + 4 * half]);
+        });
+        add_rows(st, sc, [&](int d, int y, int pair) { return v_fragment<false>(ka, d, y, pair); }, more);
+        add_rows(st, sc, [&](int d, int y, int pair) { return v_fragment<true>(vb, d, y, pair); }, more);
     }
 
-    // The waves' rows meet in LDS.
+    const float l = add_xor32(st.l);
+    float *stats = part_stats<D>(a, blockIdx.x);
+    const auto write = [&](int r, int d, const Joined &joined, f32x4 o) {
+        if (splits == 1) {
+            write_row<T>(a, s, head, first_row + r, d, joined, o);
+            return;
+        }
+        *reinterpret_cast<f32x4 *>(part_rows<D>(a, blockIdx.x) + static_cast<size_t>(r) * D + d) = o;
+        if (d == 0) {
+            stats[r] = joined.m;
+            stats[kTreeRows + r] = joined.l;
+            stats[2 * kTreeRows + r] = joined.e;
+        }
+    };
+    // The waves' rows meet in LDS, their statistics first: each wave brings its rows
+    // to the row's own unit.
     __syncthreads();
     TreeJoin<D> &j = shared.join;
-    const float l_row = add_xor32(st.l);
     if (half == 0) {
         j.m[wave][column] = st.m;
-        j.l[wave][column] = l_row;
+        j.l[wave][column] = l;
         j.e[wave][column] = st.e;
     }
+    __syncthreads();
+    Joined own = {kNegInf, 0.0f, kNegInf};
+    for (int i = 0; i < kWaves; ++i) own.m = fmaxf(own.m, j.m[i][column]);
+    const float ref = own.m == kNegInf ? 0.0f : own.m;
+    for (int i = 0; i < kWaves; ++i) {
+        own.e = fmaxf(own.e, shifted_unit(ref, j.m[i][column], j.e[i][column]));
+        own.l += j.l[i][column] * __builtin_amdgcn_exp2f(j.m[i][column] - ref);
+    }
+    if (wave == 0 && half == 0) j.joined[column] = own;
+    const float factor = part_factor(ref, own.e, st.m, st.e);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
             *reinterpret_cast<f32x4 *>(&j.o[wave][column][32 * d + 8 * x + 4 * half]) =
-                f32x4{st.o[d][4 * x], st.o[d][4 * x + 1], st.o[d][4 * x + 2], st.o[d][4 * x + 3]};
+                f32x4{st.o[d][4 * x], st.o[d][4 * x + 1], st.o[d][4 * x + 2], st.o[d][4 * x + 3]} * factor;
     __syncthreads();
-    const int live_rows = min(ROWS, rows - first_row);
-    const auto finish = [&](int r, int d, const Joined &w, f32x4 o) {
-        const int of = first_row + r, n = s.first + of / group;
-        const uint32_t to_head = head * a.group + of % group;
-        const float inv = w.l == 0.0f ? 0.0f : 1.0f / w.l;
-        const int places = static_cast<int>(fminf(fmaxf(w.e, -400.0f), 400.0f));
-        float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(o[e] * inv, places);
-        store_floats<T, 4>(static_cast<T *>(a.d.out.data) + static_cast<int64_t>(n) * a.d.out.token_stride + to_head * a.d.out.head_stride + d,
-                           a.wide_out != 0, v);
-        if (d == 0 && a.d.lse != nullptr)
-            a.d.lse[static_cast<size_t>(n) * a.d.q_heads + to_head] = (w.m + log2f(w.l) - kWeight) * (1.0f / kLog2e);
-    };
-    float *stats = a.partials + static_cast<size_t>(gridDim.x) * ROWS * D;  // [workgroup][row][m, l, e]
-    for (int x = tid; x < live_rows * (D / 4); x += kTreeThreads) {
-        const int r = x / (D / 4), d = x % (D / 4) * 4, rw = r / 32, c = r % 32;
-        const Joined w = join(BW, [&](int i) { return Joined{j.m[RW * i + rw][c], j.l[RW * i + rw][c], j.e[RW * i + rw][c]}; });
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < BW; ++i)
-            o += *reinterpret_cast<const f32x4 *>(&j.o[RW * i + rw][c][d]) * part_factor(w, j.m[RW * i + rw][c], j.e[RW * i + rw][c]);
-        if (splits == 1) {
-            finish(r, d, w, o);
-            continue;
-        }
-        float *to_part = a.partials + (static_cast<size_t>(blockIdx.x) * ROWS + r) * D + d;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) store_agent(to_part + e, o[e]);
-        if (d == 0) {
-            float *stat = stats + (static_cast<size_t>(blockIdx.x) * ROWS + r) * 3;
-            store_agent(stat, w.m);
-            store_agent(stat + 1, w.l);
-            store_agent(stat + 2, w.e);
-        }
-    }
-    if (splits == 1) return;
-
-    // The last workgroup of the row group joins the parts, in their order.
-    wait_stores();
-    __syncthreads();
-    uint32_t *arrived = a.arrived + (static_cast<size_t>(it.seq) * a.row_groups + it.row_group) * a.cache.kv_heads + head;
-    if (tid == 0) ticket = add_agent(arrived, 1u);
-    __syncthreads();
-    if (ticket != static_cast<uint32_t>(splits - 1)) return;
-    if (tid == 0) store_agent(arrived, 0u);
-    const auto slot = [&](int i, int r) { return (static_cast<size_t>(it.first) + static_cast<size_t>(i) * it.step) * ROWS + r; };
-    for (int x = tid; x < live_rows * (D / 4); x += kTreeThreads) {
+    for (int x = tid; x < 32 * (D / 4); x += kTreeThreads) {
         const int r = x / (D / 4), d = x % (D / 4) * 4;
-        const auto stat = [&](int i) {
-            const float *p = stats + slot(i, r) * 3;
-            return Joined{load_agent(p), load_agent(p + 1), load_agent(p + 2)};
-        };
-        const Joined w = join(splits, stat);
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < splits; ++i) {
-            const float *p = a.partials + slot(i, r) * D + d;
-            const f32x2 lo = load_agent2(p), hi = load_agent2(p + 2);
-            const Joined q = stat(i);
-            o += f32x4{lo[0], lo[1], hi[0], hi[1]} * part_factor(w, q.m, q.e);
-        }
-        finish(r, d, w, o);
+        if (r >= live_rows) break;
+        f32x4 o[kWaves];
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) o[i] = *reinterpret_cast<const f32x4 *>(&j.o[i][r][d]);
+        write(r, d, j.joined[r], (o[0] + o[1]) + (o[2] + o[3]));
     }
+}
+
+// Joins the parts of split tiles, in their order: a workgroup takes 1024 / D
+// rows, D / 4 threads a row, a launch of its own, since the last workgroup of a tile
+// to arrive would read them alone.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void join_tree_kernel(const TreeArgs a) {
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes, kParts = static_cast<int>(kTreeSplits), kEach = kParts / kLanes;
+    __shared__ float factor[kRows][kParts];
+    const int tid = threadIdx.x, lane = tid % kLanes, d = 4 * lane;
+    const uint32_t per = kTreeRows / kRows, job = blockIdx.x / per, heads = a.cache.kv_heads;
+    const uint32_t head = job % heads, tile = job / heads % a.tiles, i = job / heads / a.tiles;
+    const TreeJob parts = a.jobs[job];  // (of another call's where the sequence has no such tile)
+    const Seq s = draft_seq(a, i);
+    const int first_row = static_cast<int>(tile * kTreeRows), r = static_cast<int>(blockIdx.x % per) * kRows + tid / kLanes;
+    const int rows = s.ok ? s.count * static_cast<int>(a.group) : 0, here = min(rows - first_row, static_cast<int>(kTreeRows));
+    if (static_cast<int>(blockIdx.x % per) * kRows >= here) return;
+    const int splits = static_cast<int>(parts.splits);
+    if (splits <= 1) return;
+    const bool live = r < here;
+    const int at = live ? r : 0;
+    const auto load = [&](int p) {
+        return *(gptr_f32x4)(uintptr_t)(part_rows<D>(a, parts.first + static_cast<uint32_t>(min(p, splits - 1)) * heads) + static_cast<size_t>(at) * D + d);
+    };
+    // The first parts' rows are under way while the row's lanes, a part each or
+    // more, turn its statistics into the parts' factors.
+    constexpr int kBatch = 8;
+    f32x4 v[kBatch];
+#pragma unroll
+    for (int p = 0; p < kBatch; ++p) v[p] = load(p);
+    float m[kEach], l[kEach], e[kEach];
+    Joined w = {kNegInf, 0.0f, kNegInf};
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+        const int p = lane + x * kLanes;
+        m[x] = e[x] = kNegInf;
+        l[x] = 0.0f;
+        if (p < splits) {
+            const float *stat = part_stats<D>(a, parts.first + static_cast<uint32_t>(p) * heads) + at;
+            m[x] = stat[0];
+            l[x] = stat[kTreeRows];
+            e[x] = stat[2 * kTreeRows];
+        }
+        w.m = fmaxf(w.m, m[x]);
+    }
+    const auto most = [&](float x) {
+        x = fmaxf(x, dpp<kDppXor1>(x));
+        x = fmaxf(x, dpp<kDppXor2>(x));
+        x = fmaxf(x, dpp<kDppMirror8>(x));
+        x = fmaxf(x, dpp<kDppMirror16>(x));
+        return kLanes == 32 ? max_xor16(x) : x;
+    };
+    w.m = most(w.m);
+    const float ref = w.m == kNegInf ? 0.0f : w.m;
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) {
+        w.e = fmaxf(w.e, shifted_unit(ref, m[x], e[x]));
+        w.l += l[x] * __builtin_amdgcn_exp2f(m[x] - ref);
+    }
+    w.e = most(w.e);
+    w.l = lanes_sum<16>(w.l);
+    if (kLanes == 32) w.l = add_xor16(w.l);
+#pragma unroll
+    for (int x = 0; x < kEach; ++x) factor[tid / kLanes][lane + x * kLanes] = part_factor(ref, w.e, m[x], e[x]);
+    __syncthreads();
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p0 = 0; p0 < splits; p0 += kBatch) {
+#pragma unroll
+        for (int p = 0; p < kBatch; ++p)
+            if (p0 + p < splits) o += v[p] * factor[tid / kLanes][p0 + p];
+        if (p0 + kBatch < splits) {
+#pragma unroll
+            for (int p = 0; p < kBatch; ++p) v[p] = load(p0 + kBatch + p);
+        }
+    }
+    if (live) write_row<T>(a, s, head, first_row + r, d, w, o);
 }
 
 }  // namespace
 
-template <int SPLIT, int RW, typename T>
-static void launch_tree_as(const TreeArgs &a, hipStream_t stream) {
-    auto go = [&](auto kernel) { kernel<<<a.workgroups, kTreeThreads, 0, stream>>>(a); };
-    a.cache.head_dim == 64 ? go(attend_tree_kernel<64, SPLIT, RW, T>) : go(attend_tree_kernel<128, SPLIT, RW, T>);
-}
 template <int SPLIT, typename T>
 static void launch_tree_as(const TreeArgs &a, hipStream_t stream) {
-    a.row_waves == 1 ? launch_tree_as<SPLIT, 1, T>(a, stream)
-                     : a.row_waves == 2 ? launch_tree_as<SPLIT, 2, T>(a, stream) : launch_tree_as<SPLIT, 4, T>(a, stream);
+    auto go = [&](auto kernel) { kernel<<<a.workgroups, kTreeThreads, 0, stream>>>(a); };
+    a.cache.head_dim == 64 ? go(attend_tree_kernel<64, SPLIT, T>) : go(attend_tree_kernel<128, SPLIT, T>);
+    if (a.splits == 1) return;
+    const uint32_t jobs = a.batch.sequences * a.tiles * a.cache.kv_heads, rows = 1024 / a.cache.head_dim;
+    auto join = [&](auto kernel) { kernel<<<jobs * (kTreeRows / rows), 256, 0, stream>>>(a); };
+    a.cache.head_dim == 64 ? join(join_tree_kernel<64, T>) : join(join_tree_kernel<128, T>);
 }
 hipError_t launch_attend_tree(const TreeArgs &a, hipStream_t stream) {
     if (a.d.dtype == Q4RDNA_F32) launch_tree_as<2, float>(a, stream);

@@ -97,23 +97,19 @@ int attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, cons
     a.batch = *batch;
     a.d = d;
     a.group = d.q_heads / cache->kv_heads;
-    const int64_t sixteen = 16 / size_of(d.dtype);
-    a.wide = wide_rows(d.q, d.dtype, sixteen) && wide_rows(d.k, d.dtype, sixteen) && wide_rows(d.v, d.dtype, sixteen);
-    a.wide_out = wide_rows(d.out, d.dtype, 4);
     // The most rows (query token, query head) per kv head that a sequence has.
     const uint32_t most_rows = std::min(batch->max_tokens, batch->tokens) * a.group;
-    a.row_waves = most_rows <= 32 ? 1 : most_rows <= 64 ? 2 : 4;
-    const uint32_t rows = 32 * a.row_waves, block_waves = 4 / a.row_waves;
-    a.row_groups = (most_rows + rows - 1) / rows;
-    const uint64_t jobs = static_cast<uint64_t>(a.row_groups) * cache->kv_heads * batch->sequences;
+    a.tiles = (most_rows + kTreeRows - 1) / kTreeRows;
+    const uint64_t jobs = static_cast<uint64_t>(a.tiles) * cache->kv_heads * batch->sequences;
     const uint64_t most_units = (d.window == 0 ? batch->table_width
                                                : std::min<uint64_t>(batch->table_width, d.window / kKvBlock + 2)) + 1ull;
+    // A workgroup's worth for every CU.  (Two fit one in 16 bits, but with as many
+    // smaller parts 32 sequences take 65 us rather than 56, and five 17.9 rather
+    // than 17.4.  Nor are parts worth their scratch where tiles abound.)
     const uint32_t cus = cu_count(cache->device);
-    a.target = (d.dtype == Q4RDNA_F32 ? 1 : 2) * cus;
-    a.least = 2 * block_waves;
-    const bool split = most_units > a.least && batch->sequences <= kDealtSequences && jobs <= 64ull * cus &&
-                       jobs * most_units <= 0x7fffffffu;
-    a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>((most_units + a.least - 1) / a.least, 64) : 1);
+    a.target = cus;
+    const bool split = most_units > 4 && batch->sequences <= kDealtSequences && jobs <= 16ull * cus && jobs * most_units <= 0x7fffffffu;
+    a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>((most_units + 3) / 4, kTreeSplits) : 1);
     const uint64_t workgroups = split ? std::min(jobs + a.target, jobs * a.splits) : jobs;
     if (workgroups > most_workgroups(256))
         return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences of %u kv heads are too many for one call", batch->sequences, cache->kv_heads);
@@ -122,10 +118,11 @@ int attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, cons
     if (device.status() != Q4RDNA_OK) return device.status();
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (a.splits > 1) {
+        const size_t floats = workgroups * kTreeRows * (cache->head_dim + 3);
         Scratch scratch;
-        if ((rc = get_scratch(cache->device, s, workgroups * rows * (cache->head_dim + 3), jobs, &scratch)) != Q4RDNA_OK) return rc;
+        if ((rc = get_scratch(cache->device, s, floats + 2 * jobs, 0, &scratch)) != Q4RDNA_OK) return rc;
         a.partials = scratch.partials;
-        a.arrived = scratch.arrived;
+        a.jobs = reinterpret_cast<TreeJob *>(scratch.partials + floats);
     }
     return launched(launch_attend_tree(a, s), "kv_attend_tree");
 }

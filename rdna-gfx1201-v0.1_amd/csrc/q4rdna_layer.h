@@ -100,21 +100,25 @@ struct RotateArgs {
 };
 hipError_t launch_rotate(const RotateArgs &a, hipStream_t stream);
 
+// Rows (query token, query head of a kv head) of a workgroup of
+// attend_tree_kernel, a tile, and the most workgroups that share them.
+constexpr uint32_t kTreeRows = 32;
+constexpr uint32_t kTreeSplits = 64;
+struct TreeJob {
+    uint32_t first;   // workgroup of a tile's first part
+    uint32_t splits;
+};
 struct TreeArgs {
     q4rdna_kv_cache cache;
     q4rdna_kv_batch batch;
     q4rdna_kv_tree_desc d;
     uint32_t group;       // query heads per kv head
-    uint32_t row_waves;   // 1, 2 or 4 of a workgroup's waves have rows of their own, 32 each: a row group
-    uint32_t row_groups;  // of the largest sequence
-    uint32_t splits;      // the most workgroups that share a row group
-    uint32_t least;       // units (cached blocks, the drafts) of a part, the least
-    uint32_t target;      // workgroups to deal the units to
+    uint32_t tiles;       // of the largest sequence
+    uint32_t splits;      // the most workgroups that share a tile
+    uint32_t target;      // workgroups to deal the units (cached blocks, the drafts) to
     uint32_t workgroups;  // launched
-    uint32_t wide;        // rows of q, k and v can be read 16 bytes at a time
-    uint32_t wide_out;    // out rows can be written four elements at a time
-    float *partials;      // of each workgroup: [row][D], then all the maxima, sums and units, [row][3]
-    uint32_t *arrived;    // [sequence][row group][head], zero between launches
+    float *partials;      // of each workgroup [row][D], then of each [m, l, e][row]
+    TreeJob *jobs;        // [sequence][tile][head]
 };
 hipError_t launch_attend_tree(const TreeArgs &a, hipStream_t stream);
 
