@@ -920,11 +920,16 @@ def tree(batch: KVBatch, parents: torch.Tensor, positions: torch.Tensor | None =
     step = batch._of(shape[0])
     if positions is None:
         positions = torch.empty_like(parents)
+        positions_at = positions.data_ptr()
+    else:
+        positions_at = _plain(positions, "positions", torch.int32, shape, device)
     if seen is None:
         seen = torch.empty_like(parents, dtype=torch.int64)
-    to = _plain(positions, "positions", torch.int32, shape, device), _plain(seen, "seen", torch.int64, shape, device)
+        seen_at = seen.data_ptr()
+    else:
+        seen_at = _plain(seen, "seen", torch.int64, shape, device)
     s = _raw_stream(device) if stream is None else stream
-    _call(device, load().q4rdna_kv_tree, step, at, *to, s)
+    _call(device, load().q4rdna_kv_tree, step, at, positions_at, seen_at, s)
     return positions, seen
 
 
@@ -947,18 +952,26 @@ def rotate(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
         with _on_stream(stream, device):
             return rotate(q, k, positions, cos, sin, interleaved=interleaved, q_norm=q_norm, k_norm=k_norm, eps=eps,
                           q_out=q_out, k_out=k_out)
-    rows, to, heads = [_NO_ROWS, _NO_ROWS], [_NO_ROWS, _NO_ROWS], [0, 0]
-    outs = [q_out, k_out]
-    for i, (x, name, norm) in enumerate(((q, "q", q_norm), (k, "k", k_norm))):
-        if x is None:
-            if outs[i] is not None or norm is not None:
-                raise ValueError(f"{name}_out or {name}_norm without {name}")
-            continue
-        if x.dim() != 3:
-            raise ValueError(f"{name} must be [tokens, heads, head_dim]")
-        heads[i] = x.shape[1]
-        rows[i] = _rows(x, name, dtype, (tokens, heads[i], dim), device)
-        outs[i], to[i] = _out_rows(outs[i], name + "_out", x, device)
+    q_heads = k_heads = q_weight = k_weight = 0
+    q_rows = q_to = k_rows = k_to = _NO_ROWS
+    if q is not None:
+        q_heads = q.shape[1]
+        q_rows = _rows(q, "q", dtype, (tokens, q_heads, dim), device)
+        q_out, q_to = _out_rows(q_out, "q_out", q, device)
+        if q_norm is not None:
+            q_weight = _plain(q_norm, "q_norm", torch.float32, (dim,), device)
+    elif q_out is not None or q_norm is not None:
+        raise ValueError("q_out or q_norm without q")
+    if k is not None:
+        if k.dim() != 3:
+            raise ValueError("k must be [tokens, heads, head_dim]")
+        k_heads = k.shape[1]
+        k_rows = _rows(k, "k", dtype, (tokens, k_heads, dim), device)
+        k_out, k_to = _out_rows(k_out, "k_out", k, device)
+        if k_norm is not None:
+            k_weight = _plain(k_norm, "k_norm", torch.float32, (dim,), device)
+    elif k_out is not None or k_norm is not None:
+        raise ValueError("k_out or k_norm without k")
     at = cos_at = sin_at = table_rows = rotary = 0
     if cos is not None:
         table = cos.shape
@@ -970,13 +983,11 @@ def rotate(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
         table_rows, rotary = table[0], 2 * table[1]
     elif sin is not None:
         raise ValueError("sin without cos")
-    q_weight = 0 if q_norm is None else _plain(q_norm, "q_norm", torch.float32, (dim,), device)
-    k_weight = 0 if k_norm is None else _plain(k_norm, "k_norm", torch.float32, (dim,), device)
-    d = _lib.ROTATE.pack(_dtype(dtype), tokens, *heads, dim, table_rows, rotary, interleaved, *rows[0], *rows[1], *to[0], *to[1],
-                         at, cos_at, sin_at, q_weight, k_weight, eps, 0)
+    d = _lib.ROTATE.pack(_dtype(dtype), tokens, q_heads, k_heads, dim, table_rows, rotary, interleaved, *q_rows, *k_rows, *q_to,
+                         *k_to, at, cos_at, sin_at, q_weight, k_weight, eps, 0)
     s = _raw_stream(device) if stream is None else stream
     _call(device, load().q4rdna_rotate, d, s)
-    return tuple(outs)
+    return q_out, k_out
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor | None, count: int, out: tuple | None = None,
@@ -1004,14 +1015,18 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor | None, count: int, o
     scores_at = 0 if scores is None else _plain(scores, "scores", torch.float32, (groups, beams), device)
     if not 1 <= count <= min(_lib.BEAM_MAX_COUNT, beams * vocab):
         raise ValueError(f"count is {count}: 1 to {_lib.BEAM_MAX_COUNT}, and no more than there are continuations")
-    shape = (groups, count)
     if out is None:
-        ints = torch.empty((2, groups, count), dtype=torch.int32, device=logits.device)
-        out = torch.empty(shape, dtype=torch.float32, device=logits.device), ints[0], ints[1]
-    at = [_plain(t, name, dtype, shape, device) for t, name, dtype in zip(
-        out, ("out scores", "out rows", "out tokens"), (torch.float32, torch.int32, torch.int32), strict=True)]
+        # One allocation, 4 bytes a number in all three.
+        totals, rows, tokens = logits.new_empty((3, groups, count), dtype=torch.int32).unbind()
+        totals = totals.view(torch.float32)
+        at = totals.data_ptr(), rows.data_ptr(), tokens.data_ptr()
+    else:
+        totals, rows, tokens = out
+        shape = groups, count
+        at = (_plain(totals, "out scores", torch.float32, shape, device), _plain(rows, "out rows", torch.int32, shape, device),
+              _plain(tokens, "out tokens", torch.int32, shape, device))
     d = _lib.BEAM.pack(_dtype(logits.dtype), groups, beams, vocab, count, 0, logits.data_ptr(), group_stride, beam_stride,
                        scores_at, *at)
     s = _raw_stream(device) if stream is None else stream
     _call(device, load().q4rdna_beam_select, d, s)
-    return tuple(out)
+    return totals, rows, tokens
