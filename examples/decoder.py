@@ -3,9 +3,13 @@ rotation, attention over the 8-bit paged cache, norms with the residual add.
 
 Weights are random, in the shapes of Qwen3-8B by default.  A prompt goes
 through in steps of up to eight tokens (the batched products' limit), then
-tokens are decoded one by one, each step a replay of one captured HIP graph.
+tokens are decoded one by one, each step a replay of one captured HIP graph;
+with --beams along the best of several continuations; with --drafts up to seven
+guessed tokens are verified together with each one.
 
     python examples/decoder.py --layers 36 --prompt 100 --tokens 50
+    python examples/decoder.py --layers 36 --prompt 100 --tokens 50 --beams 4
+    python examples/decoder.py --layers 36 --prompt 100 --tokens 50 --drafts
 """
 from __future__ import annotations
 
@@ -34,10 +38,40 @@ class Shape:
     eps: float = 1e-6
 
 
-class Decoder:
-    """Random weights, one cache per layer, one sequence."""
+def lookup(history: list[int], most: int = 7, depth: int = 3) -> tuple[list[int], list[int]]:
+    """Guesses at what follows a history: what followed its last token before,
+    the latest first, as a tree of (tokens, parents); a parent of 0 is that last
+    token, i the i-th guess."""
+    tokens, parents, child = [], [], {}
+    for at in range(len(history) - 2, -1, -1):
+        if history[at] != history[-1]:
+            continue
+        node = 0
+        for t in history[at + 1:at + 1 + depth]:
+            if (node, t) not in child:
+                if len(tokens) == most:
+                    return tokens, parents
+                tokens.append(t)
+                parents.append(node)
+                child[node, t] = len(tokens)
+            node = child[node, t]
+    return tokens, parents
 
-    def __init__(self, shape: Shape, max_tokens: int, seed: int = 0, device: int = 0):
+
+class Drafts:
+    """A step's tokens that are not in the cache: where they stand, whom they
+    see, and their keys and values of each layer, unrotated."""
+
+    def __init__(self, batch: api.KVBatch, parents: torch.Tensor):
+        self.positions, self.seen = api.tree(batch, parents)
+        self.rows = []
+
+
+class Decoder:
+    """Random weights, one cache per layer; one sequence, or `beams` that fork
+    from it."""
+
+    def __init__(self, shape: Shape, max_tokens: int, seed: int = 0, device: int = 0, beams: int = 1):
         self.shape, self.device = shape, torch.device("cuda", device)
         gen = torch.Generator(device=self.device).manual_seed(seed)
 
@@ -56,9 +90,12 @@ class Decoder:
                        for _ in range(s.layers)]
         self.norm, self.head = weight(s.hidden), matrix(s.vocab, s.hidden)
         pages = (max_tokens + 63) // 64
-        self.caches = [api.KVCache.empty(pages, 1, s.kv_heads, s.head_dim, device) for _ in range(s.layers)]
-        self.table = torch.arange(pages, dtype=torch.int32, device=self.device)[None]
-        self.past = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.caches = [api.KVCache.empty(beams * pages, beams, s.kv_heads, s.head_dim, device) for _ in range(s.layers)]
+        self.beams, self.slots = beams, torch.arange(beams, dtype=torch.int32, device=self.device)
+        self.tables = torch.full((beams, pages), -1, dtype=torch.int32, device=self.device)
+        self.pasts = torch.zeros(beams, dtype=torch.int32, device=self.device)
+        self.table, self.past = self.tables[:1], self.pasts[:1]  # of the one sequence
+        self.table[0] = torch.arange(pages, dtype=torch.int32, device=self.device)
         angle = torch.arange(max_tokens, device=self.device).double()[:, None] * s.rope_base ** (
             -torch.arange(s.head_dim // 2, device=self.device).double() / (s.head_dim // 2))
         self.cos, self.sin = angle.cos().float(), angle.sin().float()
@@ -75,17 +112,24 @@ class Decoder:
                 api.mul_mat_batch(w, x, y)
         return ys
 
-    def forward(self, x: torch.Tensor, batch: api.KVBatch) -> torch.Tensor:
-        """Logits [n, vocab] of the step's n <= 8 embedded tokens [n, hidden]."""
+    def forward(self, x: torch.Tensor, batch: api.KVBatch, drafts: Drafts | None = None) -> torch.Tensor:
+        """Logits [n, vocab] of the step's n <= 8 embedded tokens [n, hidden],
+        which are appended to the caches, or are drafts."""
         s, n = self.shape, x.shape[0]
         h, y = x, None
         for layer, cache in zip(self.layers, self.caches):
             h, normed = api.add_norm(h, y, layer["norm1"], eps=s.eps)
             q, k, v = self._products(normed, layer["q"], layer["k"], layer["v"])
-            q = cache.append(batch, k.view(n, s.kv_heads, s.head_dim), v.view(n, s.kv_heads, s.head_dim),
-                             q=q.view(n, s.heads, s.head_dim), cos=self.cos, sin=self.sin, q_norm=layer["q_norm"],
-                             k_norm=layer["k_norm"], eps=s.eps)
-            attended = cache.attend(batch, q)
+            q, k, v = q.view(n, s.heads, s.head_dim), k.view(n, s.kv_heads, s.head_dim), v.view(n, s.kv_heads, s.head_dim)
+            if drafts is None:
+                q = cache.append(batch, k, v, q=q, cos=self.cos, sin=self.sin, q_norm=layer["q_norm"],
+                                 k_norm=layer["k_norm"], eps=s.eps)
+                attended = cache.attend(batch, q)
+            else:
+                drafts.rows.append((k, v))
+                q, k = api.rotate(q, k, drafts.positions, self.cos, self.sin, q_norm=layer["q_norm"],
+                                  k_norm=layer["k_norm"], eps=s.eps)
+                attended = cache.attend_tree(batch, q, k, v, drafts.seen)
             (y,) = self._products(attended.view(n, -1), layer["o"])
             h, normed = api.add_norm(h, y, layer["norm2"], eps=s.eps)
             inner = torch.empty((n, s.ffn), device=self.device)
@@ -106,11 +150,15 @@ class Decoder:
             n = len(ids)
             if self.length + n > self.max_tokens:
                 raise ValueError(f"more than {self.max_tokens} tokens")
-            cu = torch.tensor([0, n], dtype=torch.int32, device=self.device)
-            logits = self.forward(self.embedding[ids], api.KVBatch(self.past, self.table, cu_tokens=cu, max_tokens=n))
+            logits = self.forward(self.embedding[ids], self._step(n))
             self.past += n
             self.length += n
         return logits[-1]
+
+    def _step(self, n: int) -> api.KVBatch:
+        """A step of n tokens of the one sequence."""
+        cu = torch.tensor([0, n], dtype=torch.int32, device=self.device)
+        return api.KVBatch(self.past, self.table, cu_tokens=cu, slots=self.slots[:1], max_tokens=n)
 
     def decode(self, logits: torch.Tensor, count: int) -> tuple[list[int], float]:
         """Decode greedily from the given logits: (tokens, seconds a step).  The
@@ -120,11 +168,11 @@ class Decoder:
             raise ValueError(f"more than {self.max_tokens} tokens")
         if count == 0:
             return [], 0.0
-        batch = api.KVBatch(self.past, self.table)
-        token = logits.argmax().reshape(1)
+        batch = api.KVBatch(self.past, self.table, slots=self.slots[:1])
+        token = best(logits[None])
 
         def step():
-            return self.forward(self.embedding[token], batch)[0]
+            return best(self.forward(self.embedding[token], batch))
 
         stream = torch.cuda.Stream(self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
@@ -133,21 +181,113 @@ class Decoder:
         torch.cuda.current_stream(self.device).wait_stream(stream)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
-            logits = step()
+            token.copy_(step())
+            self.past += 1
         chosen = []
         torch.cuda.synchronize(self.device)
         began = time.perf_counter()
         for _ in range(count):
             chosen.append(token.clone())
             graph.replay()
-            # Outside the graph: torch's argmax over many logits sets memory
-            # that it counts in, and such a node must not be replayed.
-            token.copy_(logits.argmax())
-            self.past += 1
         torch.cuda.synchronize(self.device)
         spent = (time.perf_counter() - began) / count
         self.length += count
         return [int(t) for t in chosen], spent
+
+    def verify(self, tokens: list[int], parents: list[int]) -> tuple[torch.Tensor, Drafts]:
+        """Logits [n, vocab] after each of up to eight drafted tokens, a tree that
+        follows the cache: parents[i] is a place among them before i, or -1."""
+        if self.length + len(tokens) > self.max_tokens:
+            raise ValueError(f"more than {self.max_tokens} tokens")
+        batch = self._step(len(tokens))
+        drafts = Drafts(batch, torch.tensor(parents, dtype=torch.int32, device=self.device))
+        return self.forward(self.embedding[torch.tensor(tokens, device=self.device)], batch, drafts), drafts
+
+    def accept(self, drafts: Drafts, path: list[int]) -> None:
+        """Append the drafted tokens of a path from the cache's last token on."""
+        n, s, at = len(path), self.shape, torch.tensor(path, device=self.device)
+        batch = self._step(n)
+        for layer, cache, (k, v) in zip(self.layers, self.caches, drafts.rows):
+            cache.append(batch, k[at], v[at], cos=self.cos, sin=self.sin, k_norm=layer["k_norm"], eps=s.eps)
+        self.past += n
+        self.length += n
+
+    def speculate(self, history: list[int], logits: torch.Tensor, count: int, guess=lookup) -> tuple[list[int], int]:
+        """Decode greedily as decode() does, the tokens that `guess` expects
+        after each one (see lookup) verified with it: (tokens, steps)."""
+        if self.length + count > self.max_tokens:
+            raise ValueError(f"more than {self.max_tokens} tokens")
+        chosen, steps, token = [], 0, int(best(logits[None]))
+        while len(chosen) < count:
+            tokens, parents = guess(history + chosen + [token])
+            most = min(8, count - len(chosen))
+            tokens, parents = [token, *tokens][:most], [-1, *parents][:most]
+            logits, drafts = self.verify(tokens, parents)
+            after, path = best(logits).tolist(), [0]
+            while True:  # down the tree as long as a guess is the best token
+                wanted = [i for i, p in enumerate(parents) if p == path[-1] and tokens[i] == after[path[-1]]]
+                if not wanted:
+                    break
+                path.append(wanted[0])
+            self.accept(drafts, path)
+            chosen += [tokens[i] for i in path]
+            token, steps = after[path[-1]], steps + 1
+        return chosen, steps
+
+    def search(self, logits: torch.Tensor, count: int) -> tuple[list[list[int]], list[float], torch.Tensor]:
+        """The best `beams` continuations of `count` tokens that a beam search
+        finds: (tokens, scores), the best first, and the logits after that one,
+        from which the decoder goes on.  The first step aside, each is a replay of
+        one captured graph: the model's step, the choice, the fork."""
+        n = self.beams
+        if not 2 <= n <= 8:
+            raise ValueError("a search needs 2 to 8 beams")
+        if count < 1 or self.length + count > self.max_tokens:
+            raise ValueError(f"more than {self.max_tokens} tokens, or none")
+        batch = api.KVBatch(self.pasts, self.tables, slots=self.slots)
+        scores, rows, tokens = api.beam_select(logits.view(1, 1, -1), None, n)
+        batch.fork(rows[0], self.caches)  # all go on from sequence 0
+        chosen = [(rows.clone(), tokens.clone())]
+
+        def step():
+            logits = self.forward(self.embedding[tokens[0]], batch)
+            self.pasts.add_(1)
+            for new, old in zip(api.beam_select(logits[None], scores, n), (scores, rows, tokens)):
+                old.copy_(new)
+            batch.fork(rows[0], self.caches)
+
+        stream = torch.cuda.Stream(self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))
+        graph = None
+        for i in range(1, count):
+            if i == 1:
+                with torch.cuda.stream(stream):
+                    step()  # scratch grows here, not in the capture
+                torch.cuda.current_stream(self.device).wait_stream(stream)
+            else:
+                if graph is None:
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph, stream=stream):
+                        step()
+                graph.replay()
+            chosen.append((rows.clone(), tokens.clone()))
+        found = [[] for _ in range(n)]
+        up = list(range(n))
+        for rows_at, tokens_at in reversed(chosen):
+            r, t = rows_at[0].tolist(), tokens_at[0].tolist()
+            for i in range(n):
+                found[i].insert(0, t[up[i]])
+                up[i] = r[up[i]]
+        # The best one goes on alone, with pages for all that may follow.
+        self.length += count - 1
+        alone = torch.tensor([0] + [-1] * (n - 1), dtype=torch.int32, device=self.device)
+        batch.fork(alone, self.caches, room=self.max_tokens - self.length)
+        return found, scores[0].tolist(), self.prompt(found[0][-1:])
+
+
+def best(logits: torch.Tensor) -> torch.Tensor:
+    """The best token (int32) of each row."""
+    return api.beam_select(logits[:, None], None, 1)[2].view(-1)
 
 
 def main():
@@ -155,10 +295,24 @@ def main():
     ap.add_argument("--layers", type=int, default=36)
     ap.add_argument("--prompt", type=int, default=100, help="tokens of the (random) prompt")
     ap.add_argument("--tokens", type=int, default=50, help="tokens to decode")
+    ap.add_argument("--beams", type=int, default=1, help="search along so many continuations (up to 8)")
+    ap.add_argument("--drafts", action="store_true", help="verify guessed tokens with each one")
     a = ap.parse_args()
-    model = Decoder(Shape(layers=a.layers), a.prompt + a.tokens + 1)
+    model = Decoder(Shape(layers=a.layers), a.prompt + a.tokens + 1, beams=a.beams)
     ids = torch.randint(0, model.shape.vocab, (a.prompt,), generator=torch.Generator().manual_seed(1)).tolist()
-    tokens, spent = model.decode(model.prompt(ids), a.tokens)
+    logits = model.prompt(ids)
+    torch.cuda.synchronize()
+    began = time.perf_counter()
+    if a.beams > 1:
+        found, scores, _ = model.search(logits, a.tokens)
+        tokens, spent = found[0], (time.perf_counter() - began) / a.tokens
+        print("scores", [round(x, 3) for x in scores])
+    elif a.drafts:
+        tokens, steps = model.speculate(ids, logits, a.tokens)
+        spent = (time.perf_counter() - began) / a.tokens
+        print(f"{steps} steps")
+    else:
+        tokens, spent = model.decode(logits, a.tokens)
     print(f"{a.layers} layers, {a.prompt} + {a.tokens} tokens: {spent * 1e6:.1f} us a token ({1 / spent:.0f} tokens/s)")
     print("tokens", tokens[:10], "...", "cache faults", sum(c.faults() for c in model.caches))
 
