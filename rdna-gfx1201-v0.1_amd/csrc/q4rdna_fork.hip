@@ -38,10 +38,17 @@ __device__ __forceinline__ int room_end(const q4rdna_kv_fork_desc &d, int past) 
     return static_cast<int>(min(end, static_cast<uint64_t>(d.table_width)));
 }
 
+// Four entries of a row, at any of them.
+__device__ __forceinline__ i32x4 load_entries(const int32_t *p) {
+    typedef int32_t Four __attribute__((ext_vector_type(4), aligned(4)));
+    return *(__attribute__((address_space(1))) const Four *)(uintptr_t)p;
+}
+
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs a) {
     __shared__ int32_t parent[Q4RDNA_FORK_MAX_SEQUENCES], past[Q4RDNA_FORK_MAX_SEQUENCES];
     __shared__ int32_t first[Q4RDNA_FORK_MAX_SEQUENCES];  // the first that goes on from a sequence
     __shared__ int32_t vacant[Q4RDNA_FORK_MAX_SEQUENCES];  // slots of those that nobody goes on from
+    __shared__ int32_t old_past[Q4RDNA_FORK_MAX_SEQUENCES], old_slot[Q4RDNA_FORK_MAX_SEQUENCES];
     __shared__ uint32_t used[kForkPages / 32];
     __shared__ uint32_t totals[kPlanThreads / 64], copies, longest;
     const int tid = threadIdx.x, n = static_cast<int>(a.d.sequences), width = static_cast<int>(a.d.table_width);
@@ -50,16 +57,21 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs 
         if (a.faults != nullptr) atomicAdd(a.faults, 1u);
     };
     for (int w = tid; w < words; w += kPlanThreads) used[w] = 0;
-    for (int i = tid; i < n; i += kPlanThreads) first[i] = n;
+    for (int i = tid; i < n; i += kPlanThreads) {
+        first[i] = n;
+        parent[i] = a.d.parents[i];
+        old_past[i] = a.d.past[i];
+        old_slot[i] = a.d.slots[i];
+    }
     if (tid == 0) copies = longest = 0;
     __syncthreads();
     for (int i = tid; i < n; i += kPlanThreads) {
-        int p = a.d.parents[i], length = 0;
+        int p = parent[i], length = 0;
         if (p != -1) {
             bool ok = static_cast<uint32_t>(p) < static_cast<uint32_t>(n);
             if (ok) {
-                length = a.d.past[p];
-                ok = length >= 0 && length <= static_cast<int64_t>(width) * kBlock && static_cast<uint32_t>(a.d.slots[p]) < a.slot_count;
+                length = old_past[p];
+                ok = length >= 0 && length <= static_cast<int64_t>(width) * kBlock && static_cast<uint32_t>(old_slot[p]) < a.slot_count;
             }
             if (!ok) {
                 fault();
@@ -77,7 +89,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs 
         const int i = i0 + tid;
         const bool none = i < n && first[i] == n;
         const uint32_t at = base + threads_before(none, totals, &all);
-        if (none) vacant[at] = a.d.slots[i];
+        if (none) vacant[at] = old_slot[i];
         base += all;
     }
     __syncthreads();
@@ -88,7 +100,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs 
         const bool moved = i < n && (p < 0 || first[p] != i);
         const uint32_t at = later + threads_before(moved, totals, &all);
         later += all;
-        const int from = p >= 0 ? a.d.slots[p] : 0, slot = moved ? vacant[at] : from;
+        const int from = p >= 0 ? old_slot[p] : 0, slot = moved ? vacant[at] : from;
         if (p >= 0 && static_cast<uint32_t>(slot) >= a.slot_count) {
             fault();
             p = -1;
@@ -106,29 +118,56 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs 
         }
     }
     __syncthreads();
-    // The pages of full blocks, kEach entries of a thread in flight.
-    constexpr int kEach = 8;
-    const uint32_t columns = longest;
-    const uint64_t entries = static_cast<uint64_t>(n) * columns;
-    for (uint64_t e0 = tid; e0 < entries; e0 += kEach * kPlanThreads) {
-        int page[kEach];
+    // The pages of full blocks, each parent's once: four entries of a thread, kEach
+    // times in flight, 2^log2 threads a row.
+    constexpr int kEach = 4;
+    const int log2 = longest <= 4 ? 0 : 32 - __builtin_clz((longest - 1) / 4);
+    const uint64_t units = longest == 0 ? 0 : static_cast<uint64_t>(n) << log2;
+    for (uint64_t u0 = tid; u0 < units; u0 += kEach * kPlanThreads) {
+        i32x4 page[kEach];
+        int have[kEach];
 #pragma unroll
         for (int x = 0; x < kEach; ++x) {
-            const uint64_t e = e0 + static_cast<uint64_t>(x) * kPlanThreads;
-            page[x] = -1;
-            if (e < entries) {
-                const uint32_t i = entries >> 32 == 0 ? static_cast<uint32_t>(e) / columns : static_cast<uint32_t>(e / columns);
-                const int b = static_cast<int>(e - static_cast<uint64_t>(i) * columns);
-                if (b < past[i] / kBlock) page[x] = a.d.table[static_cast<size_t>(parent[i]) * width + b];
+            const uint64_t u = u0 + static_cast<uint64_t>(x) * kPlanThreads;
+            const int i = min(static_cast<int>(u >> log2), n - 1), b = 4 * static_cast<int>(u & ((1ull << log2) - 1));
+            const int p = parent[i], full = past[i] / kBlock;
+            have[x] = 0;
+            if (u < units && b < full && first[p] == i) {
+                const int at = max(min(b, width - 4), 0);  // within the row, some entries twice
+                const int32_t *row = a.d.table + static_cast<size_t>(p) * width + at;
+                have[x] = full - at;
+                if (width >= 4) page[x] = load_entries(row);
+                else page[x] = i32x4{row[0], row[width / 2], row[width - 1], 0};  // all of up to three
             }
         }
 #pragma unroll
-        for (int x = 0; x < kEach; ++x)
-            if (static_cast<uint32_t>(page[x]) < a.page_count) atomicOr(&used[page[x] / 32], 1u << (page[x] % 32));
+        for (int x = 0; x < kEach; ++x) {
+            uint32_t bits = 0, word = 0;  // neighbours often share a word: one atomic for them
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const uint32_t g = static_cast<uint32_t>(page[x][y]);
+                if (y >= have[x] || g >= a.page_count) continue;
+                if (bits != 0 && g / 32 != word) {
+                    atomicOr(&used[word], bits);
+                    bits = 0;
+                }
+                word = g / 32;
+                bits |= 1u << (g % 32);
+            }
+            if (bits != 0) atomicOr(&used[word], bits);
+        }
     }
     if (a.d.kept != nullptr)
-        for (uint32_t p = tid; p < a.page_count; p += kPlanThreads)
-            if (a.d.kept[p] != 0) atomicOr(&used[p / 32], 1u << (p % 32));
+        for (uint32_t p0 = tid; p0 < a.page_count; p0 += kEach * kPlanThreads) {
+            uint8_t kept[kEach];
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) kept[x] = a.d.kept[min(p0 + x * kPlanThreads, a.page_count - 1)];
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) {
+                const uint32_t p = min(p0 + x * kPlanThreads, a.page_count - 1);
+                if (kept[x] != 0) atomicOr(&used[p / 32], 1u << (p % 32));
+            }
+        }
     __syncthreads();
     uint32_t found = 0;
     for (int w0 = 0; w0 < words && found < given; w0 += kPlanThreads) {

@@ -189,3 +189,23 @@ def test_refusals(cuda):
     with pytest.raises(api.Q4RdnaError, match="share"):
         batch.fork(ok, caches + caches[:1])
     assert past.tolist() == [5, 6]
+
+
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 6, 7, 9])
+def test_rows_of_few_columns(cuda, width):
+    """Full to the last entry, or short of it; the last row ends where the table does."""
+    past = [64 * width, 64 * width - 1, 64 * (width - 1), 3, 64 * width]
+    for parents in ([0, 1, 2, 3, 4], [4, 4, 0, 1, 2], [4, 4, 4, 4, 4], [3, -1, 1, 0, 0]):
+        s = state(past, width, 6 * width + 1, 5, seed=width)
+        run(*s, parents, 64)
+        run(*s, [1, 0, 2, 4, 4], 64 * width)
+
+
+def test_kept_pages_of_a_large_cache(cuda):
+    """More marks than the workgroup reads at a time, the last one's included."""
+    pages = 20011
+    s = state([700, 64, 6400, 1], 200, pages, 4, seed=8)
+    kept = torch.rand(pages, generator=torch.Generator().manual_seed(9)).lt(0.9)
+    kept[-3:] = torch.tensor([False, True, True])
+    run(*s, [2, 2, 0, 1], 6000, kept=kept.cuda())
+    run(*s, [0, 1, 2, 3], 64, kept=kept.cuda())
