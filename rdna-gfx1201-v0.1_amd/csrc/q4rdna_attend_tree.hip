@@ -107,6 +107,21 @@ __device__ __forceinline__ h16x8 half_piece(i32x4 piece, int half) {
     return r;
 }
 
+// The same without the -1152: a code c is 1152 + c, exact in fp16.
+__device__ __forceinline__ h16x8 half_piece_biased(i32x4 piece, int half) {
+    union {
+        uint32_t w[4];
+        h16x8 h;
+    } r;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const uint32_t u = static_cast<uint32_t>(piece[2 * half + x]) ^ 0x80808080u;
+        r.w[2 * x] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+        r.w[2 * x + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    }
+    return r.h;
+}
+
 // Operands of the two products out of raw tiles.
 template <bool LOW, int D>
 __device__ __forceinline__ h16x8 k_fragment(const TreeRaw<D> &r, int t, int f) { return half_piece<LOW>(r.x[t * (D / 32) + f / 2], f % 2); }
@@ -154,11 +169,24 @@ __device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (
         }
     }
 }
-__device__ __forceinline__ void clear(f32x16 (&s)[2]) {
+__device__ __forceinline__ void clear(f32x16 (&s)[2], float to = 0.0f) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+        for (int i = 0; i < 16; ++i) s[t][i] = to;
+}
+// -1152 times the sum of the lane's row of q.
+template <int D>
+__device__ __forceinline__ float k_bias(const ManyState<D, 1> &st) {
+    h16x8 bias;
+    f32x16 sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bias[e] = static_cast<_Float16>(-1152.0f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
+#pragma unroll
+    for (int f = 0; f < D / 16; ++f) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(bias, st.q[f][0], sum, 0, 0, 0);
+    return sum[0];
 }
 // All ones where bit i is set.  (As an instruction of its own: the compiler would
 // make a compare of it, and 32 of them would each hold a pair of scalar registers.)
@@ -662,12 +690,21 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
         }
         return bits;
     };
+    // With one part of q the codes of K go in as 1152 + c and the products start
+    // at -1152 sum q, which saves an instruction for two codes.  What that costs:
+    // roundings of sums up to 1152 |sum q| instead of |sum q c|, a few 2^-24 of
+    // them, 2^-17 of |c| |sum q| or less; q itself and the weights have 11 bits.
+    float bias = 0.0f;
+    if constexpr (SPLIT == 1) bias = k_bias(st);
     // A full block; `masked` ones are the first of a window's.
     const auto block = [&](int n, auto masked) {
         const float nan = __builtin_nanf("");
         const float k_scale = good_next ? scale_next[0] : nan, v_scale = good_next ? scale_next[1] : nan;
-        clear(sc);
-        add_scores(st, sc, [&](int t, int f) { return k_fragment<false>(ka, t, f); });
+        clear(sc, bias);
+        add_scores(st, sc, [&](int t, int f) {
+            if constexpr (SPLIT == 1) return half_piece_biased(ka.x[t * (D / 32) + f / 2], f % 2);
+            else return k_fragment<false>(ka, t, f);
+        });
         tile_end();
         if (n + 1 < full) {
             good_next = next(n + 1);
