@@ -52,7 +52,7 @@ __device__ __forceinline__ int v_place(int row, int at) { return row * kBlock + 
 template <int D, int SPLIT>
 struct TreeStage {
     TreeTile<D> part[SPLIT];
-    float k_scale[kKvBlock], v_scale[kKvBlock];
+    float scales[2 * kKvBlock];  // K's, V's
 };
 // Parts of one row joined: its maximum m, the accumulators' exponent e (a whole
 // number) and its sum l, in units of 2^(m - 7).
@@ -72,23 +72,59 @@ template <int D>
 struct TreeRaw {
     i32x4 x[D / 16];
 };
+// (Buffer loads: their base is in scalar registers, so that all of them share
+// one vector register of offsets and need no vector instruction.)
+struct Tile {
+    __amdgpu_buffer_rsrc_t at;
+};
+__device__ __forceinline__ Tile tile_at(const int8_t *p, uint32_t bytes) {
+    return Tile{__builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(p), 0, static_cast<int>(bytes), 0x00020000)};
+}
+// 16 (8) bytes of a lane, `at` + c on, c a constant.
+__device__ __forceinline__ i32x4 load_piece(const Tile &tile, uint32_t at, uint32_t c) {
+    return __builtin_amdgcn_raw_buffer_load_b128(tile.at, at, c, 0);
+}
+typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ i32x2 load_half_piece(const Tile &tile, uint32_t at, uint32_t c) {
+    return __builtin_amdgcn_raw_buffer_load_b64(tile.at, at, c, 0);
+}
 template <int D>
-__device__ __forceinline__ void load_k(TreeRaw<D> &r, const int8_t *tile) {
-    const int lane = threadIdx.x & 63;
-    const int8_t *p = tile + (lane & 31) / 16 * (D / 64 * 1024) + (lane >> 5) * 256 + (lane & 15) * 16;
+__device__ __forceinline__ void load_k(TreeRaw<D> &r, const Tile &tile) {
+    const uint32_t lane = threadIdx.x & 63, at = (lane & 31) / 16 * (D / 64 * 1024) + (lane >> 5) * 256 + (lane & 15) * 16;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) r.x[t * (D / 32) + x] = load16(p + t * (D / 64 * 2048) + x / 2 * 1024 + x % 2 * 512);
+        for (int x = 0; x < D / 32; ++x) r.x[t * (D / 32) + x] = load_piece(tile, at, t * (D / 64 * 2048) + x / 2 * 1024 + x % 2 * 512);
 }
 template <int D>
-__device__ __forceinline__ void load_v(TreeRaw<D> &r, const int8_t *tile) {
-    const int lane = threadIdx.x & 63;
-    const int8_t *p = tile + (lane & 31) / 16 * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
+__device__ __forceinline__ void load_v(TreeRaw<D> &r, const Tile &tile) {
+    const uint32_t lane = threadIdx.x & 63, at = (lane & 31) / 16 * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) r.x[d * 2 + y] = load16(p + d * 2048 + y * 512);
+        for (int y = 0; y < 2; ++y) r.x[d * 2 + y] = load_piece(tile, at, kBlock * D + d * 2048 + y * 512);
+}
+// Of the open block's half `which`: K's planes of high and low bytes one behind the
+// other, and of V's eight tokens of each of the two in one piece.
+template <int D>
+__device__ __forceinline__ void load_open_k(TreeRaw<D> &r, const Tile &planes, uint32_t which) {
+    const uint32_t lane = threadIdx.x & 63, at = (lane & 31) / 16 * (D / 64 * 1024) + (lane >> 5) * 256 + (lane & 15) * 16 + which * (D / 64 * 2048);
+#pragma unroll
+    for (int low = 0; low < 2; ++low)
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) r.x[low * (D / 32) + x] = load_piece(planes, at, low * (kBlock * D) + x / 2 * 1024 + x % 2 * 512);
+}
+template <int D>
+__device__ __forceinline__ void load_open_v(TreeRaw<D> &r, const Tile &planes, uint32_t which) {
+    const uint32_t lane = threadIdx.x & 63, at = (lane & 31) / 16 * 1024 + (lane >> 5) * 256 + (lane & 15) * 16 + 8 * which;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const i32x2 high = load_half_piece(planes, at, 2 * kBlock * D + d * 2048 + y * 512);
+            const i32x2 low = load_half_piece(planes, at, 3 * kBlock * D + d * 2048 + y * 512);
+            r.x[d * 2 + y] = i32x4{high[0], high[1], low[0], low[1]};
+        }
 }
 // Half of 16 codes as fp16, times 2^-8 where they are low bytes.
 template <bool LOW>
@@ -129,12 +165,10 @@ template <bool LOW, int D>
 __device__ __forceinline__ h16x8 v_fragment(const TreeRaw<D> &r, int d, int y, int pair) { return half_piece<LOW>(r.x[d * 2 + y], pair); }
 
 // s[t] += the products of K's fragments (32 tokens t, 16 numbers f) with the rows.
-// `more`: there are tokens in the second 32.
-template <int D, int SPLIT, typename K>
-__device__ __forceinline__ void add_scores(const ManyState<D, SPLIT> &st, f32x16 (&s)[2], K fragment, bool more = true) {
+template <int N, int D, int SPLIT, typename K>
+__device__ __forceinline__ void add_scores(const ManyState<D, SPLIT> &st, f32x16 (&s)[N], K fragment) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        if (t == 1 && !more) return;
+    for (int t = 0; t < N; ++t) {
 #pragma unroll
         for (int f = 0; f < D / 16; ++f) {
             const h16x8 k = fragment(t, f);
@@ -144,34 +178,33 @@ __device__ __forceinline__ void add_scores(const ManyState<D, SPLIT> &st, f32x16
     }
 }
 // o += the products of V's fragments (32 numbers d; tokens 16 a + 8 y + 4 half + b,
-// a = 2 pair, 2 pair + 1) with the weights.
-template <int D, int SPLIT, typename V>
-__device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (&s)[2], V fragment, bool more = true) {
+// a = 2 t, 2 t + 1) with the weights.
+template <int N, int D, int SPLIT, typename V>
+__device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (&s)[N], V fragment) {
 #pragma unroll
-    for (int pair = 0; pair < 2; ++pair) {
-        if (pair == 1 && !more) return;
+    for (int t = 0; t < N; ++t) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             h16x8 p[SPLIT];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int eight = 2 * (2 * pair + e / 4) + y;
-                const float w = s[eight / 4][4 * (eight % 4) + e % 4];
+                const float w = s[t][4 * (2 * (e / 4) + y) + e % 4];
                 p[0][e] = static_cast<_Float16>(w);
                 if (SPLIT == 2) p[SPLIT - 1][e] = static_cast<_Float16>(w - static_cast<float>(p[0][e]));
             }
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
-                const h16x8 v = fragment(d, y, pair);
+                const h16x8 v = fragment(d, y, t);
 #pragma unroll
                 for (int x = 0; x < SPLIT; ++x) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], st.o[d], 0, 0, 0);
             }
         }
     }
 }
-__device__ __forceinline__ void clear(f32x16 (&s)[2], float to = 0.0f) {
+template <int N>
+__device__ __forceinline__ void clear(f32x16 (&s)[N], float to = 0.0f) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < N; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[t][i] = to;
 }
@@ -192,36 +225,44 @@ __device__ __forceinline__ float k_bias(const ManyState<D, 1> &st) {
 // make a compare of it, and 32 of them would each hold a pair of scalar registers.)
 __device__ __forceinline__ uint32_t bit_ones(uint32_t bits, int i) { return static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), i, 1)); }
 // `instead` where a bit is clear.
-__device__ __forceinline__ void hide(f32x16 (&s)[2], uint32_t seen, float instead) {
+template <int N>
+__device__ __forceinline__ void hide(f32x16 (&s)[N], uint32_t seen, float instead) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < N; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint32_t m = bit_ones(seen, 16 * t + i);
             s[t][i] = __uint_as_float((__float_as_uint(s[t][i]) & m) | (__float_as_uint(instead) & ~m));
         }
 }
-// The largest and the sum of the lane's 32 numbers, four chains of them side by side.
-__device__ __forceinline__ float largest(const f32x16 (&s)[2]) {
-    float top[4] = {s[0][0], s[0][8], s[1][0], s[1][8]};
+// The largest and the sum of the lane's numbers, four chains of them side by side.
+template <int N>
+__device__ __forceinline__ float largest(const f32x16 (&s)[N]) {
+    float top[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) top[x] = s[x * N / 4][4 * N * x % 16];
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top[x] = fmaxf(top[x], s[x / 2][8 * (x % 2) + i]);
+        for (int i = 1; i < 4 * N; ++i) top[x] = fmaxf(top[x], s[x * N / 4][4 * N * x % 16 + i]);
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
-__device__ __forceinline__ float total(const f32x16 (&s)[2]) {
-    float sum[4] = {s[0][0], s[0][8], s[1][0], s[1][8]};
+template <int N>
+__device__ __forceinline__ float total(const f32x16 (&s)[N]) {
+    float sum[4];
 #pragma unroll
-    for (int i = 1; i < 8; ++i)
+    for (int x = 0; x < 4; ++x) sum[x] = s[x * N / 4][4 * N * x % 16];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sum[x] += s[x / 2][8 * (x % 2) + i];
+    for (int i = 1; i < 4 * N; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum[x] += s[x * N / 4][4 * N * x % 16 + i];
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 // Scores to weights: s = 2^(s * unit + shift), zero where hidden; their sum.
-__device__ __forceinline__ float exponentials(f32x16 (&s)[2], float unit, float shift, uint32_t seen, bool masked) {
+template <int N>
+__device__ __forceinline__ float exponentials(f32x16 (&s)[N], float unit, float shift, uint32_t seen, bool masked) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < N; ++t)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unit, shift));
     if (masked) hide(s, seen, 0.0f);
@@ -246,15 +287,16 @@ __device__ __forceinline__ void soften_block(ManyState<D, SPLIT> &st, f32x16 (&s
     const float sum = exponentials(s, unit, kWeight - (st.m == kNegInf ? 0.0f : st.m) + ratio, seen, masked);
     st.l += sum * __builtin_amdgcn_exp2f(-ratio);
 }
-// The same with scales per token: `unit_log` is 8 for 16-bit codes, whose tiles
-// are in units of 256 times the scales.
-template <int D, int SPLIT, typename Scales>
-__device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&s)[2], int unit_log, uint32_t seen, Scales scales) {
+// The same of 32 tokens with a scale each, K's and 64 further on V's, the lane's
+// own four at a time; `unit_log` is 8 for 16-bit codes, whose tiles are in units
+// of 256 times the scales.
+template <int D, int SPLIT>
+__device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&s)[1], int unit_log, uint32_t seen, const float *scales) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-        const f32x4 kt = scales(0, x);
+    for (int x = 0; x < 4; ++x) {
+        const f32x4 kt = *reinterpret_cast<const f32x4 *>(scales + 8 * x);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) s[x / 4][4 * (x % 4) + b] *= kt[b];
+        for (int b = 0; b < 4; ++b) s[0][4 * x + b] *= kt[b];
     }
     hide(s, seen, kNegInf);
     const float unit = __builtin_amdgcn_ldexpf(st.q_scale, unit_log), top = max_xor32(largest(s));
@@ -264,10 +306,10 @@ __device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&
     const float m = now > st.m + kLazy ? now : st.m;
     const float sum = exponentials(s, unit, m == kNegInf ? 0.0f : -m, seen, true);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-        const f32x4 vt = scales(1, x);
+    for (int x = 0; x < 4; ++x) {
+        const f32x4 vt = *reinterpret_cast<const f32x4 *>(scales + kBlock + 8 * x);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) s[x / 4][4 * (x % 4) + b] *= vt[b] + (vt[b] - vt[b]);  // an infinite scale is made NaN
+        for (int b = 0; b < 4; ++b) s[0][4 * x + b] *= vt[b] + (vt[b] - vt[b]);  // an infinite scale is made NaN
     }
     hide(s, seen, 0.0f);
     refer(st, now, m + __builtin_amdgcn_logf(max_xor32(fmaxf(largest(s), 0.0f))) + static_cast<float>(unit_log));
@@ -275,9 +317,7 @@ __device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&
     // From units of 2^(m + unit_log) to the accumulators'.
     const int up = st.e == kNegInf ? 0 : unit_log + static_cast<int>(kWeight) - static_cast<int>(st.e);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_ldexpf(s[t][i], up);
+    for (int i = 0; i < 16; ++i) s[0][i] = __builtin_amdgcn_ldexpf(s[0][i], up);
 }
 
 // Numbers as they lie in memory, N side by side at any alignment: they become
@@ -381,7 +421,7 @@ __device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const D
             const int up = finite && top != 0 ? min(14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 110) : 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[which][b][e] = finite ? __builtin_amdgcn_ldexpf(x[which][b][e], up) : 0.0f;
-            if (octet == 0) (which == 0 ? stage.k_scale : stage.v_scale)[4 * quad + b] = finite ? __builtin_amdgcn_ldexpf(1.0f, -up) : __builtin_nanf("");
+            if (octet == 0) stage.scales[which * kBlock + 4 * quad + b] = finite ? __builtin_amdgcn_ldexpf(1.0f, -up) : __builtin_nanf("");
         }
     typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -433,7 +473,8 @@ __device__ __forceinline__ int first_block(const TreeArgs &a, int past) {
 }
 
 // What a sequence's workgroups take: each tile of 32 rows of each head is cut into
-// parts of about `chunk` of its units, the cached blocks and the drafts.
+// parts of about `chunk` of its units: full blocks of the cache, 32 tokens of the
+// open one, 32 drafts.
 struct TreeWork {
     Seq s;
     uint32_t jobs, units;
@@ -444,7 +485,7 @@ __device__ __forceinline__ TreeWork tree_work(const TreeArgs &a, uint32_t i) {
     w.s = draft_seq(a, min(i, a.batch.sequences - 1));
     if (i >= a.batch.sequences || !w.s.ok || w.s.count == 0) return w;
     w.jobs = (w.s.count * a.group + kTreeRows - 1) / kTreeRows * a.cache.kv_heads;
-    w.units = (w.s.past + kBlock - 1) / kBlock - first_block(a, w.s.past) + 1;
+    w.units = w.s.past / kBlock - first_block(a, w.s.past) + (w.s.past % kBlock + 31) / 32 + (w.s.count + 31) / 32;
     return w;
 }
 // (A part has a unit for every wave.)
@@ -570,18 +611,17 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     const int first_row = static_cast<int>(it.tile * kTreeRows);
     if (first_row >= rows) return;
     const int live_rows = min(static_cast<int>(kTreeRows), rows - first_row);
-    // Units: the cached blocks from block0 on, full ones, then the open one, then the drafts.
+    // Units: full blocks from block0 on, the halves of the open one, those of the
+    // drafts.  These four go to different waves.
     const int block0 = first_block(a, s.past), full_blocks = s.past / kBlock;
-    const int units = (s.past + kBlock - 1) / kBlock - block0 + 1;
+    const int opens = full_blocks, drafts = opens + (s.past % kBlock + 31) / 32, units = drafts + (s.count + 31) / 32 - block0;
     const int splits = min(it.splits, units), split = it.split;
     if (split >= splits) return;
     if (a.splits > 1 && split == 0 && tid == 0)
         a.jobs[(static_cast<size_t>(it.seq) * a.tiles + it.tile) * a.cache.kv_heads + head] = TreeJob{it.first, static_cast<uint32_t>(splits)};
     const int from = block0 + static_cast<int>(mul_div(split, units, splits));
     const int to = block0 + static_cast<int>(mul_div(split + 1, units, splits));
-    const int drafts = block0 + units - 1;
     const bool has_drafts = drafts < to;
-    const auto mine = [&](int unit) { return unit >= from && unit < to && (unit - from) % kWaves == wave; };
 
     // Everything that depends on the item alone is under way first.  The wave's
     // full blocks: from + wave + 4 n.  Lane x keeps the page of the x-th of
@@ -589,10 +629,13 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     const int32_t *table = a.batch.table + static_cast<size_t>(it.seq) * a.batch.table_width;
     const int start = from + wave, full_to = min(to, full_blocks);
     const int full = full_to > start ? (full_to - start + kWaves - 1) / kWaves : 0;
-    const bool open_mine = s.past % kBlock != 0 && mine(full_blocks), drafts_mine = mine(drafts);
+    int unit = max(opens, from);  // the wave's own of those of 32 tokens
+    unit += (from + wave - unit) & (kWaves - 1);
+    const bool open_mine = unit < min(to, drafts), drafts_mine = unit >= drafts && unit < to;
+    const int which = open_mine ? unit - opens : unit - drafts;  // half
     int pages = 0;
     if (full > 0) pages = table[min(start + kWaves * lane, full_to - 1)];
-    const int8_t *planes = a.cache.open + open_tile(a.cache, s.slot, full_blocks, head);
+    const Tile planes = tile_at(a.cache.open + open_tile(a.cache, s.slot, full_blocks, head), 4 * kBlock * D);
     f32x2 open_scale = {0.0f, 0.0f};
     if (open_mine) {
         const float *scales = a.cache.open_scales + open_scale_row(a.cache, s.slot, full_blocks, head);
@@ -610,9 +653,9 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     const int8_t *head_pages = a.cache.pages + head * (2 * kPlane);
     const float *head_scales = a.cache.scales + 2 * head;
     const uint32_t page_bytes = a.cache.kv_heads * static_cast<uint32_t>(2 * kPlane), page_count = a.cache.page_count;
-    TreeRaw<D> ka, vb;  // K and V of a full block, or K's (V's) high and low bytes of the open one
+    TreeRaw<D> ka, vb;  // K and V of a full block, or K's high and low bytes, V's of the open one's half
     f32x2 scale_next = {0.0f, 0.0f};
-    const int8_t *tile = nullptr;
+    Tile tile = planes;
     const auto check_pages = [&](int n) {
         if (static_cast<uint32_t>(pages) >= page_count) {
             if (n + lane < full) count_fault(a.cache);
@@ -625,7 +668,7 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
             check_pages(n);
         }
         const int page = __builtin_amdgcn_readlane(pages, n % 64), safe = max(page, 0);
-        tile = head_pages + static_cast<size_t>(static_cast<uint32_t>(safe)) * page_bytes;
+        tile = tile_at(head_pages + static_cast<size_t>(static_cast<uint32_t>(safe)) * page_bytes, 2 * kBlock * D);
         scale_next = *(gptr_f32x2)(uintptr_t)(head_scales + static_cast<size_t>(static_cast<uint32_t>(safe)) * (2 * a.cache.kv_heads));
         return page >= 0;
     };
@@ -634,10 +677,10 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
         check_pages(0);
         good_next = next(0);
         load_k(ka, tile);
-        load_v(vb, tile + kPlane);
+        load_v(vb, tile);
     } else if (open_mine) {
-        load_k(ka, planes);
-        load_k(vb, planes + kPlane);
+        load_open_k(ka, planes, which);
+        load_open_v(vb, planes, which);
     }
     tile_end();
     ManyState<D, SPLIT> st;
@@ -654,7 +697,8 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
         __syncthreads();
     }
 
-    f32x16 sc[2];
+    // Of the half of the drafts that is the wave's, in the order of its scores.
+    uint32_t drafts_seen = 0;
     if (drafts_mine) {
         if (a.d.window != 0 && a.d.window < 64) {  // drafted tokens that lie too far above
             const int depth = st.position - (s.past - 1);
@@ -662,23 +706,9 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
             for (int j = 0; j < s.count; ++j)
                 if (__builtin_amdgcn_readlane(depths, j) + static_cast<int>(a.d.window) <= depth) seen &= ~(1ull << j);
         }
-        uint32_t bits = 0;
+        const uint32_t of = static_cast<uint32_t>(seen >> (32 * which));
 #pragma unroll
-        for (int x = 0; x < 8; ++x) bits |= (static_cast<uint32_t>(seen >> (8 * x + 4 * half)) & 15u) << (4 * x);
-        clear(sc);
-#pragma unroll
-        for (int part = 0; part < SPLIT; ++part)
-            add_scores(st, sc, [&](int t, int f) {
-                return *reinterpret_cast<const h16x8 *>(shared.stage.part[part].k + (32 * t + column) * (D + 8) + fragment_number(f, half));
-            }, s.count > 32);
-        soften_tokens(st, sc, 0, bits, [&](int which, int x) {
-            return *reinterpret_cast<const f32x4 *>((which == 0 ? shared.stage.k_scale : shared.stage.v_scale) + 8 * x + 4 * half);
-        });
-#pragma unroll
-        for (int part = 0; part < SPLIT; ++part)
-            add_rows(st, sc, [&](int d, int y, int pair) {
-                return *reinterpret_cast<const h16x8 *>(shared.stage.part[part].v + v_place(32 * d + column, 32 * half + 16 * y + 8 * pair));
-            }, s.count > 32);
+        for (int x = 0; x < 4; ++x) drafts_seen |= (of >> (8 * x + 4 * half) & 15u) << (4 * x);
     }
     // Of the lane's 32 tokens of a block, in the order of its scores: those cached and within the window.
     const auto seen_from = [&](int first) {
@@ -698,6 +728,7 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     if constexpr (SPLIT == 1) bias = k_bias(st);
     // A full block; `masked` ones are the first of a window's.
     const auto block = [&](int n, auto masked) {
+        f32x16 sc[2];
         const float nan = __builtin_nanf("");
         const float k_scale = good_next ? scale_next[0] : nan, v_scale = good_next ? scale_next[1] : nan;
         clear(sc, bias);
@@ -710,15 +741,15 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
             good_next = next(n + 1);
             load_k(ka, tile);
         } else if (open_mine) {
-            load_k(ka, planes);
+            load_open_k(ka, planes, which);
         }
         tile_end();
         soften_block(st, sc, k_scale, v_scale, masked ? seen_from((start + kWaves * n) * kBlock) : 0xffffffffu, masked);
         tile_end();
         add_rows(st, sc, [&](int d, int y, int pair) { return v_fragment<false>(vb, d, y, pair); });
         tile_end();
-        if (n + 1 < full) load_v(vb, tile + kPlane);
-        else if (open_mine) load_k(vb, planes + kPlane);
+        if (n + 1 < full) load_v(vb, tile);
+        else if (open_mine) load_open_v(vb, planes, which);
         tile_end();
     };
     int n = 0;
@@ -726,20 +757,36 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
         for (; n < full && static_cast<int64_t>(s.past) + 63 - (start + kWaves * n) * kBlock >= static_cast<int64_t>(a.d.window); ++n)
             block(n, std::true_type());
     for (; n < full; ++n) block(n, std::false_type());
-    if (open_mine) {
-        const bool more = s.past % kBlock > 32;
+    // Half of the open block or of the drafts.
+    if (open_mine || drafts_mine) {
+        f32x16 sc[1];
         clear(sc);
-        add_scores(st, sc, [&](int t, int f) { return k_fragment<false>(ka, t, f); }, more);
-        add_scores(st, sc, [&](int t, int f) { return k_fragment<true>(vb, t, f); }, more);
-        tile_end();
-        load_v(ka, planes + 2 * kPlane);
-        load_v(vb, planes + 3 * kPlane);
-        tile_end();
-        soften_tokens(st, sc, 8, seen_from(full_blocks * kBlock), [&](int which, int x) {
-            return *reinterpret_cast<const f32x4 *>(&open_scales[wave][kBlock * which + 8 * x + 4 * half]);
-        });
-        add_rows(st, sc, [&](int d, int y, int pair) { return v_fragment<false>(ka, d, y, pair); }, more);
-        add_rows(st, sc, [&](int d, int y, int pair) { return v_fragment<true>(vb, d, y, pair); }, more);
+        uint32_t bits = drafts_seen;
+        const float *scales;
+        if (open_mine) {
+            add_scores(st, sc, [&](int, int f) { return half_piece<false>(ka.x[f / 2], f % 2); });
+            add_scores(st, sc, [&](int, int f) { return half_piece<true>(ka.x[D / 32 + f / 2], f % 2); });
+            bits = seen_from(full_blocks * kBlock) >> (16 * which);
+            scales = open_scales[wave];
+        } else {
+#pragma unroll
+            for (int part = 0; part < SPLIT; ++part)
+                add_scores(st, sc, [&](int, int f) {
+                    return *reinterpret_cast<const h16x8 *>(shared.stage.part[part].k + (32 * which + column) * (D + 8) + fragment_number(f, half));
+                });
+            scales = shared.stage.scales;
+        }
+        soften_tokens(st, sc, open_mine ? 8 : 0, bits, scales + 32 * which + 4 * half);
+        if (open_mine) {
+            add_rows(st, sc, [&](int d, int y, int) { return half_piece<false>(vb.x[d * 2 + y], 0); });
+            add_rows(st, sc, [&](int d, int y, int) { return half_piece<true>(vb.x[d * 2 + y], 1); });
+        } else {
+#pragma unroll
+            for (int part = 0; part < SPLIT; ++part)
+                add_rows(st, sc, [&](int d, int y, int) {
+                    return *reinterpret_cast<const h16x8 *>(shared.stage.part[part].v + v_place(32 * d + column, 32 * half + 16 * y + 8 * which));
+                });
+        }
     }
 
     const float l = add_xor32(st.l);
