@@ -455,10 +455,14 @@ __device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const D
 // One sequence of a step: as seq_of, but its tokens are not in the cache.
 __device__ __forceinline__ Seq draft_seq(const TreeArgs &a, uint32_t i) {
     Seq s;
-    s.first = a.batch.cu_tokens ? a.batch.cu_tokens[i] : static_cast<int>(i);
-    const int end = a.batch.cu_tokens ? a.batch.cu_tokens[i + 1] : static_cast<int>(i) + 1;
+    // (Loads without branches: what is not there is read from past.)
+    const bool starts = a.batch.cu_tokens != nullptr, slots = a.batch.slots != nullptr;
+    const int32_t *from = starts ? a.batch.cu_tokens : a.batch.past;
+    const int first = from[i], last = from[starts ? i + 1 : i], slot = (slots ? a.batch.slots : a.batch.past)[i];
     s.past = a.batch.past[i];
-    s.slot = a.batch.slots ? a.batch.slots[i] : static_cast<int>(i);
+    s.first = starts ? first : static_cast<int>(i);
+    const int end = starts ? last : static_cast<int>(i) + 1;
+    s.slot = slots ? slot : static_cast<int>(i);
     s.ok = s.first >= 0 && end >= s.first && static_cast<uint32_t>(end) <= a.batch.tokens;
     s.count = s.ok ? end - s.first : 0;
     const int64_t room = static_cast<int64_t>(a.batch.table_width) * kBlock;
@@ -503,17 +507,17 @@ struct TreeItem {
 };
 // The item of workgroup x: the device knows the lengths, the host does not, so
 // every wave adds up the sequences' parts, 64 at a time.
-__device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a, uint32_t x) {
+__device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a) {
+    const uint32_t x = blockIdx.x;
     TreeItem it;
     it.seq = -1;
     const int lane = threadIdx.x & 63;
     const uint32_t heads = a.cache.kv_heads;
     if (a.splits == 1) {  // as many workgroups as there may be tiles
-        const uint32_t per = a.tiles * heads;
-        it.seq = static_cast<int>(x / per);
-        it.s = draft_seq(a, x / per);
-        it.tile = x % per / heads;
-        it.head = x % heads;
+        it.seq = static_cast<int>(blockIdx.z);
+        it.s = draft_seq(a, blockIdx.z);
+        it.tile = x;
+        it.head = blockIdx.y;
         it.split = 0;
         it.splits = 1;
         it.first = x;
@@ -568,11 +572,18 @@ __device__ __forceinline__ float part_factor(float ref, float row_e, float m, fl
     return e == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((m - ref) + (e - row_e));
 }
 
+// row / group.  (A row is below 64 * 2^15 and the group up to 2^15: div_split may
+// be one too many.)
+__device__ __forceinline__ int token_of(const TreeArgs &a, int row) {
+    const uint32_t t = div_split(row, a.group, a.group_magic);
+    return static_cast<int>(t * a.group > static_cast<uint32_t>(row) ? t - 1 : t);
+}
+
 // Four numbers of a row.
 template <typename T>
 __device__ __forceinline__ void write_row(const TreeArgs &a, const Seq &s, uint32_t head, int row, int d, const Joined &w, f32x4 o) {
-    const int group = static_cast<int>(a.group), n = s.first + row / group;
-    const uint32_t to_head = head * a.group + row % group;
+    const int token = token_of(a, row), n = s.first + token;
+    const uint32_t to_head = head * a.group + (row - token * a.group);
     const float inv = w.l == 0.0f ? 0.0f : 1.0f / w.l;
     const int places = static_cast<int>(fminf(fmaxf(w.e, -400.0f), 400.0f));
     typedef __attribute__((address_space(1))) typename Numbers<T, 4>::TN *gptr;
@@ -592,7 +603,7 @@ __device__ __forceinline__ float *part_stats(const TreeArgs &a, uint32_t x) {
     return a.partials + static_cast<size_t>(a.workgroups) * kTreeRows * D + static_cast<size_t>(x) * kTreeRows * 3;
 }
 
-template <int D, int SPLIT, typename T>
+template <int D, int SPLIT, typename T, bool WINDOW>
 __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_kernel(const TreeArgs a) {
     __shared__ __align__(16) union Shared {
         TreeStage<D, SPLIT> stage;
@@ -600,9 +611,9 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     } shared;
     __shared__ __align__(16) float open_scales[kWaves][2 * kBlock];
     const int tid = threadIdx.x, lane = tid & 63, column = lane & 31, half = lane >> 5, wave = wave_id();
-    const TreeItem it = find_tree_item(a, blockIdx.x);
-    if (blockIdx.x == 0)  // bad entries, once
-        for (uint32_t i = tid; i < a.batch.sequences; i += kTreeThreads)
+    const TreeItem it = find_tree_item(a);
+    if (wave == kWaves - 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+        for (uint32_t i = lane; i < a.batch.sequences; i += 64)  // bad entries, once
             if (!draft_seq(a, i).ok) count_fault(a.cache);
     if (it.seq < 0 || !it.s.ok) return;
     const uint32_t head = it.head;
@@ -619,8 +630,9 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     if (split >= splits) return;
     if (a.splits > 1 && split == 0 && tid == 0)
         a.jobs[(static_cast<size_t>(it.seq) * a.tiles + it.tile) * a.cache.kv_heads + head] = TreeJob{it.first, static_cast<uint32_t>(splits)};
-    const int from = block0 + static_cast<int>(mul_div(split, units, splits));
-    const int to = block0 + static_cast<int>(mul_div(split + 1, units, splits));
+    // (Products of 64 parts and 2^24 columns.)
+    const int from = block0 + static_cast<int>(static_cast<uint32_t>(split * units) / static_cast<uint32_t>(splits));
+    const int to = block0 + static_cast<int>(static_cast<uint32_t>((split + 1) * units) / static_cast<uint32_t>(splits));
     const bool has_drafts = drafts < to;
 
     // Everything that depends on the item alone is under way first.  The wave's
@@ -642,7 +654,7 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
         open_scale = f32x2{scales[lane], scales[kBlock + lane]};
     }
     Eight<T> query[D / 16];
-    const int row = first_row + column, token = row < rows ? row / group : 0;
+    const int row = first_row + column, token = row < rows ? token_of(a, row) : 0;
     load_query<D, T>(query, static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(s.first + token) * a.d.q.token_stride +
                                 (head * a.group + (row < rows ? row - token * group : 0)) * a.d.q.head_stride);
     uint64_t seen = a.d.seen[s.first + token];  // of the drafts, by the lane's row
@@ -700,7 +712,7 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     // Of the half of the drafts that is the wave's, in the order of its scores.
     uint32_t drafts_seen = 0;
     if (drafts_mine) {
-        if (a.d.window != 0 && a.d.window < 64) {  // drafted tokens that lie too far above
+        if (WINDOW && a.d.window < 64) {  // drafted tokens that lie too far above
             const int depth = st.position - (s.past - 1);
             const int depths = __builtin_popcountll(a.d.seen[s.first + min(lane, s.count - 1)] & there);
             for (int j = 0; j < s.count; ++j)
@@ -714,7 +726,7 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
     const auto seen_from = [&](int first) {
         const int ahead = s.past - 1 - first - 4 * half;
         uint32_t bits = first_tokens(ahead);
-        if (a.d.window != 0) {
+        if (WINDOW) {
             const int64_t behind = static_cast<int64_t>(st.position) - first - 4 * half - a.d.window;
             bits &= ~first_tokens(static_cast<int>(max(behind, static_cast<int64_t>(-1))));
         }
@@ -753,7 +765,7 @@ __global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_
         tile_end();
     };
     int n = 0;
-    if (a.d.window != 0)  // no row stands behind past + 63
+    if (WINDOW)  // no row stands behind past + 63
         for (; n < full && static_cast<int64_t>(s.past) + 63 - (start + kWaves * n) * kBlock >= static_cast<int64_t>(a.d.window); ++n)
             block(n, std::true_type());
     for (; n < full; ++n) block(n, std::false_type());
@@ -848,9 +860,9 @@ __global__ __launch_bounds__(256) void join_tree_kernel(const TreeArgs a) {
     constexpr int kLanes = D / 4, kRows = 256 / kLanes, kParts = static_cast<int>(kTreeSplits), kEach = kParts / kLanes;
     __shared__ float factor[kRows][kParts];
     const int tid = threadIdx.x, lane = tid % kLanes, d = 4 * lane;
-    const uint32_t per = kTreeRows / kRows, job = blockIdx.x / per, heads = a.cache.kv_heads;
-    const uint32_t head = job % heads, tile = job / heads % a.tiles, i = job / heads / a.tiles;
-    const TreeJob parts = a.jobs[job];  // (of another call's where the sequence has no such tile)
+    constexpr uint32_t per = kTreeRows / kRows;
+    const uint32_t heads = a.cache.kv_heads, head = blockIdx.y, tile = blockIdx.x / per, i = blockIdx.z;
+    const TreeJob parts = a.jobs[(static_cast<size_t>(i) * a.tiles + tile) * heads + head];  // (of another call's where the sequence has no such tile)
     const Seq s = draft_seq(a, i);
     const int first_row = static_cast<int>(tile * kTreeRows), r = static_cast<int>(blockIdx.x % per) * kRows + tid / kLanes;
     const int rows = s.ok ? s.count * static_cast<int>(a.group) : 0, here = min(rows - first_row, static_cast<int>(kTreeRows));
@@ -918,14 +930,17 @@ __global__ __launch_bounds__(256) void join_tree_kernel(const TreeArgs a) {
 
 }  // namespace
 
+template <int D, int SPLIT, typename T>
+static void launch_tree_as(const TreeArgs &a, hipStream_t stream) {
+    const dim3 tiles(a.tiles, a.cache.kv_heads, a.batch.sequences);
+    auto go = [&](auto kernel) { kernel<<<a.splits == 1 ? tiles : dim3(a.workgroups), kTreeThreads, 0, stream>>>(a); };
+    a.d.window == 0 ? go(attend_tree_kernel<D, SPLIT, T, false>) : go(attend_tree_kernel<D, SPLIT, T, true>);
+    if (a.splits == 1) return;
+    join_tree_kernel<D, T><<<dim3(a.tiles * (kTreeRows * D / 1024), tiles.y, tiles.z), 256, 0, stream>>>(a);
+}
 template <int SPLIT, typename T>
 static void launch_tree_as(const TreeArgs &a, hipStream_t stream) {
-    auto go = [&](auto kernel) { kernel<<<a.workgroups, kTreeThreads, 0, stream>>>(a); };
-    a.cache.head_dim == 64 ? go(attend_tree_kernel<64, SPLIT, T>) : go(attend_tree_kernel<128, SPLIT, T>);
-    if (a.splits == 1) return;
-    const uint32_t jobs = a.batch.sequences * a.tiles * a.cache.kv_heads, rows = 1024 / a.cache.head_dim;
-    auto join = [&](auto kernel) { kernel<<<jobs * (kTreeRows / rows), 256, 0, stream>>>(a); };
-    a.cache.head_dim == 64 ? join(join_tree_kernel<64, T>) : join(join_tree_kernel<128, T>);
+    a.cache.head_dim == 64 ? launch_tree_as<64, SPLIT, T>(a, stream) : launch_tree_as<128, SPLIT, T>(a, stream);
 }
 hipError_t launch_attend_tree(const TreeArgs &a, hipStream_t stream) {
     if (a.d.dtype == Q4RDNA_F32) launch_tree_as<2, float>(a, stream);

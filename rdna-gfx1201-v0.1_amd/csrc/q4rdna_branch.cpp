@@ -97,6 +97,7 @@ int attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, cons
     a.batch = *batch;
     a.d = d;
     a.group = d.q_heads / cache->kv_heads;
+    a.group_magic = magic_of(a.group);
     // The most rows (query token, query head) per kv head that a sequence has.
     const uint32_t most_rows = std::min(batch->max_tokens, batch->tokens) * a.group;
     a.tiles = (most_rows + kTreeRows - 1) / kTreeRows;

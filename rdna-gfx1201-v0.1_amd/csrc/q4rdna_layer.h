@@ -113,6 +113,7 @@ struct TreeArgs {
     q4rdna_kv_batch batch;
     q4rdna_kv_tree_desc d;
     uint32_t group;       // query heads per kv head
+    uint32_t group_magic; // div_split's
     uint32_t tiles;       // of the largest sequence
     uint32_t splits;      // the most workgroups that share a tile
     uint32_t target;      // workgroups to deal the units (cached blocks, the drafts) to

@@ -397,3 +397,24 @@ def test_streams(cuda):
     got = api.tree(batch, parents, stream=side.cuda_stream) + cache.attend_tree(batch, q, k, v, seen, lse=True, stream=side.cuda_stream)
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, (positions, seen) + want))
+
+
+@pytest.mark.parametrize("group", [8191, 9001, 32767, 32768])
+def test_many_query_heads_of_a_kv_head(cuda, group):
+    """Rows are counted off right however many share a kv head: with one value
+    per token and head a row's result tells its token, its query its head."""
+    from q4rdna import api
+    dim, n = 64, 3
+    cache = api.KVCache.empty(1, 1, 1, dim)
+    step = api.KVBatch(torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros((1, 1), dtype=torch.int32, device="cuda"),
+                       cu_tokens=torch.tensor([0, n], dtype=torch.int32, device="cuda"), max_tokens=n)
+    k = torch.zeros(n, 1, dim, device="cuda", dtype=torch.float16)
+    k[:, 0, 0] = 1.0
+    v = torch.arange(1, n + 1, device="cuda").half()[:, None, None].expand(n, 1, dim).contiguous()
+    head = (torch.arange(group, device="cuda") % 2039 - 1019).half()
+    q = torch.zeros(n, group, dim, device="cuda", dtype=torch.float16)
+    q[:, :, 0] = head
+    seen = torch.tensor([1, 2, 4], dtype=torch.int64, device="cuda")  # each itself alone
+    out, lse = cache.attend_tree(step, q, k, v, seen, scale=1.0, lse=True)
+    assert torch.equal(out, v.expand(n, group, dim))
+    assert ((lse - head.float()).abs() <= 2.0 ** -20 * head.float().abs() + 2.0 ** -20).all()
