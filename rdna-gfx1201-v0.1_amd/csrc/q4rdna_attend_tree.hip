@@ -17,19 +17,20 @@
 // as large to join: 63 us rather than 56 for 32 sequences of 100 .. 8000 tokens,
 // 1 .. 24 drafts, 8 kv heads of 4 by 128.  The second read is the L2's.)
 //
-// The drafted tokens are one more block.  The workgroup lays their rows into LDS
+// The open block and the drafted tokens are cut into halves of 32, one for a wave
+// at most (4 drafts after 33 tokens 11.5 us, 13.0 as whole blocks).  The workgroup lays their rows into LDS
 // in fp16, scaled by a power of two for each token, fp32 ones in two parts; a
 // row's mask is 64 bits.
 //
 // A tile's blocks are split over workgroups, dealt on the device by the
 // sequences' lengths, and joined in a fixed order by a second kernel.
 //
-// What bounds it: a wave's vector instructions, some 600 for a block of 64 tokens
-// (2048 codes into fp16, 2048 weights), a 16th as many matrix instructions; for
+// What bounds it: a wave's vector instructions, some 550 for a block of 64 tokens
+// (16384 codes into fp16, 2048 weights), a 16th as many matrix instructions; for
 // one sequence, the chain of dependent loads and the first fetch of the code.
-// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 13.0 us; 16 drafts
-// after 4001 17.2 us and 4.0 us the joining; bf16, the 32 sequences above (118 MB
-// of codes) 56.4 us and 4.9 us.
+// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 11.1 us; 16 drafts
+// after 4001 17.1 us and 3.9 us the joining; bf16, the 32 sequences above (118 MB
+// of codes) 52.7 us and 4.8 us.
 #include <type_traits>
 
 #include "q4rdna_rows_device.h"

