@@ -252,8 +252,7 @@ class Decoder:
         def step():
             logits = self.forward(self.embedding[tokens[0]], batch)
             self.pasts.add_(1)
-            for new, old in zip(api.beam_select(logits[None], scores, n), (scores, rows, tokens)):
-                old.copy_(new)
+            api.beam_select(logits[None], scores, n, out=(scores, rows, tokens))
             batch.fork(rows[0], self.caches)
 
         stream = torch.cuda.Stream(self.device)

@@ -558,7 +558,8 @@ int q4rdna_kv_attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *b
  * apart), then by token.
  * scores NULL: zeros.  A beam has no continuation, all its totals are -inf, if
  * its score is not finite, if all its logits are -inf or if one of them is NaN
- * or +inf; such totals come behind all others.  Scratch as for
+ * or +inf; such totals come behind all others.  out_scores may be scores where
+ * count is beams; other overlaps are not allowed.  Scratch as for
  * q4rdna_kv_attend.  Runs on the current device. */
 #define Q4RDNA_BEAM_MAX_COUNT 128
 #define Q4RDNA_BEAM_MAX_BEAMS 256

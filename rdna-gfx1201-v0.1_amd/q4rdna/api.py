@@ -998,7 +998,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor | None, count: int, o
     None for zeros; a continuation's total is its beam's score plus the
     log-softmax of its beam's logits.  rows (int32) is group * beams + beam, what
     :meth:`KVBatch.fork` takes for a batch of all groups' beams; tokens is
-    int32; out: these three, to be written.  Equal totals go by row, then by
+    int32; out: these three, to be written (the first may be `scores` where
+    count is beams).  Equal totals go by row, then by
     logit, then by token.  A beam whose score is not finite (such as -inf) or whose logits have
     a NaN or +inf has no continuation: its totals are -inf, behind all others."""
     if logits.dim() != 3 or not logits.is_cuda:

@@ -162,3 +162,14 @@ def test_refusals(cuda):
             call()
     empty = api.beam_select(x[:0], s[:0], 2)
     assert [t.shape for t in empty] == [(0, 2)] * 3
+
+
+@pytest.mark.parametrize("beams", [1, 5, 64])
+def test_scores_in_place(cuda, beams):
+    """A search's step: the new scores where the old ones were."""
+    from q4rdna import api
+    logits, scores = normal((7, beams, 9001), "f32", 18, 2.0), normal((7, beams), "f32", 19)
+    scores[3, 0] = float("-inf")
+    want = api.beam_select(logits, scores, beams)
+    got = api.beam_select(logits, scores, beams, out=(scores, torch.empty_like(want[1]), torch.empty_like(want[2])))
+    assert got[0] is scores and all(torch.equal(a, b) for a, b in zip(want, got))

@@ -273,3 +273,86 @@ def test_graphs_that_share_scratch(cuda):
         for a, b in zip(*forked()):
             assert torch.equal(a, b), turn
     assert sum(c.faults() for c in caches) == 0
+
+
+def test_nothing_to_do(cuda):
+    """No tokens, no sequences, a sequence without drafts: outputs of no rows, and
+    rows of the others."""
+    from q4rdna import api
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = api.KVCache.empty(4, 2, 2, 64)
+    table, slots = ints([[0, 1], [2, 3]]), ints([0, 1])
+    batch = api.KVBatch(ints([0, 0]), table, cu_tokens=ints([0, 0, 0]), slots=slots, max_tokens=4)
+    positions, seen = api.tree(batch, ints([]))
+    assert positions.shape == seen.shape == (0,)
+    rows = lambda n, h: torch.randn(n, h, 64, device="cuda")  # noqa: E731
+    out, lse = cache.attend_tree(batch, rows(0, 4), rows(0, 2), rows(0, 2), seen, lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    nobody = api.KVBatch(ints([]), torch.zeros((0, 2), dtype=torch.int32, device="cuda"), cu_tokens=ints([0]), slots=ints([]), max_tokens=4)
+    nobody.fork(ints([]), [cache])
+    assert api.tree(nobody, ints([]))[0].shape == (0,)
+    # One draft of the second sequence, none of the first, nothing cached: it sees itself.
+    one = api.KVBatch(ints([0, 0]), table, cu_tokens=ints([0, 0, 1]), slots=slots, max_tokens=4)
+    v = rows(1, 2)
+    positions, seen = api.tree(one, ints([-1]))
+    out = cache.attend_tree(one, rows(1, 4), rows(1, 2), v, seen)
+    assert positions.tolist() == [0] and seen.tolist() == [1]
+    # Two fp16 parts of a number and fp32 products: 2^-21 of the row's largest at most.
+    assert (out - v.repeat_interleave(2, dim=1)).abs().max() <= 2.0 ** -21 * v.abs().max()
+    assert cache.faults() == 0
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(cuda):
+    from q4rdna import api
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda:1")  # noqa: E731
+    torch.manual_seed(0)
+    cache = api.KVCache.empty(8, 2, 2, 64, device=1)
+    past, table, slots = ints([0, 0]), ints([[0, 1, 2], [3, 4, 5]]), ints([0, 1])
+    k, q = torch.randn((140, 2, 64), device="cuda:1"), torch.randn((5, 4, 64), device="cuda:1")
+    cache.append(api.KVBatch(past, table, ints([0, 70, 140]), slots, max_tokens=70), k, k)
+    past += 70
+    step = api.KVBatch(past, table, ints([0, 2, 5]), slots, max_tokens=3)
+    parents, logits = ints([-1, 0, -1, 0, 0]), torch.randn((1, 2, 999), device="cuda:1")
+    results = []
+    for current in (1, 0):
+        with torch.cuda.device(current):
+            positions, seen = api.tree(step, parents)
+            q1, k1 = api.rotate(q, k[:5], positions)
+            results.append((positions, seen, q1, k1, cache.attend_tree(step, q1, k1, k[:5], seen), *api.beam_select(logits, None, 4)))
+            assert torch.cuda.current_device() == current
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    step.fork(ints([1, 1]), [cache])
+    assert torch.cuda.current_device() == 0 and past.tolist() == [70, 70]
+
+
+def test_offsets_past_32_bits(cuda):
+    """Pages and slots more than 4 GiB into a cache: the same bits as in a small
+    one, from drafts and after a fork."""
+    from q4rdna import api
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    torch.manual_seed(1)
+    heads, dim, length = 8, 128, 200
+    k, v = torch.randn(2, length, heads, dim, device="cuda")
+    q, dk, dv = (torch.randn(3, h, dim, device="cuda") for h in (2 * heads, heads, heads))
+    results = []
+    for pages, slots in ((12, 2), (34000, 8300)):
+        cache = api.KVCache.empty(pages, slots, heads, dim)
+        if slots > 2:
+            assert cache.pages.numel() > 2 ** 32 and cache.open.numel() > 2 ** 32
+        table = ints([list(range(pages - 4, pages)), [-1] * 4])
+        past, slot = ints([0, 0]), ints([slots - 1, 0])
+        cache.append(api.KVBatch(past, table, ints([0, length, length]), slot, max_tokens=length), k, v)
+        past[0] = length
+        step = api.KVBatch(past, table, ints([0, 3, 3]), slot, max_tokens=3)
+        _, seen = api.tree(step, ints([-1, 0, 0]))
+        out = [cache.attend_tree(step, q, dk, dv, seen)]
+        step.fork(ints([0, 0]), [cache])
+        assert slot.tolist() == [slots - 1, 0] and past.tolist() == [length, length]
+        # The second goes on from the copy of its open block.
+        step = api.KVBatch(past, table, ints([0, 0, 3]), slot, max_tokens=3)
+        out.append(cache.attend_tree(step, q, dk, dv, seen))
+        assert torch.equal(out[0], out[1]) and cache.faults() == 0
+        results.append(out)
+        del cache
+    assert all(torch.equal(a, b) for a, b in zip(*results))
