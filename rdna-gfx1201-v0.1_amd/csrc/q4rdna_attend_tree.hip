@@ -29,8 +29,9 @@
 // (16384 codes into fp16, 2048 weights), a 16th as many matrix instructions; for
 // one sequence, the chain of dependent loads and the first fetch of the code.
 // Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 11.1 us; 16 drafts
-// after 4001 17.1 us and 3.9 us the joining; bf16, the 32 sequences above (118 MB
-// of codes) 52.7 us and 4.8 us.
+// after 4001 17.0 us and 3.9 us the joining; the 32 sequences above (118 MB of codes)
+// in bf16 51.5 us and 4.9 us, in fp32 70.7 (86.2 with one workgroup a CU, whose
+// registers need no scratch).
 #include <type_traits>
 
 #include "q4rdna_rows_device.h"
@@ -530,39 +531,49 @@ __device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a) {
         w = tree_work(a, i + lane);
         all += __builtin_amdgcn_readlane(wave_scan(w.jobs * w.units), 63);
     }
-    uint32_t chunk = (max(all, 1u) - 1) / a.target + 1;
-    // Larger parts until all of them run at once, if they can.
-    if (a.batch.sequences <= 64) {
-        const uint32_t jobs = __builtin_amdgcn_readlane(wave_scan(w.jobs), 63);
-        while (jobs < a.target &&
-               static_cast<uint32_t>(__builtin_amdgcn_readlane(wave_scan(w.jobs * tree_parts(a, w, chunk)), 63)) > a.target)
+    // Up to eight units a wave a part for a CU, or fewer and larger ones, so that all
+    // of them run at once.  Beyond that two for a CU, which share it well, and as
+    // large as it takes for the long ones to run at once: a second round costs a
+    // whole part's time, while short ones fill the gaps.  (By the sequences' lengths,
+    // 32 of them as above: all of one size 60 us.)
+    uint32_t chunk = (max(all, 1u) - 1) / a.cus + 1;
+    const bool two = chunk >= 8 * kWaves;
+    if (two) chunk = (all - 1) / (2 * a.cus) + 1;
+    if (a.batch.sequences <= 64 && (two || static_cast<uint32_t>(__builtin_amdgcn_readlane(wave_scan(w.jobs), 63)) < a.cus))
+        for (int i = 0; i < 12; ++i) {
+            const float parts = ceilf(static_cast<float>(w.units) * __builtin_amdgcn_rcpf(static_cast<float>(max(chunk, static_cast<uint32_t>(kWaves)))));
+            const uint32_t n = !two || 2 * w.units > chunk ? w.jobs * static_cast<uint32_t>(parts) : 0;
+            if (static_cast<uint32_t>(__builtin_amdgcn_readlane(wave_scan(n), 63)) <= (two ? 2 * a.cus : a.cus)) break;
             chunk += chunk / 8 + 1;
-    }
-    uint32_t base = 0;
-    for (uint32_t i = 0; i < a.batch.sequences; i += 64) {
-        if (a.batch.sequences > 64) w = tree_work(a, i + lane);
-        const uint32_t parts = tree_parts(a, w, chunk), end = base + wave_scan(w.jobs * parts);
-        const uint64_t later = __builtin_amdgcn_ballot_w64(end > x);
-        if (later != 0) {
-            const int owner = __builtin_ctzll(later);
-            const uint32_t mine = __builtin_amdgcn_readlane(parts, owner);
-            const uint32_t local = x - __builtin_amdgcn_readlane(end - w.jobs * parts, owner);  // (tile, part, head)
-            it.seq = static_cast<int>(i) + owner;
-            it.s.first = __builtin_amdgcn_readlane(w.s.first, owner);
-            it.s.count = __builtin_amdgcn_readlane(w.s.count, owner);
-            it.s.past = __builtin_amdgcn_readlane(w.s.past, owner);
-            it.s.slot = __builtin_amdgcn_readlane(w.s.slot, owner);
-            it.s.length = it.s.past;
-            it.s.ok = true;
-            it.head = local % heads;
-            it.split = static_cast<int>(local / heads % mine);
-            it.tile = local / heads / mine;
-            it.splits = static_cast<int>(mine);
-            it.first = x - it.split * heads;
-            return it;
         }
-        base = __builtin_amdgcn_readlane(end, 63);
-    }
+    // Long parts first: those of more than half a chunk, then the others.
+    uint32_t base = 0;
+    for (int small = 0; small < 2; ++small)
+        for (uint32_t i = 0; i < a.batch.sequences; i += 64) {
+            if (a.batch.sequences > 64) w = tree_work(a, i + lane);
+            const uint32_t parts = tree_parts(a, w, chunk), mine = (2 * w.units <= chunk) == (small != 0) ? w.jobs * parts : 0;
+            const uint32_t end = base + wave_scan(mine);
+            const uint64_t later = __builtin_amdgcn_ballot_w64(end > x);
+            if (later != 0) {
+                const int owner = __builtin_ctzll(later);
+                const uint32_t its = __builtin_amdgcn_readlane(parts, owner);
+                const uint32_t local = x - __builtin_amdgcn_readlane(end - mine, owner);  // (tile, part, head)
+                it.seq = static_cast<int>(i) + owner;
+                it.s.first = __builtin_amdgcn_readlane(w.s.first, owner);
+                it.s.count = __builtin_amdgcn_readlane(w.s.count, owner);
+                it.s.past = __builtin_amdgcn_readlane(w.s.past, owner);
+                it.s.slot = __builtin_amdgcn_readlane(w.s.slot, owner);
+                it.s.length = it.s.past;
+                it.s.ok = true;
+                it.head = local % heads;
+                it.split = static_cast<int>(local / heads % its);
+                it.tile = local / heads / its;
+                it.splits = static_cast<int>(its);
+                it.first = x - it.split * heads;
+                return it;
+            }
+            base = __builtin_amdgcn_readlane(end, 63);
+        }
     return it;
 }
 
@@ -605,7 +616,7 @@ __device__ __forceinline__ float *part_stats(const TreeArgs &a, uint32_t x) {
 }
 
 template <int D, int SPLIT, typename T, bool WINDOW>
-__global__ __launch_bounds__(kTreeThreads, SPLIT == 1 ? 2 : 1) void attend_tree_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(kTreeThreads, 2) void attend_tree_kernel(const TreeArgs a) {
     __shared__ __align__(16) union Shared {
         TreeStage<D, SPLIT> stage;
         TreeJoin<D> join;

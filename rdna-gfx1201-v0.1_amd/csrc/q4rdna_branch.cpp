@@ -104,14 +104,13 @@ int attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, cons
     const uint64_t jobs = static_cast<uint64_t>(a.tiles) * cache->kv_heads * batch->sequences;
     const uint64_t most_units = (d.window == 0 ? batch->table_width
                                                : std::min<uint64_t>(batch->table_width, d.window / kKvBlock + 2)) + 3ull;
-    // A workgroup's worth for every CU.  (Two fit one in 16 bits, but with as many
-    // smaller parts 32 sequences take 65 us rather than 56, and five 17.9 rather
-    // than 17.4.  Nor are parts worth their scratch where tiles abound.)
     const uint32_t cus = cu_count(cache->device);
-    a.target = cus;
+    a.cus = cus;
+    // (Parts are not worth their scratch where tiles abound, nor a second launch
+    // where a wave has four units at most.)
     const bool split = most_units > 16 && batch->sequences <= kDealtSequences && jobs <= 16ull * cus && jobs * most_units <= 0x7fffffffu;
     a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>((most_units + 3) / 4, kTreeSplits) : 1);
-    const uint64_t workgroups = split ? std::min(jobs + a.target, jobs * a.splits) : jobs;
+    const uint64_t workgroups = split ? std::min(jobs + 2 * cus, jobs * a.splits) : jobs;
     if (workgroups > most_workgroups(256))
         return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences of %u kv heads are too many for one call", batch->sequences, cache->kv_heads);
     a.workgroups = static_cast<uint32_t>(workgroups);

@@ -116,7 +116,7 @@ struct TreeArgs {
     uint32_t group_magic; // div_split's
     uint32_t tiles;       // of the largest sequence
     uint32_t splits;      // the most workgroups that share a tile
-    uint32_t target;      // workgroups to deal the units (cached blocks, the drafts) to
+    uint32_t cus;         // to deal the units to
     uint32_t workgroups;  // launched
     float *partials;      // of each workgroup [row][D], then of each [m, l, e][row]
     TreeJob *jobs;        // [sequence][tile][head]
