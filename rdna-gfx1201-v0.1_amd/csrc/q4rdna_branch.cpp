@@ -211,6 +211,28 @@ int fork(const q4rdna_kv_cache *caches, uint32_t count, const q4rdna_kv_fork_des
     const uint64_t given = std::min<uint64_t>(c.page_count, touched * d.sequences);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     Scratch scratch;
+    const uint32_t cus = cu_count(c.device);
+    const auto take_layers = [&](uint32_t first) {
+        a.layers = std::min(count - first, kForkLayers);
+        for (uint32_t l = 0; l < a.layers; ++l) {
+            a.open[l] = caches[first + l].open;
+            a.open_scales[l] = caches[first + l].open_scales;
+        }
+        // All but one sequence may be copied.
+        return static_cast<uint64_t>(d.sequences - 1) * a.layers * 2 * c.kv_heads;
+    };
+    uint32_t width_log2 = 0;
+    while (1u << width_log2 < d.table_width) ++width_log2;
+    // One launch where one workgroup can rename the table at a time; a larger one
+    // takes many, after a plan.
+    if (count <= kForkLayers && d.sequences <= kForkSmall && c.page_count <= kForkSmallPages && given <= kForkSmallGiven &&
+        static_cast<uint64_t>(d.sequences) << width_log2 <= kForkEntries) {
+        if ((rc = get_scratch(c.device, s, 0, 32 * (1 + kForkGates), &scratch)) != Q4RDNA_OK) return rc;
+        a.arrived = scratch.arrived;
+        a.columns_log2 = width_log2;
+        const uint64_t most = take_layers(0);
+        return launched(launch_fork(a, static_cast<uint32_t>(std::min<uint64_t>(most, 4ull * cus)), s), "kv_fork");
+    }
     if ((rc = get_scratch(c.device, s, 7ull * d.sequences + 2 + given, 0, &scratch)) != Q4RDNA_OK) return rc;
     a.moves = reinterpret_cast<ForkMove *>(scratch.partials);
     a.copies = reinterpret_cast<ForkCopy *>(a.moves + d.sequences);
@@ -219,16 +241,10 @@ int fork(const q4rdna_kv_cache *caches, uint32_t count, const q4rdna_kv_fork_des
     while (a.columns_log2 < 6 && (d.sequences << (a.columns_log2 + 1)) <= kForkEntries) ++a.columns_log2;
     const uint32_t units = ((d.table_width - 1) >> a.columns_log2) + 1;
     if ((rc = launched(launch_fork_plan(a, s), "kv_fork")) != Q4RDNA_OK) return rc;
-    const uint32_t cus = cu_count(c.device);
     for (uint32_t i = 0; i < count; i += kForkLayers) {
-        a.layers = std::min(count - i, kForkLayers);
-        for (uint32_t l = 0; l < a.layers; ++l) {
-            a.open[l] = caches[i + l].open;
-            a.open_scales[l] = caches[i + l].open_scales;
-        }
+        const uint64_t most = take_layers(i);
         a.table_units = i == 0 ? units : 0;
-        // All but one sequence may be copied; eight workgroups a CU carry a copy.
-        const uint64_t most = static_cast<uint64_t>(d.sequences - 1) * a.layers * 2 * c.kv_heads;
+        // Eight workgroups a CU carry a copy.
         const uint32_t copiers = static_cast<uint32_t>(std::min<uint64_t>(most, 8ull * cus));
         if (a.table_units + copiers == 0) continue;
         if ((rc = launched(launch_fork_move(a, copiers, s), "kv_fork")) != Q4RDNA_OK) return rc;

@@ -156,6 +156,7 @@ struct ForkArgs {
     ForkCopy *copies;  // [sequences]
     uint32_t *counts;  // copies, pages in `free`
     int32_t *free;     // pages in the order in which they are given out
+    uint32_t *arrived; // launch_fork's, 32 * (1 + kForkGates) zeros
     uint32_t columns_log2;  // of the table, that a workgroup takes
     uint32_t table_units;
     uint32_t layers;
@@ -166,6 +167,13 @@ struct ForkArgs {
 constexpr uint32_t kForkPages = 1u << 18;
 // Entries of the table that a workgroup takes.
 constexpr uint32_t kForkEntries = 4096;
+// What one launch does: sequences, pages, pages given out at most.
+constexpr uint32_t kForkSmall = 256;
+constexpr uint32_t kForkSmallPages = 1u << 16;
+constexpr uint32_t kForkSmallGiven = 1024;
+constexpr uint32_t kForkGates = 16;
+// One workgroup for the table and `copiers` for the open blocks.
+hipError_t launch_fork(const ForkArgs &a, uint32_t copiers, hipStream_t stream);
 hipError_t launch_fork_plan(const ForkArgs &a, hipStream_t stream);
 // a.table_units workgroups for the table, the lengths and the slots, and
 // `copiers` for the open blocks.

@@ -209,3 +209,24 @@ def test_kept_pages_of_a_large_cache(cuda):
     kept[-3:] = torch.tensor([False, True, True])
     run(*s, [2, 2, 0, 1], 6000, kept=kept.cuda())
     run(*s, [0, 1, 2, 3], 64, kept=kept.cuda())
+
+
+@pytest.mark.parametrize("n,width,pages,layers", [
+    (256, 16, 2000, 1), (257, 16, 2000, 1), (256, 17, 2000, 1), (16, 256, 3000, 2), (15, 300, 3000, 2), (3, 64, 65536, 1), (3, 64, 65537, 1),
+    (1, 4096, 5000, 1), (1, 5000, 5000, 1)])
+def test_either_side_of_one_launch(cuda, n, width, pages, layers):
+    """Small tables take one launch, others two: the same results."""
+    r = np.random.RandomState(n + width)
+    past = [int(x) for x in r.randint(0, 64 * min(width, pages // n) - 100, n)]
+    s = state(past, width, pages, n + 1, layers=layers, kv_heads=1, seed=n)
+    for room in (1, 70, 0):
+        run(*s, [int(x) for x in r.randint(-1, n, n)], room)
+    run(*s, list(range(n)), 10000)
+
+
+@pytest.mark.parametrize("n", [60, 200])
+def test_more_entries_than_pages(cuda, n):
+    """Pages for 16 columns of every sequence are wanted, few are there."""
+    s = state([5] * n, 16, 100, n, layers=1, kv_heads=1, seed=n)
+    run(*s, [0] * n, 1024)
+    run(*s, [n - 1] * n, 1024)
