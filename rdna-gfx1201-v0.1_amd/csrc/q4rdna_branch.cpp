@@ -223,15 +223,19 @@ int fork(const q4rdna_kv_cache *caches, uint32_t count, const q4rdna_kv_fork_des
     };
     uint32_t width_log2 = 0;
     while (1u << width_log2 < d.table_width) ++width_log2;
-    // One launch where one workgroup can rename the table at a time; a larger one
-    // takes many, after a plan.
+    // One launch where one workgroup can see to the table: in a step, or, with 1024
+    // threads, in a few.  A larger table takes many, after a plan.
+    const uint64_t entries = static_cast<uint64_t>(d.sequences) << width_log2;
     if (count <= kForkLayers && d.sequences <= kForkSmall && c.page_count <= kForkSmallPages && given <= kForkSmallGiven &&
-        static_cast<uint64_t>(d.sequences) << width_log2 <= kForkEntries) {
+        entries <= 8 * kForkEntries) {
         if ((rc = get_scratch(c.device, s, 0, 32 * (1 + kForkGates), &scratch)) != Q4RDNA_OK) return rc;
         a.arrived = scratch.arrived;
-        a.columns_log2 = width_log2;
+        const uint32_t threads = entries <= kForkEntries ? 256 : 1024, side = threads / 256;
+        while (a.columns_log2 < width_log2 && (d.sequences << (a.columns_log2 + 1)) <= side * kForkEntries) ++a.columns_log2;
+        // 1024 threads a CU carry a copy.  (2048 where they wait for each other: 48.5 us,
+        // not 49.5, for 200 sequences.)
         const uint64_t most = take_layers(0);
-        return launched(launch_fork(a, static_cast<uint32_t>(std::min<uint64_t>(most, 4ull * cus)), s), "kv_fork");
+        return launched(launch_fork(a, threads, static_cast<uint32_t>(std::min<uint64_t>((most + side - 1) / side, (side == 1 ? 4 : 2) * cus)), s), "kv_fork");
     }
     if ((rc = get_scratch(c.device, s, 7ull * d.sequences + 2 + given, 0, &scratch)) != Q4RDNA_OK) return rc;
     a.moves = reinterpret_cast<ForkMove *>(scratch.partials);

@@ -1,15 +1,18 @@
 // Sequences that go on from others (q4rdna_kv_fork).
 //
-// Two launches.  fork_plan_kernel, one workgroup, decides: each sequence's
-// parent, length and slot, which open blocks are copied, and which pages are
-// free, in the order in which they are given out.  fork_move_kernel carries it
-// out: a workgroup renames some columns of the table, all rows of which it has
-// read before it writes the first, and others copy open blocks, at a large copy's
-// rate.  One workgroup plans since everything depends on everything: a page is
-// free if no row holds it.  Measured, plan and move: 4 sequences of 700 tokens,
-// 4 layers of 8 heads by 128 5.6 and 4.4 us; 8 of 4001, 36 layers (153 MB read and
-// written) 6.5 and 29.7; 200 of 10 .. 8000, 12 layers of 4 by 64 (212 MB) 11.4 and
-// 42.7.
+// What is decided: each sequence's parent, length and slot, which open blocks are
+// copied, and which pages are free, in the order in which they are given out.
+// What takes the time is copying the open blocks.
+//
+// fork_kernel, for up to 256 sequences and tables of up to 2^15 entries, does all
+// in one launch.  For larger ones fork_plan_kernel, one workgroup, decides, and
+// fork_move_kernel carries it out: a workgroup renames some columns of the table,
+// all rows of which it has read before it writes the first, and others copy.
+//
+// Measured, with the plan in a launch of its own and in one launch: 4 sequences
+// of 700 tokens, 4 layers of 8 heads by 128 5.6 + 4.4 and 6.6 us; 8 of 4001, 36
+// layers (153 MB read and written) 6.5 + 29.7 and 30.1, a large copy's rate; 200
+// of 10 .. 8000, 12 layers of 4 by 64 (212 MB) 11.4 + 42.5 and 48.5.
 #include "q4rdna_layer_device.h"
 
 namespace q4rdna {
@@ -208,15 +211,17 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkArgs 
 
 // Renames 2^columns_log2 columns: what sequence i becomes is move(i), the pages
 // that are given out, `given` of them, are page(rank).
-template <typename Move, typename Page>
+template <int THREADS, typename Move, typename Page>
 __device__ __forceinline__ void move_columns(const ForkArgs &a, int column0, uint32_t given, Move move, Page page) {
     constexpr int kEach = kForkEntries / 256;
-    const int tid = threadIdx.x, n = static_cast<int>(a.d.sequences), width = static_cast<int>(a.d.table_width);
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // or all entries' rows would stay in registers over the caller's loop
+    const int n = static_cast<int>(a.d.sequences), width = static_cast<int>(a.d.table_width);
     const int columns = 1 << a.columns_log2;
     int32_t entry[kEach];
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
-        const int e = tid + 256 * x, i = e >> a.columns_log2, b = column0 + (e & (columns - 1));
+        const int e = tid + THREADS * x, i = e >> a.columns_log2, b = column0 + (e & (columns - 1));
         entry[x] = -1;
         if (i >= n || b >= width) continue;
         const ForkMove m = move(i);
@@ -234,14 +239,14 @@ __device__ __forceinline__ void move_columns(const ForkArgs &a, int column0, uin
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < kEach; ++x) {
-        const int e = tid + 256 * x, i = e >> a.columns_log2, b = column0 + (e & (columns - 1));
+        const int e = tid + THREADS * x, i = e >> a.columns_log2, b = column0 + (e & (columns - 1));
         if (i < n && b < width) a.d.table[static_cast<size_t>(i) * width + b] = entry[x];
     }
 }
 
 __device__ __forceinline__ void move_table(const ForkArgs &a) {
     const int tid = threadIdx.x, n = static_cast<int>(a.d.sequences);
-    move_columns(a, static_cast<int>(blockIdx.x << a.columns_log2), a.counts[1], [&](int i) { return a.moves[i]; },
+    move_columns<256>(a, static_cast<int>(blockIdx.x << a.columns_log2), a.counts[1], [&](int i) { return a.moves[i]; },
                  [&](uint32_t rank) { return a.free[rank]; });
     if (blockIdx.x == 0)
         for (int i = tid; i < n; i += 256) {
@@ -256,7 +261,7 @@ __device__ __forceinline__ void move_table(const ForkArgs &a) {
 template <int D>
 __device__ __forceinline__ void copy_open(const ForkArgs &a, const ForkCopy *copies, uint32_t unit) {
     constexpr int kEach = 4 * kBlock * D / (16 * 256);
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x % 256;
     const uint32_t head = unit % a.kv_heads, rest = unit / a.kv_heads;
     const uint32_t layer = rest / 2 % a.layers;
     const ForkCopy c = copies[rest / 2 / a.layers];
@@ -290,16 +295,16 @@ __global__ __launch_bounds__(256) void fork_move_kernel(const ForkArgs a) {
     for (uint64_t u = blockIdx.x - a.table_units; u < units; u += copiers) copy_open<D>(a, a.copies, static_cast<uint32_t>(u));
 }
 
-// Both in one launch, for few sequences: every workgroup plans for itself, which
+// Both in one launch, for up to 256 sequences: every workgroup plans for itself, which
 // is three loads side by side and some steps in LDS.  The first one sees to the
 // pages and the table, which no other reads, the others copy; and since all
 // read the lengths and slots, the last one to have done so writes them.
-template <int D>
-__global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void fork_kernel(const ForkArgs a) {
     __shared__ int32_t parent[kForkSmall], past[kForkSmall], slot[kForkSmall], first[kForkSmall], vacant[kForkSmall];
     __shared__ int32_t old_past[kForkSmall], old_slot[kForkSmall], free[kForkSmallGiven];
     __shared__ ForkCopy copy[kForkSmall];
-    __shared__ uint32_t used[kForkSmallPages / 32], ranks[kForkSmall], totals[4], longest;
+    __shared__ uint32_t used[kForkSmallPages / 32], ranks[kForkSmall], totals[THREADS / 64], longest;
     const int tid = threadIdx.x, lane = tid & 63, n = static_cast<int>(a.d.sequences), width = static_cast<int>(a.d.table_width);
     const bool mine = tid < n, first_one = blockIdx.x == 0;
     int p = -1, length = 0;
@@ -308,9 +313,9 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
         old_past[tid] = a.d.past[tid];
         old_slot[tid] = a.d.slots[tid];
     }
-    first[tid] = n;
+    if (tid < kForkSmall) first[tid] = n;
     if (first_one)
-        for (uint32_t w = tid; w < (a.page_count + 31) / 32; w += 256) used[w] = 0;
+        for (uint32_t w = tid; w < (a.page_count + 31) / 32; w += THREADS) used[w] = 0;
     if (tid == 0) longest = 0;
     __syncthreads();  // with it, the lengths and slots have arrived
     // Arrivals are counted at gates, 128 bytes apart, and the full gates.
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
     __syncthreads();
     uint32_t all;
     const bool none = mine && first[tid] == n, moved = mine && (p < 0 || first[p] != tid);
-    const uint32_t at = threads_before<256>((none ? 1u : 0u) + (moved ? 1u << 16 : 0u), totals, &all);
+    const uint32_t at = threads_before<THREADS>((none ? 1u : 0u) + (moved ? 1u << 16 : 0u), totals, &all);
     if (none) vacant[at & 0xffffu] = old_slot[tid];
     __syncthreads();
     const int from = p >= 0 ? old_slot[p] : 0, to = moved ? vacant[at >> 16] : from;
@@ -346,12 +351,14 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
     const bool copied = moved && length > 0;
     const int blocks = p >= 0 ? max(room_end(a.d, length) - length / kBlock, 0) : 0;
     // (Fewer than 256 copies, and no more pages than the table has entries.)
-    const uint32_t rank = threads_before<256>((copied ? 1u : 0u) + (static_cast<uint32_t>(blocks) << 16), totals, &all);
+    const uint32_t rank = threads_before<THREADS>((copied ? 1u : 0u) + (static_cast<uint32_t>(blocks) << 16), totals, &all);
     if (copied) copy[rank & 0xffffu] = ForkCopy{from, to, length};
-    parent[tid] = p;
-    past[tid] = length;
-    slot[tid] = to;
-    ranks[tid] = rank >> 16;
+    if (tid < kForkSmall) {
+        parent[tid] = p;
+        past[tid] = length;
+        slot[tid] = to;
+        ranks[tid] = rank >> 16;
+    }
     if (first_one && length >= kBlock) atomicMax(&longest, static_cast<uint32_t>(length / kBlock));
     __syncthreads();
     if (tid < 64) {
@@ -372,14 +379,16 @@ __global__ __launch_bounds__(256) void fork_kernel(const ForkArgs a) {
     }
     if (!first_one) {
         const uint32_t units = (all & 0xffffu) * a.layers * 2 * a.kv_heads;  // fewer than 2^32
-        for (uint32_t u = blockIdx.x - 1; u < units; u += gridDim.x - 1) copy_open<D>(a, copy, u);
+        constexpr uint32_t kSide = THREADS / 256;  // units side by side
+        for (uint32_t u = (blockIdx.x - 1) * kSide + tid / 256; u < units; u += (gridDim.x - 1) * kSide) copy_open<D>(a, copy, u);
         return;
     }
     if (refused && a.faults != nullptr) atomicAdd(a.faults, 1u);
-    mark_pages<256>(a, longest, parent, past, first, used);
-    const uint32_t given = find_free<256>(a, all >> 16, used, totals, free);
+    mark_pages<THREADS>(a, longest, parent, past, first, used);
+    const uint32_t given = find_free<THREADS>(a, all >> 16, used, totals, free);
     __syncthreads();
-    move_columns(a, 0, given, [&](int i) { return ForkMove{parent[i], past[i], slot[i], ranks[i]}; }, [&](uint32_t r) { return free[r]; });
+    for (int column = 0; column < width; column += 1 << a.columns_log2)
+        move_columns<THREADS>(a, column, given, [&](int i) { return ForkMove{parent[i], past[i], slot[i], ranks[i]}; }, [&](uint32_t r) { return free[r]; });
 }
 
 }  // namespace
@@ -395,9 +404,10 @@ hipError_t launch_fork_move(const ForkArgs &a, uint32_t copiers, hipStream_t str
     return hipGetLastError();
 }
 
-hipError_t launch_fork(const ForkArgs &a, uint32_t copiers, hipStream_t stream) {
-    auto go = [&](auto kernel) { kernel<<<1 + copiers, 256, 0, stream>>>(a); };
-    a.head_dim == 64 ? go(fork_kernel<64>) : go(fork_kernel<128>);
+hipError_t launch_fork(const ForkArgs &a, uint32_t threads, uint32_t copiers, hipStream_t stream) {
+    auto go = [&](auto kernel) { kernel<<<1 + copiers, threads, 0, stream>>>(a); };
+    if (threads == 256) a.head_dim == 64 ? go(fork_kernel<64, 256>) : go(fork_kernel<128, 256>);
+    else a.head_dim == 64 ? go(fork_kernel<64, 1024>) : go(fork_kernel<128, 1024>);
     return hipGetLastError();
 }
 

@@ -165,15 +165,16 @@ struct ForkArgs {
 };
 // The most pages: their bits lie in LDS.
 constexpr uint32_t kForkPages = 1u << 18;
-// Entries of the table that a workgroup takes.
+// Entries of the table that a workgroup of 256 threads takes.
 constexpr uint32_t kForkEntries = 4096;
 // What one launch does: sequences, pages, pages given out at most.
 constexpr uint32_t kForkSmall = 256;
 constexpr uint32_t kForkSmallPages = 1u << 16;
 constexpr uint32_t kForkSmallGiven = 1024;
 constexpr uint32_t kForkGates = 16;
-// One workgroup for the table and `copiers` for the open blocks.
-hipError_t launch_fork(const ForkArgs &a, uint32_t copiers, hipStream_t stream);
+// One workgroup for the table and `copiers` for the open blocks, of 256 or 1024
+// threads.
+hipError_t launch_fork(const ForkArgs &a, uint32_t threads, uint32_t copiers, hipStream_t stream);
 hipError_t launch_fork_plan(const ForkArgs &a, hipStream_t stream);
 // a.table_units workgroups for the table, the lengths and the slots, and
 // `copiers` for the open blocks.

@@ -213,7 +213,7 @@ def test_kept_pages_of_a_large_cache(cuda):
 
 @pytest.mark.parametrize("n,width,pages,layers", [
     (256, 16, 2000, 1), (257, 16, 2000, 1), (256, 17, 2000, 1), (16, 256, 3000, 2), (15, 300, 3000, 2), (3, 64, 65536, 1), (3, 64, 65537, 1),
-    (1, 4096, 5000, 1), (1, 5000, 5000, 1)])
+    (1, 4096, 5000, 1), (1, 5000, 5000, 1), (256, 128, 20000, 1), (256, 129, 20000, 1), (200, 100, 20000, 3), (7, 4000, 20000, 1)])
 def test_either_side_of_one_launch(cuda, n, width, pages, layers):
     """Small tables take one launch, others two: the same results."""
     r = np.random.RandomState(n + width)
