@@ -30,8 +30,8 @@
 // one sequence, the chain of dependent loads and the first fetch of the code.
 // Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 11.1 us; 16 drafts
 // after 4001 17.0 us and 3.9 us the joining; the 32 sequences above (118 MB of codes)
-// in bf16 51.5 us and 4.9 us, in fp32 70.7 (86.2 with one workgroup a CU, whose
-// registers need no scratch).
+// in bf16 51.5 us and 4.9 us, in fp32 70.7 (86.2 with one workgroup a CU; two leave
+// registers for all but eight, and cost a few tokens' call 1%).
 #include <type_traits>
 
 #include "q4rdna_rows_device.h"
@@ -526,20 +526,22 @@ __device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a) {
         return it;
     }
     TreeWork w;
-    uint32_t all = 0;  // jobs * units, fewer than 2^32 by the host's bound
+    uint32_t all = 0, jobs = 0;  // jobs * units, fewer than 2^32 by the host's bound
     for (uint32_t i = 0; i < a.batch.sequences; i += 64) {
         w = tree_work(a, i + lane);
         all += __builtin_amdgcn_readlane(wave_scan(w.jobs * w.units), 63);
+        jobs += __builtin_amdgcn_readlane(wave_scan(w.jobs), 63);
     }
-    // Up to eight units a wave a part for a CU, or fewer and larger ones, so that all
-    // of them run at once.  Beyond that two for a CU, which share it well, and as
-    // large as it takes for the long ones to run at once: a second round costs a
-    // whole part's time, while short ones fill the gaps.  (By the sequences' lengths,
-    // 32 of them as above: all of one size 60 us.)
+    // A part for a CU, or fewer and larger ones, so that all of them run at once.
+    // Where there are as many tiles as CUs and eight units a wave, two for a CU,
+    // which share it well, and as large as it takes for the long ones to run at
+    // once: a second round costs a whole part's time, while short ones fill the
+    // gaps.  (48 sequences of 100 .. 4000 tokens 58.7 and 48.9 us, 24 of up to 12000 by
+    // 64 33.3 and 29.3; but one of 60000 39.1 and 44.8.)
     uint32_t chunk = (max(all, 1u) - 1) / a.cus + 1;
-    const bool two = chunk >= 8 * kWaves;
+    const bool two = a.per_cu == 2 && jobs >= a.cus && chunk >= 8 * kWaves;
     if (two) chunk = (all - 1) / (2 * a.cus) + 1;
-    if (a.batch.sequences <= 64 && (two || static_cast<uint32_t>(__builtin_amdgcn_readlane(wave_scan(w.jobs), 63)) < a.cus))
+    if (a.batch.sequences <= 64 && (two || jobs < a.cus))
         for (int i = 0; i < 12; ++i) {
             const float parts = ceilf(static_cast<float>(w.units) * __builtin_amdgcn_rcpf(static_cast<float>(max(chunk, static_cast<uint32_t>(kWaves)))));
             const uint32_t n = !two || 2 * w.units > chunk ? w.jobs * static_cast<uint32_t>(parts) : 0;
@@ -551,7 +553,7 @@ __device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a) {
     for (int small = 0; small < 2; ++small)
         for (uint32_t i = 0; i < a.batch.sequences; i += 64) {
             if (a.batch.sequences > 64) w = tree_work(a, i + lane);
-            const uint32_t parts = tree_parts(a, w, chunk), mine = (2 * w.units <= chunk) == (small != 0) ? w.jobs * parts : 0;
+            const uint32_t parts = tree_parts(a, w, chunk), mine = (two && 2 * w.units <= chunk) == (small != 0) ? w.jobs * parts : 0;
             const uint32_t end = base + wave_scan(mine);
             const uint64_t later = __builtin_amdgcn_ballot_w64(end > x);
             if (later != 0) {
@@ -615,8 +617,8 @@ __device__ __forceinline__ float *part_stats(const TreeArgs &a, uint32_t x) {
     return a.partials + static_cast<size_t>(a.workgroups) * kTreeRows * D + static_cast<size_t>(x) * kTreeRows * 3;
 }
 
-template <int D, int SPLIT, typename T, bool WINDOW>
-__global__ __launch_bounds__(kTreeThreads, 2) void attend_tree_kernel(const TreeArgs a) {
+template <int D, int SPLIT, typename T, bool WINDOW, int PER_CU>
+__global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const TreeArgs a) {
     __shared__ __align__(16) union Shared {
         TreeStage<D, SPLIT> stage;
         TreeJoin<D> join;
@@ -946,7 +948,9 @@ template <int D, int SPLIT, typename T>
 static void launch_tree_as(const TreeArgs &a, hipStream_t stream) {
     const dim3 tiles(a.tiles, a.cache.kv_heads, a.batch.sequences);
     auto go = [&](auto kernel) { kernel<<<a.splits == 1 ? tiles : dim3(a.workgroups), kTreeThreads, 0, stream>>>(a); };
-    a.d.window == 0 ? go(attend_tree_kernel<D, SPLIT, T, false>) : go(attend_tree_kernel<D, SPLIT, T, true>);
+    constexpr int kAlone = D == 128 && SPLIT == 2 ? 1 : 2;
+    if (a.per_cu == 1) a.d.window == 0 ? go(attend_tree_kernel<D, SPLIT, T, false, kAlone>) : go(attend_tree_kernel<D, SPLIT, T, true, kAlone>);
+    else a.d.window == 0 ? go(attend_tree_kernel<D, SPLIT, T, false, 2>) : go(attend_tree_kernel<D, SPLIT, T, true, 2>);
     if (a.splits == 1) return;
     join_tree_kernel<D, T><<<dim3(a.tiles * (kTreeRows * D / 1024), tiles.y, tiles.z), 256, 0, stream>>>(a);
 }

@@ -117,6 +117,7 @@ struct TreeArgs {
     uint32_t tiles;       // of the largest sequence
     uint32_t splits;      // the most workgroups that share a tile
     uint32_t cus;         // to deal the units to
+    uint32_t per_cu;      // workgroups that a CU takes
     uint32_t workgroups;  // launched
     float *partials;      // of each workgroup [row][D], then of each [m, l, e][row]
     TreeJob *jobs;        // [sequence][tile][head]

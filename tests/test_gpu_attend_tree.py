@@ -418,3 +418,45 @@ def test_many_query_heads_of_a_kv_head(cuda, group):
     out, lse = cache.attend_tree(step, q, k, v, seen, scale=1.0, lse=True)
     assert torch.equal(out, v.expand(n, group, dim))
     assert ((lse - head.float()).abs() <= 2.0 ** -20 * head.float().abs() + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("dtype,n,kv_heads,dim", [("f32", 40, 2, 128), ("bf16", 70, 2, 128), ("f16", 100, 1, 64), ("f32", 9, 8, 64)])
+def test_long_and_short_sequences_together(cuda, dtype, n, kv_heads, dim):
+    """Lengths of every size and tables as wide as the longest: each sequence
+    alone gives what the batch gives, up to the order of its parts (fp32
+    accumulators, two fp16 parts: 2^-18 of the largest; 16-bit outputs a rounding
+    apart)."""
+    from q4rdna import api
+    r = np.random.RandomState(n)
+    past = [int(x) for x in np.exp(r.uniform(0, np.log(9000), n))]
+    count = [int(x) for x in r.randint(0, 20, n)]
+    width = max(past) // 64 + 1
+    pages = sum(p // 64 + 1 for p in past)
+    cache = api.KVCache.empty(pages, n, kv_heads, dim)
+    order, rows, at = r.permutation(pages), np.full((n, width), -1), 0
+    for i, p in enumerate(past):
+        rows[i, :p // 64 + 1] = order[at:at + p // 64 + 1]
+        at += p // 64 + 1
+    ints = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    table, slots, starts = ints(rows), ints(r.permutation(n)), lambda c: ints(np.concatenate([[0], np.cumsum(c)]))  # noqa: E731
+    torch.manual_seed(n)
+    t = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    k, v = torch.randn(2, sum(past), kv_heads, dim, device="cuda", dtype=t)
+    cache.append(api.KVBatch(ints([0] * n), table, starts(past), slots, max_tokens=max(past)), k, v)
+    total = sum(count)
+    q, dk, dv = (torch.randn(total, h, dim, device="cuda", dtype=t) for h in (4 * kv_heads, kv_heads, kv_heads))
+    step = api.KVBatch(ints(past), table, starts(count), slots, max_tokens=20)
+    up = [j - 1 if r.rand() < 0.7 else max(j - 3, -1) for c in count for j in range(c)]
+    _, seen = api.tree(step, ints(up))
+    out, lse = cache.attend_tree(step, q, dk, dv, seen, lse=True)
+    assert cache.faults() == 0
+    at = 0
+    for i in range(n):
+        rows = slice(at, at + count[i])
+        at += count[i]
+        if count[i]:
+            one = api.KVBatch(ints(past[i:i + 1]), table[i:i + 1], starts(count[i:i + 1]), slots[i:i + 1], max_tokens=20)
+            a, b = cache.attend_tree(one, q[rows], dk[rows], dv[rows], seen[rows], lse=True)
+            step_of = 2.0 ** -18 if dtype == "f32" else torch.finfo(t).eps
+            assert ((a.float() - out[rows].float()).abs() <= step_of * a.float().abs().amax(-1, keepdim=True)).all()
+            assert ((b - lse[rows]).abs() <= 2.0 ** -18 * (1 + b.abs())).all()
