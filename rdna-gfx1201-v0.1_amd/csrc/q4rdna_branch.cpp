@@ -65,8 +65,9 @@ int rotate(const q4rdna_rotate_desc *desc, void *stream) {
     a.heads = static_cast<uint32_t>(heads);
     a.heads_magic = magic_of(a.heads);
     a.rows = static_cast<uint32_t>(rows);
-    // As q4rdna_kv_append has it for q.
-    a.unit_rows = rows <= 4096 ? 2048 / d.head_dim : 16384 / d.head_dim;
+    // A row for each group of lanes of a workgroup, or two where there are many (61 MB:
+    // one 17.1 us, two 16.1, four 16.3, eight 17.5).
+    a.unit_rows = rows <= 4096 ? 2048 / d.head_dim : 4096 / d.head_dim;
     a.wide = (d.q_heads == 0 || (wide_rows(d.q, d.dtype, 4) && wide_rows(d.q_out, d.dtype, 4))) &&
              (d.k_heads == 0 || (wide_rows(d.k, d.dtype, 4) && wide_rows(d.k_out, d.dtype, 4)));
     if ((rows + a.unit_rows - 1) / a.unit_rows > most_workgroups(256))

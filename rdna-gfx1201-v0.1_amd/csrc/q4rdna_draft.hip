@@ -50,13 +50,13 @@ __global__ __launch_bounds__(256) void tree_kernel(const q4rdna_kv_batch b, cons
     seen[first + lane] = bad ? 0 : static_cast<uint64_t>(high) << 32 | low;
 }
 
-// a.unit_rows rows (token, head of q and then of k), kEach per group of D / 8
-// lanes in flight.  A row is read and written once: 16 tokens of 32 and 8 heads by
-// 128 in fp32 3.7 us, a chain of loads (position, cosines); 61 MB in bf16 16.7 us,
-// 3.7 TB/s.
+// a.unit_rows rows (token, head of q and then of k), one at a time for a group of
+// D / 8 lanes.  A row is read and written once: 16 tokens of 32 and 8 heads by 128
+// in fp32 3.5 us, a chain of loads (position, cosines); 61 MB in bf16 16.1 us, 3.8
+// TB/s (two rows of a group in flight 16.6, with fewer waves on a CU).
 template <int D, bool INTERLEAVED, typename T>
 __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
-    constexpr int kLanes = D / 8, kRows = 256 / kLanes, kEach = 2;
+    constexpr int kLanes = D / 8, kRows = 256 / kLanes;
     const int lane = threadIdx.x % kLanes;
     const Place at = place_of<INTERLEAVED>(lane, a.d.rotary);
     Weights q_weights, k_weights;
@@ -65,44 +65,26 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
     const uint32_t row_first = blockIdx.x * a.unit_rows, row_end = min(a.rows - row_first, a.unit_rows);
     // One division per workgroup, a multiplication per row.
     const uint32_t n_first = row_first / a.heads, head_first = row_first - n_first * a.heads;
-    for (uint32_t x0 = threadIdx.x / kLanes; x0 < row_end; x0 += kEach * kRows) {
-        Row r[kEach];
-        Turn turn[kEach];
-        T *out[kEach];
-        bool live[kEach], is_k[kEach];
-        int position[kEach];
+    for (uint32_t x = threadIdx.x / kLanes; x < row_end; x += kRows) {
+        const uint32_t local = head_first + x, token = div_split(local, a.heads, a.heads_magic);
+        const uint32_t n = n_first + token, h = local - token * a.heads;
+        const bool is_k = h >= a.d.q_heads;
+        const uint32_t head = is_k ? h - a.d.q_heads : h;
+        const q4rdna_kv_rows &in = is_k ? a.d.k : a.d.q, &to = is_k ? a.d.k_out : a.d.q_out;
+        const int position = a.d.rotary != 0 ? a.d.position[n] : 0;
+        Row r;
+        load_row(r, static_cast<const T *>(in.data) + static_cast<int64_t>(n) * in.token_stride + head * in.head_stride, at, a.wide != 0);
+        const bool there = static_cast<uint32_t>(position) < a.d.positions;
+        Turn turn;
+        load_turn(turn, at, a.d.cos, a.d.sin, a.d.rotary, there ? position : 0);
+        if (a.d.rotary != 0 && !there)
 #pragma unroll
-        for (int x = 0; x < kEach; ++x) {
-            live[x] = x0 + x * kRows < row_end;
-            const uint32_t local = head_first + (live[x] ? x0 + x * kRows : 0), token = div_split(local, a.heads, a.heads_magic);
-            const uint32_t n = n_first + token, h = local - token * a.heads;
-            is_k[x] = h >= a.d.q_heads;
-            const uint32_t head = is_k[x] ? h - a.d.q_heads : h;
-            const q4rdna_kv_rows &in = is_k[x] ? a.d.k : a.d.q, &to = is_k[x] ? a.d.k_out : a.d.q_out;
-            out[x] = static_cast<T *>(to.data) + static_cast<int64_t>(n) * to.token_stride + head * to.head_stride;
-            if (live[x]) {
-                position[x] = a.d.rotary != 0 ? a.d.position[n] : 0;
-                load_row(r[x], static_cast<const T *>(in.data) + static_cast<int64_t>(n) * in.token_stride + head * in.head_stride,
-                         at, a.wide != 0);
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < kEach; ++x)
-            if (live[x]) {
-                const bool there = static_cast<uint32_t>(position[x]) < a.d.positions;
-                load_turn(turn[x], at, a.d.cos, a.d.sin, a.d.rotary, there ? position[x] : 0);
-                if (a.d.rotary != 0 && !there)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) r[x].a[e] = r[x].b[e] = __builtin_nanf("");
-            }
-#pragma unroll
-        for (int x = 0; x < kEach; ++x)
-            if (live[x]) {
-                if (is_k[x] ? a.d.k_norm != nullptr : a.d.q_norm != nullptr) norm_row<D>(r[x], is_k[x] ? k_weights : q_weights, a.d.eps);
-                turn_row<INTERLEAVED>(r[x], at, turn[x]);
-                store_floats<T, 4>(out[x] + at.a_at, a.wide != 0, r[x].a);
-                store_floats<T, 4>(out[x] + at.b_at, a.wide != 0, r[x].b);
-            }
+            for (int e = 0; e < 4; ++e) r.a[e] = r.b[e] = __builtin_nanf("");
+        if (is_k ? a.d.k_norm != nullptr : a.d.q_norm != nullptr) norm_row<D>(r, is_k ? k_weights : q_weights, a.d.eps);
+        turn_row<INTERLEAVED>(r, at, turn);
+        T *out = static_cast<T *>(to.data) + static_cast<int64_t>(n) * to.token_stride + head * to.head_stride;
+        store_floats<T, 4>(out + at.a_at, a.wide != 0, r.a);
+        store_floats<T, 4>(out + at.b_at, a.wide != 0, r.b);
     }
 }
 
