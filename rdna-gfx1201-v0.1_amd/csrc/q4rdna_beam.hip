@@ -12,7 +12,7 @@
 // count-th largest of them is a bound that `count` items at least reach, and
 // few more.  These go to LDS and each counts how many are before it.  Equal
 // logits are told apart by their token, so a bound always cuts; where more items
-// reach it than LDS takes, the bound is raised by halving.
+// reach it than LDS takes, the count-th of those that LDS has is the next bound.
 //
 // The logits are read once, at far less than a copy's rate: what takes the time
 // is one thing after another, load, bound, order, arrival, sums, totals, order.
@@ -49,14 +49,10 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
 //  Total   a continuation: by its total, then by row, logit and token.
 struct Pick {
     uint64_t key;
-    static constexpr int kParts = 1;
-    __device__ __forceinline__ uint64_t &part(int) { return key; }
     __device__ __forceinline__ bool before(const Pick &o) const { return key > o.key; }
 };
 struct Total {
     uint64_t key, place;
-    static constexpr int kParts = 2;
-    __device__ __forceinline__ uint64_t &part(int i) { return i == 0 ? key : place; }
     __device__ __forceinline__ bool before(const Total &o) const { return key > o.key || (key == o.key && place > o.place); }
 };
 __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
@@ -75,15 +71,16 @@ struct Select {
     uint64_t group[128];
     uint32_t ranks[4][128];
     uint32_t count;
+    Item chosen;
 };
 
 // A key that `count` of the workgroup's threads' largest keys, `mine`, taken
-// together by two (count > 64) or four threads, at least reach: the count-th of
+// together by two (count > 32) or four threads, at least reach: the count-th of
 // them; 1 where fewer are not zero.
 template <typename Item>
 __device__ __forceinline__ uint64_t count_th(Select<Item> &s, uint32_t count, uint64_t mine) {
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    const bool pairs = count > 64;
+    const bool pairs = count > 32;
     uint64_t g = max_dpp<kDppXor1>(mine);
     if (!pairs) g = max_dpp<kDppXor2>(g);
     if (tid % (pairs ? 2 : 4) == 0) s.group[tid / (pairs ? 2 : 4)] = g;
@@ -117,36 +114,6 @@ __device__ __forceinline__ uint64_t count_th(Select<Item> &s, uint32_t count, ui
     uint64_t key = found(a, lane);
     if (pairs && key == 0) key = found(b, lane + 64);
     return key != 0 ? key : 1;
-}
-
-// How many of the items that each(f) calls f with reach a bound: in `counter`,
-// which is zero before and after.
-template <typename Item, typename Each>
-__device__ __forceinline__ uint32_t reach(uint32_t *counter, const Item &bound, Each each) {
-    uint32_t n = 0;
-    each([&](const Item &x) { n += !bound.before(x); });
-    if (n != 0) atomicAdd(counter, n);
-    __syncthreads();
-    const uint32_t all = *counter;
-    __syncthreads();
-    if (threadIdx.x == 0) *counter = 0;
-    __syncthreads();
-    return all;
-}
-// Where more items reach a bound than LDS takes: the count-th item itself, by
-// halving its key and then its place.
-template <typename Item, typename Each>
-__device__ __forceinline__ Item count_th_item(uint32_t *counter, uint32_t count, Item bound, Each each) {
-    for (int part = 0; part < Item::kParts; ++part) {
-        uint64_t &low = bound.part(part);  // reached by enough
-        uint64_t high = ~0ull;             // not reached by enough
-        while (high - low > 1) {
-            Item mid = bound;
-            mid.part(part) = low + (high - low) / 2;
-            (reach(counter, mid, each) >= count ? low : high) = mid.part(part);
-        }
-    }
-    return bound;
 }
 
 // The `count` first of the `n` items in LDS, count <= 128, in order: take(r, item)
@@ -189,27 +156,50 @@ __device__ __forceinline__ uint32_t held_count(const Select<Item> &s) {
 }
 // A thread's share of the first `n` items that are held.
 constexpr int kShare = static_cast<int>(kHeld) / kBeamThreads;
-__device__ __forceinline__ void share_of(const Select<Pick> &s, uint32_t n, Pick (&share)[kShare]) {
+template <typename Item>
+__device__ __forceinline__ void share_of(const Select<Item> &s, uint32_t n, Item (&share)[kShare]) {
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {
         const uint32_t at = threadIdx.x + i * kBeamThreads;
-        share[i] = at < n ? s.held[at] : Pick{0};
+        share[i] = at < n ? s.held[at] : Item{};
     }
 }
 // Of n <= kHeld items that are held, those that reach a higher bound, `count` at
 // least: how many.
-__device__ __forceinline__ uint32_t tighten(Select<Pick> &s, uint32_t count, uint32_t n, Pick &bound) {
-    Pick share[kShare];
+template <typename Item>
+__device__ __forceinline__ uint32_t tighten(Select<Item> &s, uint32_t count, uint32_t n, Item &bound) {
+    Item share[kShare];
     share_of(s, n, share);
     uint64_t mine = 0;
 #pragma unroll
     for (int i = 0; i < kShare; ++i) mine = max(mine, share[i].key);
     let_go(s);
-    bound.key = max(bound.key, count_th(s, count, mine));
+    const uint64_t key = count_th(s, count, mine);
+    if (key > bound.key) bound = Item{key};
 #pragma unroll
     for (int i = 0; i < kShare; ++i)
         if (share[i].key != 0) hold(s, bound, share[i]);
     return held_count(s);
+}
+// Where more items reach the bound than LDS takes: the count-th of the kHeld that
+// are held, which as many of all reach.  Nothing is held afterwards.  (Each time
+// all but count of these fall behind, and of others as many as they stand for.)
+template <typename Item>
+__device__ __noinline__ void raise(Select<Item> &s, uint32_t count, Item *bound) {
+    uint32_t n = kHeld;
+    for (uint32_t last = 2 * n; n > 2 * count && 4 * n < 3 * last;) {
+        last = n;
+        n = tighten(s, count, n, *bound);
+    }
+    for (uint32_t i = threadIdx.x; i < n; i += kBeamThreads) {
+        const Item x = s.held[i];
+        uint32_t r = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; ++j) r += s.held[j].before(x);
+        if (r == count - 1) s.chosen = x;
+    }
+    let_go(s);
+    *bound = s.chosen;
 }
 
 // The sum over a wave, in every lane.
@@ -320,18 +310,16 @@ __device__ __noinline__ void overflown(Select<Pick> &s, const T *p, uint32_t bas
             if (x == x) f(Pick{static_cast<uint64_t>(ordered(x)) << 32 | static_cast<uint32_t>(~(base + i))});
         }
     };
-    let_go(s);
-    *bound = count_th_item(&s.count, count, *bound, [&](auto f) {
-        trip(f);
-        for (uint32_t i = threadIdx.x; i < before; i += kBeamThreads) f(s.held[i]);
-    });
     Pick share[kShare];
     share_of(s, before, share);
     __syncthreads();
+    do {
+        raise(s, count, bound);
 #pragma unroll
-    for (int i = 0; i < kShare; ++i)
-        if (share[i].key != 0) hold(s, *bound, share[i]);
-    trip([&](const Pick &x) { hold(s, *bound, x); });
+        for (int i = 0; i < kShare; ++i)
+            if (share[i].key != 0) hold(s, *bound, share[i]);
+        trip([&](const Pick &x) { hold(s, *bound, x); });
+    } while (held_count(s) > kHeld);
 }
 
 template <typename T>
@@ -524,9 +512,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         every([&](const Total &t) { hold(g, least, t); });
     }
     uint32_t found = held_count(g);
-    if (found > kHeld) {
-        let_go(g);
-        least = count_th_item(&g.count, count, least, every);
+    while (found > kHeld) {
+        raise(g, count, &least);
         every([&](const Total &t) { hold(g, least, t); });
         found = held_count(g);
     }

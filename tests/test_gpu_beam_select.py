@@ -173,3 +173,30 @@ def test_scores_in_place(cuda, beams):
     want = api.beam_select(logits, scores, beams)
     got = api.beam_select(logits, scores, beams, out=(scores, torch.empty_like(want[1]), torch.empty_like(want[2])))
     assert got[0] is scores and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("beams,vocab,count", [(32, 392, 64), (256, 150, 128), (200, 300, 33), (17, 5000, 128), (256, 4097, 16)])
+@pytest.mark.parametrize("spread", [0.0, 0.5, 30.0])
+def test_beams_far_apart(cuda, beams, vocab, count, spread):
+    """One beam's best are all before the next one's, rising and falling, and
+    all beams alike: more candidates than are ordered at a time reach any first
+    bound."""
+    logits = normal((3, beams, vocab), "f32", beams + count, 2.0)
+    logits[2] = logits[2, :1]
+    scores = spread * torch.arange(beams, dtype=torch.float32).expand(3, beams).clone()
+    scores[1] = -scores[1]
+    scores[2] = spread * torch.randn(beams, generator=torch.Generator().manual_seed(count))
+    check(logits, scores.cuda(), count)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("count", [1, 33, 128])
+def test_masked_vocabularies(cuda, dtype, count):
+    """Few tokens allowed, the others -inf: those come behind, by token."""
+    logits = normal((4, 5, 30011), dtype, count, 2.0)
+    g = torch.Generator().manual_seed(count)
+    for i, share in enumerate((0.001, 0.00004, 0.2, 0.0)):
+        allowed = torch.rand((5, 30011), generator=g) < share
+        allowed[0, 12345] = True
+        logits[i].masked_fill_(~allowed.cuda(), float("-inf"))
+    check(logits, normal((4, 5), "f32", count + 1), count)
