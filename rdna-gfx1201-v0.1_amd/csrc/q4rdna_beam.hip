@@ -133,11 +133,13 @@ __device__ __forceinline__ void take_first(const Select<Item> &s, uint32_t n, ui
         if (r < count) take(r, x);
     }
 }
+// Whether x reaches the bound.
 template <typename Item>
-__device__ __forceinline__ void hold(Select<Item> &s, const Item &bound, const Item &x) {
-    if (bound.before(x)) return;
+__device__ __forceinline__ bool hold(Select<Item> &s, const Item &bound, const Item &x) {
+    if (bound.before(x)) return false;
     const uint32_t at = atomicAdd(&s.count, 1u);
     if (at < kHeld) s.held[at] = x;
+    return true;
 }
 // Sets the count of what is held to zero, between barriers.
 template <typename Item>
@@ -420,7 +422,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
     // A list to each thread, its first items to the first ones, and so on: the
     // threads' maxima are near each other.  Where these are few a thread they
     // stay in registers, and are under way while the sums are added up.
-    const uint32_t items = lists * count, width = 1u << (32 - __builtin_clz(max(lists, 2u) - 1));  // of a row of threads
+    const uint32_t width = 1u << (32 - __builtin_clz(max(lists, 2u) - 1));  // of a row of threads
     constexpr int kKept = 4;
     const bool few = width <= kBeamThreads && count <= kKept * (kBeamThreads / width);
     const uint32_t my_list = tid & (width - 1), my_first = tid / width, my_step = kBeamThreads / width;
@@ -480,12 +482,27 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         a.d.out_rows[at] = static_cast<int32_t>(group * a.d.beams + static_cast<uint32_t>(~t.place >> 56));
         a.d.out_tokens[at] = static_cast<int32_t>(static_cast<uint32_t>(~t.place) & 0xffffffu);
     };
+    // Otherwise a thread has a block of neighbours of a list, or of several lists.
+    // These are sorted: f(t) is called from the first on until it is false.
+    const uint32_t across = min(width, static_cast<uint32_t>(kBeamThreads)), in_block = (count + kBeamThreads / across - 1) / (kBeamThreads / across);
+    const uint32_t block = tid / across * in_block, block_end = min(block + in_block, count);
     const auto every = [&](auto f) {
 #pragma unroll 1
-        for (uint32_t i = tid; i < items; i += kBeamThreads) {
-            const uint32_t r = i / lists, list = i - r * lists;
-            const Total t = item(r, list, list / a.chunks, load_agent64(tops + i));
-            if (t.key != 0) f(t);
+        for (uint32_t list = tid & (across - 1); list < lists; list += across) {
+            const uint32_t b = list / a.chunks;
+            bool on = true;
+#pragma unroll 1
+            for (uint32_t r = block; on && r < block_end; r += 4) {
+                uint64_t top[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[i] = load_agent64(tops + static_cast<size_t>(min(r + i, block_end - 1)) * lists + list);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (on && r + i < block_end) {
+                        const Total t = item(r + i, list, b, top[i]);
+                        on = t.key != 0 && f(t);
+                    }
+            }
         }
     };
     Select<Total> &g = select.group;
@@ -507,14 +524,25 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         for (int i = 0; i < kKept; ++i)
             if (i * my_step < count) hold(g, least, t[i]);
     } else {
-        every([&](const Total &t) { best = max(best, t.key); });
+        // The blocks' first items bound as above; their last ones stand for a block each.
+        uint64_t last = 0;
+#pragma unroll 1
+        for (uint32_t list = tid & (across - 1); block < count && list < lists; list += across) {
+            const uint32_t b = list / a.chunks;
+            const uint64_t top = load_agent64(tops + static_cast<size_t>(block) * lists + list);
+            const uint64_t end = load_agent64(tops + static_cast<size_t>(block_end - 1) * lists + list);
+            best = max(best, item(block, list, b, top).key);
+            if (block_end - block == in_block) last = max(last, item(block_end - 1, list, b, end).key);
+        }
         least.key = count_th(g, count, best);
-        every([&](const Total &t) { hold(g, least, t); });
+        __syncthreads();
+        least.key = max(least.key, count_th(g, (count + in_block - 1) / in_block, last));
+        every([&](const Total &t) { return hold(g, least, t); });
     }
     uint32_t found = held_count(g);
     while (found > kHeld) {
         raise(g, count, &least);
-        every([&](const Total &t) { hold(g, least, t); });
+        every([&](const Total &t) { return hold(g, least, t); });
         found = held_count(g);
     }
     take_first(g, found, count, take);
