@@ -482,29 +482,6 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         a.d.out_rows[at] = static_cast<int32_t>(group * a.d.beams + static_cast<uint32_t>(~t.place >> 56));
         a.d.out_tokens[at] = static_cast<int32_t>(static_cast<uint32_t>(~t.place) & 0xffffffu);
     };
-    // Otherwise a thread has a block of neighbours of a list, or of several lists.
-    // These are sorted: f(t) is called from the first on until it is false.
-    const uint32_t across = min(width, static_cast<uint32_t>(kBeamThreads)), in_block = (count + kBeamThreads / across - 1) / (kBeamThreads / across);
-    const uint32_t block = tid / across * in_block, block_end = min(block + in_block, count);
-    const auto every = [&](auto f) {
-#pragma unroll 1
-        for (uint32_t list = tid & (across - 1); list < lists; list += across) {
-            const uint32_t b = list / a.chunks;
-            bool on = true;
-#pragma unroll 1
-            for (uint32_t r = block; on && r < block_end; r += 4) {
-                uint64_t top[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top[i] = load_agent64(tops + static_cast<size_t>(min(r + i, block_end - 1)) * lists + list);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (on && r + i < block_end) {
-                        const Total t = item(r + i, list, b, top[i]);
-                        on = t.key != 0 && f(t);
-                    }
-            }
-        }
-    };
     Select<Total> &g = select.group;
     if (tid == 0) g.count = 0;
     uint64_t best = 0;
@@ -524,6 +501,30 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         for (int i = 0; i < kKept; ++i)
             if (i * my_step < count) hold(g, least, t[i]);
     } else {
+        // A thread has a block of neighbours of a list, or of several lists.
+        // These are sorted: f(t) is called from the first on until it is false.
+        const uint32_t across_log2 = min(31 - __builtin_clz(width), 8), across = 1u << across_log2;
+        const uint32_t in_block = (count + (kBeamThreads >> across_log2) - 1) >> (8 - across_log2);
+        const uint32_t block = (tid >> across_log2) * in_block, block_end = min(block + in_block, count);
+        const auto every = [&](auto f) {
+#pragma unroll 1
+            for (uint32_t list = tid & (across - 1); list < lists; list += across) {
+                const uint32_t b = list / a.chunks;
+                bool on = true;
+#pragma unroll 1
+                for (uint32_t r = block; on && r < block_end; r += 4) {
+                    uint64_t top[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top[i] = load_agent64(tops + static_cast<size_t>(min(r + i, block_end - 1)) * lists + list);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (on && r + i < block_end) {
+                            const Total t = item(r + i, list, b, top[i]);
+                            on = t.key != 0 && f(t);
+                        }
+                }
+            }
+        };
         // The blocks' first items bound as above; their last ones stand for a block each.
         uint64_t last = 0;
 #pragma unroll 1
@@ -538,13 +539,12 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         __syncthreads();
         least.key = max(least.key, count_th(g, (count + in_block - 1) / in_block, last));
         every([&](const Total &t) { return hold(g, least, t); });
+        while (held_count(g) > kHeld) {
+            raise(g, count, &least);
+            every([&](const Total &t) { return hold(g, least, t); });
+        }
     }
-    uint32_t found = held_count(g);
-    while (found > kHeld) {
-        raise(g, count, &least);
-        every([&](const Total &t) { return hold(g, least, t); });
-        found = held_count(g);
-    }
+    const uint32_t found = held_count(g);
     take_first(g, found, count, take);
 }
 
