@@ -49,10 +49,12 @@ __device__ __forceinline__ double unordered64(uint64_t u) {
 //  Total   a continuation: by its total, then by row, logit and token.
 struct Pick {
     uint64_t key;
+    static constexpr bool kPlaced = false;
     __device__ __forceinline__ bool before(const Pick &o) const { return key > o.key; }
 };
 struct Total {
     uint64_t key, place;
+    static constexpr bool kPlaced = true;  // keys may be alike, places not
     __device__ __forceinline__ bool before(const Total &o) const { return key > o.key || (key == o.key && place > o.place); }
 };
 __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
@@ -167,32 +169,48 @@ __device__ __forceinline__ void share_of(const Select<Item> &s, uint32_t n, Item
     }
 }
 // Of n <= kHeld items that are held, those that reach a higher bound, `count` at
-// least: how many.
-template <typename Item>
+// least: how many.  By keys, or by places among those with the bound's key.
+template <bool PLACES, typename Item>
 __device__ __forceinline__ uint32_t tighten(Select<Item> &s, uint32_t count, uint32_t n, Item &bound) {
     Item share[kShare];
     share_of(s, n, share);
     uint64_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) mine = max(mine, share[i].key);
+    for (int i = 0; i < kShare; ++i) {
+        uint64_t at = share[i].key;
+        if constexpr (PLACES) at = share[i].key > bound.key ? ~uint64_t{0} : share[i].place;
+        mine = max(mine, at);  // (of one type: max() of two would be a double's)
+    }
     let_go(s);
-    const uint64_t key = count_th(s, count, mine);
-    if (key > bound.key) bound = Item{key};
+    const uint64_t at = count_th(s, count, mine);
+    if constexpr (PLACES) bound.place = max(bound.place, at);
+    else if (at > bound.key) bound = Item{at};
 #pragma unroll
     for (int i = 0; i < kShare; ++i)
         if (share[i].key != 0) hold(s, bound, share[i]);
     return held_count(s);
+}
+// The same until few are left, or a step leaves out less than a quarter.
+__device__ __forceinline__ uint32_t few_of(uint32_t count) { return 2 * count + 64; }
+template <typename Item>
+__device__ __noinline__ uint32_t shrink(Select<Item> &s, uint32_t count, uint32_t n, Item *bound) {
+    Item b = *bound;
+    for (bool on = true; on && n > few_of(count);) {
+        uint32_t last = n;
+        n = tighten<false>(s, count, n, b);
+        if constexpr (Item::kPlaced)
+            if (4 * n > 3 * last) n = tighten<true>(s, count, last = n, b);
+        on = 4 * n <= 3 * last;
+    }
+    *bound = b;
+    return n;
 }
 // Where more items reach the bound than LDS takes: the count-th of the kHeld that
 // are held, which as many of all reach.  Nothing is held afterwards.  (Each time
 // all but count of these fall behind, and of others as many as they stand for.)
 template <typename Item>
 __device__ __noinline__ void raise(Select<Item> &s, uint32_t count, Item *bound) {
-    uint32_t n = kHeld;
-    for (uint32_t last = 2 * n; n > 2 * count && 4 * n < 3 * last;) {
-        last = n;
-        n = tighten(s, count, n, *bound);
-    }
+    const uint32_t n = shrink(s, count, kHeld, bound);
     for (uint32_t i = threadIdx.x; i < n; i += kBeamThreads) {
         const Item x = s.held[i];
         uint32_t r = 0;
@@ -382,15 +400,15 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
             if (__builtin_amdgcn_ballot_w64(!(tops_of[g] < least)) != 0) {
 #pragma unroll
                 for (int e = 8 * g; e < 8 * g + 8; ++e)
-                    if (x[e] >= least) hold(s, bound, Pick{static_cast<uint64_t>(ordered(x[e])) << 32 | static_cast<uint32_t>(~token_of<T>(base, e))});
+                    if (x[e] >= least && token_of<T>(base, e) < a.d.vocab) hold(s, bound, Pick{static_cast<uint64_t>(ordered(x[e])) << 32 | static_cast<uint32_t>(~token_of<T>(base, e))});
             }
         const uint32_t before = n;
         n = held_count(s);
         if (n > kHeld) {
             overflown<T>(s, p, base, a.d.vocab, before, count, &bound);
             n = held_count(s);
-        } else if (n > (trip < trips ? kHeld / 2 : 2 * count + 64)) {
-            n = tighten(s, count, n, bound);
+        } else if (n > (trip < trips ? kHeld / 2 : few_of(count))) {
+            n = shrink(s, count, n, &bound);
         }
     }
     take_first(s, n, count, [&](uint32_t r, const Pick &i) {
@@ -433,38 +451,63 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         kept[i] = few && my_list < lists && r < count ? load_agent64(tops + static_cast<size_t>(r) * lists + my_list) : 0;
     }
     const uint32_t parts = a.chunks * kBeamWaves;
-    for (uint32_t b = wave; b < a.d.beams; b += 4) {
-        const uint32_t r = group * a.d.beams + b;
-        const float score = a.d.scores == nullptr ? 0.0f : a.d.scores[r];
-        double lse = __builtin_nan(""), sum_of = 0.0;
-        float most_of = -__builtin_inff();  // what the lane's parts are relative to
-        constexpr int kParts = 4;           // of a lane, under way together
-#pragma unroll 1
-        for (uint32_t c0 = lane; c0 < parts; c0 += 64 * kParts) {
-            float most[kParts], now = most_of;
-            double sum[kParts];
-#pragma unroll
-            for (int i = 0; i < kParts; ++i) {
-                const uint32_t c = c0 + 64 * i;
-                const uint64_t *stat = stats + (static_cast<size_t>(b) * parts + min(c, parts - 1)) * 2;
-                sum[i] = __builtin_bit_cast(double, load_agent64(stat));
-                most[i] = c < parts ? __uint_as_float(static_cast<uint32_t>(load_agent64(stat + 1))) : -__builtin_inff();
-            }
-#pragma unroll
-            for (int i = 0; i < kParts; ++i) now = fmaxf(now, most[i]);
-            const float to = now == -__builtin_inff() ? 0.0f : now;
-            sum_of *= __builtin_amdgcn_exp2f((most_of - to) * kLog2e);
-#pragma unroll
-            for (int i = 0; i < kParts; ++i) sum_of += sum[i] * __builtin_amdgcn_exp2f((most[i] - to) * kLog2e);
-            most_of = now;
-        }
+    const bool my_beam_is = static_cast<uint32_t>(tid) < a.d.beams;
+    const float my_score = my_beam_is && a.d.scores != nullptr ? a.d.scores[group * a.d.beams + tid] : 0.0f;
+    // A wave's lanes have a beam's sums, relative to most_of.
+    const auto set_sum = [&](uint32_t b, float most_of, double sum_of) {
         const float m = wave_max(most_of);
-        if (__builtin_fabsf(score) < __builtin_inff() && __builtin_fabsf(m) < __builtin_inff())
-            lse = static_cast<double>(m) + log_of(wave_sum(sum_of * __builtin_amdgcn_exp2f((most_of - m) * kLog2e)));
+        const double all = wave_sum(sum_of * __builtin_amdgcn_exp2f((most_of - m) * kLog2e));
         if (lane == 0) {
-            beam_lse[b] = lse;
-            beam_score[b] = score;
+            beam_lse[b] = all;
+            beam_score[b] = m;
         }
+    };
+    const auto load_part = [&](uint32_t b, uint32_t c, double &sum, float &most) {
+        const uint64_t *stat = stats + (static_cast<size_t>(b) * parts + min(c, parts - 1)) * 2;
+        sum = __builtin_bit_cast(double, load_agent64(stat));
+        most = c < parts ? __uint_as_float(static_cast<uint32_t>(load_agent64(stat + 1))) : -__builtin_inff();
+    };
+    if (parts <= 64) {  // one part a lane, several beams under way together
+        constexpr int kBeams = 4;
+#pragma unroll 1
+        for (uint32_t b0 = wave; b0 < a.d.beams; b0 += 4 * kBeams) {
+            float most[kBeams];
+            double sum[kBeams];
+#pragma unroll
+            for (int i = 0; i < kBeams; ++i) load_part(min(b0 + 4 * i, a.d.beams - 1), lane, sum[i], most[i]);
+#pragma unroll
+            for (int i = 0; i < kBeams; ++i)
+                if (b0 + 4 * i < a.d.beams) set_sum(b0 + 4 * i, most[i], most[i] == -__builtin_inff() ? 0.0 : sum[i]);
+        }
+    } else {
+#pragma unroll 1
+        for (uint32_t b = wave; b < a.d.beams; b += 4) {
+            double sum_of = 0.0;
+            float most_of = -__builtin_inff();  // what the lane's parts are relative to
+            constexpr int kParts = 4;           // of a lane, under way together
+#pragma unroll 1
+            for (uint32_t c0 = lane; c0 < parts; c0 += 64 * kParts) {
+                float most[kParts], now = most_of;
+                double sum[kParts];
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) load_part(b, c0 + 64 * i, sum[i], most[i]);
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) now = fmaxf(now, most[i]);
+                const float to = now == -__builtin_inff() ? 0.0f : now;
+                sum_of *= __builtin_amdgcn_exp2f((most_of - to) * kLog2e);
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) sum_of += sum[i] * __builtin_amdgcn_exp2f((most[i] - to) * kLog2e);
+                most_of = now;
+            }
+            set_sum(b, most_of, sum_of);
+        }
+    }
+    __syncthreads();
+    if (my_beam_is) {  // its sum and maximum make way for its log-sum-exp and score
+        const float m = beam_score[tid];
+        const bool there = __builtin_fabsf(my_score) < __builtin_inff() && __builtin_fabsf(m) < __builtin_inff();
+        beam_lse[tid] = there ? static_cast<double>(m) + log_of(beam_lse[tid]) : __builtin_nan("");
+        beam_score[tid] = my_score;
     }
     __syncthreads();
     // The r-th of a list, of a beam.  A dead beam's items are its first tokens, all
@@ -544,7 +587,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
             every([&](const Total &t) { return hold(g, least, t); });
         }
     }
-    const uint32_t found = held_count(g);
+    uint32_t found = held_count(g);
+    if (found > few_of(count)) found = shrink(g, count, found, &least);
     take_first(g, found, count, take);
 }
 
