@@ -536,10 +536,10 @@ __device__ __forceinline__ TreeItem find_tree_item(const TreeArgs &a) {
     // Where there are as many tiles as CUs and eight units a wave, two for a CU,
     // which share it well, and as large as it takes for the long ones to run at
     // once: a second round costs a whole part's time, while short ones fill the
-    // gaps.  (48 sequences of 100 .. 4000 tokens 58.7 and 48.9 us, 24 of up to 12000 by
+    // gaps.  (The host has launched workgroups for as many.)  (48 sequences of 100 .. 4000 tokens 58.7 and 48.9 us, 24 of up to 12000 by
     // 64 33.3 and 29.3; but one of 60000 39.1 and 44.8.)
     uint32_t chunk = (max(all, 1u) - 1) / a.cus + 1;
-    const bool two = a.per_cu == 2 && jobs >= a.cus && chunk >= 8 * kWaves;
+    const bool two = jobs >= a.cus && chunk >= 8 * kWaves;
     if (two) chunk = (all - 1) / (2 * a.cus) + 1;
     if (a.batch.sequences <= 64 && (two || jobs < a.cus))
         for (int i = 0; i < 12; ++i) {

@@ -111,9 +111,11 @@ int attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, cons
     // where a wave has four units at most.)
     const bool split = most_units > 16 && batch->sequences <= kDealtSequences && jobs <= 16ull * cus && jobs * most_units <= 0x7fffffffu;
     a.splits = static_cast<uint32_t>(split ? std::min<uint64_t>((most_units + 3) / 4, kTreeSplits) : 1);
-    // (By the tables' width; short ones' fp32 kernel needs no scratch with one.)
-    a.per_cu = jobs * most_units > 32ull * cus ? 2 : 1;
-    const uint64_t workgroups = split ? std::min(jobs + a.per_cu * cus, jobs * a.splits) : jobs;
+    // (Blocks by the tables' width.  With one, fp32 needs no scratch: 1% for a few
+    // tokens; with two, more tiles than CUs share them.)
+    const bool many = jobs * most_units > 31ull * cus;
+    a.per_cu = jobs > cus || many ? 2 : 1;
+    const uint64_t workgroups = split ? std::min(jobs + (many ? 2 : 1) * cus, jobs * a.splits) : jobs;
     if (workgroups > most_workgroups(256))
         return set_error(Q4RDNA_ERR_ARGUMENT, "%u sequences of %u kv heads are too many for one call", batch->sequences, cache->kv_heads);
     a.workgroups = static_cast<uint32_t>(workgroups);
