@@ -37,6 +37,12 @@ except AttributeError:  # a torch build without this private function
         return torch.cuda.current_stream(device).cuda_stream
 
 
+try:  # without torch.cuda's initialisation, which has been where there is a tensor
+    _current_device = torch._C._cuda_getDevice
+except AttributeError:
+    _current_device = torch.cuda.current_device
+
+
 def _stream(device: torch.device | int | None = None) -> int:
     if isinstance(device, torch.device):
         device = device.index
@@ -495,9 +501,10 @@ def _out_rows(out: torch.Tensor | None, name: str, like: torch.Tensor, device: i
     """(out, its rows): the one given, or a new one like the input."""
     if out is None:
         out = torch.empty_like(like)
-        if out.stride(2) != 1:
+        token_stride, head_stride, stride = out.stride()
+        if stride != 1:
             out = _packed_like(like)
-        token_stride, head_stride, _ = out.stride()
+            token_stride, head_stride, _ = out.stride()
         return out, (out.data_ptr(), token_stride, head_stride)
     _no_overlap(out, name)
     return out, _rows(out, name, like.dtype, like.shape, device)
@@ -893,7 +900,7 @@ def add_norm(residual: torch.Tensor, y: torch.Tensor | None, weight: torch.Tenso
 
 def _call(device: int, entry, *args) -> None:
     """A call that runs on the current device, on its tensors' one."""
-    if torch.cuda.current_device() == device:
+    if _current_device() == device:
         check(entry(*args))
     else:
         with torch.cuda.device(device):
@@ -944,10 +951,10 @@ def rotate(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
     position outside cos and sin makes the token's rows NaN.  Without cos and
     sin nothing is rotated.  q_out may be q and k_out k."""
     first = k if q is None else q
-    if first is None or first.dim() != 3 or not first.is_cuda:
+    if first is None or first.dim() != 3 or (device := first.get_device()) < 0:
         raise ValueError("q or k must be a CUDA tensor [tokens, heads, head_dim]")
-    device, dtype = first.get_device(), first.dtype
-    tokens, _, dim = first.shape
+    dtype = first.dtype
+    tokens, heads, dim = first.shape
     if stream is not None and (q is not None and q_out is None or k is not None and k_out is None):
         with _on_stream(stream, device):
             return rotate(q, k, positions, cos, sin, interleaved=interleaved, q_norm=q_norm, k_norm=k_norm, eps=eps,
@@ -955,7 +962,7 @@ def rotate(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
     q_heads = k_heads = q_weight = k_weight = 0
     q_rows = q_to = k_rows = k_to = _NO_ROWS
     if q is not None:
-        q_heads = q.shape[1]
+        q_heads = heads
         q_rows = _rows(q, "q", dtype, (tokens, q_heads, dim), device)
         q_out, q_to = _out_rows(q_out, "q_out", q, device)
         if q_norm is not None:
