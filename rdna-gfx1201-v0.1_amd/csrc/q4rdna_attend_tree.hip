@@ -380,76 +380,83 @@ __device__ __forceinline__ void set_query(ManyState<D, SPLIT> &st, const Eight<T
         for (int i = 0; i < 16; ++i) st.o[d][i] = 0.0f;
 }
 
-// The drafted tokens' K and V into LDS: a thread takes eight numbers of four
-// tokens, D / 8 threads side by side a row.
-template <int D, typename T>
+// The drafted tokens' K and V into LDS: a thread takes eight numbers of B tokens,
+// D / 8 threads side by side a row: of four, or, where there are few, of one.
+template <int D, typename T, int B>
 struct DraftRows {
     static constexpr int kOctets = D / 8;
-    Eight<T> raw[2][4];
+    static constexpr int kTokens = B == 1 ? kTreeThreads / kOctets : kBlock;
+    Eight<T> raw[2][B];
     __device__ __forceinline__ static int octet() { return threadIdx.x % kOctets; }
-    __device__ __forceinline__ static int quad() { return threadIdx.x / kOctets; }  // of 16 (the threads behind have none)
+    __device__ __forceinline__ static int token() { return threadIdx.x / kOctets * B; }  // the first
 };
-template <int D, typename T>
-__device__ __forceinline__ void load_drafts(DraftRows<D, T> &r, const TreeArgs &a, int first, int count, uint32_t head) {
-    const int quad = r.quad();
+template <int D, typename T, int B>
+__device__ __forceinline__ void load_drafts(DraftRows<D, T, B> &r, const TreeArgs &a, int first, int count, uint32_t head) {
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         const q4rdna_kv_rows &rows = which == 0 ? a.d.k : a.d.v;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < B; ++b) {
             // (Tokens behind the last one are that one, and seen by nobody.)
-            load_numbers(r.raw[which][b], static_cast<const T *>(rows.data) + static_cast<int64_t>(first + min(4 * quad + b, count - 1)) * rows.token_stride +
+            load_numbers(r.raw[which][b], static_cast<const T *>(rows.data) + static_cast<int64_t>(first + min(r.token() + b, count - 1)) * rows.token_stride +
                                               head * rows.head_stride + 8 * r.octet());
         }
     }
 }
-template <int D, int SPLIT, typename T>
-__device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const DraftRows<D, T> &r) {
-    const int octet = r.octet(), quad = r.quad();
-    if (quad >= kBlock / 4) return;
-    float x[2][4][8];
+template <int D, int SPLIT, typename T, int B>
+__device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const DraftRows<D, T, B> &r) {
+    const int octet = r.octet(), token = r.token();
+    if (token >= kBlock) return;
+    float x[2][B][8];
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < B; ++b) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[which][b][e] = static_cast<float>(r.raw[which][b].v[e]);
             uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[which][b][e]) & 0x7fffffffu);
-            top = lanes_max<DraftRows<D, T>::kOctets>(top);
+            top = lanes_max<DraftRows<D, T, B>::kOctets>(top);
             const bool finite = top < 0x7f800000u;
             // The largest to 2^13 .. 2^14, but for numbers under 2^-96: the scale stays a normal number.
             const int up = finite && top != 0 ? min(14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)), 110) : 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[which][b][e] = finite ? __builtin_amdgcn_ldexpf(x[which][b][e], up) : 0.0f;
-            if (octet == 0) stage.scales[which * kBlock + 4 * quad + b] = finite ? __builtin_amdgcn_ldexpf(1.0f, -up) : __builtin_nanf("");
+            if (octet == 0) stage.scales[which * kBlock + token + b] = finite ? __builtin_amdgcn_ldexpf(1.0f, -up) : __builtin_nanf("");
         }
+    typedef _Float16 Tokens __attribute__((ext_vector_type(B)));
     typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int part = 0; part < SPLIT; ++part) {
         TreeTile<D> &tile = stage.part[part];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < B; ++b) {
             h16x8 k;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 k[e] = static_cast<_Float16>(x[0][b][e]);
                 x[0][b][e] -= static_cast<float>(k[e]);
             }
-            *reinterpret_cast<h16x8 *>(tile.k + (4 * quad + b) * (D + 8) + 8 * octet) = k;
+            *reinterpret_cast<h16x8 *>(tile.k + (token + b) * (D + 8) + 8 * octet) = k;
         }
         // Row d of V: the tokens in the order of the lanes' scores.
-        const int at = (quad & 1) * 32 + (quad >> 1 & 1) * 16 + (quad >> 2) * 4;
+        const int quad = token / 4, at = (quad & 1) * 32 + (quad >> 1 & 1) * 16 + (quad >> 2) * 4 + token % 4;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            h16x4 v;
+            Tokens v;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
+            for (int b = 0; b < B; ++b) {
                 v[b] = static_cast<_Float16>(x[1][b][e]);
                 x[1][b][e] -= static_cast<float>(v[b]);
             }
-            *reinterpret_cast<h16x4 *>(tile.v + v_place(8 * octet + e, at)) = v;
+            *reinterpret_cast<Tokens *>(tile.v + v_place(8 * octet + e, at)) = v;
+        }
+        // The other tokens of the first 32 are zeros (of weight zero; K's are hidden).
+        if constexpr (DraftRows<D, T, B>::kTokens == 16) {
+#pragma unroll
+            for (int i = threadIdx.x; i < 4 * D; i += kTreeThreads)
+                *reinterpret_cast<h16x4 *>(tile.v + v_place(i / 4, i % 4 * 16 + 4)) = h16x4{};
         }
     }
 }
@@ -672,8 +679,13 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
     load_query<D, T>(query, static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(s.first + token) * a.d.q.token_stride +
                                 (head * a.group + (row < rows ? row - token * group : 0)) * a.d.q.head_stride);
     uint64_t seen = a.d.seen[s.first + token];  // of the drafts, by the lane's row
-    DraftRows<D, T> draft_rows;
-    if (has_drafts) load_drafts<D, T>(draft_rows, a, s.first, s.count, head);
+    DraftRows<D, T, 4> draft_rows;
+    DraftRows<D, T, 1> few_rows;
+    const bool few = s.count <= DraftRows<D, T, 1>::kTokens;
+    if (has_drafts) {
+        if (few) load_drafts(few_rows, a, s.first, s.count, head);
+        else load_drafts(draft_rows, a, s.first, s.count, head);
+    }
     tile_end();
     constexpr size_t kPlane = kKvBlock * D;
     const int8_t *head_pages = a.cache.pages + head * (2 * kPlane);
@@ -719,7 +731,8 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
         open_scales[wave][kBlock + lane] = open_scale[1];
     }
     if (has_drafts) {  // the same for the whole workgroup
-        stage_drafts<D, SPLIT, T>(shared.stage, draft_rows);
+        if (few) stage_drafts(shared.stage, few_rows);
+        else stage_drafts(shared.stage, draft_rows);
         __syncthreads();
     }
 
