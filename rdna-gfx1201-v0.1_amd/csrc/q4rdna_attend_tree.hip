@@ -633,7 +633,8 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
     __shared__ __align__(16) float open_scales[kWaves][2 * kBlock];
     const int tid = threadIdx.x, lane = tid & 63, column = lane & 31, half = lane >> 5, wave = wave_id();
     const TreeItem it = find_tree_item(a);
-    if (wave == kWaves - 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1)
+    // (What is rare is told apart: its code goes behind the rest, which is fetched in order.)
+    if (__builtin_expect(wave == kWaves - 1 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1, 0))
         for (uint32_t i = lane; i < a.batch.sequences; i += 64)  // bad entries, once
             if (!draft_seq(a, i).ok) count_fault(a.cache);
     if (it.seq < 0 || !it.s.ok) return;
@@ -695,13 +696,13 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
     f32x2 scale_next = {0.0f, 0.0f};
     Tile tile = planes;
     const auto check_pages = [&](int n) {
-        if (static_cast<uint32_t>(pages) >= page_count) {
+        if (__builtin_expect(static_cast<uint32_t>(pages) >= page_count, 0)) {
             if (n + lane < full) count_fault(a.cache);
             pages = -1;
         }
     };
     const auto next = [&](int n) {
-        if (n % 64 == 0 && n != 0) {
+        if (__builtin_expect(n % 64 == 0 && n != 0, 0)) {
             pages = table[min(start + kWaves * (n + lane), full_to - 1)];
             check_pages(n);
         }
@@ -739,7 +740,7 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
     // Of the half of the drafts that is the wave's, in the order of its scores.
     uint32_t drafts_seen = 0;
     if (drafts_mine) {
-        if (WINDOW && a.d.window < 64) {  // drafted tokens that lie too far above
+        if (WINDOW && __builtin_expect(a.d.window < 64, 0)) {  // drafted tokens that lie too far above
             const int depth = st.position - (s.past - 1);
             const int depths = __builtin_popcountll(a.d.seen[s.first + min(lane, s.count - 1)] & there);
             for (int j = 0; j < s.count; ++j)
