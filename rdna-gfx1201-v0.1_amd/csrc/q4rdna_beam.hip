@@ -405,10 +405,14 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         const uint32_t before = n;
         n = held_count(s);
         if (n > kHeld) {
-            overflown<T>(s, p, base, a.d.vocab, before, count, &bound);
+            Pick raised = bound;  // (bound itself stays in registers)
+            overflown<T>(s, p, base, a.d.vocab, before, count, &raised);
+            bound = raised;
             n = held_count(s);
         } else if (n > (trip < trips ? kHeld / 2 : few_of(count))) {
-            n = shrink(s, count, n, &bound);
+            Pick raised = bound;
+            n = shrink(s, count, n, &raised);
+            bound = raised;
         }
     }
     take_first(s, n, count, [&](uint32_t r, const Pick &i) {
@@ -451,16 +455,10 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         kept[i] = few && my_list < lists && r < count ? load_agent64(tops + static_cast<size_t>(r) * lists + my_list) : 0;
     }
     const uint32_t parts = a.chunks * kBeamWaves;
-    const bool my_beam_is = static_cast<uint32_t>(tid) < a.d.beams;
-    const float my_score = my_beam_is && a.d.scores != nullptr ? a.d.scores[group * a.d.beams + tid] : 0.0f;
-    // A wave's lanes have a beam's sums, relative to most_of.
-    const auto set_sum = [&](uint32_t b, float most_of, double sum_of) {
-        const float m = wave_max(most_of);
-        const double all = wave_sum(sum_of * __builtin_amdgcn_exp2f((most_of - m) * kLog2e));
-        if (lane == 0) {
-            beam_lse[b] = all;
-            beam_score[b] = m;
-        }
+    const auto score_of = [&](uint32_t b) { return a.d.scores == nullptr ? 0.0f : a.d.scores[group * a.d.beams + b]; };
+    const auto lse_of = [&](float score, float m, double all) {
+        const bool there = __builtin_fabsf(score) < __builtin_inff() && __builtin_fabsf(m) < __builtin_inff();
+        return there ? static_cast<double>(m) + log_of(all) : __builtin_nan("");
     };
     const auto load_part = [&](uint32_t b, uint32_t c, double &sum, float &most) {
         const uint64_t *stat = stats + (static_cast<size_t>(b) * parts + min(c, parts - 1)) * 2;
@@ -477,11 +475,26 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
             for (int i = 0; i < kBeams; ++i) load_part(min(b0 + 4 * i, a.d.beams - 1), lane, sum[i], most[i]);
 #pragma unroll
             for (int i = 0; i < kBeams; ++i)
-                if (b0 + 4 * i < a.d.beams) set_sum(b0 + 4 * i, most[i], most[i] == -__builtin_inff() ? 0.0 : sum[i]);
+                if (b0 + 4 * i < a.d.beams) {
+                    const float m = wave_max(most[i]);
+                    const double all = wave_sum((most[i] == -__builtin_inff() ? 0.0 : sum[i]) * __builtin_amdgcn_exp2f((most[i] - m) * kLog2e));
+                    if (lane == 0) {
+                        beam_lse[b0 + 4 * i] = all;
+                        beam_score[b0 + 4 * i] = m;
+                    }
+                }
+        }
+        // A thread then has a beam: its sum and maximum make way.
+        const float score = static_cast<uint32_t>(tid) < a.d.beams ? score_of(tid) : 0.0f;
+        __syncthreads();
+        if (static_cast<uint32_t>(tid) < a.d.beams) {
+            beam_lse[tid] = lse_of(score, beam_score[tid], beam_lse[tid]);
+            beam_score[tid] = score;
         }
     } else {
 #pragma unroll 1
         for (uint32_t b = wave; b < a.d.beams; b += 4) {
+            const float score = score_of(b);
             double sum_of = 0.0;
             float most_of = -__builtin_inff();  // what the lane's parts are relative to
             constexpr int kParts = 4;           // of a lane, under way together
@@ -499,15 +512,13 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
                 for (int i = 0; i < kParts; ++i) sum_of += sum[i] * __builtin_amdgcn_exp2f((most[i] - to) * kLog2e);
                 most_of = now;
             }
-            set_sum(b, most_of, sum_of);
+            const float m = wave_max(most_of);
+            const double lse = lse_of(score, m, wave_sum(sum_of * __builtin_amdgcn_exp2f((most_of - m) * kLog2e)));
+            if (lane == 0) {
+                beam_lse[b] = lse;
+                beam_score[b] = score;
+            }
         }
-    }
-    __syncthreads();
-    if (my_beam_is) {  // its sum and maximum make way for its log-sum-exp and score
-        const float m = beam_score[tid];
-        const bool there = __builtin_fabsf(my_score) < __builtin_inff() && __builtin_fabsf(m) < __builtin_inff();
-        beam_lse[tid] = there ? static_cast<double>(m) + log_of(beam_lse[tid]) : __builtin_nan("");
-        beam_score[tid] = my_score;
     }
     __syncthreads();
     // The r-th of a list, of a beam.  A dead beam's items are its first tokens, all
@@ -583,12 +594,17 @@ __global__ __launch_bounds__(kBeamThreads) void beam_kernel(const BeamArgs a) {
         least.key = max(least.key, count_th(g, (count + in_block - 1) / in_block, last));
         every([&](const Total &t) { return hold(g, least, t); });
         while (held_count(g) > kHeld) {
-            raise(g, count, &least);
+            Total raised = least;
+            raise(g, count, &raised);
+            least = raised;
             every([&](const Total &t) { return hold(g, least, t); });
         }
     }
     uint32_t found = held_count(g);
-    if (found > few_of(count)) found = shrink(g, count, found, &least);
+    if (found > few_of(count)) {
+        Total raised = least;
+        found = shrink(g, count, found, &raised);
+    }
     take_first(g, found, count, take);
 }
 
