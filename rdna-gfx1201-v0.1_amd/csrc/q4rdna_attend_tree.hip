@@ -18,9 +18,10 @@
 // 1 .. 24 drafts, 8 kv heads of 4 by 128.  The second read is the L2's.)
 //
 // The open block and the drafted tokens are cut into halves of 32, one for a wave
-// at most (4 drafts after 33 tokens 11.5 us, 13.0 as whole blocks).  The workgroup lays their rows into LDS
-// in fp16, scaled by a power of two for each token, fp32 ones in two parts; a
-// row's mask is 64 bits.
+// at most (4 drafts after 33 tokens 11.5 us, 13.0 as whole blocks).  The workgroup
+// lays the drafts' rows into LDS in fp16, scaled by a power of two for each token,
+// fp32 ones in two parts: four tokens a thread, or one where they are few (1.2 us
+// less for these).  A row's mask is 64 bits.
 //
 // A tile's blocks are split over workgroups, dealt on the device by the
 // sequences' lengths, and joined in a fixed order by a second kernel.
@@ -28,9 +29,9 @@
 // What bounds it: a wave's vector instructions, some 550 for a block of 64 tokens
 // (16384 codes into fp16, 2048 weights), a 16th as many matrix instructions; for
 // one sequence, the chain of dependent loads and the first fetch of the code.
-// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 11.1 us; 16 drafts
-// after 4001 17.0 us and 3.9 us the joining; the 32 sequences above (118 MB of codes)
-// in bf16 51.5 us and 4.9 us, in fp32 70.7 (86.2 with one workgroup a CU; two leave
+// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 9.7 us; 16 drafts
+// after 4001 15.7 us and 4.0 us the joining; the 32 sequences above (118 MB of codes)
+// in bf16 51.2 us and 5.0 us, in fp32 70.7 (86.2 with one workgroup a CU; two leave
 // registers for all but eight, and cost a few tokens' call 1%).
 #include <type_traits>
 

@@ -157,8 +157,8 @@ int beam_select(const q4rdna_beam_desc *desc, void *stream) {
     // A trip costs a workgroup 0.8 us, its own start and end 4, and every chunk's
     // items lengthen the join: up to three workgroups a CU, and up to 128 chunks of
     // a group, a chunk is one trip (one, two and three trips: 4 rows of 151936 in
-    // fp32, 152 trips, 12.8, 12.2, 13.5 us; one row 8.6, 10.1, 10.5; 160 rows of
-    // 50257 in bf16, 2080 trips, 35.6, 23.6, 19.4, and 20.8 with four).
+    // fp32, 152 trips, 11.7, 11.5, 12.8 us; one row 7.8, 8.8, 9.5; 160 rows of
+    // 50257 in bf16, 2080 trips, 36.7, 23.7, 18.3, and 19.3 with four).
     const uint64_t rows = static_cast<uint64_t>(d.groups) * d.beams;
     const uint32_t row_trips = (d.vocab + kBeamTrip - 1) / kBeamTrip;
     const uint64_t most = 3ull * cu_count(device);
