@@ -382,11 +382,12 @@ __device__ __forceinline__ void set_query(ManyState<D, SPLIT> &st, const Eight<T
 }
 
 // The drafted tokens' K and V into LDS: a thread takes eight numbers of B tokens,
-// D / 8 threads side by side a row: of four, or, where there are few, of one.
+// D / 8 threads side by side a row: of four (of 64 numbers two), or, where there
+// are few, of one.
 template <int D, typename T, int B>
 struct DraftRows {
     static constexpr int kOctets = D / 8;
-    static constexpr int kTokens = B == 1 ? kTreeThreads / kOctets : kBlock;
+    static constexpr int kTokens = B * kTreeThreads / kOctets;
     Eight<T> raw[2][B];
     __device__ __forceinline__ static int octet() { return threadIdx.x % kOctets; }
     __device__ __forceinline__ static int token() { return threadIdx.x / kOctets * B; }  // the first
@@ -407,7 +408,6 @@ __device__ __forceinline__ void load_drafts(DraftRows<D, T, B> &r, const TreeArg
 template <int D, int SPLIT, typename T, int B>
 __device__ __forceinline__ void stage_drafts(TreeStage<D, SPLIT> &stage, const DraftRows<D, T, B> &r) {
     const int octet = r.octet(), token = r.token();
-    if (token >= kBlock) return;
     float x[2][B][8];
 #pragma unroll
     for (int which = 0; which < 2; ++which)
@@ -681,7 +681,7 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
     load_query<D, T>(query, static_cast<const T *>(a.d.q.data) + static_cast<int64_t>(s.first + token) * a.d.q.token_stride +
                                 (head * a.group + (row < rows ? row - token * group : 0)) * a.d.q.head_stride);
     uint64_t seen = a.d.seen[s.first + token];  // of the drafts, by the lane's row
-    DraftRows<D, T, 4> draft_rows;
+    DraftRows<D, T, D / 32> draft_rows;  // all 64 by all threads
     DraftRows<D, T, 1> few_rows;
     const bool few = s.count <= DraftRows<D, T, 1>::kTokens;
     if (has_drafts) {
