@@ -29,9 +29,9 @@
 // What bounds it: a wave's vector instructions, some 550 for a block of 64 tokens
 // (16384 codes into fp16, 2048 weights), a 16th as many matrix instructions; for
 // one sequence, the chain of dependent loads and the first fetch of the code.
-// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 9.7 us; 16 drafts
-// after 4001 15.7 us and 4.0 us the joining; the 32 sequences above (118 MB of codes)
-// in bf16 51.2 us and 5.0 us, in fp32 70.7 (86.2 with one workgroup a CU; two leave
+// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 9.5 us; 16 drafts
+// after 4001 15.5 us and 3.9 us the joining; the 32 sequences above (118 MB of codes)
+// in bf16 49.9 us and 4.8 us, in fp32 70.7 (86.2 with one workgroup a CU; two leave
 // registers for all but eight, and cost a few tokens' call 1%).
 #include <type_traits>
 

@@ -16,8 +16,8 @@
 //
 // The logits are read once, at far less than a copy's rate: what takes the time
 // is one thing after another, load, bound, order, arrival, sums, totals, order.
-// 1 of 151936 in fp32 8.4 us, 8 of 4 rows 11.8, 10 of each 5 of 160 rows of 50257
-// in bf16 (16 MB) 18.2.
+// 1 of 151936 in fp32 8.0 us, 8 of 4 rows 11.8, 10 of each 5 of 160 rows of 50257
+// in bf16 (16 MB) 18.5.
 #include "q4rdna_layer_device.h"
 
 namespace q4rdna {
