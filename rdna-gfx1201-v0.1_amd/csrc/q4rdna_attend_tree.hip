@@ -146,27 +146,6 @@ __device__ __forceinline__ h16x8 half_piece(i32x4 piece, int half) {
     return r;
 }
 
-// The same without the -1152: a code c is 1152 + c, exact in fp16.
-__device__ __forceinline__ h16x8 half_piece_biased(i32x4 piece, int half) {
-    union {
-        uint32_t w[4];
-        h16x8 h;
-    } r;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const uint32_t u = static_cast<uint32_t>(piece[2 * half + x]) ^ 0x80808080u;
-        r.w[2 * x] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
-        r.w[2 * x + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    }
-    return r.h;
-}
-
-// Operands of the two products out of raw tiles.
-template <bool LOW, int D>
-__device__ __forceinline__ h16x8 k_fragment(const TreeRaw<D> &r, int t, int f) { return half_piece<LOW>(r.x[t * (D / 32) + f / 2], f % 2); }
-template <bool LOW, int D>
-__device__ __forceinline__ h16x8 v_fragment(const TreeRaw<D> &r, int d, int y, int pair) { return half_piece<LOW>(r.x[d * 2 + y], pair); }
-
 // s[t] += the products of K's fragments (32 tokens t, 16 numbers f) with the rows.
 template <int N, int D, int SPLIT, typename K>
 __device__ __forceinline__ void add_scores(const ManyState<D, SPLIT> &st, f32x16 (&s)[N], K fragment) {
@@ -205,24 +184,11 @@ __device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (
     }
 }
 template <int N>
-__device__ __forceinline__ void clear(f32x16 (&s)[N], float to = 0.0f) {
+__device__ __forceinline__ void clear(f32x16 (&s)[N]) {
 #pragma unroll
     for (int t = 0; t < N; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i] = to;
-}
-// -1152 times the sum of the lane's row of q.
-template <int D>
-__device__ __forceinline__ float k_bias(const ManyState<D, 1> &st) {
-    h16x8 bias;
-    f32x16 sum;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bias[e] = static_cast<_Float16>(-1152.0f);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
-#pragma unroll
-    for (int f = 0; f < D / 16; ++f) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(bias, st.q[f][0], sum, 0, 0, 0);
-    return sum[0];
+        for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
 }
 // All ones where bit i is set.  (As an instruction of its own: the compiler would
 // make a compare of it, and 32 of them would each hold a pair of scalar registers.)
@@ -761,22 +727,13 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
         }
         return bits;
     };
-    // With one part of q the codes of K go in as 1152 + c and the products start
-    // at -1152 sum q, which saves an instruction for two codes.  What that costs:
-    // roundings of sums up to 1152 |sum q| instead of |sum q c|, a few 2^-24 of
-    // them, 2^-17 of |c| |sum q| or less; q itself and the weights have 11 bits.
-    float bias = 0.0f;
-    if constexpr (SPLIT == 1) bias = k_bias(st);
     // A full block; `masked` ones are the first of a window's.
     const auto block = [&](int n, auto masked) {
         f32x16 sc[2];
         const float nan = __builtin_nanf("");
         const float k_scale = good_next ? scale_next[0] : nan, v_scale = good_next ? scale_next[1] : nan;
-        clear(sc, bias);
-        add_scores(st, sc, [&](int t, int f) {
-            if constexpr (SPLIT == 1) return half_piece_biased(ka.x[t * (D / 32) + f / 2], f % 2);
-            else return k_fragment<false>(ka, t, f);
-        });
+        clear(sc);
+        add_scores(st, sc, [&](int t, int f) { return half_piece<false>(ka.x[t * (D / 32) + f / 2], f % 2); });
         tile_end();
         if (n + 1 < full) {
             good_next = next(n + 1);
@@ -787,7 +744,7 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
         tile_end();
         soften_block(st, sc, k_scale, v_scale, masked ? seen_from((start + kWaves * n) * kBlock) : 0xffffffffu, masked);
         tile_end();
-        add_rows(st, sc, [&](int d, int y, int pair) { return v_fragment<false>(vb, d, y, pair); });
+        add_rows(st, sc, [&](int d, int y, int pair) { return half_piece<false>(vb.x[d * 2 + y], pair); });
         tile_end();
         if (n + 1 < full) load_v(vb, tile);
         else if (open_mine) load_open_v(vb, planes, which);
