@@ -160,25 +160,36 @@ __device__ __forceinline__ void add_scores(const ManyState<D, SPLIT> &st, f32x16
     }
 }
 // o += the products of V's fragments (32 numbers d; tokens 16 a + 8 y + 4 half + b,
-// a = 2 t, 2 t + 1) with the weights.
+// a = 2 t, 2 t + 1) with the weights, which are held in two fp16 parts whatever the
+// type of the queries: 22 bits of each.  (In 11 bits an fp16 row was further off
+// by its weights than by its own rounding.)
 template <int N, int D, int SPLIT, typename V>
 __device__ __forceinline__ void add_rows(ManyState<D, SPLIT> &st, const f32x16 (&s)[N], V fragment) {
 #pragma unroll
     for (int t = 0; t < N; ++t) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-            h16x8 p[SPLIT];
+            float minus = -1.0f;
+            asm("" : "+s"(minus));  // (a product, so that one instruction takes a half as it is)
+            h16x8 p[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float w = s[t][4 * (2 * (e / 4) + y) + e % 4];
-                p[0][e] = static_cast<_Float16>(w);
-                if (SPLIT == 2) p[SPLIT - 1][e] = static_cast<_Float16>(w - static_cast<float>(p[0][e]));
+            for (int e = 0; e < 8; e += 2) {
+                const int at = 4 * (2 * (e / 4) + y) + e % 4;
+                const f32x2 w = {s[t][at], s[t][at + 1]};
+                h16x2 high = __builtin_convertvector(w, h16x2);
+                asm("" : "+v"(high));  // or each would be converted once more by itself
+                const f32x2 rest = {fmaf(static_cast<float>(high[0]), minus, w[0]), fmaf(static_cast<float>(high[1]), minus, w[1])};
+                const h16x2 low = __builtin_convertvector(rest, h16x2);
+                p[0][e] = high[0];
+                p[0][e + 1] = high[1];
+                p[1][e] = low[0];
+                p[1][e + 1] = low[1];
             }
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
                 const h16x8 v = fragment(d, y, t);
 #pragma unroll
-                for (int x = 0; x < SPLIT; ++x) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], st.o[d], 0, 0, 0);
+                for (int x = 0; x < 2; ++x) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[x], st.o[d], 0, 0, 0);
             }
         }
     }
