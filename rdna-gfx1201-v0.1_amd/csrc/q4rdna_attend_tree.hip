@@ -718,7 +718,9 @@ __global__ __launch_bounds__(kTreeThreads, PER_CU) void attend_tree_kernel(const
     // Of the half of the drafts that is the wave's, in the order of its scores.
     uint32_t drafts_seen = 0;
     if (drafts_mine) {
-        if (WINDOW && __builtin_expect(a.d.window < 64, 0)) {  // drafted tokens that lie too far above
+        // Drafted tokens that lie too far above: by 64 at most, all of a row's that sees
+        // 64 over one that sees none.
+        if (WINDOW && __builtin_expect(a.d.window <= kTreeMax, 0)) {
             const int depth = st.position - (s.past - 1);
             const int depths = __builtin_popcountll(a.d.seen[s.first + min(lane, s.count - 1)] & there);
             for (int j = 0; j < s.count; ++j)
