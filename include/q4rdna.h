@@ -436,7 +436,8 @@ int q4rdna_kv_append(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch,
  * receives log sum_t exp(scale * q . k_t), [tokens][q_heads].  Calls that
  * split a sequence use scratch per (device, stream), under the rules of the
  * GEMVs' scratch above: make one call of a shape on the stream before
- * capturing it. */
+ * capturing it.  Threads may call on one stream at once: no other call's
+ * launch that uses the scratch comes between a call's own. */
 typedef struct q4rdna_kv_attend_desc {
     uint32_t dtype;           /* of q and out */
     uint32_t q_heads;

@@ -122,9 +122,9 @@ int attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, cons
     const OnDevice device(cache->device);
     if (device.status() != Q4RDNA_OK) return device.status();
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    Scratch scratch;  // held over the launches
     if (a.splits > 1) {
         const size_t floats = workgroups * kTreeRows * (cache->head_dim + 3);
-        Scratch scratch;
         if ((rc = get_scratch(cache->device, s, floats + 2 * jobs, 0, &scratch)) != Q4RDNA_OK) return rc;
         a.partials = scratch.partials;
         a.jobs = reinterpret_cast<TreeJob *>(scratch.partials + floats);
@@ -215,7 +215,7 @@ int fork(const q4rdna_kv_cache *caches, uint32_t count, const q4rdna_kv_fork_des
     const uint64_t touched = std::min<uint64_t>(d.table_width, static_cast<uint64_t>(d.room) / kKvBlock + 2);
     const uint64_t given = std::min<uint64_t>(c.page_count, touched * d.sequences);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    Scratch scratch;
+    Scratch scratch;  // held over the launches
     const uint32_t cus = cu_count(c.device);
     const auto take_layers = [&](uint32_t first) {
         a.layers = std::min(count - first, kForkLayers);

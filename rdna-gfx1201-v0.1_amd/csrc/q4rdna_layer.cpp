@@ -6,16 +6,28 @@
 #include <algorithm>
 #include <cmath>
 #include <map>
-#include <mutex>
 #include <utility>
 #include <vector>
 
 namespace q4rdna {
 namespace {
 
-std::mutex g_scratch_mu;
-std::map<std::pair<int, hipStream_t>, Scratch> g_scratch;
-std::vector<void *> g_retired;
+// One stream's buffers.  Those that were outgrown are kept.
+struct StreamScratch {
+    std::mutex mu;
+    float *partials = nullptr;
+    size_t floats = 0;
+    uint32_t *arrived = nullptr;
+    size_t jobs = 0;
+    std::vector<void *> retired;
+};
+std::mutex g_scratch_mu;  // of the map: its entries stay where they are
+std::map<std::pair<int, hipStream_t>, StreamScratch> g_scratch;
+
+StreamScratch &stream_scratch(int device, hipStream_t stream) {
+    std::lock_guard<std::mutex> lock(g_scratch_mu);
+    return g_scratch[{device, stream}];
+}
 
 bool stream_captured(hipStream_t stream) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -41,18 +53,18 @@ hipError_t relaxed_malloc(void **p, size_t bytes, bool zero, hipStream_t stream)
 }  // namespace
 
 int get_scratch(int device, hipStream_t stream, size_t floats, size_t jobs, Scratch *out) {
-    std::lock_guard<std::mutex> lock(g_scratch_mu);
-    Scratch &s = g_scratch[{device, stream}];
+    StreamScratch &s = stream_scratch(device, stream);
+    std::unique_lock<std::mutex> lock(s.mu);
     if (s.floats < floats || s.jobs < jobs) {
         if (stream_captured(stream))
             return set_error(Q4RDNA_ERR_MEMORY, "attention scratch: it cannot grow while its stream is being captured");
-        g_retired.reserve(g_retired.size() + 2);
+        s.retired.reserve(s.retired.size() + 2);
         if (s.floats < floats) {
             const size_t count = std::max(floats, 2 * s.floats);
             void *p = nullptr;
             const hipError_t e = relaxed_malloc(&p, count * sizeof(float), false, stream);
             if (e != hipSuccess) return set_error(Q4RDNA_ERR_MEMORY, "attention scratch: %s", hipGetErrorString(e));
-            if (s.partials != nullptr) g_retired.push_back(s.partials);
+            if (s.partials != nullptr) s.retired.push_back(s.partials);
             s.partials = static_cast<float *>(p);
             s.floats = count;
         }
@@ -61,12 +73,14 @@ int get_scratch(int device, hipStream_t stream, size_t floats, size_t jobs, Scra
             void *p = nullptr;
             const hipError_t e = relaxed_malloc(&p, count * sizeof(uint32_t), true, stream);
             if (e != hipSuccess) return set_error(Q4RDNA_ERR_MEMORY, "attention scratch: %s", hipGetErrorString(e));
-            if (s.arrived != nullptr) g_retired.push_back(s.arrived);
+            if (s.arrived != nullptr) s.retired.push_back(s.arrived);
             s.arrived = static_cast<uint32_t *>(p);
             s.jobs = count;
         }
     }
-    *out = s;
+    out->partials = s.partials;
+    out->arrived = s.arrived;
+    out->held = std::move(lock);
     return Q4RDNA_OK;
 }
 
@@ -221,8 +235,8 @@ int attend(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *batch, const q4r
     const OnDevice device(cache->device);
     if (device.status() != Q4RDNA_OK) return device.status();
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    Scratch scratch;  // held over the launches
     if (jobs != 0) {
-        Scratch scratch;
         if ((rc = get_scratch(cache->device, s, floats, jobs, &scratch)) != Q4RDNA_OK) return rc;
         f.partials = m.partials = scratch.partials;
         f.arrived = m.arrived = scratch.arrived;

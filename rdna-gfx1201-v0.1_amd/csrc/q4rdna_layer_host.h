@@ -4,6 +4,7 @@
 
 #include <atomic>
 #include <exception>
+#include <mutex>
 
 #include "q4rdna_layer.h"
 #include "q4rdna_runtime.h"
@@ -127,12 +128,14 @@ inline bool wide_rows(const q4rdna_kv_rows &r, uint32_t dtype, int64_t elements)
 // Attention's partial results and arrival counters per (device, stream), under
 // the same rules as the GEMVs' exchange slots (q4rdna_runtime.cpp): outgrown
 // buffers are kept, since launches still queued and captured graphs use them,
-// and nothing is allocated while the stream is being captured.
+// and nothing is allocated while the stream is being captured.  All calls of a
+// stream share them, and some leave in one launch what the next one reads: a call
+// holds them from here to its last launch, so that no other thread's launch on
+// the stream comes between.
 struct Scratch {
     float *partials = nullptr;
-    size_t floats = 0;
     uint32_t *arrived = nullptr;
-    size_t jobs = 0;
+    std::unique_lock<std::mutex> held;
 };
 int get_scratch(int device, hipStream_t stream, size_t floats, size_t jobs, Scratch *out);
 
