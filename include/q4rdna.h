@@ -534,7 +534,8 @@ int q4rdna_rotate(const q4rdna_rotate_desc *desc, void *stream);
  * `window` before it: cached tokens at t > p - window, drafted ones at
  * p_j > p - window.
  * A row that sees nothing is zero, its lse -inf.  A drafted token with a number
- * of k (v) that is not finite makes every row that sees it NaN.
+ * of k (v) that is not finite makes every row that sees it NaN.  Scores are
+ * meant to lie within fp32's range: q and k may be of any size.
  * The cache is read only; accepted tokens are appended by q4rdna_kv_append of
  * their rows, with rotary 0.  max_tokens <= Q4RDNA_TREE_MAX.  Refusals on the
  * device, and scratch, as for q4rdna_kv_attend. */

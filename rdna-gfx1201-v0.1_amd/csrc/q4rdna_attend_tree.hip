@@ -238,6 +238,16 @@ __device__ __forceinline__ float total(const f32x16 (&s)[N]) {
         for (int x = 0; x < 4; ++x) sum[x] += s[x * N / 4][4 * N * x % 16 + i];
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
+// s * unit - m, the product rounded first: a score that is the reference becomes
+// zero, however large both are.
+template <int N>
+__device__ __forceinline__ void subtract(f32x16 (&s)[N], float unit, float m) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = s[t][i] * unit - m;
+}
 // Scores to weights: s = 2^(s * unit + shift), zero where hidden; their sum.
 template <int N>
 __device__ __forceinline__ float exponentials(f32x16 (&s)[N], float unit, float shift, uint32_t seen, bool masked) {
@@ -247,6 +257,25 @@ __device__ __forceinline__ float exponentials(f32x16 (&s)[N], float unit, float 
         for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], unit, shift));
     if (masked) hide(s, seen, 0.0f);
     return total(s);
+}
+
+// From scores of this size on (base 2) fp32 has steps that a weight would show.
+constexpr float kFar = 0x1p16f;
+// refer() for a weight times V of 2^(base + rel), which is not added up: the steps
+// of a large score are larger than rel.
+template <int D, int SPLIT>
+__device__ __forceinline__ void refer(ManyState<D, SPLIT> &st, float now, float base, float rel) {
+    const bool grown = now > st.m + kLazy, more = (base - st.m) + rel > st.e + kLazy;
+    if (__builtin_amdgcn_ballot_w64(grown || more) == 0) return;
+    if (!(grown || more)) return;
+    const float m = grown ? now : st.m, most = fmaxf((st.m - m) + st.e, (base - m) + rel);
+    const float e = most == kNegInf ? kNegInf : ceilf(most);
+    st.l *= __builtin_amdgcn_exp2f(st.m - m);  // 0 from -inf
+    const float f = st.e == kNegInf ? 1.0f : __builtin_amdgcn_exp2f((st.m - m) + (st.e - e));  // (o is zero there)
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) st.o[d] *= f;
+    st.m = m;
+    st.e = e;
 }
 
 // The softmax of a full block: integer products to weights in the accumulators'
@@ -262,9 +291,16 @@ __device__ __forceinline__ void soften_block(ManyState<D, SPLIT> &st, f32x16 (&s
     const bool finite = v_scale < __builtin_inff();
     const float v_exp = static_cast<float>(__builtin_amdgcn_frexp_expf(v_scale));
     const float v_log = finite ? __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(v_scale)) : __builtin_nanf("");
-    refer(st, now, now + (v_exp + v_log));
+    refer(st, now, now, v_exp + v_log);
     const float ratio = none ? 0.0f : finite ? fmaxf(v_log + (v_exp - st.e), kLeast) : __builtin_nanf("");
-    const float sum = exponentials(s, unit, kWeight - (st.m == kNegInf ? 0.0f : st.m) + ratio, seen, masked);
+    const float m = st.m == kNegInf ? 0.0f : st.m;
+    float times = unit, shift = kWeight - m + ratio;
+    if (__builtin_expect(!none && __builtin_fabsf(now) > kFar, 0)) {
+        subtract(s, unit, m);
+        times = 1.0f;
+        shift = kWeight + ratio;
+    }
+    const float sum = exponentials(s, times, shift, seen, masked);
     st.l += sum * __builtin_amdgcn_exp2f(-ratio);
 }
 // The same of 32 tokens with a scale each, K's and 64 further on V's, the lane's
@@ -272,19 +308,25 @@ __device__ __forceinline__ void soften_block(ManyState<D, SPLIT> &st, f32x16 (&s
 // of 256 times the scales.
 template <int D, int SPLIT>
 __device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&s)[1], int unit_log, uint32_t seen, const float *scales) {
+    // A token's scale and the row's by their exponents together: either alone may
+    // take the products out of fp32's range where the score is within it.
+    const float unit = 2.0f * __builtin_amdgcn_frexp_mantf(st.q_scale);
+    const int q_exp = st.q_scale == 0.0f ? -400 : __builtin_amdgcn_frexp_expf(st.q_scale) - 1 + unit_log;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         const f32x4 kt = *reinterpret_cast<const f32x4 *>(scales + 8 * x);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) s[0][4 * x + b] *= kt[b];
+        for (int b = 0; b < 4; ++b)
+            s[0][4 * x + b] = __builtin_amdgcn_ldexpf(s[0][4 * x + b] * __builtin_amdgcn_frexp_mantf(kt[b]), __builtin_amdgcn_frexp_expf(kt[b]) + q_exp);
     }
     hide(s, seen, kNegInf);
-    const float unit = __builtin_amdgcn_ldexpf(st.q_scale, unit_log), top = max_xor32(largest(s));
+    const float top = max_xor32(largest(s));
     const float now = top == kNegInf ? kNegInf : top * unit;
     // Weights of 2^8 at most times the scales, under 2^122, in fp32; the largest
     // of them is what the row refers to.
     const float m = now > st.m + kLazy ? now : st.m;
-    const float sum = exponentials(s, unit, m == kNegInf ? 0.0f : -m, seen, true);
+    subtract(s, unit, m == kNegInf ? 0.0f : m);
+    const float sum = exponentials(s, 1.0f, 0.0f, seen, true);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         const f32x4 vt = *reinterpret_cast<const f32x4 *>(scales + kBlock + 8 * x);
@@ -292,7 +334,7 @@ __device__ __forceinline__ void soften_tokens(ManyState<D, SPLIT> &st, f32x16 (&
         for (int b = 0; b < 4; ++b) s[0][4 * x + b] *= vt[b] + (vt[b] - vt[b]);  // an infinite scale is made NaN
     }
     hide(s, seen, 0.0f);
-    refer(st, now, m + __builtin_amdgcn_logf(max_xor32(fmaxf(largest(s), 0.0f))) + static_cast<float>(unit_log));
+    refer(st, now, m, __builtin_amdgcn_logf(max_xor32(fmaxf(largest(s), 0.0f))) + static_cast<float>(unit_log));
     st.l += __builtin_amdgcn_ldexpf(sum, static_cast<int>(kWeight));
     // From units of 2^(m + unit_log) to the accumulators'.
     const int up = st.e == kNegInf ? 0 : unit_log + static_cast<int>(kWeight) - static_cast<int>(st.e);
