@@ -590,9 +590,9 @@ int q4rdna_beam_select(const q4rdna_beam_desc *desc, void *stream);
  *    m the block m / 64 where it holds tokens, and the one before it.
  *  - table: entries of full blocks come from the parent's row.  A page that is
  *    then in no row's full blocks is free, but for those marked in `kept`, and
- *    the entries of the blocks that the next `room` tokens of each sequence
- *    (none of a dropped one) touch get free pages: the lowest numbers first, in
- *    the order of sequences and blocks.  Other entries become -1, and so do those
+ *    the entries of each sequence's open block, where it holds tokens, and of the
+ *    blocks that its next `room` tokens touch get free pages (none of a dropped
+ *    one): the lowest numbers first, in the order of sequences and blocks.  Other entries become -1, and so do those
  *    that no page is left for, each of which adds to *faults.
  * So `fork` with parents[i] = i gives out the pages for the next tokens, and a
  * program that calls it before each step needs no allocator of its own.  Every

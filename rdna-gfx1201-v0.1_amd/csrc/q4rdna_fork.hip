@@ -39,8 +39,8 @@ __device__ __forceinline__ uint32_t threads_before(uint32_t v, uint32_t *totals,
     return before + upto - v;
 }
 
-// Blocks that the next `room` tokens behind `past` touch: from past / 64 up to
-// this one.
+// The open block, where it holds tokens, and those that the next `room` tokens
+// behind `past` touch: from past / 64 up to this one.
 __device__ __forceinline__ int room_end(const q4rdna_kv_fork_desc &d, int past) {
     const uint64_t end = (static_cast<uint64_t>(past) + d.room + kBlock - 1) / kBlock;
     return static_cast<int>(min(end, static_cast<uint64_t>(d.table_width)));

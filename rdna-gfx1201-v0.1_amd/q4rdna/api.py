@@ -573,9 +573,10 @@ class KVBatch:
         -1: none) was; past, table and slots are changed in place, and so are
         the open blocks in `caches`, all layers' (q4rdna_kv_fork).
 
-        Full pages are shared.  Entries for the next `room` tokens get pages
-        that no sequence of the batch holds (and that `kept`, bool or uint8
-        [pages], does not mark), so a program that forks before each step, with
+        Full pages are shared.  Entries for the tokens of an open block, also
+        with a room of 0, and for the next `room` tokens get pages that no
+        sequence of the batch holds (and that `kept`, bool or uint8 [pages],
+        does not mark), so a program that forks before each step, with
         parents[i] = i where nothing changes, needs no allocator of its own.
         What is refused, and entries that no page is left for, count in the
         first cache's faults()."""
