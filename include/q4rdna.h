@@ -535,7 +535,10 @@ int q4rdna_rotate(const q4rdna_rotate_desc *desc, void *stream);
  * p_j > p - window.
  * A row that sees nothing is zero, its lse -inf.  A drafted token with a number
  * of k (v) that is not finite makes every row that sees it NaN.  Scores are
- * meant to lie within fp32's range: q and k may be of any size.
+ * meant to lie within fp32's range: q and k may be of any size.  fp16 and bf16 q,
+ * k and v and the cache's codes enter the products as they are, fp32 q, k and v as
+ * two fp16 parts, which hold 2^-23 of their row's largest number; weights are held
+ * to 2^-22, sums in fp32.
  * The cache is read only; accepted tokens are appended by q4rdna_kv_append of
  * their rows, with rotary 0.  max_tokens <= Q4RDNA_TREE_MAX.  Refusals on the
  * device, and scratch, as for q4rdna_kv_attend. */
@@ -557,7 +560,10 @@ int q4rdna_kv_attend_tree(const q4rdna_kv_cache *cache, const q4rdna_kv_batch *b
  * and the `count` largest of them, largest first: out_scores, out_rows (group *
  * beams + b) and out_tokens, each [groups][count].  Totals are compared in 64
  * bits; equal ones go by row, then by logit (totals that 64 bits cannot tell
- * apart), then by token.
+ * apart), then by token.  A beam's log sum comes from fp32 exponentials, added up
+ * by 16 in fp32 and then in 64 bits: it is within 2^-18 of the formula's, a few
+ * 2^-24 as a rule.  So a beam's own tokens are always in the order of their
+ * logits, but totals of two beams that lie closer than that may come either way.
  * scores NULL: zeros.  A beam has no continuation, all its totals are -inf, if
  * its score is not finite, if all its logits are -inf or if one of them is NaN
  * or +inf; such totals come behind all others.  out_scores may be scores where

@@ -14,24 +14,35 @@
 // it: no wave waits for another before the end, when their parts meet in LDS.
 // (Tiles of 128 rows, a wave per 32, read each block once rather than once a
 // tile, but left three waves idle where rows are few or odd, and parts four times
-// as large to join: 63 us rather than 56 for 32 sequences of 100 .. 8000 tokens,
-// 1 .. 24 drafts, 8 kv heads of 4 by 128.  The second read is the L2's.)
+// as large to join: an eighth slower for 32 sequences of 100 .. 8000 tokens, 1 .. 24
+// drafts, 8 kv heads of 4 by 128.  The second read is the L2's.)
 //
 // The open block and the drafted tokens are cut into halves of 32, one for a wave
-// at most (4 drafts after 33 tokens 11.5 us, 13.0 as whole blocks).  The workgroup
+// at most (as whole blocks 4 drafts after 33 tokens take 1.5 us more).  The workgroup
 // lays the drafts' rows into LDS in fp16, scaled by a power of two for each token,
 // fp32 ones in two parts: four tokens a thread, or one where they are few (1.2 us
 // less for these).  A row's mask is 64 bits.
 //
+// What is rounded: fp32 q, k and v to two fp16 parts, weights of all types to two
+// (2^-22 of each); fp16 and bf16 rows and the cache's codes are exact in one.  (One
+// part of the weights and K's codes with a bias, 8% faster for the 32 sequences in
+// bf16, put fp16 results further off than their own rounding, and scores off by
+// 2^-14 of a block's scale times sum |q|.)
+//
 // A tile's blocks are split over workgroups, dealt on the device by the
 // sequences' lengths, and joined in a fixed order by a second kernel.
 //
-// What bounds it: a wave's vector instructions, some 550 for a block of 64 tokens
-// (16384 codes into fp16, 2048 weights), a 16th as many matrix instructions; for
-// one sequence, the chain of dependent loads and the first fetch of the code.
-// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 9.5 us; 16 drafts
-// after 4001 15.5 us and 3.9 us the joining; the 32 sequences above (118 MB of codes)
-// in bf16 49.9 us and 4.8 us, in fp32 70.7 (86.2 with one workgroup a CU; two leave
+// What bounds it, for the 32 sequences above (118 MB of codes, 150 MB read, 2.6
+// TB/s) in bf16: nothing alone.  A block of 64 tokens takes a wave some 500 vector
+// instructions (16384 codes into fp16, 2048 weights) and 48 matrix ones; with the
+// workgroups' start, drafts and joining, 44% of all vector instructions, the vector
+// unit is busy 47% of the time and the matrix unit 20%.  A SIMD has 1.4 waves on
+// average of the two that fit, since parts end unevenly, and these wait 28% of their
+// time for data and as long for their turn.  For one sequence it is the chain of
+// dependent loads and the first fetch of the code.
+// Eight kv heads of 4 by 128: fp32, 4 drafts after 33 tokens 9.6 us; 16 drafts
+// after 4001 15.4 us and 3.9 us the joining; the 32 sequences in bf16 56.8 us and
+// 4.8 us, in fp32 66.9 and 5.4 (with one workgroup a CU a fifth more; two leave
 // registers for all but eight, and cost a few tokens' call 1%).
 #include <type_traits>
 

@@ -8,6 +8,14 @@
 // in the chunks' order, makes the totals in 64 bits and selects again: the
 // results do not depend on the order of arrival.
 //
+// Exponentials are fp32's, 16 of a thread's are added up in fp32 and these in 64
+// bits.  Of 2^-24 that is 5/2 |x - max| on average, the instruction's 2 and 15
+// additions at most, under 2^-18 of the sum; a few 2^-24 as a rule, since they
+// differ in sign.  Totals of two beams are off by that, less than the last place of
+// fp32 scores of 10 or so, which come in and go out.  (In 64 bits throughout,
+// 20 instructions an exponential: 24.5 us rather than 18.0 for 10 each of 5 of 160
+// rows of 50257, 12.7 rather than 11.2 for 8 of 4 of 151936, a pass.)
+//
 // Selection: threads' maxima, several threads' together, 64 or 128 in all; the
 // count-th largest of them is a bound that `count` items at least reach, and
 // few more.  These go to LDS and each counts how many are before it.  Equal

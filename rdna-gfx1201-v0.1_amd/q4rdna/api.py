@@ -769,9 +769,10 @@ class KVCache:
         seen[n] (int64 [tokens], :func:`tree`'s or any mask) is set where token n
         sees the j-th drafted one of its sequence.  The cache does not change:
         the rows of accepted tokens are appended afterwards, by :meth:`append`
-        without cos and sin.  The batch's max_tokens is 64 at most.  scale,
-        window, lse and refused sequences as for :meth:`attend`; with a window a
-        token stands at past - 1 + the number of drafted ones that it sees."""
+        without cos and sin.  The batch's max_tokens, given with cu_tokens, is 64
+        at most.  scale, window, lse and refused sequences as for :meth:`attend`;
+        with a window a token stands at past - 1 + the number of drafted ones that
+        it sees."""
         if q.dim() != 3:
             raise ValueError("q must be [tokens, q_heads, head_dim]")
         if stream is not None and (out is None or lse is True):
@@ -916,7 +917,7 @@ def tree(batch: KVBatch, parents: torch.Tensor, positions: torch.Tensor | None =
     the last cached token.  positions (int32) is past + the tokens above it,
     seen (int64) has a bit for each of them and for itself.  A token whose
     parent is out of range, and what lies below it, gets position -1 and seen
-    0.  The batch's max_tokens is 64 at most."""
+    0.  The batch's max_tokens, given with cu_tokens, is 64 at most."""
     device = batch.device
     if stream is not None and (positions is None or seen is None):
         with _on_stream(stream, device):
@@ -1007,9 +1008,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor | None, count: int, o
     log-softmax of its beam's logits.  rows (int32) is group * beams + beam, what
     :meth:`KVBatch.fork` takes for a batch of all groups' beams; tokens is
     int32; out: these three, to be written (the first may be `scores` where
-    count is beams).  Equal totals go by row, then by
-    logit, then by token.  A beam whose score is not finite (such as -inf) or whose logits have
-    a NaN or +inf has no continuation: its totals are -inf, behind all others."""
+    count is beams).  Equal totals go by row, then by logit, then by token; those
+    of two beams that are closer than 2^-18 (a few 2^-24 as a rule, a row's log sum
+    is from fp32 exponentials) may come either way.  A beam whose score is not
+    finite (such as -inf) or whose logits have a NaN or +inf has no continuation:
+    its totals are -inf, behind all others."""
     if logits.dim() != 3 or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor [groups, beams, vocab]")
     if logits.requires_grad:
